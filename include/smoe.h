@@ -394,6 +394,107 @@ SMOE_API int smoe_combine_rows(const void* y, int y_dtype, const float* row_w,
                                const int32_t* tok_row, int N, int K, int H, void* out,
                                int out_dtype, void* stream);
 
+/* ---- routing over groups of experts, and experts on block-scaled fp8 ----
+ * No counterpart in the reference, whose router is a softmax top-k and whose
+ * fp8 has one scale per tensor or channel: the routing and the weight format
+ * of larger mixture-of-experts models, beside smoe_select_topk,
+ * smoe_quantize_fp8_tensor, smoe_linear_fp8fp8 and smoe_expert_delta. */
+
+/* Group-limited routing over logits z [N,E] (SMOE_F32 / SMOE_BF16 / SMOE_F16):
+ *   s = softmax(z) or sigmoid(z) per row; c = s + bias (bias f32 [E] or NULL:
+ *   it counts in the choice, not in the weights);
+ *   groups > 1: E / groups consecutive experts make a group, its value is the
+ *   sum of its two largest c (the one c where it has one), and only the
+ *   top_groups groups of largest value stay;
+ *   top_idx i32 [N,K]: the K experts of largest c that stay, descending;
+ *   top_w f32 [N,K]: scale * s / max(sum of the chosen s, 1e-9) with renorm,
+ *   else scale * s.
+ * Ties go to the lower index.  An expert with z = -inf is masked: its score
+ * is 0, it is chosen after every other, with weight 0 (which the dispatch plan
+ * drops), so a row that masks every expert gets weights 0.  NaN compares as
+ * +infinity and gives NaN weights.  Choices are made on scores of 64 bits.
+ * 1 <= E <= 256, 1 <= K <= min(64, top_groups * E / groups), groups divides E,
+ * 1 <= top_groups <= groups.  No workspace. */
+#define SMOE_SCORE_SOFTMAX 0
+#define SMOE_SCORE_SIGMOID 1
+SMOE_API int smoe_select_groups(const void* logits, int logits_dtype, int N, int E, int K, int score,
+                                const float* bias, int groups, int top_groups, int renorm,
+                                float scale, float* top_w, int32_t* top_idx, void* stream);
+/* Gradient of the weights with respect to the logits, the choice held fixed:
+ * d_top_w f32 [N,K] -> d_logits [N,E] in logits_dtype, every entry written.
+ * top_idx as smoe_select_groups wrote it; an id given twice takes both
+ * gradients, ids outside [0, E) none.  Where the sum of the chosen scores is
+ * below 1e-9 the divisor is a constant. */
+SMOE_API int smoe_select_groups_backward(const void* logits, int logits_dtype, int N, int E, int K,
+                                         int score, int renorm, float scale, const int32_t* top_idx,
+                                         const float* d_top_w, void* d_logits, void* stream);
+
+/* Block-scaled e4m3: x [G, rows, cols] (SMOE_F32 / SMOE_BF16 / SMOE_F16; rows
+ * ldx elements apart, ldx >= cols) cut into blocks of block_rows x 128,
+ * block_rows 1 (activations: one scale per token and 128 channels) or 128
+ * (weights); blocks at the right and lower edge are smaller.  Per block
+ *   scale = max(amax|x| / 448, 1e-12) in f32, code = e4m3fn(x / scale), both
+ * divisions IEEE f32 divisions and the code rounded to nearest even, as
+ * smoe_quantize_fp8_tensor has them; a NaN in a block makes its scale and its
+ * codes NaN.  codes [G, rows, ld_out] (ld_out % 16 == 0, cols <= ld_out <= cols
+ * rounded up to 128; 16-byte aligned; code 0 past cols), scale f32
+ * [G, ceil(rows / block_rows), ceil(cols / 128)].  No workspace. */
+SMOE_API int smoe_quantize_fp8_blocks(const void* x, int x_dtype, int G, int rows, int cols,
+                                      int64_t ldx, int block_rows, uint8_t* codes, int64_t ld_out,
+                                      float* scale, void* stream);
+
+/* out [N, N_out] = act(x [N,K] . W^T + bias), W in e4m3 codes wq [N_out, K]
+ * (rows ldw bytes apart, ldw % 16 == 0, ldw >= K, 16-byte aligned, N_out * ldw
+ * bytes) with one scale per 128 x 128 block, w_scale f32 [ceil(N_out / 128),
+ * ceil(K / 128)].  x (SMOE_F32 / SMOE_BF16 / SMOE_F16, rows ldx elements apart)
+ * is quantized by the call as smoe_quantize_fp8_blocks does with block_rows 1
+ * (x_scale NULL); or it is codes already (x_dtype SMOE_FP8_E4M3, ldx bytes,
+ * with wq's alignment, x_scale f32 [N, ceil(K / 128)]).  Each block's products
+ * are summed by the matrix unit and added, times the two scales, to f32 sums.
+ * out bf16: the matrix unit multiplies e4m3 by e4m3, whose sums over a block
+ * are good to about 1e-5 of the sum; out f32: bf16 by bf16 on the same values,
+ * with f32 sums.  act SMOE_LINEAR_NONE / SMOE_LINEAR_GELU; bias f32 [N_out] or
+ * NULL; any K, any N_out. */
+SMOE_API size_t smoe_linear_fp8_blocks_workspace_bytes(int N, int K);
+SMOE_API int smoe_linear_fp8_blocks(const void* x, int x_dtype, int64_t ldx, const float* x_scale,
+                                    int N, int K, const uint8_t* wq, int64_t ldw,
+                                    const float* w_scale, const float* bias, int N_out, int act,
+                                    void* out, int out_dtype, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/* Expert FFN weights in that format, stacked over experts.
+ *   w_up [E,U,H] codes, s_up f32 [E, ceil(U/128), ceil(H/128)]; with
+ *   SMOE_ACT_SWIGLU the gate's U rows and then the up projection's, [E,2U,H],
+ *   each quantized on its own: s_up [E, 2 ceil(U/128), ceil(H/128)];
+ *   w_down [E,H,U], s_down f32 [E, ceil(H/128), ceil(U/128)];
+ *   b_up f32 [E,U] (SwiGLU: added to the up projection), b_down [E,H], or NULL.
+ * H % 16 == 0, U % 16 == 0, 1 <= E <= 256, codes 16-byte aligned. */
+typedef struct smoe_experts_fp8_blocks {
+  int act; /* SMOE_ACT_GELU / SMOE_ACT_SWIGLU */
+  int E, H, U;
+  const uint8_t* w_up;
+  const uint8_t* w_down;
+  const float* s_up;
+  const float* s_down;
+  const float* b_up;
+  const float* b_down;
+} smoe_experts_fp8_blocks;
+
+/* smoe_expert_delta on such experts: the messages msg [N,H] (SMOE_F32 /
+ * SMOE_BF16) and the hidden activations (in f32) are quantized in 1 x 128
+ * blocks on the way into the two products; delta [N,H] (SMOE_F32 / SMOE_BF16)
+ * = per token the sum over its experts, ascending, of w * (W_down act(W_up m +
+ * b_up) + b_down), in f32 until the end.  idx i32 / w f32 [N,K] as
+ * smoe_dispatch_plan takes them (equal ids merged, weights <= 0 and ids outside
+ * [0, E) dropped; a token left without experts gets 0).  1 <= K <= 64,
+ * N * K < 2^31 - 128. */
+SMOE_API size_t smoe_expert_delta_fp8_blocks_workspace_bytes(const smoe_experts_fp8_blocks* ex, int N,
+                                                             int K);
+SMOE_API int smoe_expert_delta_fp8_blocks(const smoe_experts_fp8_blocks* ex, const void* msg,
+                                          int msg_dtype, const int32_t* idx, const float* w, int N,
+                                          int K, void* delta, int out_dtype, void* workspace,
+                                          size_t workspace_bytes, void* stream);
+
 /* ---- Dobu expert residency (spider_moe/expert_store.py:121-166) ----
  * out[i] = map[ids[i]] for ids in [0, E), else -1: routed expert ids ->
  * slots of the device-resident expert slab (map[e] = -1 for experts not in

@@ -19,6 +19,7 @@
 #include <vector>
 
 #include "smoe_common.hpp"
+#include "smoe_fp8_blocks.hpp"
 #include "smoe_internal.hpp"
 
 using namespace smoe;
@@ -1365,6 +1366,289 @@ SMOE_API int smoe_linear_fp8fp8(const uint8_t* xq, const float* x_scale, int N, 
                             act == SMOE_LINEAR_GELU, out, out_dtype, N_out,
                             static_cast<hipStream_t>(stream)),
            "fp8 x fp8 GEMM");
+  return SMOE_OK;
+}
+
+// ---------------------------------------------- routing over groups ----
+namespace {
+
+int check_select_groups(int zdt, int N, int E, int K, int score) {
+  if (zdt != SMOE_F32 && zdt != SMOE_BF16 && zdt != SMOE_F16) return fail(SMOE_EUNSUPPORTED, "logits dtype");
+  if (N < 0 || E < 1 || E > 256 || K < 1 || K > E || K > 64)
+    return fail(SMOE_EINVAL, "select shape (1 <= K <= min(E, 64), E <= 256)");
+  if (score != SMOE_SCORE_SOFTMAX && score != SMOE_SCORE_SIGMOID) return fail(SMOE_EINVAL, "score");
+  return SMOE_OK;
+}
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+}  // namespace
+
+SMOE_API int smoe_select_groups(const void* logits, int logits_dtype, int N, int E, int K, int score,
+                                const float* bias, int groups, int top_groups, int renorm, float scale,
+                                float* top_w, int32_t* top_idx, void* stream) {
+  const int rc = check_select_groups(logits_dtype, N, E, K, score);
+  if (rc != SMOE_OK) return rc;
+  if (groups < 1 || groups > E || E % groups || top_groups < 1 || top_groups > groups)
+    return fail(SMOE_EINVAL, "groups must divide E, 1 <= top_groups <= groups");
+  if (K > top_groups * (E / groups)) return fail(SMOE_EINVAL, "K exceeds the experts of top_groups groups");
+  if (N == 0) return SMOE_OK;
+  if (!logits || !top_w || !top_idx) return fail(SMOE_EINVAL, "null buffer");
+  SMOE_TRY(launch_select_groups(logits, logits_dtype, N, E, K, score == SMOE_SCORE_SIGMOID, bias, groups,
+                                top_groups, renorm, scale, top_w, top_idx, static_cast<hipStream_t>(stream)),
+           "select groups");
+  return SMOE_OK;
+}
+
+SMOE_API int smoe_select_groups_backward(const void* logits, int logits_dtype, int N, int E, int K,
+                                         int score, int renorm, float scale, const int32_t* top_idx,
+                                         const float* d_top_w, void* d_logits, void* stream) {
+  const int rc = check_select_groups(logits_dtype, N, E, K, score);
+  if (rc != SMOE_OK) return rc;
+  if (N == 0) return SMOE_OK;
+  if (!logits || !top_idx || !d_top_w || !d_logits) return fail(SMOE_EINVAL, "null buffer");
+  SMOE_TRY(launch_select_groups_bwd(logits, logits_dtype, N, E, K, score == SMOE_SCORE_SIGMOID, renorm,
+                                    scale, top_idx, d_top_w, d_logits, static_cast<hipStream_t>(stream)),
+           "select groups backward");
+  return SMOE_OK;
+}
+
+// ----------------------------------------------- block-scaled fp8 ----
+SMOE_API int smoe_quantize_fp8_blocks(const void* x, int x_dtype, int G, int rows, int cols, int64_t ldx,
+                                      int block_rows, uint8_t* codes, int64_t ld_out, float* scale,
+                                      void* stream) {
+  if (x_dtype != SMOE_F32 && x_dtype != SMOE_BF16 && x_dtype != SMOE_F16)
+    return fail(SMOE_EUNSUPPORTED, "quantize input dtype");
+  if (block_rows != 1 && block_rows != kFp8Block) return fail(SMOE_EINVAL, "block_rows must be 1 or 128");
+  if (G < 0 || rows < 0 || cols < 1 || cols > 0x7fffff80 || ldx < cols || ld_out < cols || ld_out % 16 ||
+      ld_out > static_cast<int64_t>(fp8_blocks_of(cols)) * kFp8Block)
+    return fail(SMOE_EINVAL, "quantize shape (ldx >= cols, cols <= ld_out <= cols rounded up to 128, ld_out % 16 == 0)");
+  if (G == 0 || rows == 0) return SMOE_OK;
+  if (!x || !codes || !scale) return fail(SMOE_EINVAL, "null buffer");
+  if (!aligned16(codes)) return fail(SMOE_EINVAL, "codes must be 16-byte aligned");
+  BlockQuant q;
+  q.x = x;
+  q.x_dtype = x_dtype;
+  q.ldx = ldx;
+  q.groups = G;
+  q.rows = rows;
+  q.cols = cols;
+  q.block_rows = block_rows;
+  q.codes = codes;
+  q.ld_out = ld_out;
+  q.scale = scale;
+  q.s_row = fp8_blocks_of(cols);
+  q.s_col = 1;
+  SMOE_TRY(launch_quantize_fp8_blocks(q, static_cast<hipStream_t>(stream)), "quantize fp8 blocks");
+  return SMOE_OK;
+}
+
+namespace {
+
+// x quantized in 1 x 128 blocks: codes in rows of K rounded up to 16 bytes,
+// scales block by block [ceil(K / 128), N] (a tile's rows side by side)
+struct QuantWs {
+  size_t codes, scale, total;
+  int64_t ld;
+};
+QuantWs quant_ws(int64_t N, int K) {
+  QuantWs w;
+  Bump z;
+  w.ld = (static_cast<int64_t>(K) + 15) / 16 * 16;
+  w.codes = z.take(static_cast<size_t>(N) * w.ld);
+  w.scale = z.take(static_cast<size_t>(N) * fp8_blocks_of(K) * 4);
+  w.total = z.off;
+  return w;
+}
+
+int quantize_rows(const void* x, int xdt, int64_t ldx, int N, int K, void* ws, const QuantWs& l, hipStream_t s) {
+  BlockQuant q;
+  q.x = x;
+  q.x_dtype = xdt;
+  q.ldx = ldx;
+  q.rows = N;
+  q.cols = K;
+  q.codes = at<uint8_t>(ws, l.codes);
+  q.ld_out = l.ld;
+  q.scale = at<float>(ws, l.scale);
+  q.s_row = 1;
+  q.s_col = N;
+  return launch_quantize_fp8_blocks(q, s);
+}
+
+}  // namespace
+
+SMOE_API size_t smoe_linear_fp8_blocks_workspace_bytes(int N, int K) {
+  return N < 1 || K < 1 ? 0 : quant_ws(N, K).total;
+}
+
+SMOE_API int smoe_linear_fp8_blocks(const void* x, int x_dtype, int64_t ldx, const float* x_scale, int N,
+                                    int K, const uint8_t* wq, int64_t ldw, const float* w_scale,
+                                    const float* bias, int N_out, int act, void* out, int out_dtype,
+                                    void* ws, size_t ws_bytes, void* stream) {
+  const bool coded = x_dtype == SMOE_FP8_E4M3;
+  if (!coded && x_dtype != SMOE_F32 && x_dtype != SMOE_BF16 && x_dtype != SMOE_F16)
+    return fail(SMOE_EUNSUPPORTED, "linear input dtype");
+  if (N < 0 || N > 0x7fffff00 || K < 1 || K > 0x7fffff00 || N_out < 1 || N_out > 0x7fffff00 || ldx < K || ldw < K || ldw % 16)
+    return fail(SMOE_EINVAL, "fp8 block linear shape (ldx >= K, ldw >= K, ldw % 16 == 0)");
+  if (coded && ldx % 16) return fail(SMOE_EINVAL, "input codes: ldx % 16 == 0");
+  if (act != SMOE_LINEAR_NONE && act != SMOE_LINEAR_GELU) return fail(SMOE_EINVAL, "act");
+  if (out_dtype != SMOE_F32 && out_dtype != SMOE_BF16) return fail(SMOE_EUNSUPPORTED, "out dtype");
+  if (N == 0) return SMOE_OK;
+  if (!x || !wq || !w_scale || !out || (coded && !x_scale) || (!coded && !ws)) return fail(SMOE_EINVAL, "null buffer");
+  if (!coded && x_scale) return fail(SMOE_EINVAL, "x_scale belongs to input codes");
+  if (!aligned16(wq) || (coded && !aligned16(x)) || (!coded && !aligned16(ws)))
+    return fail(SMOE_EINVAL, "codes and workspace must be 16-byte aligned");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  BlockGemm g;
+  g.epi = act == SMOE_LINEAR_GELU ? BLK_GELU : BLK_LINEAR;
+  if (coded) {
+    g.X = static_cast<const uint8_t*>(x);
+    g.ldx = ldx;
+    g.xs = x_scale;
+    g.xs_row = fp8_blocks_of(K);
+    g.xs_col = 1;
+  } else {
+    const QuantWs l = quant_ws(N, K);
+    if (ws_bytes < l.total) return fail(SMOE_ECAPACITY, "workspace");
+    SMOE_TRY(quantize_rows(x, x_dtype, ldx, N, K, ws, l, s), "quantize fp8 blocks");
+    g.X = at<uint8_t>(ws, l.codes);
+    g.ldx = l.ld;
+    g.xs = at<float>(ws, l.scale);
+    g.xs_row = 1;
+    g.xs_col = N;
+  }
+  g.W = wq;
+  g.ldw = ldw;
+  g.ws = w_scale;
+  g.K = K;
+  g.N_out = N_out;
+  g.single_rows = N;
+  g.bias = bias;
+  g.out = out;
+  g.out_dtype = out_dtype;
+  g.ldo = N_out;
+  SMOE_TRY(launch_gemm_fp8_blocks(g, s), "fp8 block GEMM");
+  return SMOE_OK;
+}
+
+namespace {
+
+int check_experts_fp8_blocks(const smoe_experts_fp8_blocks* ex, int N, int K) {
+  if (!ex) return fail(SMOE_EINVAL, "null experts");
+  if (ex->act != SMOE_ACT_GELU && ex->act != SMOE_ACT_SWIGLU) return fail(SMOE_EINVAL, "act");
+  if (ex->E < 1 || ex->E > 256 || ex->H < 16 || ex->H % 16 || ex->U < 16 || ex->U % 16 || ex->H > (1 << 24) ||
+      ex->U > (1 << 24))
+    return fail(SMOE_EINVAL, "fp8 block experts: 1 <= E <= 256, H % 16 == 0, U % 16 == 0");
+  if (!ex->w_up || !ex->w_down || !ex->s_up || !ex->s_down) return fail(SMOE_EINVAL, "expert weights or scales missing");
+  if (!aligned16(ex->w_up) || !aligned16(ex->w_down)) return fail(SMOE_EINVAL, "expert codes must be 16-byte aligned");
+  if (N < 0 || K < 1 || K > 64 || static_cast<int64_t>(N) * K > 0x7fffff7f)
+    return fail(SMOE_EINVAL, "shape (1 <= top_k <= 64, N * top_k < 2^31 - 128)");
+  if (N > 65535 && (ex->H > 4096)) return fail(SMOE_EINVAL, "H > 4096: N <= 65535");
+  return SMOE_OK;
+}
+
+struct ExpertsWs {
+  size_t plan, off, cnt, rows, roww, tokrow, act, ascale, y, total;
+  QuantWs x;
+  size_t x_at;
+};
+ExpertsWs experts_ws(const smoe_experts_fp8_blocks& ex, int N, int K) {
+  const size_t n = N > 0 ? N : 1, r = n * K;
+  ExpertsWs w;
+  Bump z;
+  w.plan = z.take(smoe_dispatch_workspace_bytes(N, K, ex.E));
+  w.off = z.take((ex.E + 1) * 4);
+  w.cnt = z.take(ex.E * 4);
+  w.rows = z.take(r * 4);
+  w.roww = z.take(r * 4);
+  w.tokrow = z.take(r * 4);
+  w.x = quant_ws(n, ex.H);
+  w.x_at = z.take(w.x.total);
+  w.act = z.take(r * ex.U);
+  w.ascale = z.take(r * fp8_blocks_of(ex.U) * 4);
+  w.y = z.take(r * ex.H * 4);
+  w.total = z.off;
+  return w;
+}
+
+}  // namespace
+
+SMOE_API size_t smoe_expert_delta_fp8_blocks_workspace_bytes(const smoe_experts_fp8_blocks* ex, int N, int K) {
+  return check_experts_fp8_blocks(ex, N, K) != SMOE_OK ? 0 : experts_ws(*ex, N, K).total;
+}
+
+SMOE_API int smoe_expert_delta_fp8_blocks(const smoe_experts_fp8_blocks* ex, const void* msg, int msg_dtype,
+                                          const int32_t* idx, const float* w, int N, int K, void* delta,
+                                          int out_dtype, void* ws, size_t ws_bytes, void* stream) {
+  int rc = check_experts_fp8_blocks(ex, N, K);
+  if (rc != SMOE_OK) return rc;
+  if (msg_dtype != SMOE_F32 && msg_dtype != SMOE_BF16) return fail(SMOE_EUNSUPPORTED, "message dtype");
+  if (out_dtype != SMOE_F32 && out_dtype != SMOE_BF16) return fail(SMOE_EUNSUPPORTED, "out dtype");
+  if (N == 0) return SMOE_OK;
+  if (!msg || !idx || !w || !delta || !ws) return fail(SMOE_EINVAL, "null buffer");
+  if (!aligned16(ws)) return fail(SMOE_EINVAL, "workspace must be 16-byte aligned");
+  const ExpertsWs l = experts_ws(*ex, N, K);
+  if (ws_bytes < l.total) return fail(SMOE_ECAPACITY, "workspace");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  const int E = ex->E, H = ex->H, U = ex->U, hb = fp8_blocks_of(H), ub = fp8_blocks_of(U);
+  const int halves = ex->act == SMOE_ACT_SWIGLU ? 2 : 1;
+  int32_t *off = at<int32_t>(ws, l.off), *rows = at<int32_t>(ws, l.rows), *tokrow = at<int32_t>(ws, l.tokrow);
+  float* roww = at<float>(ws, l.roww);
+  rc = smoe_dispatch_plan(idx, w, N, K, E, at<int32_t>(ws, l.cnt), off, rows, roww, tokrow, at<void>(ws, l.plan),
+                          smoe_dispatch_workspace_bytes(N, K, E), stream);
+  if (rc != SMOE_OK) return rc;
+  void* xw = at<void>(ws, l.x_at);
+  SMOE_TRY(quantize_rows(msg, msg_dtype, H, N, H, xw, l.x, s), "quantize messages");
+  BlockGemm up;
+  up.epi = halves == 2 ? BLK_UP_SWIGLU : BLK_UP_GELU;
+  up.X = at<uint8_t>(xw, l.x.codes);
+  up.ldx = l.x.ld;
+  up.xs = at<float>(xw, l.x.scale);
+  up.xs_row = 1;
+  up.xs_col = N;
+  up.a_rows = rows;
+  up.W = ex->w_up;
+  up.w_gstride = static_cast<int64_t>(halves) * U * H;
+  up.ldw = H;
+  up.ws = ex->s_up;
+  up.ws_gstride = static_cast<int64_t>(halves) * ub * hb;
+  up.K = H;
+  up.N_out = U;
+  up.grp_off = off;
+  up.G = E;
+  up.max_rows = N * K;
+  up.bias = ex->b_up;
+  up.bias_gstride = U;
+  up.out = at<void>(ws, l.act);
+  up.ldo = U;
+  up.out_scale = at<float>(ws, l.ascale);
+  up.os_col = static_cast<int64_t>(N) * K;
+  SMOE_TRY(launch_gemm_fp8_blocks(up, s), "expert up GEMM");
+  BlockGemm dn;
+  dn.epi = BLK_DOWN;
+  dn.X = at<uint8_t>(ws, l.act);
+  dn.ldx = U;
+  dn.xs = up.out_scale;
+  dn.xs_row = 1;
+  dn.xs_col = up.os_col;
+  dn.W = ex->w_down;
+  dn.w_gstride = static_cast<int64_t>(H) * U;
+  dn.ldw = U;
+  dn.ws = ex->s_down;
+  dn.ws_gstride = static_cast<int64_t>(hb) * ub;
+  dn.K = U;
+  dn.N_out = H;
+  dn.grp_off = off;
+  dn.G = E;
+  dn.max_rows = N * K;
+  dn.bias = ex->b_down;
+  dn.bias_gstride = H;
+  dn.row_scale = roww;
+  dn.out = at<void>(ws, l.y);
+  dn.ldo = H;
+  SMOE_TRY(launch_gemm_fp8_blocks(dn, s), "expert down GEMM");
+  SMOE_TRY(launch_delta_combine(at<void>(ws, l.y), SMOE_F32, tokrow, N, K, H, delta, out_dtype, s), "delta combine");
   return SMOE_OK;
 }
 

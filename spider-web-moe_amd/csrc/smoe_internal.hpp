@@ -232,6 +232,14 @@ int launch_gemm_f8f8(const uint8_t* xq, int ldx, const float* xs, const uint8_t*
                      void* out, int odt, int ldo, hipStream_t s);
 int launch_select_topk(const float* logits, int N, int E, int K, int mode, float* top_w,
                        int32_t* top_idx, hipStream_t s);
+// group-limited routing of logits [N, E] (f32 / bf16 / f16) and its gradient
+// (smoe_select_groups.hip); the entry points check the shapes
+int launch_select_groups(const void* logits, int zdt, int N, int E, int K, int sigmoid,
+                         const float* bias, int groups, int top_groups, int renorm, float scale,
+                         float* top_w, int32_t* top_idx, hipStream_t s);
+int launch_select_groups_bwd(const void* logits, int zdt, int N, int E, int K, int sigmoid,
+                             int renorm, float scale, const int32_t* top_idx, const float* d_w,
+                             void* d_logits, hipStream_t s);
 // out[t] = sum over the token's rows tok_row [N, K] of y[row] * row_w[row]
 int launch_combine_rows(const void* y, int ydt, const float* row_w, const int32_t* tok_row,
                         int N, int K, int H, void* out, int odt, hipStream_t s);

@@ -18,10 +18,12 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libs
 F32, BF16, FP8_E4M3, INT4, F16 = 0, 1, 2, 3, 4
 ACT_GELU, ACT_SWIGLU = 0, 1
 SMOE_SELECT_ROUTER, SMOE_SELECT_TOPK_SOFTMAX = 0, 1
+SCORES = {"softmax": 0, "sigmoid": 1}
 STATUS = {0: "ok", 1: "invalid argument", 2: "index out of range", 3: "capacity",
           -2: "unsupported dtype/format", 4: "HIP runtime error"}
 
 _c_int, _c_float, _vp, _sz = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
+_i64 = ctypes.c_int64
 
 
 class SmoeExperts(ctypes.Structure):
@@ -29,6 +31,11 @@ class SmoeExperts(ctypes.Structure):
                 ("group_size", _c_int), ("scale_dtype", _c_int),
                 ("w_up", _vp), ("w_gate", _vp), ("w_down", _vp), ("s_up", _vp), ("s_down", _vp),
                 ("b_up", _vp), ("b_down", _vp), ("w_up_tiles", _vp), ("w_down_tiles", _vp)]
+
+
+class SmoeExpertsFp8Blocks(ctypes.Structure):
+    _fields_ = [("act", _c_int), ("E", _c_int), ("H", _c_int), ("U", _c_int), ("w_up", _vp),
+                ("w_down", _vp), ("s_up", _vp), ("s_down", _vp), ("b_up", _vp), ("b_down", _vp)]
 
 
 class SmoeBlock(ctypes.Structure):
@@ -95,6 +102,20 @@ SIGNATURES = {
                                     _c_int, _vp]),
     "smoe_linear": (_c_int, [_vp, _c_int, _c_int, _vp, _c_int, _vp, _vp, _c_int, _c_int, _vp,
                              _c_int, _vp]),
+    "smoe_select_groups": (_c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _c_int,
+                                    _c_int, _c_int, _c_float, _vp, _vp, _vp]),
+    "smoe_select_groups_backward": (_c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                             _c_float, _vp, _vp, _vp, _vp]),
+    "smoe_quantize_fp8_blocks": (_c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _i64, _c_int, _vp,
+                                          _i64, _vp, _vp]),
+    "smoe_linear_fp8_blocks_workspace_bytes": (_sz, [_c_int, _c_int]),
+    "smoe_linear_fp8_blocks": (_c_int, [_vp, _c_int, _i64, _vp, _c_int, _c_int, _vp, _i64, _vp,
+                                        _vp, _c_int, _c_int, _vp, _c_int, _vp, _sz, _vp]),
+    "smoe_expert_delta_fp8_blocks_workspace_bytes": (_sz, [ctypes.POINTER(SmoeExpertsFp8Blocks),
+                                                           _c_int, _c_int]),
+    "smoe_expert_delta_fp8_blocks": (_c_int, [ctypes.POINTER(SmoeExpertsFp8Blocks), _vp, _c_int,
+                                              _vp, _vp, _c_int, _c_int, _vp, _c_int, _vp, _sz,
+                                              _vp]),
     "smoe_combine_rows": (_c_int, [_vp, _c_int, _vp, _vp, _c_int, _c_int, _c_int, _vp, _c_int,
                                    _vp]),
     "smoe_remap_ids": (_c_int, [_vp, ctypes.c_int64, _vp, _c_int, _vp, _vp]),
@@ -285,6 +306,11 @@ def require_gpu(*tensors) -> torch.device:
         elif t.device != dev:
             raise RuntimeError("all tensors must be on the same GPU")
     return dev
+
+
+def float_code(dt: torch.dtype) -> int:
+    """dtype_code of the calls that read f16 too."""
+    return F16 if dt == torch.float16 else dtype_code(dt)
 
 
 def dtype_code(dt: torch.dtype) -> int:

@@ -19,6 +19,14 @@ forge/gemm, forge/ep).  Here they run on libsmoe.so:
                        callback per assignment with the weighted combine
                        on the GPU (dispatch.dispatch_expert_ffn)
 
+Beside them, without a counterpart in the reference:
+
+  ForgeSelect.route_groups   softmax or sigmoid scores, a balance bias,
+                       top-k within the best groups of experts, with its
+                       gradient -> smoe_select_groups(_backward)
+  ForgeGEMM.linear_fp8_blocks   fp8 with a scale per block of 128 ->
+                       smoe_linear_fp8_blocks
+
 One GPU: the cross-rank combine is the identity (no process group), as
 the reference's combine_across_ranks is at world size 1.
 """
@@ -33,7 +41,7 @@ import torch
 
 from . import _native as nat
 from .dispatch import DispatchPlan, build_dispatch_plan, dispatch_expert_ffn
-from .quant import quantize_fp8_per_tensor
+from .quant import FP8_BLOCK, quantize_fp8_per_tensor
 
 
 class ForgeBackend(str, Enum):
@@ -76,6 +84,30 @@ class ForgeSelect:
         k = max(1, min(k, e))
         return select_topk(logits, k, nat.SMOE_SELECT_TOPK_SOFTMAX)
 
+    def route_groups(self, logits: torch.Tensor, *, top_k: int | None = None,
+                     score: str = "sigmoid", bias: torch.Tensor | None = None,
+                     num_groups: int = 1, top_groups: int = 1, renormalize: bool = True,
+                     scale: float = 1.0):
+        """logits [..., E] (float32, bfloat16 or float16) -> (weights float32,
+        indices int32) [..., k], as the dispatch plan and the experts read
+        them.
+
+        s = softmax(logits) or sigmoid(logits); s + bias (bias [E], which
+        evens out the experts' load) decides the choice, s alone the weights.
+        With num_groups > 1 consecutive experts form groups, a group's value
+        is the sum of its two largest s + bias, and only the top_groups best
+        groups take part.  The k largest are chosen, ties to the lower index,
+        and weigh scale * s, divided by the chosen scores' sum (at least 1e-9)
+        with renormalize.  Experts whose logit is -inf are chosen last, with
+        weight 0.
+
+        Differentiable in logits (the choice held fixed; the bias gets no
+        gradient)."""
+        self.calls += 1
+        k = int(top_k if top_k is not None else self.config.select_top_k)
+        return select_groups(logits, k, score=score, bias=bias, num_groups=num_groups,
+                             top_groups=top_groups, renormalize=renormalize, scale=scale)
+
     def top_dobu_budget(self) -> int:
         return int(self.config.select_top_dobu)
 
@@ -100,6 +132,66 @@ def select_topk(logits: torch.Tensor, k: int, mode: int):
     return w.view(*lead, k).to(out_dtype), idx.view(*lead, k).long()
 
 
+def _select_groups_fwd(logits, k, score, bias, num_groups, top_groups, renormalize, scale):
+    dev = logits.device
+    e = logits.shape[-1]
+    x = logits.contiguous()
+    shape = (*logits.shape[:-1], k)
+    w = torch.empty(shape, dtype=torch.float32, device=dev)
+    idx = torch.empty(shape, dtype=torch.int32, device=dev)
+    n = x.numel() // e if e else 0
+    with torch.cuda.device(dev):
+        nat.check(nat.lib().smoe_select_groups(
+            x.data_ptr(), nat.float_code(x.dtype), n, e, k, score, nat.ptr(bias), num_groups,
+            top_groups, renormalize, scale, w.data_ptr(), idx.data_ptr(), nat.stream_of(dev)),
+            "smoe_select_groups")
+    return w, idx
+
+
+class _SelectGroups(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, k, score, bias, num_groups, top_groups, renormalize, scale):
+        w, idx = _select_groups_fwd(logits, k, score, bias, num_groups, top_groups, renormalize, scale)
+        ctx.save_for_backward(logits, idx)
+        ctx.how = (score, renormalize, scale)
+        ctx.mark_non_differentiable(idx)
+        return w, idx
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_w, _):
+        logits, idx = ctx.saved_tensors
+        score, renormalize, scale = ctx.how
+        x = logits.contiguous()
+        d = torch.empty_like(x)
+        e, k = x.shape[-1], idx.shape[-1]
+        d_w = d_w.float().contiguous()
+        with torch.cuda.device(x.device):
+            nat.check(nat.lib().smoe_select_groups_backward(
+                x.data_ptr(), nat.float_code(x.dtype), x.numel() // e, e, k, score, renormalize,
+                scale, idx.data_ptr(), d_w.data_ptr(), d.data_ptr(), nat.stream_of(x.device)),
+                "smoe_select_groups_backward")
+        return d, None, None, None, None, None, None, None
+
+
+def select_groups(logits: torch.Tensor, k: int, *, score: str = "sigmoid", bias=None,
+                  num_groups: int = 1, top_groups: int = 1, renormalize: bool = True,
+                  scale: float = 1.0):
+    """smoe_select_groups over the last dimension (ForgeSelect.route_groups)."""
+    nat.require_gpu(logits, bias)
+    if score not in nat.SCORES:
+        raise ValueError("score must be 'softmax' or 'sigmoid'")
+    if bias is not None:
+        if bias.shape != logits.shape[-1:]:
+            raise ValueError(f"bias must be [{logits.shape[-1]}], got {tuple(bias.shape)}")
+        bias = bias.detach().float().contiguous()
+    how = (int(k), nat.SCORES[score], bias, int(num_groups), int(top_groups), int(renormalize),
+           float(scale))
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _SelectGroups.apply(logits, *how)
+    return _select_groups_fwd(logits.detach(), *how)
+
+
 # ------------------------------------------------------------------ gemm ----
 _ACT = {None: 0, "gelu": 1}
 
@@ -118,6 +210,58 @@ def _linear(x: torch.Tensor, w: torch.Tensor, w_format: int, scale, bias, act, o
                                     nat.ptr(b), n_out, _ACT[act], out.data_ptr(),
                                     nat.dtype_code(out_dtype), nat.stream_of(dev)), "smoe_linear")
     return out.view(*lead, n_out)
+
+
+def _linear_fp8_blocks(x, codes, scale, bias, act):
+    dev = nat.require_gpu(x, codes, scale, bias)
+    k, lead = x.shape[-1], x.shape[:-1]
+    if codes.dtype != torch.float8_e4m3fn or codes.ndim != 2 or codes.shape[1] != k:
+        raise ValueError(f"codes must be float8_e4m3fn [N_out, {k}], got {codes.dtype} {tuple(codes.shape)}")
+    n_out = codes.shape[0]
+    if scale.dtype != torch.float32 or scale.shape != (-(-n_out // FP8_BLOCK), -(-k // FP8_BLOCK)):
+        raise ValueError("scale must be float32 [ceil(N_out / 128), ceil(K / 128)], "
+                         f"got {scale.dtype} {tuple(scale.shape)}")
+    if act not in _ACT:
+        raise ValueError("act must be None or 'gelu'")
+    if bias is not None:
+        if bias.shape != (n_out,):
+            raise ValueError(f"bias must be [{n_out}], got {tuple(bias.shape)}")
+        bias = bias.detach().float().contiguous()
+    if x.ndim == 2 and x.stride(1) == 1 and x.stride(0) >= k:
+        ldx = x.stride(0)
+    else:
+        x, ldx = x.contiguous(), k
+    codes, ldw = _rows16(codes)
+    scale = scale.contiguous()
+    out_dtype = torch.bfloat16 if x.dtype == torch.bfloat16 else torch.float32
+    out = torch.empty(*lead, n_out, dtype=out_dtype, device=dev)
+    n = out.numel() // n_out if n_out else 0
+    lib = nat.lib()
+    need = lib.smoe_linear_fp8_blocks_workspace_bytes(n, k)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        nat.check(lib.smoe_linear_fp8_blocks(
+            x.data_ptr(), nat.float_code(x.dtype), ldx, None, n, k, codes.data_ptr(), ldw,
+            scale.data_ptr(), nat.ptr(bias), n_out, _ACT[act], out.data_ptr(),
+            nat.dtype_code(out_dtype), ws.data_ptr(), need, nat.stream_of(dev)),
+            "smoe_linear_fp8_blocks")
+    return out if out_dtype == x.dtype else out.to(x.dtype)
+
+
+def _rows16(codes):
+    """Codes [rows, cols] in rows that start a multiple of 16 bytes apart,
+    each whole in memory, and that distance: the tensor itself where it is
+    laid out so, else a copy."""
+    rows, cols = codes.shape
+    ld = codes.stride(0) if rows > 1 else -(-cols // 16) * 16
+    room = codes.untyped_storage().nbytes() - codes.storage_offset()
+    if (codes.stride(1) == 1 or cols == 1) and ld >= cols and ld % 16 == 0 and \
+            codes.data_ptr() % 16 == 0 and room >= rows * ld:
+        return codes, ld
+    ld = -(-cols // 16) * 16
+    c = torch.zeros(rows, ld, dtype=torch.uint8, device=codes.device)
+    c[:, :cols] = codes.view(torch.uint8)
+    return c, ld
 
 
 class _Fp8Cache:
@@ -254,6 +398,17 @@ class ForgeGEMM:
         return self._run(x, weight, bias, None, True, quantize_input).to(x.dtype)
 
     @torch.no_grad()
+    def linear_fp8_blocks(self, x, codes, scale, bias=None, *, act: str | None = None):
+        """act(x . W^T + bias) with W held as e4m3 codes [N_out, K] and one
+        scale per 128 x 128 block (quantize_fp8_blocks), x [..., K] quantized
+        in 1 x 128 blocks on the way (smoe_linear_fp8_blocks); act None or
+        "gelu" (erf).  Result in x's dtype: bfloat16 from e4m3 x e4m3
+        products, float32 (and float16) from the same values' products with
+        f32 sums throughout."""
+        self.calls += 1
+        return _linear_fp8_blocks(x, codes, scale, bias, act)
+
+    @torch.no_grad()
     def expert_ffn(self, x, w_up, b_up, w_down, b_down):
         self.calls += 1
         fp8 = self.config.gemm_fp8
@@ -380,5 +535,5 @@ def get_forge() -> ForgeRuntime:
 
 
 __all__ = ["ForgeBackend", "ForgeConfig", "ForgeSelect", "ForgeGEMM", "ForgeEP", "ForgeRuntime",
-           "init_forge", "get_forge", "select_topk", "fp8_linear", "fp8_expert_ffn",
+           "init_forge", "get_forge", "select_topk", "select_groups", "fp8_linear", "fp8_expert_ffn",
            "get_last_fp8_gemm_backend", "quantize_fp8_input"]

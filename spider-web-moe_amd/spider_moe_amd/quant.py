@@ -11,6 +11,10 @@ fp8: per-output-channel e4m3 — scale = max(amax_K / 448, 1e-12) and
 codes = (w / scale).to(float8_e4m3fn), as quantize_fp8_with_scale_tensor
 (quant.py:146-158) with a [.., N] scale; dequant = code * scale
 (quant.py:161-169).
+
+fp8 in blocks: e4m3 codes with one f32 scale per 128 x 128 block of a weight
+or per 1 x 128 block of activations (no counterpart in the reference):
+quantize_fp8_blocks / dequantize_fp8_blocks.
 """
 from __future__ import annotations
 
@@ -134,6 +138,86 @@ def quantize_fp8_per_tensor(weight: torch.Tensor):
     w = weight.detach().float()
     scale = (w.abs().amax() / FP8_E4M3_MAX).clamp_min(1e-12)
     return (w / scale).to(torch.float8_e4m3fn).contiguous(), scale
+
+
+# ------------------------------------------------------- fp8 in blocks ----
+FP8_BLOCK = 128
+
+
+def _row_stride(x: torch.Tensor):
+    """Elements between rows when x [.., rows, cols] is rows of contiguous
+    elements at one distance throughout, else None."""
+    if x.ndim < 2 or (x.shape[-1] > 1 and x.stride(-1) != 1):
+        return None
+    ld = x.stride(-2) if x.shape[-2] > 1 else x.shape[-1]
+    if x.shape[-2] == 1 and x.ndim > 2:  # the rows of the leading dimension
+        for n, st in zip(reversed(x.shape[:-2]), reversed(x.stride()[:-2])):
+            if n > 1:
+                ld = st
+                break
+    step = ld * x.shape[-2]
+    for n, st in zip(reversed(x.shape[:-2]), reversed(x.stride()[:-2])):
+        if n > 1 and st != step:
+            return None
+        step *= n
+    return ld if ld >= x.shape[-1] else None
+
+
+def quantize_fp8_blocks(x: torch.Tensor, *, block_rows: int = FP8_BLOCK):
+    """x [.., rows, cols] -> (float8_e4m3fn codes of that shape, float32 scale
+    [.., ceil(rows / block_rows), ceil(cols / 128)]): one scale for each block
+    of block_rows x 128 elements, block_rows 128 (weights) or 1 (activations).
+    scale = max(amax|block| / 448, 1e-12), code = x / scale rounded to nearest
+    even, both divisions in f32 (a NaN makes its block's scale and codes NaN).
+    The codes' rows start a multiple of 16 bytes apart, as the GEMMs read
+    them (a view where cols % 16 != 0).  On a GPU: the HIP quantizer (same
+    bits as the CPU formula)."""
+    if block_rows not in (1, FP8_BLOCK):
+        raise ValueError("block_rows must be 1 or 128")
+    if x.ndim < 2 or x.shape[-1] < 1:
+        raise ValueError("x must be [.., rows, cols] with cols >= 1")
+    x = x.detach()
+    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        x = x.float()
+    *lead, rows, cols = x.shape
+    cb, ld = -(-cols // FP8_BLOCK), -(-cols // 16) * 16
+    rb = -(-rows // block_rows)
+    if x.is_cuda:
+        from . import _native as nat
+        ldx = _row_stride(x)
+        if ldx is None:
+            x, ldx = x.contiguous(), cols
+        g = 1
+        for n in lead:
+            g *= n
+        codes = torch.empty(*lead, rows, ld, dtype=torch.float8_e4m3fn, device=x.device)
+        scale = torch.empty(*lead, rb, cb, dtype=torch.float32, device=x.device)
+        with torch.cuda.device(x.device):
+            nat.check(nat.lib().smoe_quantize_fp8_blocks(
+                x.data_ptr(), nat.float_code(x.dtype), g, rows, cols, ldx, block_rows,
+                codes.data_ptr(), ld, scale.data_ptr(), nat.stream_of(x.device)),
+                "smoe_quantize_fp8_blocks")
+        return (codes if ld == cols else codes[..., :cols]), scale
+    p = torch.zeros(*lead, rb * block_rows, cb * FP8_BLOCK)
+    p[..., :rows, :cols] = x
+    p = p.view(*lead, rb, block_rows, cb, FP8_BLOCK)
+    scale = (p.abs().amax(dim=(-3, -1)) / FP8_E4M3_MAX).clamp_min(1e-12)
+    q = (p / scale[..., :, None, :, None]).view(*lead, rb * block_rows, cb * FP8_BLOCK)
+    codes = torch.zeros(*lead, rows, ld, dtype=torch.uint8)
+    codes[..., :cols] = q[..., :rows, :cols].to(torch.float8_e4m3fn).view(torch.uint8)
+    return codes.view(torch.float8_e4m3fn)[..., :cols], scale
+
+
+def dequantize_fp8_blocks(codes: torch.Tensor, scale: torch.Tensor, *, block_rows: int = FP8_BLOCK,
+                          dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """code * scale of its block, in f32, as dtype."""
+    rows, cols = codes.shape[-2:]
+    if scale.shape != (*codes.shape[:-2], -(-rows // block_rows), -(-cols // FP8_BLOCK)):
+        raise ValueError("scale does not match the codes' blocks")
+    s = scale.float().repeat_interleave(FP8_BLOCK, dim=-1)[..., :cols]
+    if block_rows > 1:
+        s = s.repeat_interleave(block_rows, dim=-2)[..., :rows, :]
+    return (codes.float() * s).to(dtype)
 
 
 # ------------------------------------------------------ SwiGLU layout ----

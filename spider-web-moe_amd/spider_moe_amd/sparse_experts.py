@@ -11,6 +11,9 @@ outside [0, E) match no expert.  Weights may be float32 or bfloat16
 With expert parallelism active (torch.distributed world > 1) the reference
 computes its local experts and SUM-all-reduces; this single-GPU module
 computes every expert on every rank, which yields the same delta.
+
+sparse_expert_delta_fp8_blocks is the same step on experts whose weights are
+e4m3 codes with a scale per 128 x 128 block (Fp8BlockExperts).
 """
 from __future__ import annotations
 
@@ -19,6 +22,7 @@ import ctypes
 import torch
 
 from . import _native as nat
+from .quant import FP8_BLOCK, quantize_fp8_blocks
 
 
 def _experts_desc(w_up, b_up, w_down, b_down, act=nat.ACT_GELU):
@@ -75,3 +79,110 @@ def sparse_expert_delta(
               "smoe_expert_delta")
     del keep
     return delta.view(b, t, width).to(messages.dtype)
+
+
+class Fp8BlockExperts:
+    """Expert FFN weights as e4m3 codes with one f32 scale per 128 x 128 block.
+
+    w_up [E,U,H] codes and s_up [E, ceil(U/128), ceil(H/128)]; for
+    activation "swiglu" [E,2U,H], the gate's rows first, and s_up
+    [E, 2 ceil(U/128), ceil(H/128)] (gate and up projection are quantized
+    each on its own).  w_down [E,H,U], s_down [E, ceil(H/128), ceil(U/128)].
+    b_up [E,U] (swiglu: added to the up projection) and b_down [E,H] or None.
+    H % 16 == 0 and U % 16 == 0.  The tensors are kept, not copied (a copy is
+    made of what is not contiguous); a kept object follows in-place changes
+    of them.  Fp8BlockExperts.quantize makes one from float weights."""
+
+    def __init__(self, w_up, s_up, w_down, s_down, *, b_up=None, b_down=None,
+                 activation: str = "gelu"):
+        if activation not in ("gelu", "swiglu"):
+            raise ValueError("activation must be 'gelu' or 'swiglu'")
+        self.device = nat.require_gpu(w_up, s_up, w_down, s_down, b_up, b_down)
+        if w_up.ndim != 3 or w_down.ndim != 3:
+            raise ValueError("w_up and w_down must be stacked over experts: [E, .., ..]")
+        halves = 2 if activation == "swiglu" else 1
+        e, h, u = w_down.shape
+        hb, ub = -(-h // FP8_BLOCK), -(-u // FP8_BLOCK)
+        if w_up.shape != (e, halves * u, h):
+            raise ValueError(f"w_up must be {(e, halves * u, h)}, got {tuple(w_up.shape)}")
+        for name, t, shape in (("s_up", s_up, (e, halves * ub, hb)), ("s_down", s_down, (e, hb, ub))):
+            if t.shape != shape or t.dtype != torch.float32:
+                raise ValueError(f"{name} must be float32 {shape}, got {t.dtype} {tuple(t.shape)}")
+        for name, t in (("w_up", w_up), ("w_down", w_down)):
+            if t.dtype != torch.float8_e4m3fn:
+                raise ValueError(f"{name} must be float8_e4m3fn codes, got {t.dtype}")
+        for name, t, shape in (("b_up", b_up, (e, u)), ("b_down", b_down, (e, h))):
+            if t is not None and t.shape != shape:
+                raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+        if h % 16 or u % 16 or not 1 <= e <= 256:
+            raise ValueError("Fp8BlockExperts: H % 16 == 0, U % 16 == 0, 1 <= E <= 256")
+        self.num_experts, self.hidden_size, self.expert_ffn_size = e, h, u
+        self.activation = activation
+
+        def whole(t):
+            t = t.contiguous()
+            return t if t.data_ptr() % 16 == 0 else t.clone()
+
+        self.w_up, self.s_up = whole(w_up), s_up.contiguous()
+        self.w_down, self.s_down = whole(w_down), s_down.contiguous()
+        self.b_up = None if b_up is None else b_up.detach().float().contiguous()
+        self.b_down = None if b_down is None else b_down.detach().float().contiguous()
+        d = nat.SmoeExpertsFp8Blocks()
+        d.act = nat.ACT_SWIGLU if halves == 2 else nat.ACT_GELU
+        d.E, d.H, d.U = e, h, u
+        d.w_up, d.w_down = self.w_up.data_ptr(), self.w_down.data_ptr()
+        d.s_up, d.s_down = self.s_up.data_ptr(), self.s_down.data_ptr()
+        d.b_up, d.b_down = nat.ptr(self.b_up), nat.ptr(self.b_down)
+        self._desc = d
+        self._ref = ctypes.byref(d)
+
+    @classmethod
+    def quantize(cls, w_up, w_down, *, b_up=None, b_down=None, activation: str = "gelu"):
+        """From float weights w_up [E, U or 2U, H] and w_down [E,H,U]."""
+        e, _, u = w_down.shape
+        if activation == "swiglu":
+            if w_up.shape[1] != 2 * u:
+                raise ValueError("swiglu: w_up must hold the gate's and the up projection's rows, [E,2U,H]")
+            q, s = quantize_fp8_blocks(w_up.reshape(2 * e, u, w_up.shape[-1]))
+            q = q.contiguous().view(e, 2 * u, w_up.shape[-1])
+            s = s.view(e, -1, s.shape[-1])
+        else:
+            q, s = quantize_fp8_blocks(w_up)
+        qd, sd = quantize_fp8_blocks(w_down)
+        return cls(q, s, qd, sd, b_up=b_up, b_down=b_down, activation=activation)
+
+
+@torch.no_grad()
+def sparse_expert_delta_fp8_blocks(messages: torch.Tensor, top_indices: torch.Tensor,
+                                   top_weights: torch.Tensor, experts: Fp8BlockExperts) -> torch.Tensor:
+    """sparse_expert_delta on Fp8BlockExperts: messages [..,H] (float32 or
+    bfloat16), top_indices / top_weights [..,K] -> delta [..,H] in messages'
+    dtype.  Messages and hidden activations are quantized in 1 x 128 blocks on
+    the way into the two products; everything else is summed in f32."""
+    dev = nat.require_gpu(messages, top_indices, top_weights, experts.w_up)
+    h, k = messages.shape[-1], top_indices.shape[-1]
+    if h != experts.hidden_size:
+        raise ValueError(f"messages have {h} channels, the experts {experts.hidden_size}")
+    if top_indices.shape[:-1] != messages.shape[:-1] or top_weights.shape != top_indices.shape:
+        raise ValueError("top_indices and top_weights must be messages' shape with K last")
+    code = nat.dtype_code(messages.dtype)
+    idx, wts = top_indices, top_weights
+    if idx.dtype != torch.int32:
+        idx = idx.to(torch.int32)
+    if wts.dtype != torch.float32:
+        wts = wts.float()
+    msg, idx, wts = messages.contiguous(), idx.contiguous(), wts.contiguous()
+    n = idx.numel() // k if k else 0
+    delta = torch.empty(messages.shape, dtype=messages.dtype, device=dev)
+    lib = nat.lib()
+    need = lib.smoe_expert_delta_fp8_blocks_workspace_bytes(experts._ref, n, k)
+    if need == 0:
+        raise RuntimeError("smoe_expert_delta_fp8_blocks: "
+                           f"unsupported shapes ({lib.smoe_last_error().decode()})")
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        nat.check(lib.smoe_expert_delta_fp8_blocks(
+            experts._ref, msg.data_ptr(), code, idx.data_ptr(), wts.data_ptr(), n, k,
+            delta.data_ptr(), code, ws.data_ptr(), need, nat.stream_of(dev)),
+            "smoe_expert_delta_fp8_blocks")
+    return delta
