@@ -454,7 +454,8 @@ SMOE_API int smoe_quantize_fp8_blocks(const void* x, int x_dtype, int G, int row
  * out bf16: the matrix unit multiplies e4m3 by e4m3, whose sums over a block
  * are good to about 1e-5 of the sum; out f32: bf16 by bf16 on the same values,
  * with f32 sums.  act SMOE_LINEAR_NONE / SMOE_LINEAR_GELU; bias f32 [N_out] or
- * NULL; any K, any N_out. */
+ * NULL; any K, any N_out.  Where the workspace query gives 0 (a few rows) the
+ * workspace may be NULL. */
 SMOE_API size_t smoe_linear_fp8_blocks_workspace_bytes(int N, int K);
 SMOE_API int smoe_linear_fp8_blocks(const void* x, int x_dtype, int64_t ldx, const float* x_scale,
                                     int N, int K, const uint8_t* wq, int64_t ldw,

@@ -1461,7 +1461,7 @@ QuantWs quant_ws(int64_t N, int K) {
   return w;
 }
 
-int quantize_rows(const void* x, int xdt, int64_t ldx, int N, int K, void* ws, const QuantWs& l, hipStream_t s) {
+BlockQuant rows_quant(const void* x, int xdt, int64_t ldx, int N, int K, void* ws, const QuantWs& l) {
   BlockQuant q;
   q.x = x;
   q.x_dtype = xdt;
@@ -1473,13 +1473,13 @@ int quantize_rows(const void* x, int xdt, int64_t ldx, int N, int K, void* ws, c
   q.scale = at<float>(ws, l.scale);
   q.s_row = 1;
   q.s_col = N;
-  return launch_quantize_fp8_blocks(q, s);
+  return q;
 }
 
 }  // namespace
 
 SMOE_API size_t smoe_linear_fp8_blocks_workspace_bytes(int N, int K) {
-  return N < 1 || K < 1 ? 0 : quant_ws(N, K).total;
+  return N < 1 || K < 1 || linear_quantizes_inside(N, K) ? 0 : quant_ws(N, K).total;
 }
 
 SMOE_API int smoe_linear_fp8_blocks(const void* x, int x_dtype, int64_t ldx, const float* x_scale, int N,
@@ -1495,9 +1495,11 @@ SMOE_API int smoe_linear_fp8_blocks(const void* x, int x_dtype, int64_t ldx, con
   if (act != SMOE_LINEAR_NONE && act != SMOE_LINEAR_GELU) return fail(SMOE_EINVAL, "act");
   if (out_dtype != SMOE_F32 && out_dtype != SMOE_BF16) return fail(SMOE_EUNSUPPORTED, "out dtype");
   if (N == 0) return SMOE_OK;
-  if (!x || !wq || !w_scale || !out || (coded && !x_scale) || (!coded && !ws)) return fail(SMOE_EINVAL, "null buffer");
+  const bool inside = !coded && linear_quantizes_inside(N, K);
+  if (!x || !wq || !w_scale || !out || (coded && !x_scale) || (!coded && !inside && !ws))
+    return fail(SMOE_EINVAL, "null buffer");
   if (!coded && x_scale) return fail(SMOE_EINVAL, "x_scale belongs to input codes");
-  if (!aligned16(wq) || (coded && !aligned16(x)) || (!coded && !aligned16(ws)))
+  if (!aligned16(wq) || (coded && !aligned16(x)) || (!coded && !inside && !aligned16(ws)))
     return fail(SMOE_EINVAL, "codes and workspace must be 16-byte aligned");
   hipStream_t s = static_cast<hipStream_t>(stream);
   BlockGemm g;
@@ -1508,10 +1510,15 @@ SMOE_API int smoe_linear_fp8_blocks(const void* x, int x_dtype, int64_t ldx, con
     g.xs = x_scale;
     g.xs_row = fp8_blocks_of(K);
     g.xs_col = 1;
+  } else if (inside) {
+    g.x_float = x;
+    g.x_dtype = x_dtype;
+    g.ld_float = ldx;
+    g.ldx = (static_cast<int64_t>(K) + 15) / 16 * 16;
   } else {
     const QuantWs l = quant_ws(N, K);
     if (ws_bytes < l.total) return fail(SMOE_ECAPACITY, "workspace");
-    SMOE_TRY(quantize_rows(x, x_dtype, ldx, N, K, ws, l, s), "quantize fp8 blocks");
+    SMOE_TRY(launch_quantize_fp8_blocks(rows_quant(x, x_dtype, ldx, N, K, ws, l), s), "quantize fp8 blocks");
     g.X = at<uint8_t>(ws, l.codes);
     g.ldx = l.ld;
     g.xs = at<float>(ws, l.scale);
@@ -1595,11 +1602,26 @@ SMOE_API int smoe_expert_delta_fp8_blocks(const smoe_experts_fp8_blocks* ex, con
   const int halves = ex->act == SMOE_ACT_SWIGLU ? 2 : 1;
   int32_t *off = at<int32_t>(ws, l.off), *rows = at<int32_t>(ws, l.rows), *tokrow = at<int32_t>(ws, l.tokrow);
   float* roww = at<float>(ws, l.roww);
-  rc = smoe_dispatch_plan(idx, w, N, K, E, at<int32_t>(ws, l.cnt), off, rows, roww, tokrow, at<void>(ws, l.plan),
-                          smoe_dispatch_workspace_bytes(N, K, E), stream);
-  if (rc != SMOE_OK) return rc;
   void* xw = at<void>(ws, l.x_at);
-  SMOE_TRY(quantize_rows(msg, msg_dtype, H, N, H, xw, l.x, s), "quantize messages");
+  const BlockQuant mq = rows_quant(msg, msg_dtype, H, N, H, xw, l.x);
+  if (prep_fits(N, K, E)) {
+    PrepArgs pa;
+    pa.idx = idx;
+    pa.w = w;
+    pa.N = N;
+    pa.K = K;
+    pa.E = E;
+    pa.off = off;
+    pa.rows = rows;
+    pa.tokrow = tokrow;
+    pa.roww = roww;
+    SMOE_TRY(launch_prep(pa, mq, s), "plan and messages");
+  } else {
+    rc = smoe_dispatch_plan(idx, w, N, K, E, at<int32_t>(ws, l.cnt), off, rows, roww, tokrow, at<void>(ws, l.plan),
+                            smoe_dispatch_workspace_bytes(N, K, E), stream);
+    if (rc != SMOE_OK) return rc;
+    SMOE_TRY(launch_quantize_fp8_blocks(mq, s), "quantize messages");
+  }
   BlockGemm up;
   up.epi = halves == 2 ? BLK_UP_SWIGLU : BLK_UP_GELU;
   up.X = at<uint8_t>(xw, l.x.codes);

@@ -2,112 +2,17 @@
 // or 128 x 128 block) and the products on such operands, dense and grouped by
 // expert.
 #include "smoe_common.hpp"
-#include "smoe_fp8_blocks.hpp"
+#include "smoe_fp8_blocks_dev.hpp"
 #include "smoe_internal.hpp"
 
 namespace smoe {
 namespace {
 
-typedef int i32x8 __attribute__((ext_vector_type(8)));
-
-constexpr float kE4m3Max = 448.0f;
-
-// max that keeps a NaN once seen: a block with a NaN has a NaN scale
-__device__ __forceinline__ float nan_max(float m, float a) { return (a > m || a != a) ? a : m; }
-// ... over the 16 lanes of a DPP row
-__device__ __forceinline__ float row16_nan_max(float v) {
-  v = nan_max(v, dpp_f<kDppXor1>(v));
-  v = nan_max(v, dpp_f<kDppXor2>(v));
-  v = nan_max(v, dpp_f<kDppHalfMirror>(v));
-  v = nan_max(v, dpp_f<kDppMirror>(v));
-  return v;
-}
-
-// scale = max(amax / 448, 1e-12), the quotient an IEEE one; a NaN stays
-__device__ __forceinline__ float block_scale(float amax) {
-  const float s = __fdiv_rn(amax, kE4m3Max);
-  return s < 1e-12f ? 1e-12f : s;
-}
-
-// Four e4m3 codes of values that a block's scale has brought to +-448 (plus
-// half a unit in the last place of the quotient, which rounds to 448): round
-// to nearest even, NaN to NaN.
-__device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d) {
-  int w = 0;
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, w, false);
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
-  return static_cast<uint32_t>(w);
-}
-
-// Eight elements from column c of a row that ends at cols, 0 past the end;
-// one 16- or 32-byte load where the row's start and c allow it (vec).
-template <int XDT>
-__device__ __forceinline__ void load_cols8(const void* row, int c, int cols, bool vec, float (&v)[8]) {
-  if (vec && c + 8 <= cols) {
-    if constexpr (XDT == SMOE_F32) {
-      const f32x4* p = reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(row) + c);
-      const f32x4 a = p[0], b = p[1];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        v[j] = a[j];
-        v[4 + j] = b[j];
-      }
-    } else {
-      const u32x4 a = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(row) + c);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint16_t h = static_cast<uint16_t>(a[j >> 1] >> (16 * (j & 1)));
-        v[j] = XDT == SMOE_BF16 ? bf2f(h) : static_cast<float>(__builtin_bit_cast(_Float16, h));
-      }
-    }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    float x = 0.f;
-    if (c + j < cols) {
-      if constexpr (XDT == SMOE_F32) x = reinterpret_cast<const float*>(row)[c + j];
-      else if constexpr (XDT == SMOE_BF16) x = bf2f(reinterpret_cast<const uint16_t*>(row)[c + j]);
-      else x = static_cast<float>(reinterpret_cast<const _Float16*>(row)[c + j]);
-    }
-    v[j] = x;
-  }
-}
-
-template <int XDT>
-constexpr int elt_bytes() { return XDT == SMOE_F32 ? 4 : 2; }
-
-__device__ __forceinline__ float amax8(const float (&v)[8]) {
-  float m = 0.f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) m = nan_max(m, fabsf(v[j]));
-  return m;
-}
-
-__device__ __forceinline__ u32x2 codes8(const float (&v)[8], float sc) {
-  float q[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) q[j] = __fdiv_rn(v[j], sc);
-  return u32x2{pack_e4m3(q[0], q[1], q[2], q[3]), pack_e4m3(q[4], q[5], q[6], q[7])};
-}
-
-// 1 x 128 blocks: sixteen lanes hold a block, eight elements each.
+// 1 x 128 blocks (quant_row_block), sixteen a workgroup.
 template <int XDT>
 __global__ __launch_bounds__(256) void k_quant_row_blocks(const BlockQuant q, int nblk, int64_t total) {
-  const int64_t b = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 4;
-  const int l16 = threadIdx.x & 15;
-  const int64_t bc = b < total ? b : total - 1;  // every lane of the wave stays for the DPP steps
-  const int64_t row = bc / nblk;
-  const int kb = static_cast<int>(bc - row * nblk);
-  const int c = kb * kFp8Block + 8 * l16;
-  const char* rp = reinterpret_cast<const char*>(q.x) + row * q.ldx * elt_bytes<XDT>();
-  const bool vec = (reinterpret_cast<uintptr_t>(q.x) | static_cast<uintptr_t>(q.ldx * elt_bytes<XDT>())) % 16 == 0;
-  float v[8];
-  load_cols8<XDT>(rp, c, q.cols, vec, v);
-  const float sc = block_scale(row16_nan_max(amax8(v)));
-  if (b >= total) return;
-  if (l16 == 0) q.scale[row * q.s_row + kb * q.s_col] = sc;
-  if (c < q.ld_out) *reinterpret_cast<u32x2*>(q.codes + row * q.ld_out + c) = codes8(v, sc);
+  quant_row_block<XDT>(q, nblk, total, (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 4,
+                       threadIdx.x & 15);
 }
 
 // 128 x 128 blocks: a workgroup holds a block, thread t the columns
@@ -147,87 +52,6 @@ __global__ __launch_bounds__(256) void k_quant_square_blocks(const BlockQuant q,
 }
 
 // ------------------------------------------------------------------ GEMM ----
-// Rows of the 64 groups from b on: first, end and BM-row tiles of group
-// b + lane.
-__device__ __forceinline__ void groups64(const BlockGemm& p, int BM, int b, int& lo, int& hi, int& t) {
-  const int i = b + static_cast<int>(threadIdx.x & 63);
-  const int ic = i < p.G ? i : p.G - 1;
-  lo = p.grp_off[ic];
-  hi = p.grp_off[ic + 1];
-  t = i < p.G ? (hi - lo + BM - 1) / BM : 0;
-}
-
-// The tile of workgroup bid: group by group, within a group strip by strip
-// and the strip's row tiles next to each other; workgroup ids are dealt to
-// the 8 XCDs round robin and each XCD takes one contiguous part of the order.
-template <int BM, int BN>
-__device__ __forceinline__ bool block_tile(const BlockGemm& p, int bid, int& g, int& m0, int& mrows,
-                                           int& n0) {
-  const int strips = (p.N_out + BN - 1) / BN;
-  int tiles = 0;
-  if (p.G == 0) {
-    tiles = (p.single_rows + BM - 1) / BM;
-  } else {
-    for (int b = 0; b < p.G; b += 64) {
-      int lo, hi, t;
-      groups64(p, BM, b, lo, hi, t);
-      tiles += __builtin_amdgcn_readlane(wave_incl_scan(t), 63);
-    }
-  }
-  const int T = tiles * strips;
-  if (bid >= T) return false;
-  const int x = bid & 7, base = T >> 3, rem = T & 7;
-  const int logical = x * base + min(x, rem) + (bid >> 3);
-  int lo = 0, hi = p.single_rows, in = logical;
-  g = 0;
-  if (p.G > 0) {
-    int acc = 0;
-    for (int b = 0; b < p.G; b += 64) {
-      int l, h, t;
-      groups64(p, BM, b, l, h, t);
-      const int incl = wave_incl_scan(t) * strips + acc;
-      const uint64_t m = __ballot(logical < incl);
-      if (m) {
-        const int f = __builtin_ctzll(m);
-        g = b + f;
-        in = logical - __builtin_amdgcn_readlane(incl - t * strips, f);
-        lo = __builtin_amdgcn_readlane(l, f);
-        hi = __builtin_amdgcn_readlane(h, f);
-        break;
-      }
-      acc = __builtin_amdgcn_readlane(incl, 63);
-    }
-  }
-  const int tm = (hi - lo + BM - 1) / BM;
-  m0 = lo + (in % tm) * BM;
-  mrows = min(BM, hi - m0);
-  n0 = (in / tm) * BN;
-  return true;
-}
-
-// The codes of a fragment past the end of K, set to code 0 (both operands:
-// what lies behind a row's end may decode to NaN).  left: bytes of this
-// lane's 32 that belong to K.
-__device__ __forceinline__ i32x8 cut_frag(i32x8 f, int left) {
-#pragma unroll
-  for (int d = 0; d < 8; ++d) {
-    const int n = left - 4 * d;
-    const uint32_t keep = n >= 4 ? 0xFFFFFFFFu : (n <= 0 ? 0u : (1u << (8 * n)) - 1u);
-    f[d] = static_cast<int>(static_cast<uint32_t>(f[d]) & keep);
-  }
-  return f;
-}
-
-// 32 codes of a lane as four bf16 MFMA operands (every e4m3 value is a bf16)
-__device__ __forceinline__ void widen_frag(i32x8 f, bf16x8 (&o)[4]) {
-#pragma unroll
-  for (int p = 0; p < 4; ++p) {
-    const u32x2 a = fp8x4_to_bf16x4(static_cast<uint32_t>(f[2 * p]));
-    const u32x2 b = fp8x4_to_bf16x4(static_cast<uint32_t>(f[2 * p + 1]));
-    o[p] = __builtin_bit_cast(bf16x8, u32x4{a.x, a.y, b.x, b.y});
-  }
-}
-
 // 128 rows x 128 output channels a workgroup (SwiGLU: 128 gate and the 128
 // up channels of the same outputs), K one block of 128 a stage through a
 // two-stage LDS ring filled by DMA; wave tile 64 x 64 channels (SwiGLU 32
@@ -448,42 +272,13 @@ __global__ __launch_bounds__(EPI == BLK_UP_SWIGLU ? 512 : 256, 2) void k_gemm_bl
           const float y = acc[j][i][v] + b4[v];
           o[v] = EPI == BLK_GELU ? gelu_erf(y) : (EPI == BLK_DOWN ? y * rs : y);
         }
-        const int64_t at = static_cast<int64_t>(m0 + r) * p.ldo + n;
-        if constexpr (ODT == SMOE_F32) {
-          float* po = reinterpret_cast<float*>(p.out) + at;
-          if (n + 3 < p.N_out && (reinterpret_cast<uintptr_t>(po) & 15) == 0) {
-            *reinterpret_cast<f32x4*>(po) = f32x4{o[0], o[1], o[2], o[3]};
-          } else {
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-              if (n + v < p.N_out) po[v] = o[v];
-          }
-        } else {
-          uint16_t* po = reinterpret_cast<uint16_t*>(p.out) + at;
-          if (n + 3 < p.N_out && (reinterpret_cast<uintptr_t>(po) & 7) == 0) {
-            *reinterpret_cast<u32x2*>(po) = u32x2{pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3])};
-          } else {
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-              if (n + v < p.N_out) po[v] = f2bf(o[v]);
-          }
-        }
+        store4<ODT>(p, m0 + r, n, o);
       }
     }
   }
 }
 
 int rc() { return hipGetLastError() == hipSuccess ? SMOE_OK : SMOE_EHIP; }
-
-template <typename F>
-int by_xdt(int dt, F&& f) {
-  switch (dt) {
-    case SMOE_F32: return f(std::integral_constant<int, SMOE_F32>{});
-    case SMOE_BF16: return f(std::integral_constant<int, SMOE_BF16>{});
-    case SMOE_F16: return f(std::integral_constant<int, SMOE_F16>{});
-    default: return SMOE_EUNSUPPORTED;
-  }
-}
 
 }  // namespace
 
@@ -514,6 +309,8 @@ int launch_gemm_fp8_blocks(const BlockGemm& a, hipStream_t s) {
   if (rows <= 0) return SMOE_OK;
   if (a.K < 1 || a.N_out < 1 || a.ldx < a.K || a.ldw < a.K || a.ldx % 16 || a.ldw % 16 || a.w_gstride % 16)
     return SMOE_EINVAL;
+  if (gemm_blocks_few_fits(a)) return launch_gemm_blocks_few(a, s);
+  if (a.x_float) return SMOE_EINVAL;
   // at most one partly filled row tile for every group with rows
   const int64_t tiles = (rows + 127) / 128 + (a.G > 0 ? std::min(a.G, rows) : 0);
   const int64_t grid = tiles * ((a.N_out + 127) / 128);

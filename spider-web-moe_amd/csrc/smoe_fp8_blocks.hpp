@@ -45,6 +45,11 @@ struct BlockGemm {
   const float* xs = nullptr;   // scale of (row r, block b): xs[r * xs_row + b * xs_col]
   int64_t xs_row = 0, xs_col = 0;
   const int32_t* a_rows = nullptr;  // plan row -> X row; nullptr = identity
+  // instead of X / xs (linear_quantizes_inside): x [single_rows, K] itself,
+  // rows ld_float elements apart, quantized by the product's workgroups
+  const void* x_float = nullptr;
+  int x_dtype = SMOE_BF16;
+  int64_t ld_float = 0;
   const uint8_t* W = nullptr;  // codes [G, N_out (SwiGLU: gate rows, then up rows), K]
   int64_t w_gstride = 0, ldw = 0;
   const float* ws = nullptr;   // [G, row blocks (SwiGLU: gate's, then up's), blocks of K]
@@ -63,5 +68,24 @@ struct BlockGemm {
   int64_t os_col = 0;
 };
 int launch_gemm_fp8_blocks(const BlockGemm& g, hipStream_t s);
+// the products of a few rows per group (smoe_fp8_blocks_few.hip)
+bool gemm_blocks_few_fits(const BlockGemm& g);
+int launch_gemm_blocks_few(const BlockGemm& g, hipStream_t s);
+// whether a linear product of N rows takes x_float
+bool linear_quantizes_inside(int N, int K);
+
+// A small step's dispatch plan (smoe_dispatch_plan's: offsets [E + 1], rows,
+// row weights, tokrow [N, K]) and the quantized messages in one launch.
+constexpr int kPrepMaxN = 1024, kPrepMaxEntries = 4096;
+struct PrepArgs {
+  const int32_t* idx = nullptr;
+  const float* w = nullptr;
+  int N = 0, K = 0, E = 0;
+  int win = 0;  // groups a wave ranks (set by the launch)
+  int32_t *off = nullptr, *rows = nullptr, *tokrow = nullptr;
+  float* roww = nullptr;
+};
+bool prep_fits(int N, int K, int E);
+int launch_prep(const PrepArgs& a, const BlockQuant& q, hipStream_t s);
 
 }  // namespace smoe

@@ -150,39 +150,7 @@ int launch_route_topk(const float* logits, int N, int E, int K, int32_t* top_idx
 }
 
 // --------------------------------------------------------- slot merge ----
-// Arbitrary (idx, w) [N,K] -> distinct groups ascending with merged weights
-// (sum over the token's slots of that group, in slot order, from 0 — the
-// accumulation of sparse_experts.py:52-55).  Ids outside [0, E) never match
-// an expert and are dropped, as in the reference; drop_nonpos also drops
-// merged weights <= 0 (sparse_experts.py:56).  w == nullptr: every slot
-// weighs 1 (a binary source mask, model.py:277-279).
-__device__ __forceinline__ void merge_token(const int32_t* ti, const float* tw, int K, int E,
-                                            int drop_nonpos, int32_t* og, float* ow) {
-  int out = 0;
-  int last = -1;
-  // emit groups in ascending order: repeatedly take the smallest id > last
-  for (int it = 0; it < K; ++it) {
-    int best = kBig;
-    for (int s = 0; s < K; ++s) {
-      const int e = ti[s];
-      if (e > last && e < E && e >= 0 && e < best) best = e;
-    }
-    if (best == kBig) break;
-    float acc = 0.f;
-    for (int s = 0; s < K; ++s)
-      if (ti[s] == best) acc = acc + (tw ? tw[s] : 1.f);
-    last = best;
-    if (drop_nonpos && !(acc > 0.f)) continue;
-    og[out] = best;
-    ow[out] = acc;
-    ++out;
-  }
-  for (; out < K; ++out) {
-    og[out] = -1;
-    ow[out] = 0.f;
-  }
-}
-
+// (merge_token: smoe_routing.hpp)
 __global__ __launch_bounds__(256) void k_merge_slots(const int32_t* __restrict__ idx,
                                                      const float* __restrict__ w, int N, int K,
                                                      int E, int drop_nonpos,
@@ -480,65 +448,8 @@ int launch_dest_coeffs(const int32_t* src_idx, const int32_t* eidx, const float*
 }
 
 // -------------------------------------------------------------- plan ----
-// (the plan's outline and rank_chunk: smoe_routing.hpp)
-// Scatter of one token: row = goff[g] + base[g * bs] + rank (group offset,
-// the chunk's prefix inside the group, the rank inside the chunk).
-template <typename P>
-__device__ __forceinline__ void scatter_token(const int32_t* __restrict__ tok_g,
-                                              const float* __restrict__ tok_w, int t, int S,
-                                              int G, P base, int bs, const int* goff,
-                                              int32_t* __restrict__ rows,
-                                              float* __restrict__ roww,
-                                              int32_t* __restrict__ tokrow) {
-  const int64_t e0 = static_cast<int64_t>(t) * S;
-  for (int j0 = 0; j0 < S; j0 += 8) {
-    int gv[8], rv[8], bv[8], ov[8];
-    float wv[8];
-    // every load unconditional (clamped indices), so each batch is one
-    // round trip to memory
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int jj = j0 + u < S ? j0 + u : S - 1;
-      gv[u] = tok_g[e0 + jj];
-      rv[u] = tokrow[e0 + jj];
-      wv[u] = tok_w[e0 + jj];
-    }
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int gc = (gv[u] >= 0 && gv[u] < G) ? gv[u] : 0;
-      bv[u] = base[gc * bs];
-      ov[u] = goff[gc];
-    }
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      if (j0 + u >= S || rv[u] < 0 || gv[u] < 0 || gv[u] >= G) continue;
-      const int row = ov[u] + bv[u] + rv[u];
-      tokrow[e0 + j0 + u] = row;
-      rows[row] = t;
-      roww[row] = wv[u];
-    }
-  }
-}
-
-// Exclusive scan of tot[0..G) into goff[0..G].  Every thread of the
-// workgroup calls it (it holds barriers); the first 256 do the work.
-__device__ __forceinline__ void block_group_offsets(const int32_t* tot, int G, int* goff,
-                                                    int* wsum) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const bool act = tid < 256;
-  const int v = (act && tid < G) ? tot[tid] : 0;
-  const int incl = wave_incl_scan(v);
-  if (act && lane == 63) wsum[wave] = incl;
-  __syncthreads();
-  if (act) {
-    int before = 0;
-    for (int w = 0; w < wave; ++w) before += wsum[w];
-    if (tid < G) goff[tid] = before + incl - v;
-    if (tid == 0) goff[G] = wsum[0] + wsum[1] + wsum[2] + wsum[3];
-  }
-  __syncthreads();
-}
-
+// (the plan's outline, rank_chunk, scatter_token and block_group_offsets:
+// smoe_routing.hpp)
 // ccnt / cacnt are [G, C] (group-major).  Wave w of the grid ranks chunk
 // w / W for the window w % W (W = ceil(G / 64)).
 __global__ __launch_bounds__(256) void k_plan_rank(const int32_t* __restrict__ tok_g,

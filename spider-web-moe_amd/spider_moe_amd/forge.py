@@ -132,45 +132,44 @@ def select_topk(logits: torch.Tensor, k: int, mode: int):
     return w.view(*lead, k).to(out_dtype), idx.view(*lead, k).long()
 
 
-def _select_groups_fwd(logits, k, score, bias, num_groups, top_groups, renormalize, scale):
-    dev = logits.device
-    e = logits.shape[-1]
-    x = logits.contiguous()
-    shape = (*logits.shape[:-1], k)
-    w = torch.empty(shape, dtype=torch.float32, device=dev)
-    idx = torch.empty(shape, dtype=torch.int32, device=dev)
-    n = x.numel() // e if e else 0
-    with torch.cuda.device(dev):
-        nat.check(nat.lib().smoe_select_groups(
-            x.data_ptr(), nat.float_code(x.dtype), n, e, k, score, nat.ptr(bias), num_groups,
-            top_groups, renormalize, scale, w.data_ptr(), idx.data_ptr(), nat.stream_of(dev)),
-            "smoe_select_groups")
+def _select_groups_fwd(x, k, score, bias, num_groups, top_groups, renormalize, scale):
+    """x: contiguous logits."""
+    dev, shape = x.device, x.shape
+    out = (*shape[:-1], k)
+    w = torch.empty(out, dtype=torch.float32, device=dev)
+    idx = torch.empty(out, dtype=torch.int32, device=dev)
+    e = shape[-1]
+    nat.launch(dev, "smoe_select_groups", x.data_ptr(), nat.float_code(x.dtype),
+               x.numel() // e if e else 0, e, k, score, None if bias is None else bias.data_ptr(),
+               num_groups, top_groups, renormalize, scale, w.data_ptr(), idx.data_ptr())
     return w, idx
 
 
 class _SelectGroups(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, k, score, bias, num_groups, top_groups, renormalize, scale):
-        w, idx = _select_groups_fwd(logits, k, score, bias, num_groups, top_groups, renormalize, scale)
-        ctx.save_for_backward(logits, idx)
+        x = logits.contiguous()
+        w, idx = _select_groups_fwd(x, k, score, bias, num_groups, top_groups, renormalize, scale)
+        ctx.save_for_backward(x, idx)
         ctx.how = (score, renormalize, scale)
         ctx.mark_non_differentiable(idx)
+        ctx.set_materialize_grads(False)  # no zeros for idx
         return w, idx
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_w, _):
-        logits, idx = ctx.saved_tensors
+        if d_w is None:
+            return (None,) * 8
+        if torch.is_grad_enabled():
+            raise RuntimeError("route_groups is not twice differentiable")
+        x, idx = ctx.saved_tensors
         score, renormalize, scale = ctx.how
-        x = logits.contiguous()
         d = torch.empty_like(x)
         e, k = x.shape[-1], idx.shape[-1]
-        d_w = d_w.float().contiguous()
-        with torch.cuda.device(x.device):
-            nat.check(nat.lib().smoe_select_groups_backward(
-                x.data_ptr(), nat.float_code(x.dtype), x.numel() // e, e, k, score, renormalize,
-                scale, idx.data_ptr(), d_w.data_ptr(), d.data_ptr(), nat.stream_of(x.device)),
-                "smoe_select_groups_backward")
+        d_w = d_w.contiguous()
+        nat.launch(x.device, "smoe_select_groups_backward", x.data_ptr(), nat.float_code(x.dtype),
+                   x.numel() // e, e, k, score, renormalize, scale, idx.data_ptr(), d_w.data_ptr(),
+                   d.data_ptr())
         return d, None, None, None, None, None, None, None
 
 
@@ -184,12 +183,14 @@ def select_groups(logits: torch.Tensor, k: int, *, score: str = "sigmoid", bias=
     if bias is not None:
         if bias.shape != logits.shape[-1:]:
             raise ValueError(f"bias must be [{logits.shape[-1]}], got {tuple(bias.shape)}")
-        bias = bias.detach().float().contiguous()
-    how = (int(k), nat.SCORES[score], bias, int(num_groups), int(top_groups), int(renormalize),
-           float(scale))
+        if bias.dtype != torch.float32:
+            bias = bias.float()
+        bias = bias.detach().contiguous()
     if torch.is_grad_enabled() and logits.requires_grad:
-        return _SelectGroups.apply(logits, *how)
-    return _select_groups_fwd(logits.detach(), *how)
+        return _SelectGroups.apply(logits, k, nat.SCORES[score], bias, num_groups, top_groups,
+                                   renormalize, scale)
+    return _select_groups_fwd(logits.contiguous(), k, nat.SCORES[score], bias, num_groups,
+                              top_groups, renormalize, scale)
 
 
 # ------------------------------------------------------------------ gemm ----
@@ -238,13 +239,10 @@ def _linear_fp8_blocks(x, codes, scale, bias, act):
     n = out.numel() // n_out if n_out else 0
     lib = nat.lib()
     need = lib.smoe_linear_fp8_blocks_workspace_bytes(n, k)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        nat.check(lib.smoe_linear_fp8_blocks(
-            x.data_ptr(), nat.float_code(x.dtype), ldx, None, n, k, codes.data_ptr(), ldw,
-            scale.data_ptr(), nat.ptr(bias), n_out, _ACT[act], out.data_ptr(),
-            nat.dtype_code(out_dtype), ws.data_ptr(), need, nat.stream_of(dev)),
-            "smoe_linear_fp8_blocks")
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    nat.launch(dev, "smoe_linear_fp8_blocks", x.data_ptr(), nat.float_code(x.dtype), ldx, None, n, k,
+               codes.data_ptr(), ldw, scale.data_ptr(), nat.ptr(bias), n_out, _ACT[act],
+               out.data_ptr(), nat.dtype_code(out_dtype), nat.ptr(ws), need)
     return out if out_dtype == x.dtype else out.to(x.dtype)
 
 
@@ -254,9 +252,9 @@ def _rows16(codes):
     laid out so, else a copy."""
     rows, cols = codes.shape
     ld = codes.stride(0) if rows > 1 else -(-cols // 16) * 16
-    room = codes.untyped_storage().nbytes() - codes.storage_offset()
     if (codes.stride(1) == 1 or cols == 1) and ld >= cols and ld % 16 == 0 and \
-            codes.data_ptr() % 16 == 0 and room >= rows * ld:
+            codes.data_ptr() % 16 == 0 and (cols % 16 == 0 or codes.untyped_storage().nbytes() -
+                                            codes.storage_offset() >= rows * ld):
         return codes, ld
     ld = -(-cols // 16) * 16
     c = torch.zeros(rows, ld, dtype=torch.uint8, device=codes.device)

@@ -184,7 +184,7 @@ def quantize_fp8_blocks(x: torch.Tensor, *, block_rows: int = FP8_BLOCK):
     rb = -(-rows // block_rows)
     if x.is_cuda:
         from . import _native as nat
-        ldx = _row_stride(x)
+        ldx = cols if x.is_contiguous() else _row_stride(x)
         if ldx is None:
             x, ldx = x.contiguous(), cols
         g = 1
@@ -192,11 +192,8 @@ def quantize_fp8_blocks(x: torch.Tensor, *, block_rows: int = FP8_BLOCK):
             g *= n
         codes = torch.empty(*lead, rows, ld, dtype=torch.float8_e4m3fn, device=x.device)
         scale = torch.empty(*lead, rb, cb, dtype=torch.float32, device=x.device)
-        with torch.cuda.device(x.device):
-            nat.check(nat.lib().smoe_quantize_fp8_blocks(
-                x.data_ptr(), nat.float_code(x.dtype), g, rows, cols, ldx, block_rows,
-                codes.data_ptr(), ld, scale.data_ptr(), nat.stream_of(x.device)),
-                "smoe_quantize_fp8_blocks")
+        nat.launch(x.device, "smoe_quantize_fp8_blocks", x.data_ptr(), nat.float_code(x.dtype), g, rows,
+                   cols, ldx, block_rows, codes.data_ptr(), ld, scale.data_ptr())
         return (codes if ld == cols else codes[..., :cols]), scale
     p = torch.zeros(*lead, rb * block_rows, cb * FP8_BLOCK)
     p[..., :rows, :cols] = x

@@ -180,9 +180,6 @@ def sparse_expert_delta_fp8_blocks(messages: torch.Tensor, top_indices: torch.Te
         raise RuntimeError("smoe_expert_delta_fp8_blocks: "
                            f"unsupported shapes ({lib.smoe_last_error().decode()})")
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        nat.check(lib.smoe_expert_delta_fp8_blocks(
-            experts._ref, msg.data_ptr(), code, idx.data_ptr(), wts.data_ptr(), n, k,
-            delta.data_ptr(), code, ws.data_ptr(), need, nat.stream_of(dev)),
-            "smoe_expert_delta_fp8_blocks")
+    nat.launch(dev, "smoe_expert_delta_fp8_blocks", experts._ref, msg.data_ptr(), code,
+               idx.data_ptr(), wts.data_ptr(), n, k, delta.data_ptr(), code, ws.data_ptr(), need)
     return delta
