@@ -52,39 +52,44 @@ __global__ __launch_bounds__(256) void k_quant_square_blocks(const BlockQuant q,
 }
 
 // ------------------------------------------------------------------ GEMM ----
-// 128 rows x 128 output channels a workgroup (SwiGLU: 128 gate and the 128
-// up channels of the same outputs), K one block of 128 a stage through a
-// two-stage LDS ring filled by DMA; wave tile 64 x 64 channels (SwiGLU 32
-// gate + 32 up).  A block's products are summed by the matrix instruction
-// from zero and enter the f32 accumulators times the block's two scales.
+// BM rows x BN weight rows a workgroup (SwiGLU: BN / 2 gate channels and the
+// up channels of the same outputs), K one block of 128 a stage through an LDS
+// ring of NS stages filled by DMA.  WM x WN waves, wave tile BM / WM rows x 64
+// weight rows (SwiGLU 32 gate + 32 up).  A block's products are summed by the
+// matrix instruction from zero and enter the f32 accumulators times the
+// block's two scales.
 //
 // The f8f6f4 instruction sums a block below f32 precision (measured on normal
 // codes: 1.5e-5 of the sum, 1 / 100 of a bf16 rounding), which suits outputs
 // of 8 to 16 bits.  WIDE (f32 outputs): the codes are widened to bf16, exactly,
 // and multiplied at a quarter of the rate with f32 sums.
-template <int EPI, int ODT, bool WIDE>
-__global__ __launch_bounds__(EPI == BLK_UP_SWIGLU ? 512 : 256, 2) void k_gemm_blocks(const BlockGemm p) {
+template <int EPI, int ODT, bool WIDE, int BM, int BN, int WM, int WN, int NS>
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm_blocks(const BlockGemm p) {
   constexpr bool SWIGLU = EPI == BLK_UP_SWIGLU, UP = EPI == BLK_UP_GELU || SWIGLU;
-  constexpr int BM = 128, BN = 128, WN = SWIGLU ? 4 : 2, NW = 2 * WN, WROWS = 64 * WN;
-  constexpr int NS = 2, XB = BM * 128, WB = WROWS * 128, SCB = BM * 4, STAGE = XB + WB + SCB;
-  constexpr int X_LD = BM / 8 / NW, W_LD = WROWS / 8 / NW;
+  constexpr int NW = WM * WN, CH = SWIGLU ? BN / 2 : BN, CHW = CH / WN, TM = BM / WM, FM = TM / 16;
+  static_assert(BN == 64 * WN && TM % 16 == 0 && (BM == 128 || BM == 256), "wave tile: 64 weight rows");
+  static_assert(!UP || CH % 128 == 0, "activations are quantized in blocks of 128 channels");
+  constexpr int XB = BM * 128, WB = BN * 128, STAGE = XB + WB + BM * 4;
+  constexpr int X_LD = BM / 8 / NW, W_LD = BN / 8 / NW, LD = X_LD + W_LD + 1;
+  static_assert(X_LD * NW * 8 == BM && W_LD * NW * 8 == BN && NW % (BM / 64) == 0, "whole DMA instructions");
   __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * STAGE];
   int g, m0, mrows, n0;
-  if (!block_tile<BM, BN>(p, blockIdx.x, g, m0, mrows, n0)) return;  // uniform
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (!block_tile<BM, CH>(p, blockIdx.x, g, m0, mrows, n0)) return;  // uniform
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
   const int KB = (p.K + 127) / 128;
 
   // DMA sources: lane i of instruction j loads 16 bytes of row
-  // 8 (NW j + wave) + i / 8, the chunk that the swizzle puts at i % 8
+  // 8 (NW j + wave) + i / 8, the chunk cl that the swizzle puts at i % 8 (the
+  // same one for every j: 4 NW j is a multiple of 8)
+  static_assert(4 * NW % 8 == 0, "one chunk per lane");
+  const int cl = 16 * sw_chunk<8>(8 * wave + (lane >> 3), lane & 7);
   const uint8_t* xsrc[X_LD];
   const uint8_t* wsrc[W_LD];
-  int xc[X_LD], wc[W_LD];
 #pragma unroll
   for (int j = 0; j < X_LD; ++j) {
-    const int r = 8 * (NW * j + wave) + (lane >> 3);
-    const int pr = m0 + min(r, mrows - 1);  // rows past the tile's end: a valid row, never stored
-    xc[j] = 16 * sw_chunk<8>(r, lane & 7);
+    const int pr = m0 + min(8 * (NW * j + wave) + (lane >> 3), mrows - 1);  // rows past the end: a valid one, never stored
     xsrc[j] = p.X + static_cast<int64_t>(p.a_rows ? p.a_rows[pr] : pr) * p.ldx;
   }
 #pragma unroll
@@ -92,127 +97,137 @@ __global__ __launch_bounds__(EPI == BLK_UP_SWIGLU ? 512 : 256, 2) void k_gemm_bl
     const int r = 8 * (NW * j + wave) + (lane >> 3);
     const int ch = SWIGLU ? n0 + 32 * (r >> 6) + (r & 31) : n0 + r;
     const int64_t row = min(ch, p.N_out - 1) + (SWIGLU && (r & 32) ? p.N_out : 0);
-    wc[j] = 16 * sw_chunk<8>(r, lane & 7);
     wsrc[j] = p.W + g * p.w_gstride + row * p.ldw;
   }
-  // the rows' scales: waves of even number load rows 0-63, of odd number 64-127
-  const int sr = 64 * (wave & 1) + lane;
-  const int spr = m0 + min(sr, mrows - 1);
+  // the rows' scales: wave w loads rows 64 (w % (BM / 64)) .. + 63
+  const int sw = wave % (BM / 64);
+  const int spr = m0 + min(64 * sw + lane, mrows - 1);
   const float* ssrc = p.xs + static_cast<int64_t>(p.a_rows ? p.a_rows[spr] : spr) * p.xs_row;
   auto issue = [&](int s) {
     uint8_t* base = ring + (s % NS) * STAGE;
     const int k0 = s * 128;
+    const int at = k0 + cl < p.K ? k0 + cl : 0;  // chunks past K: the row's first one, cut before use
 #pragma unroll
-    for (int j = 0; j < X_LD; ++j)  // chunks past K: the row's first one, cut before use
-      __builtin_amdgcn_global_load_lds((gbl_vptr)(xsrc[j] + (k0 + xc[j] < p.K ? k0 + xc[j] : 0)),
-                                       (lds_vptr)(base + (NW * j + wave) * 1024), 16, 0, 0);
+    for (int j = 0; j < X_LD; ++j)
+      __builtin_amdgcn_global_load_lds((gbl_vptr)(xsrc[j] + at), (lds_vptr)(base + (NW * j + wave) * 1024), 16, 0, 0);
 #pragma unroll
     for (int j = 0; j < W_LD; ++j)
-      __builtin_amdgcn_global_load_lds((gbl_vptr)(wsrc[j] + (k0 + wc[j] < p.K ? k0 + wc[j] : 0)),
-                                       (lds_vptr)(base + XB + (NW * j + wave) * 1024), 16, 0, 0);
-    __builtin_amdgcn_global_load_lds((gbl_vptr)(ssrc + s * p.xs_col),
-                                     (lds_vptr)(base + XB + WB + 256 * (wave & 1)), 4, 0, 0);
+      __builtin_amdgcn_global_load_lds((gbl_vptr)(wsrc[j] + at), (lds_vptr)(base + XB + (NW * j + wave) * 1024), 16, 0, 0);
+    __builtin_amdgcn_global_load_lds((gbl_vptr)(ssrc + s * p.xs_col), (lds_vptr)(base + XB + WB + 256 * sw), 4, 0, 0);
   };
   const int fr = lane & 15, q = lane >> 4;
-  auto frag = [&](const uint8_t* op, int r) {
-    const u32x4 lo = *reinterpret_cast<const u32x4*>(op + r * 128 + (sw_chunk<8>(r, 2 * q) << 4));
-    const u32x4 hi = *reinterpret_cast<const u32x4*>(op + r * 128 + (sw_chunk<8>(r, 2 * q + 1) << 4));
+  // fragment of 16 rows from tile row 16 t on: row fr, chunks q and q + 4 (both
+  // operands pair the same k, in whatever order); the swizzle is the same for
+  // every t.  Chunks 2 q and 2 q + 1 meet in the same banks: a ds_read_b128
+  // serves lanes 0-3, 12-15, 20-23, 24-27 together (half the LDS cycles were
+  // conflicts).
+  const int flo = fr * 128 + (sw_chunk<8>(fr, q) << 4), fhi = flo ^ 64;
+  auto frag = [&](const uint8_t* op) {
+    const u32x4 lo = *reinterpret_cast<const u32x4*>(op + flo);
+    const u32x4 hi = *reinterpret_cast<const u32x4*>(op + fhi);
     return __builtin_bit_cast(i32x8, (uint32_t __attribute__((ext_vector_type(8)))){
                                          lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w});
   };
 
-  f32x4 acc[4][4];
+  f32x4 acc[4][FM];
 #pragma unroll
   for (int j = 0; j < 4; ++j)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const float* wsp = p.ws + g * p.ws_gstride + static_cast<int64_t>(n0 / 128) * KB;
-  const float* wsp_up = wsp + static_cast<int64_t>((p.N_out + 127) / 128) * KB;  // SwiGLU
+    for (int i = 0; i < FM; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int nblk = (p.N_out + 127) / 128;
+  const int cblk = min((n0 + CHW * wn) / 128, nblk - 1);  // the wave's channels' block of weight scales
+  const float* wsp = p.ws + g * p.ws_gstride + static_cast<int64_t>(cblk) * KB;
+  const float* wsp_up = wsp + static_cast<int64_t>(nblk) * KB;  // SwiGLU
 
-  issue(0);
+#pragma unroll
+  for (int s = 0; s < NS - 1; ++s)
+    if (s < KB) issue(s);
   for (int s = 0; s < KB; ++s) {
-    // own part of stage s landed; after the barrier everybody's, and nobody
-    // reads stage s - 1 any more
-    wait_vmcnt<0>();
+    // own part of stage s landed (the later ones may be on their way); after
+    // the barrier everybody's, and nobody reads stage s - 1 any more
+    if (NS > 2 && s + NS - 2 < KB) wait_vmcnt<(NS - 2) * LD>();
+    else wait_vmcnt<0>();
     wait_lgkm0();
     __builtin_amdgcn_s_barrier();
-    if (s + 1 < KB) issue(s + 1);  // into the slot of stage s - 1
-    const uint8_t* sx = ring + (s % NS) * STAGE;
-    const float* sc = reinterpret_cast<const float*>(sx + XB + WB) + wm * 64;
-    i32x8 xf[4], wf[4];
-    float xsv[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      xf[i] = frag(sx, wm * 64 + i * 16 + fr);
-      xsv[i] = sc[i * 16 + fr];
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) wf[j] = frag(sx + XB, wn * 64 + j * 16 + fr);
-    const int left = p.K - s * 128;
-    if (left < 128) {  // uniform: the last stage of a ragged K
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        xf[i] = cut_frag(xf[i], left - 32 * q);
-        wf[i] = cut_frag(wf[i], left - 32 * q);
-      }
+    if (s + NS - 1 < KB) issue(s + NS - 1);  // into the slot of stage s - 1
+    uint8_t* sx = ring + (s % NS) * STAGE;
+    const float* sc = reinterpret_cast<const float*>(sx + XB + WB) + wm * TM;
+    if (p.K - s * 128 < 128) {  // uniform: the last stage of a ragged K
+      cut_stage(sx, BM + BN, p.K - s * 128, tid, NW * 64);
+      lds_barrier();
     }
     const float w0 = wsp[s], w1 = SWIGLU ? wsp_up[s] : 0.f;
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (WIDE) {
-      bf16x8 xw[4][4];
+    i32x8 wf[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) widen_frag(xf[i], xw[i]);
+    for (int j = 0; j < 4; ++j) wf[j] = frag(sx + XB + (wn * 64 + j * 16) * 128);
+    auto xfrag = [&](int i) { return frag(sx + (wm * TM + i * 16) * 128); };
+    // sixteen rows at a time: the next rows' fragment is read, and the sums of
+    // the rows before enter the accumulators, under this one's products
+    i32x8 xf = xfrag(0);
+    f32x4 part[4];
+    float s0 = 0.f, s1 = 0.f;
+    auto add = [&](int i) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        bf16x8 ww[4];
-        widen_frag(wf[j], ww);
-        const float wsc = SWIGLU && j >= 2 ? w1 : w0;
+      for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          f32x4 part = zero;
+        for (int v = 0; v < 4; ++v)
+          acc[j][i][v] = fmaf(part[j][v], SWIGLU && j >= 2 ? s1 : s0, acc[j][i][v]);
+    };
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const float xsv = sc[i * 16 + fr];
+      const i32x8 nx = xfrag(i + 1 < FM ? i + 1 : i);
+      f32x4 now[4];
+      if constexpr (WIDE) {
+        bf16x8 xw[4];
+        widen_frag(xf, xw);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          bf16x8 ww[4];
+          widen_frag(wf[j], ww);
+          now[j] = zero;
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            part = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ww[u], xw[i][u], part, 0, 0, 0);
-#pragma unroll
-          for (int v = 0; v < 4; ++v) acc[j][i][v] = fmaf(part[v], xsv[i] * wsc, acc[j][i][v]);
+            now[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ww[u], xw[u], now[j], 0, 0, 0);
         }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          now[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], xf, zero, 0, 0, 0, 0, 0, 0);
       }
-    } else {
+      if (i > 0) add(i - 1);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float wsc = SWIGLU && j >= 2 ? w1 : w0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4 part = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], xf[i], zero, 0, 0, 0,
-                                                                              0, 0, 0);
-#pragma unroll
-          for (int v = 0; v < 4; ++v) acc[j][i][v] = fmaf(part[v], xsv[i] * wsc, acc[j][i][v]);
-        }
-      }
+      for (int j = 0; j < 4; ++j) part[j] = now[j];
+      s0 = xsv * w0;
+      s1 = xsv * w1;
+      xf = nx;
+      __builtin_amdgcn_sched_barrier(0);
     }
+    add(FM - 1);
   }
 
   // epilogue: lane holds channels 4 q + v of row fr of each 16 x 16 tile
   const float* bias = p.bias ? p.bias + g * p.bias_gstride : nullptr;
   if constexpr (UP) {
-    // activations of 128 channels: amax per row over the wave's channels, then
-    // over the waves of the row through LDS; codes staged in the ring
-    constexpr int JN = SWIGLU ? 2 : 4;
-    const int cw = SWIGLU ? 32 * wn : 64 * wn;  // the wave's first channel of the 128
+    // amax per row over the wave's channels, then over the waves of a block
+    // of 128 channels through LDS; codes staged in the ring
+    constexpr int JN = SWIGLU ? 2 : 4, BW = 128 / CHW;  // BW waves share a block
     float* red = reinterpret_cast<float*>(ring);  // [WN][BM]
-    uint8_t* stg = ring + WN * BM * 4;            // [BM][128], 16-byte chunks swizzled by row
-    float m[4];
+    uint8_t* stg = ring + WN * BM * 4;            // [BM][CH], 16-byte chunks swizzled by row
+    static_assert(WN * BM * 4 + BM * CH <= NS * STAGE, "staging in the ring");
+    float m[FM];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) m[i] = 0.f;
+    for (int i = 0; i < FM; ++i) m[i] = 0.f;
 #pragma unroll
     for (int j = 0; j < JN; ++j) {
-      const int c = cw + j * 16 + 4 * q;
+      const int c = CHW * wn + j * 16 + 4 * q;
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const bool in = n0 + c + v < p.N_out;
         const float b = bias && in ? bias[n0 + c + v] : 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < FM; ++i) {
           float y;
           if constexpr (SWIGLU) y = silu(acc[j][i][v]) * (acc[j + 2][i][v] + b);
           else y = gelu_erf(acc[j][i][v] + b);
@@ -224,61 +239,131 @@ __global__ __launch_bounds__(EPI == BLK_UP_SWIGLU ? 512 : 256, 2) void k_gemm_bl
     }
     __syncthreads();  // every wave is done with the ring
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < FM; ++i) {
       m[i] = nan_max(m[i], __shfl_xor(m[i], 16));
       m[i] = nan_max(m[i], __shfl_xor(m[i], 32));
-      if (q == 0) red[wn * BM + wm * 64 + i * 16 + fr] = m[i];
+      if (q == 0) red[wn * BM + wm * TM + i * 16 + fr] = m[i];
     }
     __syncthreads();
+    const int bw0 = wn / BW * BW;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = wm * 64 + i * 16 + fr;
-      float a = red[r];
+    for (int i = 0; i < FM; ++i) {
+      const int r = wm * TM + i * 16 + fr;
+      float a = red[bw0 * BM + r];
 #pragma unroll
-      for (int w = 1; w < WN; ++w) a = nan_max(a, red[w * BM + r]);
+      for (int w = 1; w < BW; ++w) a = nan_max(a, red[(bw0 + w) * BM + r]);
       const float sc = block_scale(a);
-      if (wn == 0 && q == 0 && r < mrows) p.out_scale[(n0 / 128) * p.os_col + m0 + r] = sc;
+      if (wn == bw0 && q == 0 && r < mrows && n0 + CHW * wn < p.N_out)
+        p.out_scale[((n0 + CHW * wn) / 128) * p.os_col + m0 + r] = sc;
 #pragma unroll
       for (int j = 0; j < JN; ++j) {
-        const int c = cw + j * 16 + 4 * q;
-        *reinterpret_cast<uint32_t*>(stg + r * 128 + (((c >> 4) ^ (r & 7)) << 4) + (c & 15)) =
+        const int c = CHW * wn + j * 16 + 4 * q;
+        *reinterpret_cast<uint32_t*>(stg + r * CH + (((c >> 4) ^ (r & 7)) << 4) + (c & 15)) =
             pack_e4m3(__fdiv_rn(acc[j][i][0], sc), __fdiv_rn(acc[j][i][1], sc),
                       __fdiv_rn(acc[j][i][2], sc), __fdiv_rn(acc[j][i][3], sc));
       }
     }
     __syncthreads();
     uint8_t* out = reinterpret_cast<uint8_t*>(p.out);
-    for (int e = tid; e < BM * 8; e += NW * 64) {
-      const int r = e >> 3, c = e & 7;
+    for (int e = tid; e < BM * (CH / 16); e += NW * 64) {
+      const int r = e / (CH / 16), c = e % (CH / 16);
       if (r < mrows && n0 + 16 * c < p.N_out)  // N_out % 16 == 0: whole chunks
         *reinterpret_cast<u32x4*>(out + static_cast<int64_t>(m0 + r) * p.ldo + n0 + 16 * c) =
-            *reinterpret_cast<const u32x4*>(stg + r * 128 + ((c ^ (r & 7)) << 4));
+            *reinterpret_cast<const u32x4*>(stg + r * CH + ((c ^ (r & 7)) << 4));
     }
   } else {
+    float b4[4][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + wn * 64 + j * 16 + 4 * q;
-      float b4[4];
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int v = 0; v < 4; ++v) b4[v] = (bias && n + v < p.N_out) ? bias[n + v] : 0.f;
+      for (int v = 0; v < 4; ++v) {
+        const int n = n0 + wn * 64 + j * 16 + 4 * q + v;
+        b4[j][v] = (bias && n < p.N_out) ? bias[n] : 0.f;
+      }
+    auto value = [&](int j, int i, float rs, float (&o)[4]) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = wm * 64 + i * 16 + fr;
+      for (int v = 0; v < 4; ++v) {
+        const float y = acc[j][i][v] + b4[j][v];
+        o[v] = EPI == BLK_GELU ? gelu_erf(y) : (EPI == BLK_DOWN ? y * rs : y);
+      }
+    };
+    // whole 16-byte chunks: the tile is staged in the ring (chunk c of row r at
+    // c ^ (r & 7)) and leaves in whole rows.  Straight from the registers a row
+    // is written in 32- or 64-byte pieces, which reach memory as twice the
+    // write requests.
+    constexpr int EB = ODT == SMOE_F32 ? 4 : 2, CPR = BN * EB / 16;
+    constexpr int PASS = BM * BN * EB <= NS * STAGE ? 1 : 2, FP = FM / PASS, TP = TM / PASS;
+    static_assert(BM / PASS * BN * EB <= NS * STAGE, "staging in the ring");
+    const bool whole = (static_cast<int64_t>(p.N_out) * EB) % 16 == 0 && (p.ldo * EB) % 16 == 0 &&
+                       reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+    if (whole) {
+#pragma unroll
+      for (int h = 0; h < PASS; ++h) {
+        __syncthreads();  // every wave is done with the ring (or the pass before)
+#pragma unroll
+        for (int i = h * FP; i < (h + 1) * FP; ++i) {
+          const int r = wm * TM + i * 16 + fr, lr = wm * TP + (i - h * FP) * 16 + fr;
+          const float rs = EPI == BLK_DOWN ? p.row_scale[m0 + min(r, mrows - 1)] : 1.f;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float o[4];
+            value(j, i, rs, o);
+            const int c4 = wn * 16 + j * 4 + q;  // group of four channels
+            if constexpr (ODT == SMOE_F32)
+              *reinterpret_cast<f32x4*>(ring + (lr * CPR + (c4 ^ (lr & 7))) * 16) = f32x4{o[0], o[1], o[2], o[3]};
+            else
+              *reinterpret_cast<u32x2*>(ring + (lr * CPR + ((c4 >> 1) ^ (lr & 7))) * 16 + (c4 & 1) * 8) =
+                  u32x2{pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3])};
+          }
+        }
+        __syncthreads();
+        for (int e = tid; e < BM / PASS * CPR; e += NW * 64) {
+          const int lr = e / CPR, c = e % CPR;
+          const int r = lr / TP * TM + h * FP * 16 + lr % TP;
+          if (r < mrows && n0 + c * (16 / EB) < p.N_out)
+            *reinterpret_cast<u32x4*>(static_cast<uint8_t*>(p.out) + ((m0 + static_cast<int64_t>(r)) * p.ldo + n0) * EB + c * 16) =
+                *reinterpret_cast<const u32x4*>(ring + (lr * CPR + (c ^ (lr & 7))) * 16);
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int r = wm * TM + i * 16 + fr;
         if (r >= mrows) continue;
         float o[4];
-        const float rs = EPI == BLK_DOWN ? p.row_scale[m0 + r] : 1.f;
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const float y = acc[j][i][v] + b4[v];
-          o[v] = EPI == BLK_GELU ? gelu_erf(y) : (EPI == BLK_DOWN ? y * rs : y);
-        }
-        store4<ODT>(p, m0 + r, n, o);
+        value(j, i, EPI == BLK_DOWN ? p.row_scale[m0 + r] : 1.f, o);
+        store4<ODT>(p, m0 + r, n0 + wn * 64 + j * 16 + 4 * q, o);
       }
-    }
   }
 }
 
 int rc() { return hipGetLastError() == hipSuccess ? SMOE_OK : SMOE_EHIP; }
+
+template <int EPI, int ODT, bool WIDE, int BM, int BN, int WM, int WN, int NS>
+int go_tile(const BlockGemm& a, hipStream_t s) {
+  constexpr int CH = EPI == BLK_UP_SWIGLU ? BN / 2 : BN;
+  const int rows = a.G > 0 ? a.max_rows : a.single_rows;
+  // at most one partly filled row tile for every group with rows
+  const int64_t tiles = (static_cast<int64_t>(rows) + BM - 1) / BM + (a.G > 0 ? std::min(a.G, rows) : 0);
+  const int64_t grid = tiles * ((static_cast<int64_t>(a.N_out) + CH - 1) / CH);
+  if (grid > 0x7fffffff) return SMOE_EINVAL;
+  SMOE_LAUNCH((k_gemm_blocks<EPI, ODT, WIDE, BM, BN, WM, WN, NS>), dim3(static_cast<unsigned>(grid)),
+              dim3(64 * WM * WN), 0, s, a);
+  return rc();
+}
+
+template <int EPI, int ODT, bool WIDE>
+int go_tiles(const BlockGemm& a, hipStream_t s) {
+  const int rows = a.G > 0 ? a.max_rows / a.G : a.single_rows;
+  if constexpr (!WIDE) {
+    if (rows >= 512) return go_tile<EPI, ODT, WIDE, 256, 256, 2, 4, 2>(a, s);
+  }
+  if constexpr (EPI == BLK_UP_SWIGLU) return go_tile<EPI, ODT, WIDE, 128, 256, 2, 4, 2>(a, s);
+  else return go_tile<EPI, ODT, WIDE, 128, 128, 2, 2, 2>(a, s);
+}
 
 }  // namespace
 
@@ -311,33 +396,13 @@ int launch_gemm_fp8_blocks(const BlockGemm& a, hipStream_t s) {
     return SMOE_EINVAL;
   if (gemm_blocks_few_fits(a)) return launch_gemm_blocks_few(a, s);
   if (a.x_float) return SMOE_EINVAL;
-  // at most one partly filled row tile for every group with rows
-  const int64_t tiles = (rows + 127) / 128 + (a.G > 0 ? std::min(a.G, rows) : 0);
-  const int64_t grid = tiles * ((a.N_out + 127) / 128);
-  if (grid > 0x7fffffff) return SMOE_EINVAL;
-  auto go = [&](auto epi, auto odt, auto wide) {
-    constexpr int EPI = decltype(epi)::value;
-    SMOE_LAUNCH((k_gemm_blocks<EPI, decltype(odt)::value, decltype(wide)::value>),
-                dim3(static_cast<unsigned>(grid)), dim3(EPI == BLK_UP_SWIGLU ? 512 : 256), 0, s, a);
-    return rc();
-  };
-  using F = std::integral_constant<int, SMOE_F32>;
-  using B = std::integral_constant<int, SMOE_BF16>;
-  using T = std::true_type;
-  using N = std::false_type;
   const bool f32 = a.out_dtype == SMOE_F32;
   switch (a.epi) {
-    case BLK_LINEAR: {
-      using E = std::integral_constant<int, BLK_LINEAR>;
-      return f32 ? go(E{}, F{}, T{}) : go(E{}, B{}, N{});
-    }
-    case BLK_GELU: {
-      using E = std::integral_constant<int, BLK_GELU>;
-      return f32 ? go(E{}, F{}, T{}) : go(E{}, B{}, N{});
-    }
-    case BLK_UP_GELU: return go(std::integral_constant<int, BLK_UP_GELU>{}, F{}, N{});
-    case BLK_UP_SWIGLU: return go(std::integral_constant<int, BLK_UP_SWIGLU>{}, F{}, N{});
-    case BLK_DOWN: return go(std::integral_constant<int, BLK_DOWN>{}, F{}, N{});
+    case BLK_LINEAR: return f32 ? go_tiles<BLK_LINEAR, SMOE_F32, true>(a, s) : go_tiles<BLK_LINEAR, SMOE_BF16, false>(a, s);
+    case BLK_GELU: return f32 ? go_tiles<BLK_GELU, SMOE_F32, true>(a, s) : go_tiles<BLK_GELU, SMOE_BF16, false>(a, s);
+    case BLK_UP_GELU: return go_tiles<BLK_UP_GELU, SMOE_F32, false>(a, s);
+    case BLK_UP_SWIGLU: return go_tiles<BLK_UP_SWIGLU, SMOE_F32, false>(a, s);
+    case BLK_DOWN: return go_tiles<BLK_DOWN, SMOE_F32, false>(a, s);
     default: return SMOE_EINVAL;
   }
 }

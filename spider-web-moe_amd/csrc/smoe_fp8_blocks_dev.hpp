@@ -145,9 +145,12 @@ __device__ __forceinline__ void groups64(const BlockGemm& p, int BM, int b, int&
   t = i < p.G ? (hi - lo + BM - 1) / BM : 0;
 }
 
-// The tile of workgroup bid: group by group, within a group strip by strip
-// and the strip's row tiles next to each other; workgroup ids are dealt to
-// the 8 XCDs round robin and each XCD takes one contiguous part of the order.
+// The tile of workgroup bid: group by group; within a group kSuperRows row
+// tiles at a time, over them strip by strip with the strip's row tiles next to
+// each other, so that the rows in use stay in an L2 while the strips' weights
+// pass.  Workgroup ids are dealt to the 8 XCDs round robin and each XCD takes
+// one contiguous part of the order.
+constexpr int kSuperRows = 8;
 template <int BM, int BN>
 __device__ __forceinline__ bool block_tile(const BlockGemm& p, int bid, int& g, int& m0, int& mrows,
                                            int& n0) {
@@ -187,23 +190,36 @@ __device__ __forceinline__ bool block_tile(const BlockGemm& p, int bid, int& g, 
     }
   }
   const int tm = (hi - lo + BM - 1) / BM;
-  m0 = lo + (in % tm) * BM;
+  const int super = in / (kSuperRows * strips), rest = in - super * kSuperRows * strips;
+  const int sr = min(kSuperRows, tm - super * kSuperRows);  // row tiles of this part
+  m0 = lo + (super * kSuperRows + rest % sr) * BM;
   mrows = min(BM, hi - m0);
-  n0 = (in / tm) * BN;
+  n0 = (rest / sr) * BN;
   return true;
 }
 
-// The codes of a fragment past the end of K, set to code 0 (both operands:
-// what lies behind a row's end may decode to NaN).  left: bytes of this
-// lane's 32 that belong to K.
-__device__ __forceinline__ i32x8 cut_frag(i32x8 f, int left) {
+// keeps the first `left` bytes
+__device__ __forceinline__ u32x4 cut16(u32x4 v, int left) {
 #pragma unroll
-  for (int d = 0; d < 8; ++d) {
+  for (int d = 0; d < 4; ++d) {
     const int n = left - 4 * d;
-    const uint32_t keep = n >= 4 ? 0xFFFFFFFFu : (n <= 0 ? 0u : (1u << (8 * n)) - 1u);
-    f[d] = static_cast<int>(static_cast<uint32_t>(f[d]) & keep);
+    v[d] &= n >= 4 ? 0xFFFFFFFFu : (n <= 0 ? 0u : (1u << (8 * n)) - 1u);
   }
-  return f;
+  return v;
+}
+
+// The codes past the end of K in a stage of `rows` 128-byte rows (swizzled as
+// sw_chunk says), set to code 0: what lies behind a row's end may decode to
+// NaN, in either operand.  left: bytes of the stage that belong to K.
+__device__ __forceinline__ void cut_stage(uint8_t* stage, int rows, int left, int tid, int threads) {
+  const int c0 = left >> 4, per = 8 - c0;  // the first chunk that is not whole
+  for (int e = tid; e < rows * per; e += threads) {
+    const int r = e / per, c = c0 + e % per;
+    u32x4* at = reinterpret_cast<u32x4*>(stage + r * 128 + (sw_chunk<8>(r, c) << 4));
+    u32x4 v = c == c0 ? *at : u32x4{0u, 0u, 0u, 0u};
+    if (c == c0) v = cut16(v, left & 15);
+    *at = v;
+  }
 }
 
 // 32 codes of a lane as four bf16 MFMA operands (every e4m3 value is a bf16)

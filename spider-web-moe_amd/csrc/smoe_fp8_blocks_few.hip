@@ -20,14 +20,6 @@ __device__ __forceinline__ Piece load_piece(const uint8_t* row, int k0, int q, i
   return {*reinterpret_cast<const u32x4*>(row + (a < K ? a : 0)),
           *reinterpret_cast<const u32x4*>(row + (b < K ? b : 0))};
 }
-__device__ __forceinline__ u32x4 cut16(u32x4 v, int left) {  // keeps the first `left` bytes
-#pragma unroll
-  for (int d = 0; d < 4; ++d) {
-    const int n = left - 4 * d;
-    v[d] &= n >= 4 ? 0xFFFFFFFFu : (n <= 0 ? 0u : (1u << (8 * n)) - 1u);
-  }
-  return v;
-}
 __device__ __forceinline__ Piece cut_piece(Piece p, int q, int left) {
   return {cut16(p.lo, left - 16 * q), cut16(p.hi, left - 64 - 16 * q)};
 }

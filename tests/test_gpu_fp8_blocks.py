@@ -148,7 +148,8 @@ def _weights(g, *shape):
 @pytest.mark.parametrize("n,k,n_out", [(1, 128, 16), (1, 2048, 1408), (2, 1, 1), (3, 16, 5), (7, 100, 130),
                                        (16, 129, 128), (17, 1000, 300), (33, 256, 257), (64, 1408, 64),
                                        (65, 130, 1000), (127, 512, 129), (129, 384, 384), (200, 1000, 700),
-                                       (257, 2816, 256), (300, 272, 2800)])
+                                       (257, 2816, 256), (300, 272, 2800), (600, 200, 520),
+                                       (1029, 384, 300)])
 def test_linear(dtype, n, k, n_out):
     from spider_moe_amd import ForgeGEMM
     say("linear", dtype, n, k, n_out)
@@ -166,7 +167,8 @@ def test_linear(dtype, n, k, n_out):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("n,k,n_out", [(1, 384, 260), (5, 640, 512), (40, 640, 260), (130, 640, 515), (300, 1100, 200)])
+@pytest.mark.parametrize("n,k,n_out", [(1, 384, 260), (5, 640, 512), (40, 640, 260), (130, 640, 515), (300, 1100, 200),
+                                       (777, 400, 700)])
 def test_linear_is_exact_on_small_integers(dtype, n, k, n_out):
     """One nonzero element a block and row, of value 448 times a power of two:
     every code is +-448, every product a power of two times the weight's
@@ -305,6 +307,7 @@ SHAPES = [  # n, e, k, h, u
     (1, 1, 1, 16, 16), (1, 8, 2, 256, 512), (1, 64, 2, 2048, 1408), (2, 4, 3, 144, 208), (5, 12, 3, 528, 1200),
     (16, 8, 2, 256, 384), (33, 16, 4, 512, 272), (64, 16, 2, 1024, 256), (100, 3, 2, 128, 128),
     (260, 5, 2, 400, 336), (300, 2, 1, 1024, 640), (515, 33, 6, 272, 144),
+    (1100, 2, 1, 272, 400), (1300, 3, 2, 128, 272),
 ]
 
 
