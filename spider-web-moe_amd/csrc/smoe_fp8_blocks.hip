@@ -19,7 +19,7 @@ __global__ __launch_bounds__(256) void k_quant_row_blocks(const BlockQuant q, in
 // 8 (t % 16) .. + 7 of rows t / 16, t / 16 + 16, ..
 template <int XDT>
 __global__ __launch_bounds__(256) void k_quant_square_blocks(const BlockQuant q, int rblk, int nblk) {
-  __shared__ float red[4];
+  __shared__ uint32_t red[4];
   const int kb = blockIdx.x % nblk;
   const int64_t grb = blockIdx.x / nblk;  // group * row blocks + row block
   const int64_t g = grb / rblk;
@@ -27,20 +27,18 @@ __global__ __launch_bounds__(256) void k_quant_square_blocks(const BlockQuant q,
   const int c = kb * kFp8Block + 8 * (threadIdx.x & 15);
   const bool vec = (reinterpret_cast<uintptr_t>(q.x) | static_cast<uintptr_t>(q.ldx * elt_bytes<XDT>())) % 16 == 0;
   float v[8][8];
-  float m = 0.f;
+  uint32_t m = 0u;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = r0 + (threadIdx.x >> 4) + 16 * i;
     const char* rp = reinterpret_cast<const char*>(q.x) + (g * q.rows + min(r, q.rows - 1)) * q.ldx * elt_bytes<XDT>();
     load_cols8<XDT>(rp, c, r < q.rows ? q.cols : 0, vec, v[i]);
-    m = nan_max(m, amax8(v[i]));
+    m = max(m, amax8(v[i]));
   }
-  m = row16_nan_max(m);
-  m = nan_max(m, __shfl_xor(m, 16));
-  m = nan_max(m, __shfl_xor(m, 32));
+  m = quarters_max(row16_max(m));
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
   __syncthreads();
-  const float sc = block_scale(nan_max(nan_max(red[0], red[1]), nan_max(red[2], red[3])));
+  const float sc = block_scale(max(max(red[0], red[1]), max(red[2], red[3])));
   if (threadIdx.x == 0) q.scale[grb * q.s_row + kb * q.s_col] = sc;
   if (c >= q.ld_out) return;
 #pragma unroll
@@ -139,6 +137,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm_blocks(const BlockGemm
   const float* wsp = p.ws + g * p.ws_gstride + static_cast<int64_t>(cblk) * KB;
   const float* wsp_up = wsp + static_cast<int64_t>(nblk) * KB;  // SwiGLU
 
+  // The weight scales of a stage are uniform: scalar loads, a stage ahead.  As
+  // vector loads each made the wave wait for every DMA issued before it.
+  const uniform_f32 wsc = as_uniform(wsp), wsc_up = as_uniform(wsp_up);
+  float nw0 = wsc[0], nw1 = SWIGLU ? wsc_up[0] : 0.f;
 #pragma unroll
   for (int s = 0; s < NS - 1; ++s)
     if (s < KB) issue(s);
@@ -156,7 +158,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm_blocks(const BlockGemm
       cut_stage(sx, BM + BN, p.K - s * 128, tid, NW * 64);
       lds_barrier();
     }
-    const float w0 = wsp[s], w1 = SWIGLU ? wsp_up[s] : 0.f;
+    const float w0 = nw0, w1 = nw1;
+    const int ns = min(s + 1, KB - 1);
+    nw0 = wsc[ns];
+    if (SWIGLU) nw1 = wsc_up[ns];
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     i32x8 wf[4];
 #pragma unroll
@@ -213,12 +218,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm_blocks(const BlockGemm
     // amax per row over the wave's channels, then over the waves of a block
     // of 128 channels through LDS; codes staged in the ring
     constexpr int JN = SWIGLU ? 2 : 4, BW = 128 / CHW;  // BW waves share a block
-    float* red = reinterpret_cast<float*>(ring);  // [WN][BM]
+    uint32_t* red = reinterpret_cast<uint32_t*>(ring);  // [WN][BM]
     uint8_t* stg = ring + WN * BM * 4;            // [BM][CH], 16-byte chunks swizzled by row
     static_assert(WN * BM * 4 + BM * CH <= NS * STAGE, "staging in the ring");
-    float m[FM];
+    uint32_t m[FM];
 #pragma unroll
-    for (int i = 0; i < FM; ++i) m[i] = 0.f;
+    for (int i = 0; i < FM; ++i) m[i] = 0u;
 #pragma unroll
     for (int j = 0; j < JN; ++j) {
       const int c = CHW * wn + j * 16 + 4 * q;
@@ -233,15 +238,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm_blocks(const BlockGemm
           else y = gelu_erf(acc[j][i][v] + b);
           y = in ? y : 0.f;
           acc[j][i][v] = y;
-          m[i] = nan_max(m[i], fabsf(y));
+          m[i] = amax_bits(m[i], y);
         }
       }
     }
     __syncthreads();  // every wave is done with the ring
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
-      m[i] = nan_max(m[i], __shfl_xor(m[i], 16));
-      m[i] = nan_max(m[i], __shfl_xor(m[i], 32));
+      m[i] = quarters_max(m[i]);
       if (q == 0) red[wn * BM + wm * TM + i * 16 + fr] = m[i];
     }
     __syncthreads();
@@ -249,18 +253,19 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm_blocks(const BlockGemm
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int r = wm * TM + i * 16 + fr;
-      float a = red[bw0 * BM + r];
+      uint32_t a = red[bw0 * BM + r];
 #pragma unroll
-      for (int w = 1; w < BW; ++w) a = nan_max(a, red[(bw0 + w) * BM + r]);
+      for (int w = 1; w < BW; ++w) a = max(a, red[(bw0 + w) * BM + r]);
       const float sc = block_scale(a);
+      const Divisor d = divisor(sc);
       if (wn == bw0 && q == 0 && r < mrows && n0 + CHW * wn < p.N_out)
         p.out_scale[((n0 + CHW * wn) / 128) * p.os_col + m0 + r] = sc;
 #pragma unroll
       for (int j = 0; j < JN; ++j) {
         const int c = CHW * wn + j * 16 + 4 * q;
         *reinterpret_cast<uint32_t*>(stg + r * CH + (((c >> 4) ^ (r & 7)) << 4) + (c & 15)) =
-            pack_e4m3(__fdiv_rn(acc[j][i][0], sc), __fdiv_rn(acc[j][i][1], sc),
-                      __fdiv_rn(acc[j][i][2], sc), __fdiv_rn(acc[j][i][3], sc));
+            pack_e4m3(quotient(acc[j][i][0], d), quotient(acc[j][i][1], d), quotient(acc[j][i][2], d),
+                      quotient(acc[j][i][3], d));
       }
     }
     __syncthreads();

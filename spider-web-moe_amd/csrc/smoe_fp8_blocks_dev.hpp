@@ -12,21 +12,52 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 
 constexpr float kE4m3Max = 448.0f;
 
-// max that keeps a NaN once seen: a block with a NaN has a NaN scale
-__device__ __forceinline__ float nan_max(float m, float a) { return (a > m || a != a) ? a : m; }
+// Constant memory that every lane of a wave reads at one address (s_load)
+typedef const float __attribute__((address_space(4)))* uniform_f32;
+__device__ __forceinline__ uniform_f32 as_uniform(const float* p) {
+  return (uniform_f32)(reinterpret_cast<uintptr_t>(p));
+}
+
+// amax over |v| as bit patterns: the largest unsigned word is the largest
+// magnitude, NaN above infinity above the rest, so a block with a NaN has a NaN
+// scale.
+__device__ __forceinline__ uint32_t amax_bits(uint32_t m, float v) {
+  return max(m, __float_as_uint(v) & 0x7FFFFFFFu);
+}
 // ... over the 16 lanes of a DPP row
-__device__ __forceinline__ float row16_nan_max(float v) {
-  v = nan_max(v, dpp_f<kDppXor1>(v));
-  v = nan_max(v, dpp_f<kDppXor2>(v));
-  v = nan_max(v, dpp_f<kDppHalfMirror>(v));
-  v = nan_max(v, dpp_f<kDppMirror>(v));
+__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
+  v = max(v, static_cast<uint32_t>(dpp_i<kDppXor1>(static_cast<int>(v))));
+  v = max(v, static_cast<uint32_t>(dpp_i<kDppXor2>(static_cast<int>(v))));
+  v = max(v, static_cast<uint32_t>(dpp_i<kDppHalfMirror>(static_cast<int>(v))));
+  v = max(v, static_cast<uint32_t>(dpp_i<kDppMirror>(static_cast<int>(v))));
   return v;
+}
+// ... over lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ uint32_t quarters_max(uint32_t v) {
+  v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 16)));
+  return max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), 32)));
 }
 
 // scale = max(amax / 448, 1e-12), the quotient an IEEE one; a NaN stays
-__device__ __forceinline__ float block_scale(float amax) {
-  const float s = __fdiv_rn(amax, kE4m3Max);
+__device__ __forceinline__ float block_scale(uint32_t amax) {
+  const float s = __fdiv_rn(__uint_as_float(amax), kE4m3Max);
   return s < 1e-12f ? 1e-12f : s;
+}
+
+// Quotients by one divisor, correctly rounded: with r the correctly rounded
+// reciprocal and q0 = x r, the residual e = x - q0 s is exact and q0 + e r
+// rounds to x / s (P. Markstein, IBM J. Res. Dev. 34, 1990), where neither q0
+// nor e underflows; below, the code is 0 either way.  4 operations for an
+// IEEE division's 12.  s = infinity: 0 for finite x, NaN for infinite x.
+struct Divisor {
+  float r, s;
+};
+__device__ __forceinline__ Divisor divisor(float s) {
+  return {__fdiv_rn(1.0f, s), s == INFINITY ? 0.0f : s};
+}
+__device__ __forceinline__ float quotient(float x, Divisor d) {
+  const float q = mul_rn(x, d.r);
+  return copysignf(fmaf(fmaf(-q, d.s, x), d.r, q), x);  // x = -0 keeps its sign
 }
 
 // Four e4m3 codes of values that a block's scale has brought to +-448 (plus
@@ -77,17 +108,18 @@ __device__ __forceinline__ void load_cols8(const void* row, int c, int cols, boo
 template <int XDT>
 constexpr int elt_bytes() { return XDT == SMOE_F32 ? 4 : 2; }
 
-__device__ __forceinline__ float amax8(const float (&v)[8]) {
-  float m = 0.f;
+__device__ __forceinline__ uint32_t amax8(const float (&v)[8]) {
+  uint32_t m = 0u;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) m = nan_max(m, fabsf(v[j]));
+  for (int j = 0; j < 8; ++j) m = amax_bits(m, v[j]);
   return m;
 }
 
 __device__ __forceinline__ u32x2 codes8(const float (&v)[8], float sc) {
+  const Divisor d = divisor(sc);
   float q[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) q[j] = __fdiv_rn(v[j], sc);
+  for (int j = 0; j < 8; ++j) q[j] = quotient(v[j], d);
   return u32x2{pack_e4m3(q[0], q[1], q[2], q[3]), pack_e4m3(q[4], q[5], q[6], q[7])};
 }
 
@@ -104,7 +136,7 @@ __device__ __forceinline__ void quant_row_block(const BlockQuant& q, int nblk, i
   const bool vec = (reinterpret_cast<uintptr_t>(q.x) | static_cast<uintptr_t>(q.ldx * elt_bytes<XDT>())) % 16 == 0;
   float v[8];
   load_cols8<XDT>(rp, c, q.cols, vec, v);
-  const float sc = block_scale(row16_nan_max(amax8(v)));
+  const float sc = block_scale(row16_max(amax8(v)));
   if (b >= total) return;
   if (l16 == 0) q.scale[row * q.s_row + kb * q.s_col] = sc;
   if (c < q.ld_out) *reinterpret_cast<u32x2*>(q.codes + row * q.ld_out + c) = codes8(v, sc);

@@ -62,6 +62,7 @@ void k_blocks_few(const BlockGemm p) {
   constexpr int D = MT == 1 ? (SWIGLU ? 3 : 4) : (WIDE || SWIGLU ? 2 : 3);
   static_assert(!UP || NT == (SWIGLU ? 2 : 1), "one or two weight tiles a wave");
   __shared__ __attribute__((aligned(16))) float red[UP ? 8 * BM : NW * MT * NT * 64 * 4];
+  uint32_t* const redm = reinterpret_cast<uint32_t*>(red);  // UP: amax bits [8][BM]
   extern __shared__ __attribute__((aligned(16))) uint8_t xlds[];  // XQ >= 0
   int g, m0, mrows, n0;
   if (!block_tile<BM, BN>(p, blockIdx.x, g, m0, mrows, n0)) return;  // uniform
@@ -124,7 +125,7 @@ void k_blocks_few(const BlockGemm p) {
           const bool vec = (reinterpret_cast<uintptr_t>(p.x_float) | static_cast<uintptr_t>(p.ld_float * elt_bytes<XD>())) % 16 == 0;
           float v[8];
           load_cols8<XD>(rp, 128 * b + 8 * l16, p.K, vec, v);
-          const float sc = block_scale(row16_nan_max(amax8(v)));
+          const float sc = block_scale(row16_max(amax8(v)));
           if (l16 == 0) xsl[b * BM + r] = sc;
           *reinterpret_cast<u32x2*>(xlds + r * ldl + 128 * b + 8 * l16) = codes8(v, sc);
         }
@@ -173,7 +174,7 @@ void k_blocks_few(const BlockGemm p) {
     float y[MT][4];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      float m = 0.f;
+      uint32_t m = 0u;
 #pragma unroll
       for (int v = 0; v < 4; ++v) {
         const bool in = c + v < p.N_out;
@@ -182,25 +183,25 @@ void k_blocks_few(const BlockGemm p) {
         if constexpr (SWIGLU) t = silu(acc[0][i][v]) * (acc[NT - 1][i][v] + b);
         else t = gelu_erf(acc[0][i][v] + b);
         y[i][v] = in ? t : 0.f;
-        m = nan_max(m, fabsf(y[i][v]));
+        m = amax_bits(m, y[i][v]);
       }
-      m = nan_max(m, __shfl_xor(m, 16));
-      m = nan_max(m, __shfl_xor(m, 32));
-      if (q == 0) red[wave * BM + 16 * i + l16] = m;
+      m = quarters_max(m);
+      if (q == 0) redm[wave * BM + 16 * i + l16] = m;
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
       const int r = 16 * i + l16;
-      float a = red[r];
+      uint32_t a = redm[r];
 #pragma unroll
-      for (int w = 1; w < 8; ++w) a = nan_max(a, red[w * BM + r]);
+      for (int w = 1; w < 8; ++w) a = max(a, redm[w * BM + r]);
       const float sc = block_scale(a);
+      const Divisor dv = divisor(sc);
       if (r >= mrows) continue;
       if (wave == 0 && q == 0) p.out_scale[(n0 / 128) * p.os_col + m0 + r] = sc;
       if (c < p.N_out)  // N_out % 16 == 0: four channels of one side
         *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out) + static_cast<int64_t>(m0 + r) * p.ldo + c) =
-            pack_e4m3(__fdiv_rn(y[i][0], sc), __fdiv_rn(y[i][1], sc), __fdiv_rn(y[i][2], sc), __fdiv_rn(y[i][3], sc));
+            pack_e4m3(quotient(y[i][0], dv), quotient(y[i][1], dv), quotient(y[i][2], dv), quotient(y[i][3], dv));
     }
   } else {
 #pragma unroll
