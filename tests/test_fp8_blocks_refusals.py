@@ -57,7 +57,7 @@ def test_quantizer_refusals(lib):
 def test_linear_refusals(lib):
     from spider_moe_amd import _native as nat
 
-    def go(x=FAKE, dt=nat.BF16, ldx=100, xs=None, n=4, k=100, w=FAKE, ldw=112, ws=FAKE, no=30, act=0, out=FAKE,
+    def go(x=FAKE, dt=nat.BF16, ldx=100, xs=None, n=40, k=100, w=FAKE, ldw=112, ws=FAKE, no=30, act=0, out=FAKE,
            od=nat.BF16, wk=FAKE, wb=1 << 20):
         return lib.smoe_linear_fp8_blocks(x, dt, ldx, xs, n, k, w, ldw, ws, None, no, act, out, od, wk, wb, None)
 
@@ -67,9 +67,11 @@ def test_linear_refusals(lib):
                 dict(wk=FAKE + 1), dict(dt=nat.FP8_E4M3, ldx=112), dict(dt=nat.FP8_E4M3, ldx=100, xs=FAKE),
                 dict(dt=nat.FP8_E4M3, ldx=112, xs=FAKE, x=FAKE + 2)):
         assert go(**bad) == 1, bad
-    need = lib.smoe_linear_fp8_blocks_workspace_bytes(4, 100)
-    assert need >= 4 * 112 + 4 * 4 and go(wb=need - 1) == 3
+    need = lib.smoe_linear_fp8_blocks_workspace_bytes(40, 100)
+    assert need >= 40 * 112 + 40 * 4 and go(wb=need - 1) == 3
     assert go(n=0) == 0
+    # a few rows are quantized by the product itself
+    assert lib.smoe_linear_fp8_blocks_workspace_bytes(4, 100) == 0
     assert lib.smoe_linear_fp8_blocks_workspace_bytes(0, 100) == 0
 
 
