@@ -1582,7 +1582,9 @@ ExpertsWs experts_ws(const smoe_experts_fp8_blocks& ex, int N, int K) {
 }  // namespace
 
 SMOE_API size_t smoe_expert_delta_fp8_blocks_workspace_bytes(const smoe_experts_fp8_blocks* ex, int N, int K) {
-  return check_experts_fp8_blocks(ex, N, K) != SMOE_OK ? 0 : experts_ws(*ex, N, K).total;
+  if (check_experts_fp8_blocks(ex, N, K) != SMOE_OK) return 0;
+  if (N > 0 && tokens_fit(N, K, ex->H, ex->U)) return align_up(static_cast<size_t>(N) * K * ex->U * 4);
+  return experts_ws(*ex, N, K).total;
 }
 
 SMOE_API int smoe_expert_delta_fp8_blocks(const smoe_experts_fp8_blocks* ex, const void* msg, int msg_dtype,
@@ -1595,9 +1597,33 @@ SMOE_API int smoe_expert_delta_fp8_blocks(const smoe_experts_fp8_blocks* ex, con
   if (N == 0) return SMOE_OK;
   if (!msg || !idx || !w || !delta || !ws) return fail(SMOE_EINVAL, "null buffer");
   if (!aligned16(ws)) return fail(SMOE_EINVAL, "workspace must be 16-byte aligned");
-  const ExpertsWs l = experts_ws(*ex, N, K);
-  if (ws_bytes < l.total) return fail(SMOE_ECAPACITY, "workspace");
+  if (ws_bytes < smoe_expert_delta_fp8_blocks_workspace_bytes(ex, N, K)) return fail(SMOE_ECAPACITY, "workspace");
   hipStream_t s = static_cast<hipStream_t>(stream);
+  if (tokens_fit(N, K, ex->H, ex->U)) {
+    TokensArgs t;
+    t.msg = msg;
+    t.msg_dtype = msg_dtype;
+    t.idx = idx;
+    t.w = w;
+    t.N = N;
+    t.K = K;
+    t.E = ex->E;
+    t.H = ex->H;
+    t.U = ex->U;
+    t.act_fn = ex->act;
+    t.w_up = ex->w_up;
+    t.w_down = ex->w_down;
+    t.s_up = ex->s_up;
+    t.s_down = ex->s_down;
+    t.b_up = ex->b_up;
+    t.b_down = ex->b_down;
+    t.act = static_cast<float*>(ws);
+    t.out = delta;
+    t.out_dtype = out_dtype;
+    SMOE_TRY(launch_tokens(t, s), "expert step of a few tokens");
+    return SMOE_OK;
+  }
+  const ExpertsWs l = experts_ws(*ex, N, K);
   const int E = ex->E, H = ex->H, U = ex->U, hb = fp8_blocks_of(H), ub = fp8_blocks_of(U);
   const int halves = ex->act == SMOE_ACT_SWIGLU ? 2 : 1;
   int32_t *off = at<int32_t>(ws, l.off), *rows = at<int32_t>(ws, l.rows), *tokrow = at<int32_t>(ws, l.tokrow);

@@ -88,4 +88,21 @@ struct PrepArgs {
 bool prep_fits(int N, int K, int E);
 int launch_prep(const PrepArgs& a, const BlockQuant& q, hipStream_t s);
 
+// The expert step of a few tokens (N * K <= 16) in two launches.
+struct TokensArgs {
+  const void* msg = nullptr;  // [N, H] f32 / bf16
+  int msg_dtype = SMOE_BF16;
+  const int32_t* idx = nullptr;
+  const float* w = nullptr;
+  int N = 0, K = 0, E = 0, H = 0, U = 0;
+  int act_fn = SMOE_ACT_GELU;
+  const uint8_t *w_up = nullptr, *w_down = nullptr;
+  const float *s_up = nullptr, *s_down = nullptr, *b_up = nullptr, *b_down = nullptr;
+  float* act = nullptr;  // f32 [N * K, U], 16-byte aligned
+  void* out = nullptr;   // [N, H]
+  int out_dtype = SMOE_BF16;
+};
+bool tokens_fit(int N, int K, int H, int U);
+int launch_tokens(const TokensArgs& a, hipStream_t s);
+
 }  // namespace smoe

@@ -229,6 +229,239 @@ void k_blocks_few(const BlockGemm p) {
   }
 }
 
+// ------------------------------------------------- a few tokens' experts ----
+// At most 16 (token, slot) entries: the whole expert step in two launches that
+// keep the dispatch plan in registers and quantize their own operands.
+//
+// The plan, by one wave, lane j = entry j (token j / K): an id's slots of one
+// token merged into the first (weights added in slot order from 0, as
+// smoe_dispatch_plan adds them), ids outside [0, E) and sums that are not > 0
+// left out.  row: the entry's place among the kept ones by (expert, token);
+// ord: how many smaller experts have rows.
+struct Entry {
+  int e, row, ord;
+  float w;
+  bool keep;
+};
+__device__ __forceinline__ Entry plan_entries(const int32_t* __restrict__ idx, const float* __restrict__ w, int NK,
+                                              int K, int E) {
+  const int j = threadIdx.x & 63;
+  const int jc = min(j, NK - 1), t = jc / K;
+  const int e = idx[jc];
+  const float wj = w[jc];
+  Entry r{e, 0, 0, 0.f, j < NK && e >= 0 && e < E};
+  for (int i = 0; i < NK; ++i) {
+    const int ei = __builtin_amdgcn_readlane(e, i);
+    const float wi = lane_f(wj, i);
+    const bool same = ei == e && i / K == t;
+    r.keep = r.keep && !(same && i < j);
+    r.w = same ? r.w + wi : r.w;
+  }
+  r.keep = r.keep && r.w > 0.f;
+  const uint64_t kept = __ballot(r.keep);
+  bool lead = r.keep;  // the expert's first kept entry
+  for (int i = 0; i < NK; ++i) {
+    const int ei = __builtin_amdgcn_readlane(e, i);
+    const bool k = kept >> i & 1;
+    lead = lead && !(k && ei == e && i < j);
+    r.row += k && (ei < e || (ei == e && i < j)) ? 1 : 0;
+  }
+  const uint64_t leads = __ballot(lead);
+  for (int i = 0; i < NK; ++i)
+    r.ord += (leads >> i & 1) && __builtin_amdgcn_readlane(e, i) < e ? 1 : 0;
+  return r;
+}
+
+constexpr int kTokensMax = 16;  // entries (and so tokens, experts and rows)
+
+// Up product of one expert's rows and 16 channels (SwiGLU: of gate and up):
+// four waves take every fourth block of K, the rows' messages are quantized
+// into LDS under the first weights' loads; activations leave in f32 at their
+// plan rows.
+template <bool SWIGLU, int XDT>
+__global__ __launch_bounds__(256, 4) void k_tokens_up(const TokensArgs a) {
+  constexpr int NT = SWIGLU ? 2 : 1, D = SWIGLU ? 3 : 4;
+  __shared__ __attribute__((aligned(16))) float red[4 * NT * 256];
+  __shared__ int s_tok[kTokensMax];
+  extern __shared__ __attribute__((aligned(16))) uint8_t xlds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int q = lane >> 4, l16 = lane & 15;
+  const int NK = a.N * a.K, strips = (a.U + 15) / 16;
+  const int o = blockIdx.x / strips, n0 = (blockIdx.x - o * strips) * 16;
+  const Entry en = plan_entries(a.idx, a.w, NK, a.K, a.E);
+  const bool mine = en.keep && en.ord == o;
+  const uint64_t mask = __ballot(mine);
+  if (!mask) return;  // uniform: fewer experts than that have rows
+  const int f = __builtin_ctzll(mask);
+  const int e = __builtin_amdgcn_readlane(en.e, f), row0 = __builtin_amdgcn_readlane(en.row, f);
+  const int rows = __popcll(mask);  // <= N <= kTokensMax
+  if (wave == 0 && mine) s_tok[en.row - row0] = lane / a.K;
+
+  const int KB = (a.H + 127) / 128, ldl = KB * 128;
+  float* const xsl = reinterpret_cast<float*>(xlds + a.N * ldl);  // [KB][N]
+  const uint8_t* wrow[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+    wrow[j] = a.w_up + (static_cast<int64_t>(e) * NT * a.U + j * a.U + n0 + l16) * a.H;  // U % 16 == 0
+  const int ub = (a.U + 127) / 128;
+  const float* wsp = a.s_up + (static_cast<int64_t>(e) * NT * ub + n0 / 128) * KB;
+  f32x4 acc[NT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  bool first = true;
+  for (int b0 = wave; b0 < KB || first; b0 += 4 * D) {
+    Piece w[D][NT];
+    float ws[D][NT];
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      const int b = min(b0 + 4 * d, KB - 1);  // past the end: the last block again, not used
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        w[d][j] = load_piece(wrow[j], 128 * b, q, a.H);
+        ws[d][j] = wsp[j * ub * KB + b];
+      }
+    }
+    if (first) {
+      __syncthreads();  // s_tok
+      const bool vec = (reinterpret_cast<uintptr_t>(a.msg) | static_cast<uintptr_t>(a.H) * elt_bytes<XDT>()) % 16 == 0;
+      for (int i = tid >> 4; i < rows * KB; i += 16) {
+        const int r = i / KB, b = i - r * KB;
+        const char* rp = reinterpret_cast<const char*>(a.msg) + static_cast<int64_t>(s_tok[r]) * a.H * elt_bytes<XDT>();
+        float v[8];
+        load_cols8<XDT>(rp, 128 * b + 8 * l16, a.H, vec, v);
+        const float sc = block_scale(row16_max(amax8(v)));
+        if (l16 == 0) xsl[b * a.N + r] = sc;
+        *reinterpret_cast<u32x2*>(xlds + r * ldl + 128 * b + 8 * l16) = codes8(v, sc);
+      }
+      __syncthreads();
+      first = false;
+    }
+    const int r = min(l16, rows - 1);
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      const int b = b0 + 4 * d;
+      if (b >= KB) break;  // uniform
+      const Piece x = load_piece(xlds + r * ldl, 128 * b, q, ldl);
+      const float xs = xsl[b * a.N + r];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        if (a.H - 128 * b < 128) w[d][j] = cut_piece(w[d][j], q, a.H - 128 * b);
+        const f32x4 part = block_product<false>(w[d][j], x);
+        const float sc = xs * ws[d][j];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) acc[j][v] = fmaf(part[v], sc, acc[j][v]);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j) *reinterpret_cast<f32x4*>(red + (wave * NT + j) * 256 + lane * 4) = acc[j];
+  __syncthreads();
+  if (wave > 0 || l16 >= rows) return;
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int u = 1; u < 4; ++u) acc[j] += *reinterpret_cast<const f32x4*>(red + (u * NT + j) * 256 + lane * 4);
+  const int c = n0 + 4 * q;
+  f32x4 y;
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    const float b = a.b_up ? a.b_up[static_cast<int64_t>(e) * a.U + c + v] : 0.f;
+    y[v] = SWIGLU ? silu(acc[0][v]) * (acc[NT - 1][v] + b) : gelu_erf(acc[0][v] + b);
+  }
+  *reinterpret_cast<f32x4*>(a.act + static_cast<int64_t>(row0 + l16) * a.U + c) = y;
+}
+
+// Down products of every expert that has rows, 16 channels a workgroup, added
+// over the experts as they are multiplied: a tile's 16 columns are the tokens,
+// a token's column holds its row of the expert at hand (a token without one
+// leaves its sum as it is) and its weight goes into the scale.  Eight waves
+// take every eighth (expert, block of K), their sums added in wave order.
+template <int ODT>
+__global__ __launch_bounds__(512, 4) void k_tokens_down(const TokensArgs a) {
+  constexpr int D = 4;
+  __shared__ __attribute__((aligned(16))) float red[8 * 256];
+  __shared__ int s_row[kTokensMax * kTokensMax], s_exp[kTokensMax];
+  __shared__ float s_w[kTokensMax * kTokensMax];
+  extern __shared__ __attribute__((aligned(16))) uint8_t xlds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int q = lane >> 4, l16 = lane & 15;
+  const int NK = a.N * a.K, n0 = blockIdx.x * 16;
+  const Entry en = plan_entries(a.idx, a.w, NK, a.K, a.E);
+  const int rows = __popcll(__ballot(en.keep));
+  int experts = 0;
+  for (int i = 0; i < NK; ++i) {
+    const int k = __builtin_amdgcn_readlane(en.keep ? en.ord + 1 : 0, i);
+    experts = max(experts, k);
+  }
+  for (int i = tid; i < kTokensMax * kTokensMax; i += 512) s_row[i] = -1;
+  __syncthreads();
+  if (wave == 0 && en.keep) {
+    const int at = en.ord * kTokensMax + lane / a.K;
+    s_row[at] = en.row;
+    s_w[at] = en.w;
+    s_exp[en.ord] = en.e;  // equal from every entry of the expert
+  }
+  const int KB = (a.U + 127) / 128, ldl = KB * 128, hb = (a.H + 127) / 128;
+  float* const xsl = reinterpret_cast<float*>(xlds + rows * ldl);  // [KB][rows]
+  const bool vec = reinterpret_cast<uintptr_t>(a.act) % 16 == 0;  // U % 16 == 0
+  for (int i = tid >> 4; i < rows * KB; i += 32) {
+    const int r = i / KB, b = i - r * KB;
+    float v[8];
+    load_cols8<SMOE_F32>(a.act + static_cast<int64_t>(r) * a.U, 128 * b + 8 * l16, a.U, vec, v);
+    const float sc = block_scale(row16_max(amax8(v)));
+    if (l16 == 0) xsl[b * rows + r] = sc;
+    *reinterpret_cast<u32x2*>(xlds + r * ldl + 128 * b + 8 * l16) = codes8(v, sc);
+  }
+  __syncthreads();
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const int items = experts * KB;
+  for (int i0 = wave; i0 < items; i0 += 8 * D) {
+    Piece w[D];
+    float ws[D];
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      const int i = min(i0 + 8 * d, items - 1), o = i / KB, b = i - o * KB;
+      const int64_t e = s_exp[o];
+      w[d] = load_piece(a.w_down + (e * a.H + n0 + l16) * a.U, 128 * b, q, a.U);  // H % 16 == 0
+      ws[d] = a.s_down[(e * hb + n0 / 128) * KB + b];
+    }
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      const int i = i0 + 8 * d;
+      if (i >= items) break;  // uniform
+      const int o = i / KB, b = i - o * KB;
+      const int r = s_row[o * kTokensMax + l16], rc = max(r, 0);
+      if (a.U - 128 * b < 128) w[d] = cut_piece(w[d], q, a.U - 128 * b);
+      const f32x4 part = block_product<false>(w[d], load_piece(xlds + rc * ldl, 128 * b, q, ldl));
+      const float sc = xsl[b * rows + rc] * ws[d] * s_w[o * kTokensMax + l16];
+#pragma unroll
+      for (int v = 0; v < 4; ++v) acc[v] = r >= 0 ? fmaf(part[v], sc, acc[v]) : acc[v];
+    }
+  }
+  *reinterpret_cast<f32x4*>(red + wave * 256 + lane * 4) = acc;
+  __syncthreads();
+  if (wave > 0 || l16 >= a.N) return;
+#pragma unroll
+  for (int u = 1; u < 8; ++u) acc += *reinterpret_cast<const f32x4*>(red + u * 256 + lane * 4);
+  const int n = n0 + 4 * q;
+  if (a.b_down)
+    for (int o = 0; o < experts; ++o) {
+      const int at = o * kTokensMax + l16;
+      if (s_row[at] < 0) continue;
+#pragma unroll
+      for (int v = 0; v < 4; ++v)
+        acc[v] = fmaf(a.b_down[static_cast<int64_t>(s_exp[o]) * a.H + n + v], s_w[at], acc[v]);
+    }
+  const int64_t at = static_cast<int64_t>(l16) * a.H + n;
+  if constexpr (ODT == SMOE_F32) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) reinterpret_cast<float*>(a.out)[at + v] = acc[v];
+  } else {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) reinterpret_cast<uint16_t*>(a.out)[at + v] = f2bf(acc[v]);
+  }
+}
+
 // The merged slots of one token (merge_token's result) from registers: the
 // ids that occur, ascending, each with its slots' weights added in slot order
 // from 0; ids outside [0, E) and sums that are not > 0 left out, -1 padded.
@@ -377,6 +610,30 @@ int launch_prep(const PrepArgs& args, const BlockQuant& q, hipStream_t s) {
   else if (a.K <= 4) hipLaunchKernelGGL((k_prep<4>), grid, block, 0, s, a, q, nblk, total);
   else if (a.K <= 8) hipLaunchKernelGGL((k_prep<8>), grid, block, 0, s, a, q, nblk, total);
   else hipLaunchKernelGGL((k_prep<16>), grid, block, 0, s, a, q, nblk, total);
+  return rc();
+}
+
+// LDS of the two launches: quantized rows of up to N messages or N * K
+// activations, and their scales
+constexpr int64_t kTokensLds = 49152;
+
+bool tokens_fit(int N, int K, int H, int U) {
+  return N * static_cast<int64_t>(K) <= kTokensMax && static_cast<int64_t>(N) * fp8_blocks_of(H) * 132 <= kTokensLds &&
+         static_cast<int64_t>(N) * K * fp8_blocks_of(U) * 132 <= kTokensLds;
+}
+
+int launch_tokens(const TokensArgs& a, hipStream_t s) {
+  const dim3 up(static_cast<unsigned>(std::min(a.E, a.N * a.K) * ((a.U + 15) / 16)));
+  const size_t lds_up = static_cast<size_t>(a.N) * fp8_blocks_of(a.H) * 132;
+  const size_t lds_down = static_cast<size_t>(a.N) * a.K * fp8_blocks_of(a.U) * 132;
+  const bool sw = a.act_fn == SMOE_ACT_SWIGLU, f32 = a.msg_dtype == SMOE_F32;
+  if (sw && f32) hipLaunchKernelGGL((k_tokens_up<true, SMOE_F32>), up, dim3(256), lds_up, s, a);
+  else if (sw) hipLaunchKernelGGL((k_tokens_up<true, SMOE_BF16>), up, dim3(256), lds_up, s, a);
+  else if (f32) hipLaunchKernelGGL((k_tokens_up<false, SMOE_F32>), up, dim3(256), lds_up, s, a);
+  else hipLaunchKernelGGL((k_tokens_up<false, SMOE_BF16>), up, dim3(256), lds_up, s, a);
+  const dim3 down(static_cast<unsigned>((a.H + 15) / 16));
+  if (a.out_dtype == SMOE_F32) hipLaunchKernelGGL((k_tokens_down<SMOE_F32>), down, dim3(512), lds_down, s, a);
+  else hipLaunchKernelGGL((k_tokens_down<SMOE_BF16>), down, dim3(512), lds_down, s, a);
   return rc();
 }
 
