@@ -6,6 +6,9 @@
 #include "smoe_internal.hpp"
 
 namespace smoe {
+
+int device_cus();
+
 namespace {
 
 // 1 x 128 blocks (quant_row_block), sixteen a workgroup.
@@ -65,11 +68,12 @@ template <int EPI, int ODT, bool WIDE, int BM, int BN, int WM, int WN, int NS>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm_blocks(const BlockGemm p) {
   constexpr bool SWIGLU = EPI == BLK_UP_SWIGLU, UP = EPI == BLK_UP_GELU || SWIGLU;
   constexpr int NW = WM * WN, CH = SWIGLU ? BN / 2 : BN, CHW = CH / WN, TM = BM / WM, FM = TM / 16;
-  static_assert(BN == 64 * WN && TM % 16 == 0 && (BM == 128 || BM == 256), "wave tile: 64 weight rows");
+  static_assert(BN == 64 * WN && TM % 16 == 0 && (BM == 32 || BM == 64 || BM == 128 || BM == 256), "wave tile: 64 weight rows");
   static_assert(!UP || CH % 128 == 0, "activations are quantized in blocks of 128 channels");
-  constexpr int XB = BM * 128, WB = BN * 128, STAGE = XB + WB + BM * 4;
-  constexpr int X_LD = BM / 8 / NW, W_LD = BN / 8 / NW, LD = X_LD + W_LD + 1;
-  static_assert(X_LD * NW * 8 == BM && W_LD * NW * 8 == BN && NW % (BM / 64) == 0, "whole DMA instructions");
+  constexpr int XB = BM * 128, WB = BN * 128, SR = BM < 64 ? 64 : BM, STAGE = XB + WB + SR * 4;
+  constexpr int XI = BM / 8;  // DMA instructions of a stage's rows (fewer than waves: some load the same)
+  constexpr int X_LD = (XI + NW - 1) / NW, W_LD = BN / 8 / NW, LD = X_LD + W_LD + 1;
+  static_assert((XI % NW == 0 || NW % XI == 0) && W_LD * NW * 8 == BN && NW % (SR / 64) == 0, "whole DMA instructions");
   __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * STAGE];
   int g, m0, mrows, n0;
   if (!block_tile<BM, CH>(p, blockIdx.x, g, m0, mrows, n0)) return;  // uniform
@@ -87,7 +91,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm_blocks(const BlockGemm
   const uint8_t* wsrc[W_LD];
 #pragma unroll
   for (int j = 0; j < X_LD; ++j) {
-    const int pr = m0 + min(8 * (NW * j + wave) + (lane >> 3), mrows - 1);  // rows past the end: a valid one, never stored
+    const int pr = m0 + min(8 * ((NW * j + wave) % XI) + (lane >> 3), mrows - 1);  // rows past the end: a valid one, never stored
     xsrc[j] = p.X + static_cast<int64_t>(p.a_rows ? p.a_rows[pr] : pr) * p.ldx;
   }
 #pragma unroll
@@ -97,21 +101,21 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm_blocks(const BlockGemm
     const int64_t row = min(ch, p.N_out - 1) + (SWIGLU && (r & 32) ? p.N_out : 0);
     wsrc[j] = p.W + g * p.w_gstride + row * p.ldw;
   }
-  // the rows' scales: wave w loads rows 64 (w % (BM / 64)) .. + 63
-  const int sw = wave % (BM / 64);
+  // the rows' scales: wave w loads rows 64 (w % (SR / 64)) .. + 63
+  const int sw = wave % (SR / 64);
   const int spr = m0 + min(64 * sw + lane, mrows - 1);
   const float* ssrc = p.xs + static_cast<int64_t>(p.a_rows ? p.a_rows[spr] : spr) * p.xs_row;
-  auto issue = [&](int s) {
+  // DMA d of stage s: X_LD of rows, W_LD of weights, one of the rows' scales
+  auto issue_one = [&](int s, int d) {
     uint8_t* base = ring + (s % NS) * STAGE;
-    const int k0 = s * 128;
-    const int at = k0 + cl < p.K ? k0 + cl : 0;  // chunks past K: the row's first one, cut before use
-#pragma unroll
-    for (int j = 0; j < X_LD; ++j)
-      __builtin_amdgcn_global_load_lds((gbl_vptr)(xsrc[j] + at), (lds_vptr)(base + (NW * j + wave) * 1024), 16, 0, 0);
-#pragma unroll
-    for (int j = 0; j < W_LD; ++j)
-      __builtin_amdgcn_global_load_lds((gbl_vptr)(wsrc[j] + at), (lds_vptr)(base + XB + (NW * j + wave) * 1024), 16, 0, 0);
-    __builtin_amdgcn_global_load_lds((gbl_vptr)(ssrc + s * p.xs_col), (lds_vptr)(base + XB + WB + 256 * sw), 4, 0, 0);
+    const int at = s * 128 + cl < p.K ? s * 128 + cl : 0;  // chunks past K: the row's first one, cut before use
+    if (d < X_LD)
+      __builtin_amdgcn_global_load_lds((gbl_vptr)(xsrc[d < X_LD ? d : 0] + at), (lds_vptr)(base + (NW * d + wave) % XI * 1024), 16, 0, 0);
+    else if (d < X_LD + W_LD)
+      __builtin_amdgcn_global_load_lds((gbl_vptr)(wsrc[d >= X_LD && d < X_LD + W_LD ? d - X_LD : 0] + at),
+                                       (lds_vptr)(base + XB + (NW * (d - X_LD) + wave) * 1024), 16, 0, 0);
+    else
+      __builtin_amdgcn_global_load_lds((gbl_vptr)(ssrc + s * p.xs_col), (lds_vptr)(base + XB + WB + 256 * sw), 4, 0, 0);
   };
   const int fr = lane & 15, q = lane >> 4;
   // fragment of 16 rows from tile row 16 t on: row fr, chunks q and q + 4 (both
@@ -143,21 +147,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm_blocks(const BlockGemm
   float nw0 = wsc[0], nw1 = SWIGLU ? wsc_up[0] : 0.f;
 #pragma unroll
   for (int s = 0; s < NS - 1; ++s)
-    if (s < KB) issue(s);
-  for (int s = 0; s < KB; ++s) {
-    // own part of stage s landed (the later ones may be on their way); after
-    // the barrier everybody's, and nobody reads stage s - 1 any more
-    if (NS > 2 && s + NS - 2 < KB) wait_vmcnt<(NS - 2) * LD>();
-    else wait_vmcnt<0>();
-    wait_lgkm0();
-    __builtin_amdgcn_s_barrier();
-    if (s + NS - 1 < KB) issue(s + NS - 1);  // into the slot of stage s - 1
+    if (s < KB) {
+#pragma unroll
+      for (int d = 0; d < LD; ++d) issue_one(s, d);
+    }
+  // stage s, whose part of the ring holds for every wave when it is called;
+  // `more`: stage s + NS - 1 is requested meanwhile
+  auto stage = [&](int s, auto more) {
     uint8_t* sx = ring + (s % NS) * STAGE;
     const float* sc = reinterpret_cast<const float*>(sx + XB + WB) + wm * TM;
-    if (p.K - s * 128 < 128) {  // uniform: the last stage of a ragged K
-      cut_stage(sx, BM + BN, p.K - s * 128, tid, NW * 64);
-      lds_barrier();
-    }
     const float w0 = nw0, w1 = nw1;
     const int ns = min(s + 1, KB - 1);
     nw0 = wsc[ns];
@@ -167,49 +165,79 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm_blocks(const BlockGemm
 #pragma unroll
     for (int j = 0; j < 4; ++j) wf[j] = frag(sx + XB + (wn * 64 + j * 16) * 128);
     auto xfrag = [&](int i) { return frag(sx + (wm * TM + i * 16) * 128); };
-    // sixteen rows at a time: the next rows' fragment is read, and the sums of
-    // the rows before enter the accumulators, under this one's products
+    // Step (i, j): the product of rows 16 i and weight rows 16 j, under it the
+    // four multiply-adds that bring the step LAG before into the accumulators
+    // and now and then a DMA of stage s + NS - 1 (into the slot of stage s - 1);
+    // the next rows' fragment is read four steps ahead.  All DMAs at the stage's
+    // start kept the matrix unit waiting about as long as its products take.
+    constexpr int LAG = 2, STEPS = 4 * FM;
     i32x8 xf = xfrag(0);
-    f32x4 part[4];
-    float s0 = 0.f, s1 = 0.f;
-    auto add = [&](int i) {
+    f32x4 part[LAG + 1];
+    float s0[2], s1[2];  // the scales of rows 16 i: [i % 2]
+    auto add = [&](int t) {
+      const int i = t / 4, j = t % 4;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int v = 0; v < 4; ++v)
-          acc[j][i][v] = fmaf(part[j][v], SWIGLU && j >= 2 ? s1 : s0, acc[j][i][v]);
+      for (int v = 0; v < 4; ++v)
+        acc[j][i][v] = fmaf(part[t % (LAG + 1)][v], SWIGLU && j >= 2 ? s1[i % 2] : s0[i % 2], acc[j][i][v]);
     };
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const float xsv = sc[i * 16 + fr];
       const i32x8 nx = xfrag(i + 1 < FM ? i + 1 : i);
-      f32x4 now[4];
-      if constexpr (WIDE) {
-        bf16x8 xw[4];
-        widen_frag(xf, xw);
+      bf16x8 xw[4];
+      if constexpr (WIDE) widen_frag(xf, xw);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 4; ++j) {
+        const int t = 4 * i + j;
+        f32x4 now = zero;
+        if constexpr (WIDE) {
           bf16x8 ww[4];
           widen_frag(wf[j], ww);
-          now[j] = zero;
 #pragma unroll
           for (int u = 0; u < 4; ++u)
-            now[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ww[u], xw[u], now[j], 0, 0, 0);
+            now = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ww[u], xw[u], now, 0, 0, 0);
+        } else {
+          now = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], xf, zero, 0, 0, 0, 0, 0, 0);
         }
-      } else {
+        part[t % (LAG + 1)] = now;
+        __builtin_amdgcn_sched_barrier(0);
+        if (t >= LAG) add(t - LAG);
+        if (j == LAG - 1) {  // the rows before are done with theirs at j = LAG - 1
+          s0[i % 2] = xsv * w0;
+          s1[i % 2] = xsv * w1;
+        }
+        if constexpr (decltype(more)::value) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          now[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], xf, zero, 0, 0, 0, 0, 0, 0);
+          for (int d = 0; d < LD; ++d)
+            if (d * STEPS / LD == t) issue_one(s + NS - 1, d);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      if (i > 0) add(i - 1);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) part[j] = now[j];
-      s0 = xsv * w0;
-      s1 = xsv * w1;
       xf = nx;
-      __builtin_amdgcn_sched_barrier(0);
     }
-    add(FM - 1);
+#pragma unroll
+    for (int t = STEPS - LAG; t < STEPS; ++t) add(t);
+  };
+  // own part of a stage landed (the later ones may be on their way); after the
+  // barrier everybody's, and nobody reads the stage before any more.  Two
+  // loops: a branch around each DMA made the compiler move the multiply-adds
+  // away from the products they should hide under.
+  int s = 0;
+  for (; s + NS - 1 < KB; ++s) {
+    wait_vmcnt<(NS - 2) * LD>();
+    wait_lgkm0();
+    __builtin_amdgcn_s_barrier();
+    stage(s, std::true_type{});
+  }
+  for (; s < KB; ++s) {
+    wait_vmcnt<0>();
+    wait_lgkm0();
+    __builtin_amdgcn_s_barrier();
+    if (p.K - s * 128 < 128) {  // uniform: the last stage of a ragged K
+      cut_stage(ring + (s % NS) * STAGE, BM + BN, p.K - s * 128, tid, NW * 64);
+      lds_barrier();
+    }
+    stage(s, std::false_type{});
   }
 
   // epilogue: lane holds channels 4 q + v of row fr of each 16 x 16 tile
@@ -360,14 +388,62 @@ int go_tile(const BlockGemm& a, hipStream_t s) {
   return rc();
 }
 
+// Tiles of BM rows and CH channels: over groups, as if the rows were spread
+// evenly (the host does not know the counts).
+int64_t tiles_of(const BlockGemm& a, int BM, int CH) {
+  const int64_t strips = (static_cast<int64_t>(a.N_out) + CH - 1) / CH;
+  if (a.G == 0) return (static_cast<int64_t>(a.single_rows) + BM - 1) / BM * strips;
+  const int64_t per = (static_cast<int64_t>(a.max_rows) + a.G - 1) / a.G;
+  return std::min(a.G, a.max_rows) * ((per + BM - 1) / BM) * strips;
+}
+
+// Dense products: the smallest tile that one round of the CUs covers, since a
+// tile alone on its CU takes about as long as its stages' bytes (200 x 1000 ->
+// 2800: 128 x 128 tiles 10.0 us, 32 x 64 6.6, 64 x 64 6.3); past one round 64 x
+// 128 and 128 x 128 (2048 rows: 17.0 and 15.4), whose workgroups share a CU, and
+// 256 x 256, which reads the operands least often, once it fills about two
+// thirds of the CUs (8192 x 1024 -> 5632: 72 -> 64 us; 2048 x 1000 -> 2800, 88 such
+// tiles: 15.4 -> 20.5).
 template <int EPI, int ODT, bool WIDE>
-int go_tiles(const BlockGemm& a, hipStream_t s) {
-  const int rows = a.G > 0 ? a.max_rows / a.G : a.single_rows;
+int go_dense(const BlockGemm& a, hipStream_t s) {
+  const int64_t cus = device_cus();
+  if (tiles_of(a, 32, 64) <= cus) return go_tile<EPI, ODT, WIDE, 32, 64, 2, 1, 4>(a, s);
+  if (tiles_of(a, 64, 64) <= cus) return go_tile<EPI, ODT, WIDE, 64, 64, 4, 1, 4>(a, s);
+  if (tiles_of(a, 64, 128) <= cus) return go_tile<EPI, ODT, WIDE, 64, 128, 2, 2, 3>(a, s);
   if constexpr (!WIDE) {
-    if (rows >= 512) return go_tile<EPI, ODT, WIDE, 256, 256, 2, 4, 2>(a, s);
+    if (tiles_of(a, 256, 256) * 8 >= cus * 5) return go_tile<EPI, ODT, WIDE, 256, 256, 2, 4, 2>(a, s);
   }
-  if constexpr (EPI == BLK_UP_SWIGLU) return go_tile<EPI, ODT, WIDE, 128, 256, 2, 4, 2>(a, s);
-  else return go_tile<EPI, ODT, WIDE, 128, 128, 2, 2, 2>(a, s);
+  if (tiles_of(a, 128, 128) <= cus) return go_tile<EPI, ODT, WIDE, 64, 128, 2, 2, 2>(a, s);
+  return go_tile<EPI, ODT, WIDE, 128, 128, 2, 2, 2>(a, s);
+}
+
+// Grouped products: the row tile by the rows a group has on average, smaller
+// where that leaves CUs without a tile; a third stage where a tile has its CU
+// for itself.  Whole expert steps: 32 rows up to 40 a group (64 tokens, top-2 of
+// 64: 77 us with 64-row tiles, 72 with 32, 59 with the third stage), 64 up to
+// 112 (777 tokens, top-4 of 32: 59 us with 128-row tiles, 54 with 64, 62 with
+// 32), 128 above (1500 tokens: 75, 79, 89), 256 from 512 on (12000 tokens, top-2
+// of 16 SwiGLU: 422 -> 357; 3000 tokens: 122 -> 130).
+template <int EPI>
+int go_grouped(const BlockGemm& a, hipStream_t s) {
+  constexpr int O = SMOE_F32;
+  constexpr bool SW = EPI == BLK_UP_SWIGLU;
+  const int64_t cus = device_cus(), per = (static_cast<int64_t>(a.max_rows) + a.G - 1) / a.G;
+  if (per >= 512 && tiles_of(a, 256, SW ? 128 : 256) * 8 >= cus * 5) return go_tile<EPI, O, false, 256, 256, 2, 4, 2>(a, s);
+  int BM = per <= (SW ? 28 : 40) ? 32 : (per <= 112 ? 64 : 128);
+  while (BM > 32 && tiles_of(a, BM, 128) < cus) BM /= 2;
+  if constexpr (SW) {  // 256 weight rows a stage: one workgroup a CU with two stages already
+    if (BM == 32) return go_tile<EPI, O, false, 32, 256, 2, 4, 3>(a, s);
+    if (BM == 64) return go_tile<EPI, O, false, 64, 256, 2, 4, 3>(a, s);
+    return go_tile<EPI, O, false, 128, 256, 2, 4, 2>(a, s);
+  } else {
+    const bool deep = tiles_of(a, BM, 128) <= 2 * cus;
+    if (BM == 32 && deep) return go_tile<EPI, O, false, 32, 128, 2, 2, 3>(a, s);
+    if (BM == 32) return go_tile<EPI, O, false, 32, 128, 2, 2, 2>(a, s);
+    if (BM == 64 && deep) return go_tile<EPI, O, false, 64, 128, 2, 2, 3>(a, s);
+    if (BM == 64) return go_tile<EPI, O, false, 64, 128, 2, 2, 2>(a, s);
+    return go_tile<EPI, O, false, 128, 128, 2, 2, 2>(a, s);
+  }
 }
 
 }  // namespace
@@ -403,11 +479,11 @@ int launch_gemm_fp8_blocks(const BlockGemm& a, hipStream_t s) {
   if (a.x_float) return SMOE_EINVAL;
   const bool f32 = a.out_dtype == SMOE_F32;
   switch (a.epi) {
-    case BLK_LINEAR: return f32 ? go_tiles<BLK_LINEAR, SMOE_F32, true>(a, s) : go_tiles<BLK_LINEAR, SMOE_BF16, false>(a, s);
-    case BLK_GELU: return f32 ? go_tiles<BLK_GELU, SMOE_F32, true>(a, s) : go_tiles<BLK_GELU, SMOE_BF16, false>(a, s);
-    case BLK_UP_GELU: return go_tiles<BLK_UP_GELU, SMOE_F32, false>(a, s);
-    case BLK_UP_SWIGLU: return go_tiles<BLK_UP_SWIGLU, SMOE_F32, false>(a, s);
-    case BLK_DOWN: return go_tiles<BLK_DOWN, SMOE_F32, false>(a, s);
+    case BLK_LINEAR: return f32 ? go_dense<BLK_LINEAR, SMOE_F32, true>(a, s) : go_dense<BLK_LINEAR, SMOE_BF16, false>(a, s);
+    case BLK_GELU: return f32 ? go_dense<BLK_GELU, SMOE_F32, true>(a, s) : go_dense<BLK_GELU, SMOE_BF16, false>(a, s);
+    case BLK_UP_GELU: return go_grouped<BLK_UP_GELU>(a, s);
+    case BLK_UP_SWIGLU: return go_grouped<BLK_UP_SWIGLU>(a, s);
+    case BLK_DOWN: return go_grouped<BLK_DOWN>(a, s);
     default: return SMOE_EINVAL;
   }
 }

@@ -68,7 +68,7 @@ struct BlockGemm {
   int64_t os_col = 0;
 };
 int launch_gemm_fp8_blocks(const BlockGemm& g, hipStream_t s);
-// the products of a few rows per group (smoe_fp8_blocks_few.hip)
+// the dense products of a few rows (smoe_fp8_blocks_few.hip)
 bool gemm_blocks_few_fits(const BlockGemm& g);
 int launch_gemm_blocks_few(const BlockGemm& g, hipStream_t s);
 // whether a linear product of N rows takes x_float

@@ -1,7 +1,6 @@
-// Block-scaled fp8 products of a few rows per group (decode steps): the
-// weights are streamed once, each wave loading the fragments it multiplies
-// straight into registers, and what a step needs besides (dispatch plan,
-// quantized messages) comes from one launch.
+// Block-scaled fp8 steps of a few rows: dense products and expert steps whose
+// waves load the weights' fragments straight into registers, and the launch
+// that makes a decode step's plan and quantizes its messages.
 #include "smoe_fp8_blocks_dev.hpp"
 #include "smoe_internal.hpp"
 #include "smoe_routing.hpp"
@@ -44,68 +43,50 @@ __device__ __forceinline__ f32x4 block_product(const Piece& w, const Piece& x) {
   }
 }
 
-// 16 MT rows of one group.  UP: 128 channels a workgroup, 8 waves of 16
-// channels (SwiGLU: 16 gate and 16 up), each over the whole of K, whose
-// activations are quantized where they are.  Else: 16 NT channels, 4 waves
-// taking every fourth block of K, their sums added through LDS in wave order.
+// Dense products of 16 MT rows: 16 channels a workgroup, four waves taking
+// every fourth block of K straight into registers, D blocks at once; their sums
+// are added through LDS in wave order.
 //
-// XQ: -1 X is codes; else its dtype, dense rows (a.x_float, a.ld_float), which
-// the workgroup quantizes into LDS while its first weights are on their way.
-//
-// A wave loads D blocks' fragments at once and then multiplies them; what
-// hides the latency is the number of waves (UP 2, else 4 or more on a SIMD).
-template <int EPI, int ODT, bool WIDE, int MT, int NT, int XQ>
-__global__ __launch_bounds__((EPI == BLK_UP_GELU || EPI == BLK_UP_SWIGLU) ? 512 : 256, 4)
-void k_blocks_few(const BlockGemm p) {
-  constexpr bool SWIGLU = EPI == BLK_UP_SWIGLU, UP = EPI == BLK_UP_GELU || SWIGLU;
-  constexpr int BM = 16 * MT, BN = UP ? 128 : 16 * NT, NW = UP ? 8 : 4, STEP = UP ? 1 : 4;
-  constexpr int D = MT == 1 ? (SWIGLU ? 3 : 4) : (WIDE || SWIGLU ? 2 : 3);
-  static_assert(!UP || NT == (SWIGLU ? 2 : 1), "one or two weight tiles a wave");
-  __shared__ __attribute__((aligned(16))) float red[UP ? 8 * BM : NW * MT * NT * 64 * 4];
-  uint32_t* const redm = reinterpret_cast<uint32_t*>(red);  // UP: amax bits [8][BM]
+// XQ: -1 X is codes; else its dtype (x_float), which the workgroup quantizes
+// into LDS while its first weights are on their way: one launch for a few
+// tokens (1 x 2048 -> 1408: 4.8 us; quantizer and product 3 + 4.2).
+template <int EPI, int ODT, bool WIDE, int MT, int XQ>
+__global__ __launch_bounds__(256, 4) void k_blocks_few(const BlockGemm p) {
+  constexpr int BM = 16 * MT, NW = 4, D = MT == 1 ? 4 : (WIDE ? 2 : 3);
+  __shared__ __attribute__((aligned(16))) float red[NW * MT * 256];
   extern __shared__ __attribute__((aligned(16))) uint8_t xlds[];  // XQ >= 0
-  int g, m0, mrows, n0;
-  if (!block_tile<BM, BN>(p, blockIdx.x, g, m0, mrows, n0)) return;  // uniform
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int strips = (p.N_out + 15) / 16;
+  const int m0 = static_cast<int>(blockIdx.x) / strips * BM, n0 = static_cast<int>(blockIdx.x) % strips * 16;
+  const int mrows = min(BM, p.single_rows - m0);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4, l16 = lane & 15;
   const int KB = (p.K + 127) / 128;
 
-  const uint8_t* wrow[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int ch = UP ? n0 + 16 * wave + l16 : n0 + 16 * j + l16;
-    const int64_t row = min(ch, p.N_out - 1) + (SWIGLU && j ? p.N_out : 0);
-    wrow[j] = p.W + g * p.w_gstride + row * p.ldw;
-  }
+  const uint8_t* wrow = p.W + static_cast<int64_t>(min(n0 + l16, p.N_out - 1)) * p.ldw;
   const uint8_t* xrow[MT];
   const float* srow[MT];
   const int ldl = KB * 128;  // XQ: row pitch in LDS
   float* const xsl = reinterpret_cast<float*>(xlds + BM * ldl);  // [KB][BM]
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
-    const int pr = m0 + min(16 * i + l16, mrows - 1);  // rows past the end: a valid one, never stored
-    const int64_t r = XQ >= 0 ? 0 : (p.a_rows ? p.a_rows[pr] : pr);
+    const int64_t r = XQ >= 0 ? 0 : m0 + min(16 * i + l16, mrows - 1);  // rows past the end: a valid one, never stored
     xrow[i] = p.X + r * p.ldx;
     srow[i] = p.xs + r * p.xs_row;
   }
-  const float* wsp = p.ws + g * p.ws_gstride + static_cast<int64_t>(n0 / 128) * KB;
-  const float* wsp_up = wsp + static_cast<int64_t>((p.N_out + 127) / 128) * KB;  // SwiGLU
+  const float* wsp = p.ws + static_cast<int64_t>(n0 / 128) * KB;
 
-  f32x4 acc[NT][MT];
+  f32x4 acc[MT];
 #pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int i = 0; i < MT; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   bool first = true;
-  for (int b0 = UP ? 0 : wave; b0 < KB || (XQ >= 0 && first); b0 += D * STEP) {
-    Piece w[D][NT], x[D][MT];
-    float xsv[D][MT], ws0[D], ws1[D];
+  for (int b0 = wave; b0 < KB || (XQ >= 0 && first); b0 += D * NW) {
+    Piece w[D], x[D][MT];
+    float xsv[D][MT], ws[D];
 #pragma unroll
     for (int d = 0; d < D; ++d) {
-      const int b = min(b0 + d * STEP, KB - 1);  // past the end: the last block again, not used
-#pragma unroll
-      for (int j = 0; j < NT; ++j) w[d][j] = load_piece(wrow[j], 128 * b, q, p.K);
+      const int b = min(b0 + d * NW, KB - 1);  // past the end: the last block again, not used
+      w[d] = load_piece(wrow, 128 * b, q, p.K);
       if constexpr (XQ < 0) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
@@ -113,16 +94,15 @@ void k_blocks_few(const BlockGemm p) {
           xsv[d][i] = srow[i][b * p.xs_col];
         }
       }
-      ws0[d] = wsp[b];
-      ws1[d] = SWIGLU ? wsp_up[b] : 0.f;
+      ws[d] = wsp[b];
     }
     if constexpr (XQ >= 0) {
       if (first) {  // sixteen lanes quantize a block
         constexpr int XD = XQ;
+        const bool vec = (reinterpret_cast<uintptr_t>(p.x_float) | static_cast<uintptr_t>(p.ld_float * elt_bytes<XD>())) % 16 == 0;
         for (int e = tid >> 4; e < mrows * KB; e += NW * 4) {
           const int r = e / KB, b = e - r * KB;
           const char* rp = reinterpret_cast<const char*>(p.x_float) + static_cast<int64_t>(m0 + r) * p.ld_float * elt_bytes<XD>();
-          const bool vec = (reinterpret_cast<uintptr_t>(p.x_float) | static_cast<uintptr_t>(p.ld_float * elt_bytes<XD>())) % 16 == 0;
           float v[8];
           load_cols8<XD>(rp, 128 * b + 8 * l16, p.K, vec, v);
           const float sc = block_scale(row16_max(amax8(v)));
@@ -134,7 +114,7 @@ void k_blocks_few(const BlockGemm p) {
       }
 #pragma unroll
       for (int d = 0; d < D; ++d) {
-        const int b = min(b0 + d * STEP, KB - 1);
+        const int b = min(b0 + d * NW, KB - 1);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
           const int r = min(16 * i + l16, mrows - 1);
@@ -145,88 +125,42 @@ void k_blocks_few(const BlockGemm p) {
     }
 #pragma unroll
     for (int d = 0; d < D; ++d) {
-      const int b = b0 + d * STEP;
+      const int b = b0 + d * NW;
       if (b >= KB) break;  // uniform
       const int left = p.K - 128 * b;
       if (left < 128) {  // uniform: the last block of a ragged K
-#pragma unroll
-        for (int j = 0; j < NT; ++j) w[d][j] = cut_piece(w[d][j], q, left);
+        w[d] = cut_piece(w[d], q, left);
         if constexpr (XQ < 0)
 #pragma unroll
           for (int i = 0; i < MT; ++i) x[d][i] = cut_piece(x[d][i], q, left);
       }
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+      for (int i = 0; i < MT; ++i) {
+        const f32x4 part = block_product<WIDE>(w[d], x[d][i]);
+        const float sc = xsv[d][i] * ws[d];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const f32x4 part = block_product<WIDE>(w[d][j], x[d][i]);
-          const float sc = xsv[d][i] * (SWIGLU && j ? ws1[d] : ws0[d]);
-#pragma unroll
-          for (int v = 0; v < 4; ++v) acc[j][i][v] = fmaf(part[v], sc, acc[j][i][v]);
-        }
+        for (int v = 0; v < 4; ++v) acc[i][v] = fmaf(part[v], sc, acc[i][v]);
+      }
     }
   }
 
   // lane: channels 4 q + v of row l16 of each 16 x 16 tile
-  const float* bias = p.bias ? p.bias + g * p.bias_gstride : nullptr;
-  if constexpr (UP) {
-    const int c = n0 + 16 * wave + 4 * q;
-    float y[MT][4];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      uint32_t m = 0u;
+  for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4*>(red + (wave * MT + i) * 256 + lane * 4) = acc[i];
+  __syncthreads();
+  const int i = wave;  // a tile a wave
+  const int r = 16 * i + l16, n = n0 + 4 * q;
+  if (i >= MT || r >= mrows) return;
+  f32x4 sum = *reinterpret_cast<const f32x4*>(red + i * 256 + lane * 4);
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const bool in = c + v < p.N_out;
-        const float b = bias && in ? bias[c + v] : 0.f;
-        float t;
-        if constexpr (SWIGLU) t = silu(acc[0][i][v]) * (acc[NT - 1][i][v] + b);
-        else t = gelu_erf(acc[0][i][v] + b);
-        y[i][v] = in ? t : 0.f;
-        m = amax_bits(m, y[i][v]);
-      }
-      m = quarters_max(m);
-      if (q == 0) redm[wave * BM + 16 * i + l16] = m;
-    }
-    __syncthreads();
+  for (int w = 1; w < NW; ++w) sum += *reinterpret_cast<const f32x4*>(red + (w * MT + i) * 256 + lane * 4);
+  float o[4];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const int r = 16 * i + l16;
-      uint32_t a = redm[r];
-#pragma unroll
-      for (int w = 1; w < 8; ++w) a = max(a, redm[w * BM + r]);
-      const float sc = block_scale(a);
-      const Divisor dv = divisor(sc);
-      if (r >= mrows) continue;
-      if (wave == 0 && q == 0) p.out_scale[(n0 / 128) * p.os_col + m0 + r] = sc;
-      if (c < p.N_out)  // N_out % 16 == 0: four channels of one side
-        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(p.out) + static_cast<int64_t>(m0 + r) * p.ldo + c) =
-            pack_e4m3(quotient(y[i][0], dv), quotient(y[i][1], dv), quotient(y[i][2], dv), quotient(y[i][3], dv));
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-        *reinterpret_cast<f32x4*>(red + ((wave * NT + j) * MT + i) * 256 + lane * 4) = acc[j][i];
-    __syncthreads();
-    for (int t = wave; t < NT * MT; t += NW) {  // a tile a wave
-      const int j = t / MT, i = t % MT;
-      f32x4 s = *reinterpret_cast<const f32x4*>(red + t * 256 + lane * 4);
-#pragma unroll
-      for (int w = 1; w < NW; ++w) s += *reinterpret_cast<const f32x4*>(red + (w * NT * MT + t) * 256 + lane * 4);
-      const int r = 16 * i + l16, n = n0 + 16 * j + 4 * q;
-      if (r >= mrows) continue;
-      const float rs = EPI == BLK_DOWN ? p.row_scale[m0 + r] : 1.f;
-      float o[4];
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const float y = s[v] + (bias && n + v < p.N_out ? bias[n + v] : 0.f);
-        o[v] = EPI == BLK_GELU ? gelu_erf(y) : (EPI == BLK_DOWN ? y * rs : y);
-      }
-      store4<ODT>(p, m0 + r, n, o);
-    }
+  for (int v = 0; v < 4; ++v) {
+    const float y = sum[v] + (p.bias && n + v < p.N_out ? p.bias[n + v] : 0.f);
+    o[v] = EPI == BLK_GELU ? gelu_erf(y) : y;
   }
+  store4<ODT>(p, m0 + r, n, o);
 }
 
 // ------------------------------------------------- a few tokens' experts ----
@@ -546,51 +480,36 @@ __global__ __launch_bounds__(1024) void k_prep(const PrepArgs a, const BlockQuan
 
 int rc() { return hipGetLastError() == hipSuccess ? SMOE_OK : SMOE_EHIP; }
 
-template <int EPI, int ODT, bool WIDE, int MT, int NT, int XQ>
+template <int EPI, int ODT, bool WIDE, int MT, int XQ>
 int go_few(const BlockGemm& a, hipStream_t s) {
-  constexpr bool UP = EPI == BLK_UP_GELU || EPI == BLK_UP_SWIGLU;
-  constexpr int BM = 16 * MT, BN = UP ? 128 : 16 * NT;
-  const int rows = a.G > 0 ? a.max_rows : a.single_rows;
-  const int64_t tiles = (rows + BM - 1) / BM + (a.G > 0 ? std::min(a.G, rows) : 0);
-  const int64_t grid = tiles * ((a.N_out + BN - 1) / BN);
+  const int64_t grid = (static_cast<int64_t>(a.single_rows) + 16 * MT - 1) / (16 * MT) * ((static_cast<int64_t>(a.N_out) + 15) / 16);
   if (grid > 0x7fffffff) return SMOE_EINVAL;
-  const int KB = fp8_blocks_of(a.K);
-  const size_t lds = XQ >= 0 ? static_cast<size_t>(BM) * KB * 132 : 0;
-  SMOE_LAUNCH((k_blocks_few<EPI, ODT, WIDE, MT, NT, XQ>), dim3(static_cast<unsigned>(grid)), dim3(UP ? 512 : 256), lds, s, a);
+  const size_t lds = XQ >= 0 ? static_cast<size_t>(16 * MT) * fp8_blocks_of(a.K) * 132 : 0;
+  SMOE_LAUNCH((k_blocks_few<EPI, ODT, WIDE, MT, XQ>), dim3(static_cast<unsigned>(grid)), dim3(256), lds, s, a);
   return rc();
 }
 
-template <int EPI, int ODT, bool WIDE, int NT>
-int go_rows(const BlockGemm& a, int mt, hipStream_t s) {
-  if constexpr (EPI == BLK_LINEAR || EPI == BLK_GELU) {
-    if (a.x_float)
-      return by_xdt(a.x_dtype, [&](auto xd) { return go_few<EPI, ODT, WIDE, 1, NT, decltype(xd)::value>(a, s); });
-  }
-  return mt == 1 ? go_few<EPI, ODT, WIDE, 1, NT, -1>(a, s) : go_few<EPI, ODT, WIDE, 2, NT, -1>(a, s);
+template <int EPI, int ODT, bool WIDE>
+int go_rows(const BlockGemm& a, hipStream_t s) {
+  if (a.x_float) return by_xdt(a.x_dtype, [&](auto xd) { return go_few<EPI, ODT, WIDE, 1, decltype(xd)::value>(a, s); });
+  return a.single_rows <= 16 ? go_few<EPI, ODT, WIDE, 1, -1>(a, s) : go_few<EPI, ODT, WIDE, 2, -1>(a, s);
 }
 
 }  // namespace
 
-bool gemm_blocks_few_fits(const BlockGemm& a) {
-  if (a.G == 0) return a.single_rows <= 32;
-  return a.max_rows <= 24 * static_cast<int64_t>(a.G);
-}
+// Up to 24 rows (24 x 2816 -> 1024: 6.5 us, tiles through LDS 7.9; 32 x 2048 ->
+// 1408: 7.9 and 6.6).
+bool gemm_blocks_few_fits(const BlockGemm& a) { return a.G == 0 && a.single_rows <= 24; }
 
 bool linear_quantizes_inside(int N, int K) {
   return N <= 16 && static_cast<int64_t>(N) * K <= 16384 && 16 * static_cast<int64_t>(fp8_blocks_of(K)) * 132 <= 49152;
 }
 
 int launch_gemm_blocks_few(const BlockGemm& a, hipStream_t s) {
-  const int mt = a.G == 0 ? (a.single_rows <= 16 ? 1 : 2) : (a.max_rows <= 8 * static_cast<int64_t>(a.G) ? 1 : 2);
   const bool f32 = a.out_dtype == SMOE_F32;
-  switch (a.epi) {
-    case BLK_LINEAR: return f32 ? go_rows<BLK_LINEAR, SMOE_F32, true, 1>(a, mt, s) : go_rows<BLK_LINEAR, SMOE_BF16, false, 1>(a, mt, s);
-    case BLK_GELU: return f32 ? go_rows<BLK_GELU, SMOE_F32, true, 1>(a, mt, s) : go_rows<BLK_GELU, SMOE_BF16, false, 1>(a, mt, s);
-    case BLK_UP_GELU: return go_rows<BLK_UP_GELU, SMOE_F32, false, 1>(a, mt, s);
-    case BLK_UP_SWIGLU: return go_rows<BLK_UP_SWIGLU, SMOE_F32, false, 2>(a, mt, s);
-    case BLK_DOWN: return go_rows<BLK_DOWN, SMOE_F32, false, 1>(a, mt, s);
-    default: return SMOE_EINVAL;
-  }
+  if (a.epi == BLK_LINEAR) return f32 ? go_rows<BLK_LINEAR, SMOE_F32, true>(a, s) : go_rows<BLK_LINEAR, SMOE_BF16, false>(a, s);
+  if (a.epi == BLK_GELU) return f32 ? go_rows<BLK_GELU, SMOE_F32, true>(a, s) : go_rows<BLK_GELU, SMOE_BF16, false>(a, s);
+  return SMOE_EINVAL;
 }
 
 bool prep_fits(int N, int K, int E) {
