@@ -437,6 +437,9 @@ int go_grouped(const BlockGemm& a, hipStream_t s) {
     if (BM == 64) return go_tile<EPI, O, false, 64, 256, 2, 4, 3>(a, s);
     return go_tile<EPI, O, false, 128, 256, 2, 4, 2>(a, s);
   } else {
+    if constexpr (EPI == BLK_DOWN) {  // its channels need not come in blocks of 128
+      if (tiles_of(a, 32, 128) * 8 <= cus * 5) return go_tile<EPI, O, false, 32, 64, 2, 1, 4>(a, s);
+    }
     const bool deep = tiles_of(a, BM, 128) <= 2 * cus;
     if (BM == 32 && deep) return go_tile<EPI, O, false, 32, 128, 2, 2, 3>(a, s);
     if (BM == 32) return go_tile<EPI, O, false, 32, 128, 2, 2, 2>(a, s);

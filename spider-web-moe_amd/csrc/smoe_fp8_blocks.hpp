@@ -76,12 +76,11 @@ bool linear_quantizes_inside(int N, int K);
 
 // A small step's dispatch plan (smoe_dispatch_plan's: offsets [E + 1], rows,
 // row weights, tokrow [N, K]) and the quantized messages in one launch.
-constexpr int kPrepMaxN = 1024, kPrepMaxEntries = 4096;
+constexpr int kPrepMaxN = 1024;
 struct PrepArgs {
   const int32_t* idx = nullptr;
   const float* w = nullptr;
   int N = 0, K = 0, E = 0;
-  int win = 0;  // groups a wave ranks (set by the launch)
   int32_t *off = nullptr, *rows = nullptr, *tokrow = nullptr;
   float* roww = nullptr;
 };

@@ -396,58 +396,25 @@ __global__ __launch_bounds__(512, 4) void k_tokens_down(const TokensArgs a) {
   }
 }
 
-// The merged slots of one token (merge_token's result) from registers: the
-// ids that occur, ascending, each with its slots' weights added in slot order
-// from 0; ids outside [0, E) and sums that are not > 0 left out, -1 padded.
-template <int KB>
-__device__ __forceinline__ void merge_slots(const int32_t* ti, const float* tw, int K, int E, int32_t* og, float* ow) {
-  int id[KB];
-  float w[KB], sum[KB];
-  bool use[KB];
-#pragma unroll
-  for (int j = 0; j < KB; ++j) {  // unconditional loads at clamped indices
-    id[j] = ti[min(j, K - 1)];
-    w[j] = tw[min(j, K - 1)];
-  }
-#pragma unroll
-  for (int j = 0; j < KB; ++j) {
-    use[j] = j < K && id[j] >= 0 && id[j] < E;
-    sum[j] = 0.f;
-#pragma unroll
-    for (int i = 0; i < KB; ++i) {
-      if (i < j) use[j] = use[j] && id[i] != id[j];  // its first slot speaks for an id
-      sum[j] = i < K && id[i] == id[j] ? sum[j] + w[i] : sum[j];
-    }
-    use[j] = use[j] && sum[j] > 0.f;
-  }
-  int n = 0;
-#pragma unroll
-  for (int j = 0; j < KB; ++j) {
-    int rank = 0;
-#pragma unroll
-    for (int i = 0; i < KB; ++i) rank += use[i] && id[i] < id[j] ? 1 : 0;
-    if (use[j]) {
-      og[rank] = id[j];
-      ow[rank] = sum[j];
-      ++n;
-    }
-  }
-  for (int j = n; j < K; ++j) {
-    og[j] = -1;
-    ow[j] = 0.f;
-  }
-}
-
-// The plan of a decode step or a short prompt and its quantized messages in
-// one launch (K <= KB): workgroup 0 merges every token's slots, ranks, scans and
-// scatters (smoe_routing.hpp: the same plan as smoe_dispatch_plan), the
-// others quantize 64 blocks each.
+// The plan of a decode step or a short prompt (K <= KB) and its quantized
+// messages in one launch: workgroup 0 makes the plan (the one
+// smoe_dispatch_plan makes), the others quantize 64 blocks each.
+//
+// A token per thread, its slots in registers: ids that occur twice are merged
+// into their first slot (weights added in slot order from 0), ids outside
+// [0, E) and sums that are not > 0 left out.  Every kept (token, expert) sets
+// the token's bit in the expert's masks, one word for 64 tokens, by an LDS
+// atomic OR (its result does not depend on the order); a row is then the
+// expert's offset, its counts in the words before and the bits below.
+// 777 tokens, top-4 of 32: 15.6 -> 5.6 us against ranking by ballots through
+// memory.
 template <int KB>
 __global__ __launch_bounds__(1024) void k_prep(const PrepArgs a, const BlockQuant bq, int nblk, int64_t total) {
-  __shared__ int32_t sg[kPrepMaxEntries];
-  __shared__ float sw[kPrepMaxEntries];
-  __shared__ int cc[kPlanMaxG * (kPrepMaxN / 64)], tot[kPlanMaxG], goff[kPlanMaxG + 1], wsum[4];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  constexpr int MAXC = kPrepMaxN / 64;
+  __shared__ unsigned long long mask[kPlanMaxG * MAXC];
+  __shared__ uint16_t before[kPlanMaxG * MAXC];
+  __shared__ int tot[kPlanMaxG], goff[kPlanMaxG + 1], wsum[4];
+  const int tid = threadIdx.x;
   if (blockIdx.x > 0) {
     auto run = [&](auto xd) {
       quant_row_block<decltype(xd)::value>(bq, nblk, total,
@@ -458,24 +425,61 @@ __global__ __launch_bounds__(1024) void k_prep(const PrepArgs a, const BlockQuan
     return;
   }
   const int N = a.N, K = a.K, E = a.E, C = (N + 63) / 64;
-  if (tid < N) merge_slots<KB>(a.idx + tid * K, a.w + tid * K, K, E, sg + tid * K, sw + tid * K);
-  __syncthreads();
-  const int win = a.win, W = (E + win - 1) / win;
-  for (int item = wave; item < C * W; item += 16) {
-    const int c = item / W;
-    rank_chunk(sg, sw, N, K, E, 1, c * 64, (item % W) * win, win, cc + c, cc + c, C, a.tokrow);
+  int id[KB];
+  float w[KB], sum[KB];
+  bool use[KB];
+  const int tc = min(tid, N - 1);
+#pragma unroll
+  for (int j = 0; j < KB; ++j) {  // unconditional loads at clamped indices
+    id[j] = a.idx[tc * K + min(j, K - 1)];
+    w[j] = a.w[tc * K + min(j, K - 1)];
+  }
+  for (int i = tid; i < E * C; i += 1024) mask[i] = 0ull;
+#pragma unroll
+  for (int j = 0; j < KB; ++j) {
+    use[j] = tid < N && j < K && id[j] >= 0 && id[j] < E;
+    sum[j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < KB; ++i) {
+      if (i < j) use[j] = use[j] && id[i] != id[j];  // its first slot speaks for an id
+      sum[j] = i < K && id[i] == id[j] ? sum[j] + w[i] : sum[j];
+    }
+    use[j] = use[j] && sum[j] > 0.f;
   }
   __syncthreads();
-  for (int g = wave; g < E; g += 16) {
-    const int v = lane < C ? cc[g * C + lane] : 0;
-    const int incl = wave_incl_scan(v);
-    if (lane < C) cc[g * C + lane] = incl - v;
-    if (lane == 63) tot[g] = incl;
+  const int c = tid >> 6;
+  const unsigned long long bit = 1ull << (tid & 63);
+#pragma unroll
+  for (int j = 0; j < KB; ++j)
+    if (use[j]) atomicOr(&mask[id[j] * C + c], bit);
+  __syncthreads();
+  if (tid < E) {
+    int n = 0;
+    for (int i = 0; i < C; ++i) {
+      before[tid * C + i] = static_cast<uint16_t>(n);
+      n += __popcll(mask[tid * C + i]);
+    }
+    tot[tid] = n;
   }
   __syncthreads();
   block_group_offsets(tot, E, goff, wsum);
   for (int g = tid; g <= E; g += 1024) a.off[g] = goff[g];
-  if (tid < N) scatter_token(sg, sw, tid, K, E, cc + (tid >> 6), C, goff, a.rows, a.roww, a.tokrow);
+  if (tid >= N) return;
+  int n = 0;
+#pragma unroll
+  for (int j = 0; j < KB; ++j) {
+    int rank = 0;  // among the token's experts, ascending
+#pragma unroll
+    for (int i = 0; i < KB; ++i) rank += use[i] && id[i] < id[j] ? 1 : 0;
+    if (!use[j]) continue;
+    const int at = id[j] * C + c;
+    const int row = goff[id[j]] + before[at] + __popcll(mask[at] & (bit - 1ull));
+    a.rows[row] = tid;
+    a.roww[row] = sum[j];
+    a.tokrow[tid * K + rank] = row;
+    ++n;
+  }
+  for (int j = n; j < K; ++j) a.tokrow[tid * K + j] = -1;
 }
 
 int rc() { return hipGetLastError() == hipSuccess ? SMOE_OK : SMOE_EHIP; }
@@ -513,14 +517,10 @@ int launch_gemm_blocks_few(const BlockGemm& a, hipStream_t s) {
 }
 
 bool prep_fits(int N, int K, int E) {
-  return N <= kPrepMaxN && K <= 16 && N * K <= kPrepMaxEntries && E <= kPlanMaxG;
+  return N <= kPrepMaxN && K <= 16 && E <= kPlanMaxG;
 }
 
-int launch_prep(const PrepArgs& args, const BlockQuant& q, hipStream_t s) {
-  PrepArgs a = args;
-  const int C = (a.N + 63) / 64;
-  a.win = 64;  // narrower rank windows until the 16 waves have work
-  while (a.win > 8 && C * ((a.E + a.win - 1) / a.win) < 16) a.win >>= 1;
+int launch_prep(const PrepArgs& a, const BlockQuant& q, hipStream_t s) {
   const int nblk = fp8_blocks_of(q.cols);
   const int64_t total = static_cast<int64_t>(q.rows) * nblk, wgs = (total + 63) / 64 + 1;
   if (wgs > 0x7fffffff) return SMOE_EINVAL;
