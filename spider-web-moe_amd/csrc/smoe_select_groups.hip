@@ -14,8 +14,6 @@
 namespace smoe {
 namespace {
 
-constexpr int kSgMaxE = 256;
-
 template <int DT>
 __device__ __forceinline__ float load_logit(const void* z, int64_t i) {
   if constexpr (DT == SMOE_F32) return reinterpret_cast<const float*>(z)[i];
@@ -23,208 +21,378 @@ __device__ __forceinline__ float load_logit(const void* z, int64_t i) {
   else return static_cast<float>(reinterpret_cast<const _Float16*>(z)[i]);
 }
 
-__device__ __forceinline__ double wave_max64(double v) {
+// A wave's token: lane l holds experts V l .. V l + V - 1, in one load where
+// rows keep its alignment (E % V == 0: the base of the array is aligned or the
+// caller passes vec = false); -inf past E.
+template <int DT, int V>
+__device__ __forceinline__ void load_logits(const void* z, int64_t base, int E, bool vec, float (&v)[V]) {
+  const int e0 = V * static_cast<int>(threadIdx.x & 63);
+  if constexpr (V == 4) {
+    if (vec) {  // uniform
+      const int64_t at = base + (e0 < E ? e0 : 0);
+      if constexpr (DT == SMOE_F32) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(z) + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = a[i];
+      } else {
+        const u32x2 a = *reinterpret_cast<const u32x2*>(reinterpret_cast<const uint16_t*>(z) + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint16_t h = static_cast<uint16_t>(a[i >> 1] >> (16 * (i & 1)));
+          v[i] = DT == SMOE_BF16 ? bf2f(h) : static_cast<float>(__builtin_bit_cast(_Float16, h));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = e0 + i < E ? v[i] : -INFINITY;
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float x = load_logit<DT>(z, base + (e0 + i < E ? e0 + i : 0));
+    v[i] = e0 + i < E ? x : -INFINITY;
+  }
+}
+
+// ---- the same arithmetic in f32 and in f64 ----
+__device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ double max_of(double a, double b) { return fmax(a, b); }
+__device__ __forceinline__ float min_of(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ double min_of(double a, double b) { return fmin(a, b); }
+__device__ __forceinline__ float exp_of(float a) { return expf(a); }
+__device__ __forceinline__ double exp_of(double a) { return exp(a); }
+__device__ __forceinline__ float wave_max_of(float v) { return wave_max(v); }
+__device__ __forceinline__ double wave_max_of(double v) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) v = fmax(v, __shfl_xor(v, o));
   return v;
 }
-__device__ __forceinline__ double wave_sum64(double v) {
+__device__ __forceinline__ float wave_sum_of(float v) { return wave_sum(v); }
+__device__ __forceinline__ double wave_sum_of(double v) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
   return v;
 }
-__device__ __forceinline__ double key64(double v) { return fmin(v, static_cast<double>(INFINITY)); }
+__device__ __forceinline__ float lane_of(float v, int l) { return lane_f(v, l); }
+__device__ __forceinline__ double lane_of(double v, int l) { return __shfl(v, l); }
+// lane ^ (1 << step), or a lane that holds the same after the steps before
+template <int STEP>
+__device__ __forceinline__ float partner(float v) {
+  if constexpr (STEP == 0) return dpp_f<kDppXor1>(v);
+  else if constexpr (STEP == 1) return dpp_f<kDppXor2>(v);
+  else if constexpr (STEP == 2) return dpp_f<kDppHalfMirror>(v);
+  else if constexpr (STEP == 3) return dpp_f<kDppMirror>(v);
+  else return __shfl_xor(v, 1 << STEP);
+}
+template <int STEP>
+__device__ __forceinline__ double partner(double v) { return __shfl_xor(v, 1 << STEP); }
 
-// One wave per token, lane l holding experts l, l + 64, ..; all in 64 bits, so
-// that which of two near scores is the larger does not depend on how an exp
-// rounds.
-template <int DT>
-__global__ __launch_bounds__(256) void k_select_groups(const void* __restrict__ logits, int N, int E,
-                                                       int K, int sigmoid, const float* __restrict__ bias,
-                                                       int groups, int top_groups, int renorm, float scale,
-                                                       float* __restrict__ top_w,
+// LDS of a wave's own: what any lane wrote before is read by any lane after
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+struct SelectArgs {
+  int E, K, sigmoid, groups, top_groups, renorm;
+  const float* bias;
+  float scale;
+};
+
+// The choice of one token (z: its logits, -inf past E).  Lane j < K returns
+// slot j: its expert and score.  Returns whether every comparison that decided
+// was by more than `tol` (scaled as below); T = double with tol 0 always is.
+//
+// Error of c in f32: the score is off by at most 2^-20 of the largest score
+// (expf 1 ulp, its argument |z - max| 2^-24 times at most e^-t t < 0.4 of it, a
+// sum of 10 levels, a division), the sum by 2^-24 of |c|.  Two compared values
+// differ by twice that, two groups' values by four times and a rounding: with
+// 2^-18 of the largest score and 2^-21 of the magnitudes that were added as the
+// border, order in f32 is order.
+template <typename T, int V>
+__device__ __forceinline__ bool choose(const float (&z)[V], const SelectArgs& a, T* group_lds, int& slot_e,
+                                       T& slot_s) {
+  const int lane = threadIdx.x & 63, e0 = V * lane, E = a.E;
+  const T ninf = -INFINITY;
+  T s[V], c[V];
+  T smax = 1;
+  if (a.sigmoid) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) s[v] = z[v] == -INFINITY ? T(0) : T(1) / (T(1) + exp_of(-T(z[v])));
+  } else {
+    float m = -INFINITY;  // NaN if there is one: then every score is
+#pragma unroll
+    for (int v = 0; v < V; ++v) m = z[v] > m ? z[v] : m;
+    m = wave_max(m);
+    T part = 0;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      s[v] = z[v] == -INFINITY ? T(0) : exp_of(T(z[v]) - T(m));
+      part += s[v];
+    }
+    const T sum = wave_sum_of(part);
+#pragma unroll
+    for (int v = 0; v < V; ++v) s[v] = z[v] == -INFINITY ? T(0) : s[v] / sum;
+    smax = T(1) / sum;
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const T b = a.bias && e0 + v < E ? T(a.bias[e0 + v]) : T(0);
+    c[v] = z[v] == -INFINITY ? ninf : min_of(s[v] + b, T(INFINITY));  // NaN -> +infinity
+  }
+  const T border = smax * T(0x1p-18f);
+  bool sure = true;
+  bool open[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) open[v] = e0 + v < E;
+  if (a.groups > 1) {
+    const int per = E / a.groups;
+    const int lanes = per / V;  // of a group
+    T mine[V];                  // the value of each expert's group
+    int gid[V];
+    if (per % V == 0 && (lanes & (lanes - 1)) == 0) {  // uniform: groups are aligned runs of 2^n lanes
+      T x = c[0], y = ninf;                            // the two largest
+#pragma unroll
+      for (int v = 1; v < V; ++v) {
+        y = max_of(y, min_of(x, c[v]));
+        x = max_of(x, c[v]);
+      }
+      auto merge = [&](T px, T py) {
+        y = max_of(min_of(x, px), max_of(y, py));
+        x = max_of(x, px);
+      };
+      if (lanes >= 2) merge(partner<0>(x), partner<0>(y));
+      if (lanes >= 4) merge(partner<1>(x), partner<1>(y));
+      if (lanes >= 8) merge(partner<2>(x), partner<2>(y));
+      if (lanes >= 16) merge(partner<3>(x), partner<3>(y));
+      if (lanes >= 32) merge(partner<4>(x), partner<4>(y));
+      if (lanes >= 64) merge(partner<5>(x), partner<5>(y));
+      const T value = y == ninf ? x : min_of(x + y, T(INFINITY));
+      const int g = lane / lanes;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        mine[v] = value;
+        gid[v] = g;
+      }
+      int ahead = 0;
+      for (int o = 0; o < a.groups; ++o) {
+        const T w = lane_of(value, o * lanes);
+        ahead += w > value || (w == value && o < g) ? 1 : 0;
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) open[v] = open[v] && ahead < a.top_groups;
+    } else {
+      // any other shape: through LDS, [0, 256) the values of c, then of the groups
+      wave_sync();
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (e0 + v < E) group_lds[e0 + v] = c[v];
+      wave_sync();
+      T gval[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {  // this lane's groups: V lane + v
+        T x = ninf, y = ninf;
+        if (e0 + v < a.groups)
+          for (int i = 0; i < per; ++i) {
+            const T w = group_lds[(e0 + v) * per + i];
+            y = max_of(y, min_of(x, w));
+            x = max_of(x, w);
+          }
+        gval[v] = y == ninf ? x : min_of(x + y, T(INFINITY));
+      }
+      wave_sync();  // every value of c is read
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (e0 + v < a.groups) group_lds[e0 + v] = gval[v];
+      wave_sync();
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (e0 + v >= E) continue;
+        gid[v] = (e0 + v) / per;
+        mine[v] = group_lds[gid[v]];
+        int ahead = 0;
+        for (int o = 0; o < a.groups; ++o) {
+          const T w = group_lds[o];
+          ahead += w > mine[v] || (w == mine[v] && o < gid[v]) ? 1 : 0;
+        }
+        open[v] = ahead < a.top_groups;
+      }
+    }
+    if constexpr (sizeof(T) == 4) {
+      T low = INFINITY, high = ninf, cmag = 0;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (e0 + v >= E) continue;
+        if (c[v] != ninf) cmag = max_of(cmag, T(fabsf(c[v])));
+        if (open[v]) low = min_of(low, mine[v]);
+        else high = max_of(high, mine[v]);
+      }
+      low = -wave_max_of(-low);
+      high = wave_max_of(high);
+      cmag = wave_max_of(cmag);
+      sure = high == ninf || low - high > border + T(0x1p-21f) * cmag;
+    }
+  }
+  T last = 0;
+  slot_e = 0;
+  slot_s = 0;
+  // one more than K: the first that is left out decides too
+  const int rounds = sizeof(T) == 4 ? a.K + 1 : a.K;
+#pragma unroll 1
+  for (int j = 0; j < rounds; ++j) {
+    T best = ninf, bs = 0;
+    int bv = -1;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const bool take = open[v] && (bv < 0 || c[v] > best);
+      best = take ? c[v] : best;
+      bs = take ? s[v] : bs;
+      bv = take ? v : bv;
+    }
+    const T top = wave_max_of(best);
+    const uint64_t at = __ballot(bv >= 0 && best == top);
+    if (!at) break;  // uniform: nothing is left (the round after the last pick)
+    const int src = __builtin_ctzll(at);  // the lowest lane: the lowest index
+    if constexpr (sizeof(T) == 4)
+      if (j > 0 && top != ninf) sure = sure && last - top > border + T(0x1p-21f) * max_of(fabsf(last), fabsf(top));
+    last = top;
+    const int e = V * src + __builtin_amdgcn_readlane(bv, src);
+    const T sc = lane_of(bs, src);
+    if (lane == j) {
+      slot_e = e;
+      slot_s = sc;
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) open[v] = open[v] && e0 + v != e;
+  }
+  return sure;
+}
+
+// One wave per token.  The choice is made in f32 and, where two values that
+// decide lie nearer than f32 tells apart, once more in f64 (sigmoid scores of
+// 256 experts: about 1 token in 100), so that it is the order of the real
+// values: 16384 tokens over 256 experts 66 us all in f64, 17 so.
+template <int DT, int V>
+__global__ __launch_bounds__(256) void k_select_groups(const void* __restrict__ logits, int N, bool vec,
+                                                       const SelectArgs a, float* __restrict__ top_w,
                                                        int32_t* __restrict__ top_idx) {
-  constexpr int V = kSgMaxE / 64;
-  __shared__ double cs[4][kSgMaxE], gv[4][kSgMaxE];
+  __shared__ double lds[4][64 * V];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int t = blockIdx.x * 4 + wave;
-  const bool live = t < N;
-  const int64_t base = static_cast<int64_t>(live ? t : N - 1) * E;
-  double s[V], key[V];
-  bool cand[V];
-  double mx = -INFINITY;
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = lane + 64 * v;
-    s[v] = e < E ? load_logit<DT>(logits, base + e) : -INFINITY;
-    cand[v] = e < E;
-    mx = (s[v] > mx || s[v] != s[v]) ? s[v] : mx;
+  if (t >= N) return;  // wave-uniform; no workgroup barrier below
+  float z[V];
+  load_logits<DT, V>(logits, static_cast<int64_t>(t) * a.E, a.E, vec, z);
+  int e;
+  float s;
+  if (!choose<float, V>(z, a, reinterpret_cast<float*>(lds[wave]), e, s)) {  // uniform
+    double d;
+    choose<double, V>(z, a, lds[wave], e, d);
+    s = static_cast<float>(d);
   }
-  double sum = 0.0;
-  if (!sigmoid) {
-    mx = wave_max64(mx);
-#pragma unroll
-    for (int v = 0; v < V; ++v) sum += s[v] == -INFINITY ? 0.0 : exp(s[v] - mx);
-    sum = wave_sum64(sum);
-  }
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = lane + 64 * v;
-    const bool masked = s[v] == -INFINITY;
-    s[v] = masked ? 0.0 : (sigmoid ? 1.0 / (1.0 + exp(-s[v])) : exp(s[v] - mx) / sum);
-    key[v] = masked ? -INFINITY : key64(s[v] + (bias && e < E ? static_cast<double>(bias[e]) : 0.0));
-    if (e < E) cs[wave][e] = key[v];
-  }
-  __syncthreads();
-  if (groups > 1) {
-    const int per = E / groups;
-    for (int g = lane; g < groups; g += 64) {
-      double a = -INFINITY, b = -INFINITY;
-      for (int i = 0; i < per; ++i) {
-        const double x = cs[wave][g * per + i];
-        b = fmax(b, fmin(a, x));
-        a = fmax(a, x);
-      }
-      gv[wave][g] = b == -INFINITY ? a : key64(a + b);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int e = lane + 64 * v;
-      if (e >= E) continue;
-      const int g = e / per;
-      int before = 0;
-      for (int o = 0; o < groups; ++o)
-        before += gv[wave][o] > gv[wave][g] || (gv[wave][o] == gv[wave][g] && o < g);
-      cand[v] = before < top_groups;
-    }
-  }
-  double slot = 0.0, total = 0.0;
-  int slot_i = 0;
-  for (int j = 0; j < K; ++j) {
-    double bv = -INFINITY, bs = 0.0;
-    int bi = 1 << 20;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-      const int e = lane + 64 * v;
-      if (cand[v] && (key[v] > bv || (key[v] == bv && e < bi))) {
-        bv = key[v];
-        bi = e;
-        bs = s[v];
-      }
-    }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-      const double ov = __shfl_xor(bv, o), os = __shfl_xor(bs, o);
-      const int oi = __shfl_xor(bi, o);
-      if (ov > bv || (ov == bv && oi < bi)) {
-        bv = ov;
-        bi = oi;
-        bs = os;
-      }
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) cand[v] = cand[v] && lane + 64 * v != bi;
-    total += bs;
-    if (lane == j) {
-      slot = bs;
-      slot_i = bi;
-    }
-  }
-  if (live && lane < K) {
-    const double w = renorm ? slot / (total < 1e-9 ? 1e-9 : total) : slot;
-    top_w[static_cast<int64_t>(t) * K + lane] = static_cast<float>(w * scale);
-    top_idx[static_cast<int64_t>(t) * K + lane] = slot_i;
-  }
+  const float total = wave_sum(lane < a.K ? s : 0.f);
+  if (lane >= a.K) return;
+  const float w = a.renorm ? s / (total < 1e-9f ? 1e-9f : total) : s;
+  top_w[static_cast<int64_t>(t) * a.K + lane] = w * a.scale;
+  top_idx[static_cast<int64_t>(t) * a.K + lane] = e;
 }
 
 // d loss / d z_e.  With S = sum of the chosen s and g_j = d loss / d w_j:
-//   renorm, S > 1e-9:  ds_j = scale / S * (g_j - sum_i g_i s_i / S)
+//   renorm, S >= 1e-9: ds_j = scale / S * (g_j - sum_i g_i s_i / S)
 //   renorm, otherwise: ds_j = scale / 1e-9 * g_j       (the clamped sum is a constant)
 //   else               ds_j = scale * g_j
 //   sigmoid: dz_e = ds_e s_e (1 - s_e);  softmax: dz_e = s_e (ds_e - sum_i s_i ds_i)
 // An expert chosen in several slots takes all their gradients; ids outside
-// [0, E) none.
-template <int DT>
-__global__ __launch_bounds__(256) void k_select_groups_bwd(const void* __restrict__ logits, int N, int E,
-                                                           int K, int sigmoid, int renorm, float scale,
+// [0, E) none.  One wave per token, lane j < K the slot j as well: bound by the
+// logits read and the gradients written.
+template <int DT, int V>
+__global__ __launch_bounds__(256) void k_select_groups_bwd(const void* __restrict__ logits, int N, bool vec,
+                                                           const SelectArgs a,
                                                            const int32_t* __restrict__ top_idx,
                                                            const float* __restrict__ d_w,
                                                            void* __restrict__ d_logits) {
-  constexpr int V = kSgMaxE / 64;
   const int lane = threadIdx.x & 63;
   const int t = blockIdx.x * 4 + (threadIdx.x >> 6);
   if (t >= N) return;  // wave-uniform
+  const int E = a.E, K = a.K, e0 = V * lane;
   const int64_t base = static_cast<int64_t>(t) * E;
-  float z[V], s[V], om[V], ds[V];
-  float mx = -INFINITY;
+  const int64_t slot = static_cast<int64_t>(t) * K + (lane < K ? lane : 0);
+  const int id_in = top_idx[slot];
+  const float g = d_w[slot];
+  float z[V];
+  load_logits<DT, V>(logits, base, E, vec, z);
+  const bool used = lane < K && id_in >= 0 && id_in < E;
+  const int id = used ? id_in : -1;
+  const float zs = load_logit<DT>(logits, base + (used ? id : 0));  // the slot's logit
+  float m = -INFINITY, sum = 1.f;
+  if (!a.sigmoid) {
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = lane + 64 * v;
-    z[v] = e < E ? load_logit<DT>(logits, base + e) : -INFINITY;
-    mx = fmaxf(mx, z[v]);
-    ds[v] = 0.f;
-  }
-  float sum = 1.f;
-  if (!sigmoid) {
-    mx = wave_max(mx);
+    for (int v = 0; v < V; ++v) m = z[v] > m ? z[v] : m;
+    m = wave_max(m);
     float part = 0.f;
 #pragma unroll
-    for (int v = 0; v < V; ++v) part += z[v] == -INFINITY ? 0.f : expf(z[v] - mx);
+    for (int v = 0; v < V; ++v) part += z[v] == -INFINITY ? 0.f : expf(z[v] - m);
     sum = wave_sum(part);
   }
+  // score and its slope (sigmoid: s (1 - s) without the cancellation)
+  auto score = [&](float x, float& slope) {
+    if (x == -INFINITY) {
+      slope = 0.f;
+      return 0.f;
+    }
+    if (!a.sigmoid) {
+      slope = 1.f;
+      return expf(x - m) / sum;
+    }
+    const float u = expf(-fabsf(x)), big = 1.f / (1.f + u), small = u / (1.f + u);
+    slope = big * small;
+    return x >= 0.f ? big : (x < 0.f ? small : x);
+  };
+  float unused;
+  const float ss = used ? score(zs, unused) : 0.f;
+  const float total = wave_sum(ss), dot = wave_sum(used ? g * ss : 0.f);
+  const bool over = total >= 1e-9f || total != total;
+  const float f = a.renorm ? a.scale / (over ? total : 1e-9f) : a.scale;
+  const float ds_slot = used ? f * (g - (a.renorm && over ? dot / total : 0.f)) : 0.f;
+  const float mean = a.sigmoid ? 0.f : wave_sum(used ? ss * ds_slot : 0.f);
+  float d[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) d[v] = 0.f;
+#pragma unroll 1
+  for (int j = 0; j < K; ++j) {
+    const int e = __builtin_amdgcn_readlane(id, j);
+    const float dj = lane_f(ds_slot, j);
+#pragma unroll
+    for (int v = 0; v < V; ++v) d[v] += e0 + v == e ? dj : 0.f;
+  }
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    const bool masked = z[v] == -INFINITY;
-    if (sigmoid) {  // 1 - s without the cancellation
-      const float x = expf(-fabsf(z[v]));
-      const float big = 1.f / (1.f + x), small = x / (1.f + x);
-      s[v] = masked ? 0.f : (z[v] >= 0.f ? big : (z[v] < 0.f ? small : z[v]));
-      om[v] = z[v] >= 0.f ? small : (z[v] < 0.f ? big : z[v]);
-    } else {
-      s[v] = masked ? 0.f : expf(z[v] - mx) / sum;
-      om[v] = 1.f;
+    float slope;
+    const float s = score(z[v], slope);
+    if (a.sigmoid) d[v] = d[v] == 0.f ? 0.f : d[v] * slope;
+    else d[v] = s * (d[v] - mean);
+  }
+  if constexpr (V == 4) {
+    if (vec) {
+      if (e0 >= E) return;
+      if constexpr (DT == SMOE_F32) {
+        *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(d_logits) + base + e0) = f32x4{d[0], d[1], d[2], d[3]};
+      } else if constexpr (DT == SMOE_BF16) {
+        *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(d_logits) + base + e0) =
+            u32x2{pack_bf2(d[0], d[1]), pack_bf2(d[2], d[3])};
+      } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) reinterpret_cast<_Float16*>(d_logits)[base + e0 + v] = static_cast<_Float16>(d[v]);
+      }
+      return;
     }
   }
-  const int id = lane < K ? top_idx[static_cast<int64_t>(t) * K + lane] : -1;
-  const float g = lane < K ? d_w[static_cast<int64_t>(t) * K + lane] : 0.f;
-  float total = 0.f, dot = 0.f;
-  for (int j = 0; j < K; ++j) {
-    const int e = __shfl(id, j);
-    const float gj = __shfl(g, j);
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-      if (lane + 64 * v == e) {
-        total += s[v];
-        dot += gj * s[v];
-        ds[v] += gj;
-      }
-  }
-  total = wave_sum(total);
-  dot = wave_sum(dot);
-  const bool over = total >= 1e-9f || total != total;
-  const float f = renorm ? scale / (over ? total : 1e-9f) : scale;
-  const float sub = renorm && over ? dot / total : 0.f;
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    float n = 0.f;  // how many slots chose the expert
-    for (int j = 0; j < K; ++j) n += lane + 64 * v == __shfl(id, j) ? 1.f : 0.f;
-    ds[v] = n > 0.f ? f * (ds[v] - n * sub) : 0.f;
-  }
-  float mean = 0.f;
-  if (!sigmoid) {
-#pragma unroll
-    for (int v = 0; v < V; ++v) mean += s[v] * ds[v];
-    mean = wave_sum(mean);
-  }
-#pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const int e = lane + 64 * v;
-    if (e >= E) continue;
-    const float d = sigmoid ? (ds[v] == 0.f ? 0.f : ds[v] * s[v] * om[v]) : s[v] * (ds[v] - mean);
-    if constexpr (DT == SMOE_F32) reinterpret_cast<float*>(d_logits)[base + e] = d;
-    else if constexpr (DT == SMOE_BF16) reinterpret_cast<uint16_t*>(d_logits)[base + e] = f2bf(d);
-    else reinterpret_cast<_Float16*>(d_logits)[base + e] = static_cast<_Float16>(d);
+    if (e0 + v >= E) continue;
+    if constexpr (DT == SMOE_F32) reinterpret_cast<float*>(d_logits)[base + e0 + v] = d[v];
+    else if constexpr (DT == SMOE_BF16) reinterpret_cast<uint16_t*>(d_logits)[base + e0 + v] = f2bf(d[v]);
+    else reinterpret_cast<_Float16*>(d_logits)[base + e0 + v] = static_cast<_Float16>(d[v]);
   }
 }
 
@@ -240,16 +408,32 @@ int by_zdt(int dt, F&& f) {
   }
 }
 
+// experts a lane holds: E <= 64, <= 128, <= 256
+template <typename F>
+int by_lane(int E, F&& f) {
+  if (E <= 64) return f(std::integral_constant<int, 1>{});
+  if (E <= 128) return f(std::integral_constant<int, 2>{});
+  return f(std::integral_constant<int, 4>{});
+}
+
+// whether rows of E logits load (and store) as vectors of four
+bool vec4(const void* p, int zdt, int E) {
+  return E % 4 == 0 && reinterpret_cast<uintptr_t>(p) % (zdt == SMOE_F32 ? 16 : 8) == 0;
+}
+
 }  // namespace
 
 int launch_select_groups(const void* logits, int zdt, int N, int E, int K, int sigmoid, const float* bias,
                          int groups, int top_groups, int renorm, float scale, float* top_w,
                          int32_t* top_idx, hipStream_t s) {
   if (N <= 0) return SMOE_OK;
+  const SelectArgs a{E, K, sigmoid, groups, top_groups, renorm, bias, scale};
   return by_zdt(zdt, [&](auto dt) {
-    hipLaunchKernelGGL((k_select_groups<decltype(dt)::value>), dim3((N + 3) / 4), dim3(256), 0, s, logits,
-                       N, E, K, sigmoid, bias, groups, top_groups, renorm, scale, top_w, top_idx);
-    return rc();
+    return by_lane(E, [&](auto v) {
+      hipLaunchKernelGGL((k_select_groups<decltype(dt)::value, decltype(v)::value>), dim3((N + 3) / 4), dim3(256), 0,
+                         s, logits, N, vec4(logits, zdt, E), a, top_w, top_idx);
+      return rc();
+    });
   });
 }
 
@@ -257,10 +441,13 @@ int launch_select_groups_bwd(const void* logits, int zdt, int N, int E, int K, i
                              float scale, const int32_t* top_idx, const float* d_w, void* d_logits,
                              hipStream_t s) {
   if (N <= 0) return SMOE_OK;
+  const SelectArgs a{E, K, sigmoid, 1, 1, renorm, nullptr, scale};
   return by_zdt(zdt, [&](auto dt) {
-    hipLaunchKernelGGL((k_select_groups_bwd<decltype(dt)::value>), dim3((N + 3) / 4), dim3(256), 0, s,
-                       logits, N, E, K, sigmoid, renorm, scale, top_idx, d_w, d_logits);
-    return rc();
+    return by_lane(E, [&](auto v) {
+      hipLaunchKernelGGL((k_select_groups_bwd<decltype(dt)::value, decltype(v)::value>), dim3((N + 3) / 4), dim3(256),
+                         0, s, logits, N, vec4(logits, zdt, E) && vec4(d_logits, zdt, E), a, top_idx, d_w, d_logits);
+      return rc();
+    });
   });
 }
 
