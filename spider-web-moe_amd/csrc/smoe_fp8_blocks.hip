@@ -146,98 +146,164 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm_blocks(const BlockGemm
   const uniform_f32 wsc = as_uniform(wsp), wsc_up = as_uniform(wsp_up);
   float nw0 = wsc[0], nw1 = SWIGLU ? wsc_up[0] : 0.f;
 #pragma unroll
-  for (int s = 0; s < NS - 1; ++s)
+  for (int s = 0; s < NS; ++s)
     if (s < KB) {
 #pragma unroll
       for (int d = 0; d < LD; ++d) issue_one(s, d);
     }
+  // A stage's last ROT rows of fragments are multiplied after the barrier that
+  // opens the next stage, each weight fragment replaced by the next stage's
+  // after its last use: otherwise the matrix unit waits there for the LDS
+  // (80 KB at 128 bytes a cycle with 256 x 256 tiles).
+  // Step t: TA steps of those rows, weights outside, then the rows before them.
+  // Under the product of a step the four multiply-adds that bring the step LAG
+  // before into the accumulators and, in the stage's first half, the DMAs of a
+  // later one.  (16384 x 1024 -> 5632: DMAs over the
+  // whole stage 139, over its first half 132.)
+  constexpr int ROT = FM >= 4 ? 2 : 1, TA = 4 * ROT, STEPS = 4 * FM, LAG = 2;
+  constexpr bool CARRY = FM > ROT;  // the last steps' multiply-adds go under the next stage's first ones
+  i32x8 wf[4], xa[ROT];
+  float za0[ROT], za1[ROT], zb0[2], zb1[2];  // the scales of the last ROT rows, of row i before them: [i % 2]
+  f32x4 part[4];
+  auto product = [&](const i32x8& w, const i32x8& x) {
+    f32x4 now = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (WIDE) {
+      bf16x8 ww[4], xw[4];
+      widen_frag(w, ww);
+      widen_frag(x, xw);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) now = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ww[u], xw[u], now, 0, 0, 0);
+    } else {
+      now = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, now, 0, 0, 0, 0, 0, 0);
+    }
+    return now;
+  };
+  auto add = [&](int t) {
+    const int j = t < TA ? t / ROT : t % 4, i = t < TA ? FM - ROT + t % ROT : (t - TA) / 4;
+    const float z0 = t < TA ? za0[t % ROT] : zb0[i % 2], z1 = t < TA ? za1[t % ROT] : zb1[i % 2];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) acc[j][i][v] = fmaf(part[t % 4][v], SWIGLU && j >= 2 ? z1 : z0, acc[j][i][v]);
+  };
+  // the last ROT rows of the stage before; `fill(j)`: the weights' fragment j is free
+  auto last_rows = [&](auto fill, auto dma) {
+#pragma unroll
+    for (int t = 0; t < TA; ++t) {
+      part[t % 4] = product(wf[t / ROT], xa[t % ROT]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (t % ROT == ROT - 1) fill(t / ROT);
+      if (t >= LAG) add(t - LAG);
+      else if (CARRY) add(STEPS + t - LAG);
+      dma(t);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (!CARRY) {
+#pragma unroll
+      for (int t = TA - LAG; t < TA; ++t) add(t);
+    }
+  };
   // stage s, whose part of the ring holds for every wave when it is called;
-  // `more`: stage s + NS - 1 is requested meanwhile
-  auto stage = [&](int s, auto more) {
-    uint8_t* sx = ring + (s % NS) * STAGE;
-    const float* sc = reinterpret_cast<const float*>(sx + XB + WB) + wm * TM;
+  // `more`: stage s - 1 + NS is requested meanwhile, into the slot of stage s - 1
+  auto stage = [&](int s, auto first, auto more) {
+    const uint8_t* sx = ring + (s % NS) * STAGE;
+    const float* sc = reinterpret_cast<const float*>(sx + XB + WB) + wm * TM + fr;
     const float w0 = nw0, w1 = nw1;
     const int ns = min(s + 1, KB - 1);
     nw0 = wsc[ns];
     if (SWIGLU) nw1 = wsc_up[ns];
-    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    i32x8 wf[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) wf[j] = frag(sx + XB + (wn * 64 + j * 16) * 128);
     auto xfrag = [&](int i) { return frag(sx + (wm * TM + i * 16) * 128); };
-    // Step (i, j): the product of rows 16 i and weight rows 16 j, under it the
-    // four multiply-adds that bring the step LAG before into the accumulators
-    // and now and then a DMA of stage s + NS - 1 (into the slot of stage s - 1);
-    // the next rows' fragment is read four steps ahead.  All DMAs at the stage's
-    // start kept the matrix unit waiting about as long as its products take.
-    constexpr int LAG = 2, STEPS = 4 * FM;
-    i32x8 xf = xfrag(0);
-    f32x4 part[LAG + 1];
-    float s0[2], s1[2];  // the scales of rows 16 i: [i % 2]
-    auto add = [&](int t) {
-      const int i = t / 4, j = t % 4;
+    auto fill = [&](int j) { wf[j] = frag(sx + XB + (wn * 64 + j * 16) * 128); };
+    auto dma = [&](int t) {
+      if constexpr (decltype(more)::value) {
 #pragma unroll
-      for (int v = 0; v < 4; ++v)
-        acc[j][i][v] = fmaf(part[t % (LAG + 1)][v], SWIGLU && j >= 2 ? s1[i % 2] : s0[i % 2], acc[j][i][v]);
-    };
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      const float xsv = sc[i * 16 + fr];
-      const i32x8 nx = xfrag(i + 1 < FM ? i + 1 : i);
-      bf16x8 xw[4];
-      if constexpr (WIDE) widen_frag(xf, xw);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = 4 * i + j;
-        f32x4 now = zero;
-        if constexpr (WIDE) {
-          bf16x8 ww[4];
-          widen_frag(wf[j], ww);
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            now = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ww[u], xw[u], now, 0, 0, 0);
-        } else {
-          now = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], xf, zero, 0, 0, 0, 0, 0, 0);
-        }
-        part[t % (LAG + 1)] = now;
-        __builtin_amdgcn_sched_barrier(0);
-        if (t >= LAG) add(t - LAG);
-        if (j == LAG - 1) {  // the rows before are done with theirs at j = LAG - 1
-          s0[i % 2] = xsv * w0;
-          s1[i % 2] = xsv * w1;
-        }
-        if constexpr (decltype(more)::value) {
-#pragma unroll
-          for (int d = 0; d < LD; ++d)
-            if (d * STEPS / LD == t) issue_one(s + NS - 1, d);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        for (int d = 0; d < LD; ++d)
+          if (d * STEPS / (2 * LD) == t) issue_one(s - 1 + NS, d);
       }
-      xf = nx;
+    };
+    i32x8 xf = xfrag(0);
+    float xsv = sc[0];
+    if constexpr (decltype(first)::value) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) fill(j);
+    } else {
+      last_rows(fill, dma);
     }
 #pragma unroll
-    for (int t = STEPS - LAG; t < STEPS; ++t) add(t);
+    for (int i = 0; i < FM - ROT; ++i) {
+      i32x8 nx = xf;
+      float nv[ROT];
+      if (i + 1 < FM - ROT) {
+        nx = xfrag(i + 1);
+        nv[0] = sc[(i + 1) * 16];
+      } else {
+#pragma unroll
+        for (int u = 0; u < ROT; ++u) {
+          xa[u] = xfrag(FM - ROT + u);
+          nv[u] = sc[(FM - ROT + u) * 16];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int t = TA + 4 * i + j;
+        part[t % 4] = product(wf[j], xf);
+        __builtin_amdgcn_sched_barrier(0);
+        if (t - LAG >= (decltype(first)::value ? TA : 0)) add(t - LAG);
+        if (j == LAG - 1) {
+          zb0[i % 2] = xsv * w0;
+          zb1[i % 2] = xsv * w1;
+        }
+        dma(t);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (i + 1 < FM - ROT) {
+        xf = nx;
+        xsv = nv[0];
+      } else {
+#pragma unroll
+        for (int u = 0; u < ROT; ++u) {
+          za0[u] = nv[u] * w0;
+          za1[u] = nv[u] * w1;
+        }
+      }
+    }
+    if constexpr (FM == ROT) {
+      xa[0] = xf;
+      za0[0] = xsv * w0;
+      za1[0] = xsv * w1;
+    }
+  };
+  auto cut = [&](int s) {
+    if (s == KB - 1 && p.K - s * 128 < 128) {  // uniform: the last stage of a ragged K
+      cut_stage(ring + (s % NS) * STAGE, BM + BN, p.K - s * 128, tid, NW * 64);
+      lds_barrier();
+    }
   };
   // own part of a stage landed (the later ones may be on their way); after the
   // barrier everybody's, and nobody reads the stage before any more.  Two
   // loops: a branch around each DMA made the compiler move the multiply-adds
   // away from the products they should hide under.
-  int s = 0;
-  for (; s + NS - 1 < KB; ++s) {
+  if (KB >= NS) wait_vmcnt<(NS - 1) * LD>();
+  else wait_vmcnt<0>();
+  __builtin_amdgcn_s_barrier();
+  cut(0);
+  stage(0, std::true_type{}, std::false_type{});
+  int s = 1;
+  for (; s - 1 + NS < KB; ++s) {
     wait_vmcnt<(NS - 2) * LD>();
     wait_lgkm0();
     __builtin_amdgcn_s_barrier();
-    stage(s, std::true_type{});
+    stage(s, std::false_type{}, std::true_type{});
   }
   for (; s < KB; ++s) {
     wait_vmcnt<0>();
     wait_lgkm0();
     __builtin_amdgcn_s_barrier();
-    if (p.K - s * 128 < 128) {  // uniform: the last stage of a ragged K
-      cut_stage(ring + (s % NS) * STAGE, BM + BN, p.K - s * 128, tid, NW * 64);
-      lds_barrier();
-    }
-    stage(s, std::false_type{});
+    cut(s);
+    stage(s, std::false_type{}, std::false_type{});
+  }
+  last_rows([](int) {}, [](int) {});
+  if constexpr (CARRY) {
+#pragma unroll
+    for (int t = TA - LAG; t < TA; ++t) add(t);
   }
 
   // epilogue: lane holds channels 4 q + v of row fr of each 16 x 16 tile
@@ -246,28 +312,35 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm_blocks(const BlockGemm
     // amax per row over the wave's channels, then over the waves of a block
     // of 128 channels through LDS; codes staged in the ring
     constexpr int JN = SWIGLU ? 2 : 4, BW = 128 / CHW;  // BW waves share a block
-    uint32_t* red = reinterpret_cast<uint32_t*>(ring);  // [WN][BM]
-    uint8_t* stg = ring + WN * BM * 4;            // [BM][CH], 16-byte chunks swizzled by row
-    static_assert(WN * BM * 4 + BM * CH <= NS * STAGE, "staging in the ring");
+    uint32_t* red = reinterpret_cast<uint32_t*>(ring);     // [WN][BM]
+    float* inv = reinterpret_cast<float*>(red + WN * BM);  // [CH / 128][BM]
+    uint8_t* stg = ring + (WN + CH / 128) * BM * 4;        // [BM][CH], 16-byte chunks swizzled by row
+    static_assert((WN + CH / 128) * BM * 4 + BM * CH <= NS * STAGE, "staging in the ring");
     uint32_t m[FM];
 #pragma unroll
     for (int i = 0; i < FM; ++i) m[i] = 0u;
 #pragma unroll
     for (int j = 0; j < JN; ++j) {
-      const int c = CHW * wn + j * 16 + 4 * q;
+      const int c = n0 + CHW * wn + j * 16;
+      if (c < p.N_out) {  // uniform: N_out % 16 == 0
+        float b[4] = {0.f, 0.f, 0.f, 0.f};
+        if (bias) {
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const bool in = n0 + c + v < p.N_out;
-        const float b = bias && in ? bias[n0 + c + v] : 0.f;
-#pragma unroll
-        for (int i = 0; i < FM; ++i) {
-          float y;
-          if constexpr (SWIGLU) y = silu(acc[j][i][v]) * (acc[j + 2][i][v] + b);
-          else y = gelu_erf(acc[j][i][v] + b);
-          y = in ? y : 0.f;
-          acc[j][i][v] = y;
-          m[i] = amax_bits(m[i], y);
+          for (int v = 0; v < 4; ++v) b[v] = bias[c + 4 * q + v];
         }
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            float y;
+            if constexpr (SWIGLU) y = silu(acc[j][i][v]) * (acc[j + 2][i][v] + b[v]);
+            else y = gelu_erf(acc[j][i][v] + b[v]);
+            acc[j][i][v] = y;
+            m[i] = amax_bits(m[i], y);
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < FM; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
     }
     __syncthreads();  // every wave is done with the ring
@@ -277,23 +350,27 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm_blocks(const BlockGemm
       if (q == 0) red[wn * BM + wm * TM + i * 16 + fr] = m[i];
     }
     __syncthreads();
-    const int bw0 = wn / BW * BW;
+    for (int e = tid; e < CH / 128 * BM; e += NW * 64) {
+      const int blk = e / BM, r = e % BM;
+      uint32_t a = red[blk * BW * BM + r];
+#pragma unroll
+      for (int w = 1; w < BW; ++w) a = max(a, red[(blk * BW + w) * BM + r]);
+      const float sc = block_scale(a);
+      inv[e] = __fdiv_rn(1.0f, sc);
+      if (r < mrows && n0 + 128 * blk < p.N_out) p.out_scale[(n0 / 128 + blk) * p.os_col + m0 + r] = sc;
+    }
+    __syncthreads();
+    // times the reciprocal: within 2^-23 of the quotient, where the activation
+    // itself is known to about 2^-16
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int r = wm * TM + i * 16 + fr;
-      uint32_t a = red[bw0 * BM + r];
-#pragma unroll
-      for (int w = 1; w < BW; ++w) a = max(a, red[(bw0 + w) * BM + r]);
-      const float sc = block_scale(a);
-      const Divisor d = divisor(sc);
-      if (wn == bw0 && q == 0 && r < mrows && n0 + CHW * wn < p.N_out)
-        p.out_scale[((n0 + CHW * wn) / 128) * p.os_col + m0 + r] = sc;
+      const float d = inv[wn / BW * BM + r];
 #pragma unroll
       for (int j = 0; j < JN; ++j) {
         const int c = CHW * wn + j * 16 + 4 * q;
         *reinterpret_cast<uint32_t*>(stg + r * CH + (((c >> 4) ^ (r & 7)) << 4) + (c & 15)) =
-            pack_e4m3(quotient(acc[j][i][0], d), quotient(acc[j][i][1], d), quotient(acc[j][i][2], d),
-                      quotient(acc[j][i][3], d));
+            pack_e4m3(acc[j][i][0] * d, acc[j][i][1] * d, acc[j][i][2] * d, acc[j][i][3] * d);
       }
     }
     __syncthreads();
