@@ -1374,8 +1374,8 @@ namespace {
 
 int check_select_groups(int zdt, int N, int E, int K, int score) {
   if (zdt != SMOE_F32 && zdt != SMOE_BF16 && zdt != SMOE_F16) return fail(SMOE_EUNSUPPORTED, "logits dtype");
-  if (N < 0 || E < 1 || E > 256 || K < 1 || K > E || K > 64)
-    return fail(SMOE_EINVAL, "select shape (1 <= K <= min(E, 64), E <= 256)");
+  if (N < 0 || N >= 1 << 26 || E < 1 || E > 256 || K < 1 || K > E || K > 64)
+    return fail(SMOE_EINVAL, "select shape (N < 2^26, 1 <= K <= min(E, 64), E <= 256)");
   if (score != SMOE_SCORE_SOFTMAX && score != SMOE_SCORE_SIGMOID) return fail(SMOE_EINVAL, "score");
   return SMOE_OK;
 }
@@ -1423,6 +1423,9 @@ SMOE_API int smoe_quantize_fp8_blocks(const void* x, int x_dtype, int G, int row
   if (G < 0 || rows < 0 || cols < 1 || cols > 0x7fffff80 || ldx < cols || ld_out < cols || ld_out % 16 ||
       ld_out > static_cast<int64_t>(fp8_blocks_of(cols)) * kFp8Block)
     return fail(SMOE_EINVAL, "quantize shape (ldx >= cols, cols <= ld_out <= cols rounded up to 128, ld_out % 16 == 0)");
+  const int64_t blocks = static_cast<int64_t>(G) * (block_rows == 1 ? rows : fp8_blocks_of(rows));
+  if (blocks > ((block_rows == 1 ? 1 << 28 : 1 << 24) - 1) / fp8_blocks_of(cols))
+    return fail(SMOE_EINVAL, "quantize shape (fewer than 2^28 blocks of 1 x 128, 2^24 of 128 x 128)");
   if (G == 0 || rows == 0) return SMOE_OK;
   if (!x || !codes || !scale) return fail(SMOE_EINVAL, "null buffer");
   if (!aligned16(codes)) return fail(SMOE_EINVAL, "codes must be 16-byte aligned");
@@ -1551,7 +1554,7 @@ int check_experts_fp8_blocks(const smoe_experts_fp8_blocks* ex, int N, int K) {
   if (!aligned16(ex->w_up) || !aligned16(ex->w_down)) return fail(SMOE_EINVAL, "expert codes must be 16-byte aligned");
   if (N < 0 || K < 1 || K > 64 || static_cast<int64_t>(N) * K > 0x7fffff7f)
     return fail(SMOE_EINVAL, "shape (1 <= top_k <= 64, N * top_k < 2^31 - 128)");
-  if (N > 65535 && (ex->H > 4096)) return fail(SMOE_EINVAL, "H > 4096: N <= 65535");
+  if (N > (ex->H > 4096 ? 65535 : 65535 * 64)) return fail(SMOE_EINVAL, "N <= 4194240, with H > 4096 N <= 65535");
   return SMOE_OK;
 }
 

@@ -459,7 +459,7 @@ int go_tile(const BlockGemm& a, hipStream_t s) {
   // at most one partly filled row tile for every group with rows
   const int64_t tiles = (static_cast<int64_t>(rows) + BM - 1) / BM + (a.G > 0 ? std::min(a.G, rows) : 0);
   const int64_t grid = tiles * ((static_cast<int64_t>(a.N_out) + CH - 1) / CH);
-  if (grid > 0x7fffffff) return SMOE_EINVAL;
+  if (grid * 64 * WM * WN > 0xffffffffll) return SMOE_EINVAL;  // threads of a launch
   SMOE_LAUNCH((k_gemm_blocks<EPI, ODT, WIDE, BM, BN, WM, WN, NS>), dim3(static_cast<unsigned>(grid)),
               dim3(64 * WM * WN), 0, s, a);
   return rc();
@@ -539,7 +539,7 @@ int launch_quantize_fp8_blocks(const BlockQuant& q, hipStream_t s) {
   const int64_t total = square ? static_cast<int64_t>(q.groups) * rblk * nblk
                                : static_cast<int64_t>(q.groups) * q.rows * nblk;
   const int64_t wgs = square ? total : (total + 15) / 16;
-  if (wgs > 0x7fffffff) return SMOE_EINVAL;
+  if (wgs * 256 > 0xffffffffll) return SMOE_EINVAL;  // threads of a launch
   return by_xdt(q.x_dtype, [&](auto xd) {
     constexpr int XD = decltype(xd)::value;
     if (square)

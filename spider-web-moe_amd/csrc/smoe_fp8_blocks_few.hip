@@ -487,7 +487,7 @@ int rc() { return hipGetLastError() == hipSuccess ? SMOE_OK : SMOE_EHIP; }
 template <int EPI, int ODT, bool WIDE, int MT, int XQ>
 int go_few(const BlockGemm& a, hipStream_t s) {
   const int64_t grid = (static_cast<int64_t>(a.single_rows) + 16 * MT - 1) / (16 * MT) * ((static_cast<int64_t>(a.N_out) + 15) / 16);
-  if (grid > 0x7fffffff) return SMOE_EINVAL;
+  if (grid * 256 > 0xffffffffll) return SMOE_EINVAL;  // threads of a launch
   const size_t lds = XQ >= 0 ? static_cast<size_t>(16 * MT) * fp8_blocks_of(a.K) * 132 : 0;
   SMOE_LAUNCH((k_blocks_few<EPI, ODT, WIDE, MT, XQ>), dim3(static_cast<unsigned>(grid)), dim3(256), lds, s, a);
   return rc();
@@ -523,7 +523,7 @@ bool prep_fits(int N, int K, int E) {
 int launch_prep(const PrepArgs& a, const BlockQuant& q, hipStream_t s) {
   const int nblk = fp8_blocks_of(q.cols);
   const int64_t total = static_cast<int64_t>(q.rows) * nblk, wgs = (total + 63) / 64 + 1;
-  if (wgs > 0x7fffffff) return SMOE_EINVAL;
+  if (wgs * 1024 > 0xffffffffll) return SMOE_EINVAL;  // threads of a launch
   const dim3 grid(static_cast<unsigned>(wgs)), block(1024);
   if (a.K <= 2) hipLaunchKernelGGL((k_prep<2>), grid, block, 0, s, a, q, nblk, total);
   else if (a.K <= 4) hipLaunchKernelGGL((k_prep<4>), grid, block, 0, s, a, q, nblk, total);

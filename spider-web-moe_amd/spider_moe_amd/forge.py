@@ -178,6 +178,8 @@ def select_groups(logits: torch.Tensor, k: int, *, score: str = "sigmoid", bias=
                   scale: float = 1.0):
     """smoe_select_groups over the last dimension (ForgeSelect.route_groups)."""
     nat.require_gpu(logits, bias)
+    if logits.ndim < 1 or logits.numel() > 0x7fffffff * logits.shape[-1]:
+        raise ValueError(f"logits must be [.., E], got {tuple(logits.shape)}")
     if score not in nat.SCORES:
         raise ValueError("score must be 'softmax' or 'sigmoid'")
     if bias is not None:
@@ -224,6 +226,8 @@ def _linear_fp8_blocks(x, codes, scale, bias, act):
                          f"got {scale.dtype} {tuple(scale.shape)}")
     if act not in _ACT:
         raise ValueError("act must be None or 'gelu'")
+    if max(k, n_out) > 0x7fffff00 or x.numel() > 0x7fffff00 * k:
+        raise ValueError("more than 2^31 - 256 rows, K or N_out")
     if bias is not None:
         if bias.shape != (n_out,):
             raise ValueError(f"bias must be [{n_out}], got {tuple(bias.shape)}")

@@ -18,6 +18,7 @@ quantize_fp8_blocks / dequantize_fp8_blocks.
 """
 from __future__ import annotations
 
+import math
 from dataclasses import dataclass
 
 import torch
@@ -187,9 +188,9 @@ def quantize_fp8_blocks(x: torch.Tensor, *, block_rows: int = FP8_BLOCK):
         ldx = cols if x.is_contiguous() else _row_stride(x)
         if ldx is None:
             x, ldx = x.contiguous(), cols
-        g = 1
-        for n in lead:
-            g *= n
+        g = math.prod(lead)
+        if max(g, rows, cols) > 0x7fffffff:
+            raise ValueError("more than 2^31 - 1 rows, columns or matrices")
         codes = torch.empty(*lead, rows, ld, dtype=torch.float8_e4m3fn, device=x.device)
         scale = torch.empty(*lead, rb, cb, dtype=torch.float32, device=x.device)
         nat.launch(x.device, "smoe_quantize_fp8_blocks", x.data_ptr(), nat.float_code(x.dtype), g, rows,

@@ -167,12 +167,14 @@ def sparse_expert_delta_fp8_blocks(messages: torch.Tensor, top_indices: torch.Te
         raise ValueError("top_indices and top_weights must be messages' shape with K last")
     code = nat.dtype_code(messages.dtype)
     idx, wts = top_indices, top_weights
-    if idx.dtype != torch.int32:
-        idx = idx.to(torch.int32)
+    if idx.dtype != torch.int32:  # ids past 32 bits stay outside [0, E)
+        idx = idx.clamp(-1, experts.num_experts).to(torch.int32)
     if wts.dtype != torch.float32:
         wts = wts.float()
     msg, idx, wts = messages.contiguous(), idx.contiguous(), wts.contiguous()
     n = idx.numel() // k if k else 0
+    if n > 0x7fffffff:
+        raise ValueError("more than 2^31 - 1 tokens")
     delta = torch.empty(messages.shape, dtype=messages.dtype, device=dev)
     lib = nat.lib()
     need = lib.smoe_expert_delta_fp8_blocks_workspace_bytes(experts._ref, n, k)

@@ -30,6 +30,7 @@ def test_select_groups_refusals(lib):
                 dict(z=None), dict(w=None), dict(i=None)):
         assert go(**bad) == 1, bad
     assert go(n=0, z=None, w=None, i=None) == 0
+    assert go(n=1 << 26) == 1
 
     def back(dt=nat.F32, n=4, e=16, k=2, score=0, z=FAKE, i=FAKE, g=FAKE, d=FAKE):
         return lib.smoe_select_groups_backward(z, dt, n, e, k, score, 1, 1.0, i, g, d, None)
@@ -52,6 +53,8 @@ def test_quantizer_refusals(lib):
                 dict(q=FAKE + 8), dict(q=None), dict(s=None), dict(x=None)):
         assert go(**bad) == 1, bad
     assert go(r=0) == 0 and go(g=0) == 0
+    assert go(g=1 << 15, r=1 << 13, c=129, ldx=129, ld=144) == 1  # 2^28 rows of two blocks
+    assert go(g=1 << 24, r=129, br=128) == 1
 
 
 def test_linear_refusals(lib):
@@ -99,7 +102,8 @@ def test_expert_refusals(lib):
                 dict(out=None), dict(ws=None), dict(ws=FAKE + 8)):
         assert go(ok, **bad) == 1, bad
     assert go(ok, dt=nat.F16) == -2 and go(ok, od=nat.FP8_E4M3) == -2
-    assert go(desc(H=8192), n=70000) == 1
+    assert go(desc(H=8192), n=70000) == 1 and go(ok, n=65535 * 64 + 1) == 1
+    assert size(ctypes.byref(ok), 65535 * 64 + 1, 2) == 0
     need = size(ctypes.byref(ok), 4, 2)
     assert need > 0 and go(ok, wb=need - 1) == 3
     assert go(ok, n=0) == 0

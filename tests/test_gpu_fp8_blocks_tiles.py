@@ -1,8 +1,8 @@
-"""Block-scaled fp8 products with more tiles than the card has CUs, where a
-workgroup walks from tile to tile: ragged rows, channels and K, one to four
-stages of K (an odd number swaps the ring's slots from tile to tile), channels
-that cannot leave in whole 16-byte chunks, more groups than a wave has lanes,
-groups without rows.  Tolerances: those of tests/test_gpu_fp8_blocks.py."""
+"""Block-scaled fp8 products with more tiles than the card has CUs: ragged
+rows, channels and K, one to four stages of K, channels that cannot leave in
+whole 16-byte chunks, more groups than a wave has lanes, groups without rows;
+every kind of dispatch plan; captured steps.  Tolerances: those of
+tests/test_gpu_fp8_blocks.py."""
 import pytest
 import torch
 
@@ -47,3 +47,60 @@ def test_expert_delta_over_many_tiles(activation, bias, n, e, k, h, u):
     assert torch.equal(got, again)
     _check_delta(got, O.expert_delta(msg.view(n, h), idx, w, ex.w_up, ex.s_up, ex.w_down, ex.s_down, ex.b_up, ex.b_down,
                                      activation))
+
+
+@pytest.mark.parametrize("n,e,k", [(3, 70, 4), (300, 70, 6), (300, 5, 20), (1300, 70, 6), (1300, 24, 20)])
+def test_expert_delta_every_plan(n, e, k):
+    """The few-token step, the plan by bit masks and the general one: more
+    experts than a wave has lanes, more choices than the bit masks take
+    (k > 16), the same id several times in a row of choices, int64 ids past 32
+    bits (outside [0, E), as any other id there)."""
+    from spider_moe_amd import sparse_expert_delta_fp8_blocks
+    say("expert delta, plans", n, e, k)
+    g = torch.Generator().manual_seed(n + e + k)
+    ex = _experts(g, e, 144, 80, "swiglu", True)
+    msg = torch.randn(n, 144, generator=g)
+    idx = torch.randint(0, e, (n, k), generator=g)
+    w = torch.rand(n, k, generator=g)
+    idx[0] = e - 1
+    idx[1, :2] = torch.tensor([1 << 32, -(1 << 32)])
+    got = sparse_expert_delta_fp8_blocks(msg.to(dev), idx.to(dev), w.to(dev), ex)
+    ids = torch.where((idx >= 0) & (idx < e), idx, torch.full_like(idx, -1))
+    _check_delta(got, O.expert_delta(msg, ids, w, ex.w_up, ex.s_up, ex.w_down, ex.s_down, ex.b_up, ex.b_down, "swiglu"))
+
+
+def test_captured_steps_beside_eager_ones():
+    """Two captured steps of different sizes replayed in turn with eager calls
+    and another stream's between them: each replay gives the eager result."""
+    from spider_moe_amd import ForgeSelect, sparse_expert_delta_fp8_blocks
+    say("captured steps")
+    g = torch.Generator().manual_seed(21)
+    ex = _experts(g, 16, 272, 144, "swiglu", True)
+    select = ForgeSelect()
+
+    def step(x, z):
+        w, idx = select.route_groups(z, top_k=2, num_groups=4, top_groups=2)
+        return sparse_expert_delta_fp8_blocks(x, idx, w, ex)
+
+    held, graphs = [], []
+    for n in (5, 300, 1100):  # few tokens, plan by bit masks, general plan
+        x = torch.randn(n, 272, generator=g).bfloat16().to(dev)
+        z = torch.randn(n, 16, generator=g).to(dev)
+        step(x, z)
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = step(x, z)
+        held.append((x, z, out))
+        graphs.append(gr)
+    side = torch.cuda.Stream()
+    for r in range(3):
+        for (x, z, out), gr in zip(held, graphs):
+            x.copy_(torch.randn(x.shape, generator=g).bfloat16())
+            z.copy_(torch.randn(z.shape, generator=g))
+            torch.cuda.synchronize()
+            gr.replay()
+            with torch.cuda.stream(side):  # at the same time
+                beside = step(x, z)
+            torch.cuda.synchronize()
+            assert torch.equal(out, step(x, z)) and torch.equal(beside, out), (r, len(x))
