@@ -498,15 +498,19 @@ int go_dense(const BlockGemm& a, hipStream_t s) {
 // where that leaves CUs without a tile; a third stage where a tile has its CU
 // for itself.  Whole expert steps: 32 rows up to 40 a group (64 tokens, top-2 of
 // 64: 77 us with 64-row tiles, 72 with 32, 59 with the third stage), 64 up to
-// 112 (777 tokens, top-4 of 32: 59 us with 128-row tiles, 54 with 64, 62 with
-// 32), 128 above (1500 tokens: 75, 79, 89), 256 from 512 on (12000 tokens, top-2
-// of 16 SwiGLU: 422 -> 357; 3000 tokens: 122 -> 130).
+// 112 (777 tokens, top-4 of 32: 49 us with 128-row tiles, 45 with 64, 52 with
+// 32), 128 above (1500 tokens, top-2 of 16 SwiGLU: 81, 84, 114), 256 from 512 on
+// (6000 tokens: 208 -> 181 us; 2500: 102 -> 119).  GELU's up product keeps 128
+// rows, whose two workgroups a CU hide one's epilogue under the other's products
+// (6000 tokens, top-4 of 32: 183 us with 256, 172).
 template <int EPI>
 int go_grouped(const BlockGemm& a, hipStream_t s) {
   constexpr int O = SMOE_F32;
   constexpr bool SW = EPI == BLK_UP_SWIGLU;
   const int64_t cus = device_cus(), per = (static_cast<int64_t>(a.max_rows) + a.G - 1) / a.G;
-  if (per >= 512 && tiles_of(a, 256, SW ? 128 : 256) * 8 >= cus * 5) return go_tile<EPI, O, false, 256, 256, 2, 4, 2>(a, s);
+  if constexpr (EPI != BLK_UP_GELU) {
+    if (per >= 512 && tiles_of(a, 256, SW ? 128 : 256) * 8 >= cus * 5) return go_tile<EPI, O, false, 256, 256, 2, 4, 2>(a, s);
+  }
   int BM = per <= (SW ? 28 : 40) ? 32 : (per <= 112 ? 64 : 128);
   while (BM > 32 && tiles_of(a, BM, 128) < cus) BM /= 2;
   if constexpr (SW) {  // 256 weight rows a stage: one workgroup a CU with two stages already
