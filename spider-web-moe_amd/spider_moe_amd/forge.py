@@ -132,45 +132,40 @@ def select_topk(logits: torch.Tensor, k: int, mode: int):
     return w.view(*lead, k).to(out_dtype), idx.view(*lead, k).long()
 
 
-def _select_groups_fwd(x, k, score, bias, num_groups, top_groups, renormalize, scale):
-    """x: contiguous logits."""
-    dev, shape = x.device, x.shape
-    out = (*shape[:-1], k)
-    w = torch.empty(out, dtype=torch.float32, device=dev)
-    idx = torch.empty(out, dtype=torch.int32, device=dev)
-    e = shape[-1]
+def _select_groups_fwd(x, idx, k, score, bias, num_groups, top_groups, renormalize, scale):
+    """x: contiguous logits; fills idx, returns the weights."""
+    dev = x.device
+    w = torch.empty(idx.shape, dtype=torch.float32, device=dev)
+    e = x.shape[-1]
     nat.launch(dev, "smoe_select_groups", x.data_ptr(), nat.float_code(x.dtype),
                x.numel() // e if e else 0, e, k, score, None if bias is None else bias.data_ptr(),
                num_groups, top_groups, renormalize, scale, w.data_ptr(), idx.data_ptr())
-    return w, idx
+    return w
 
 
 class _SelectGroups(torch.autograd.Function):
+    # idx is filled, not returned: a second output and its bookkeeping cost the
+    # host 4 us of a step's 86
     @staticmethod
-    def forward(ctx, logits, k, score, bias, num_groups, top_groups, renormalize, scale):
+    def forward(ctx, logits, idx, how):
         x = logits.contiguous()
-        w, idx = _select_groups_fwd(x, k, score, bias, num_groups, top_groups, renormalize, scale)
         ctx.save_for_backward(x, idx)
-        ctx.how = (score, renormalize, scale)
-        ctx.mark_non_differentiable(idx)
-        ctx.set_materialize_grads(False)  # no zeros for idx
-        return w, idx
+        ctx.how = how
+        return _select_groups_fwd(x, idx, *how)
 
     @staticmethod
-    def backward(ctx, d_w, _):
-        if d_w is None:
-            return (None,) * 8
+    def backward(ctx, d_w):
         if torch.is_grad_enabled():
             raise RuntimeError("route_groups is not twice differentiable")
         x, idx = ctx.saved_tensors
-        score, renormalize, scale = ctx.how
+        k, score, _, _, _, renormalize, scale = ctx.how
         d = torch.empty_like(x)
-        e, k = x.shape[-1], idx.shape[-1]
+        e = x.shape[-1]
         d_w = d_w.contiguous()
         nat.launch(x.device, "smoe_select_groups_backward", x.data_ptr(), nat.float_code(x.dtype),
                    x.numel() // e, e, k, score, renormalize, scale, idx.data_ptr(), d_w.data_ptr(),
                    d.data_ptr())
-        return d, None, None, None, None, None, None, None
+        return d, None, None
 
 
 def select_groups(logits: torch.Tensor, k: int, *, score: str = "sigmoid", bias=None,
@@ -188,11 +183,11 @@ def select_groups(logits: torch.Tensor, k: int, *, score: str = "sigmoid", bias=
         if bias.dtype != torch.float32:
             bias = bias.float()
         bias = bias.detach().contiguous()
+    idx = torch.empty((*logits.shape[:-1], k), dtype=torch.int32, device=logits.device)
+    how = (k, nat.SCORES[score], bias, num_groups, top_groups, renormalize, scale)
     if torch.is_grad_enabled() and logits.requires_grad:
-        return _SelectGroups.apply(logits, k, nat.SCORES[score], bias, num_groups, top_groups,
-                                   renormalize, scale)
-    return _select_groups_fwd(logits.contiguous(), k, nat.SCORES[score], bias, num_groups,
-                              top_groups, renormalize, scale)
+        return _SelectGroups.apply(logits, idx, how), idx
+    return _select_groups_fwd(logits.contiguous(), idx, *how), idx
 
 
 # ------------------------------------------------------------------ gemm ----
