@@ -177,12 +177,13 @@ __device__ __forceinline__ void groups64(const BlockGemm& p, int BM, int b, int&
   t = i < p.G ? (hi - lo + BM - 1) / BM : 0;
 }
 
-// The tile of workgroup bid: group by group; within a group kSuperRows row
-// tiles at a time, over them strip by strip with the strip's row tiles next to
-// each other, so that the rows in use stay in an L2 while the strips' weights
-// pass.  Workgroup ids are dealt to the 8 XCDs round robin and each XCD takes
-// one contiguous part of the order.
-constexpr int kSuperRows = 8;
+// The tile of workgroup bid: group by group; within a group SUPER row tiles at
+// a time, over them strip by strip with the strip's row tiles next to each
+// other, so that the rows in use stay in an L2 while the strips' weights pass.
+// Workgroup ids are dealt to the 8 XCDs round robin and each XCD takes one
+// contiguous part of the order.  SUPER: an XCD holds 32 tiles of 256 rows (64 of
+// 128) at a time (32768 routed rows, 2048 -> 1408 SwiGLU, 256 rows a tile: 2
+// row tiles 250 us, 4 252, 8 260, 16 256; 1024 -> 5632: 119, 117, 118, 121).
 template <int BM, int BN>
 __device__ __forceinline__ bool block_tile(const BlockGemm& p, int bid, int& g, int& m0, int& mrows,
                                            int& n0) {
@@ -222,9 +223,10 @@ __device__ __forceinline__ bool block_tile(const BlockGemm& p, int bid, int& g, 
     }
   }
   const int tm = (hi - lo + BM - 1) / BM;
-  const int super = in / (kSuperRows * strips), rest = in - super * kSuperRows * strips;
-  const int sr = min(kSuperRows, tm - super * kSuperRows);  // row tiles of this part
-  m0 = lo + (super * kSuperRows + rest % sr) * BM;
+  constexpr int SUPER = BM == 256 ? 4 : 8;
+  const int super = in / (SUPER * strips), rest = in - super * SUPER * strips;
+  const int sr = min(SUPER, tm - super * SUPER);  // row tiles of this part
+  m0 = lo + (super * SUPER + rest % sr) * BM;
   mrows = min(BM, hi - m0);
   n0 = (rest / sr) * BN;
   return true;
