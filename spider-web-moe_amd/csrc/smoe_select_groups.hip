@@ -272,7 +272,9 @@ __device__ __forceinline__ bool choose(const float (&z)[V], const SelectArgs& a,
 // One wave per token.  The choice is made in f32 and, where two values that
 // decide lie nearer than f32 tells apart, once more in f64 (sigmoid scores of
 // 256 experts: about 1 token in 100), so that it is the order of the real
-// values: 16384 tokens over 256 experts 66 us all in f64, 17 so.
+// values: 16384 tokens over 256 experts in 8 groups, top 8 of 4 groups, 66 us
+// all in f64, 37 so.  Bound by instructions: about 1200 a token, half of them
+// the K rounds of a maximum over the wave; the bytes are 4 us.
 template <int DT, int V>
 __global__ __launch_bounds__(256) void k_select_groups(const void* __restrict__ logits, int N, bool vec,
                                                        const SelectArgs a, float* __restrict__ top_w,
@@ -303,8 +305,8 @@ __global__ __launch_bounds__(256) void k_select_groups(const void* __restrict__ 
 //   else               ds_j = scale * g_j
 //   sigmoid: dz_e = ds_e s_e (1 - s_e);  softmax: dz_e = s_e (ds_e - sum_i s_i ds_i)
 // An expert chosen in several slots takes all their gradients; ids outside
-// [0, E) none.  One wave per token, lane j < K the slot j as well: bound by the
-// logits read and the gradients written.
+// [0, E) none.  One wave per token, lane j < K the slot j as well: 16384 tokens
+// over 256 experts in 15.6 us, 34 MB at 2.2 TB/s.
 template <int DT, int V>
 __global__ __launch_bounds__(256) void k_select_groups_bwd(const void* __restrict__ logits, int N, bool vec,
                                                            const SelectArgs a,
