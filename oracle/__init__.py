@@ -12,6 +12,9 @@ quant   int4 / fp8-e4m3 weight formats (numpy, integer / byte arithmetic)
 plan    dispatch plan: per-expert token lists (numpy, integer)
 block   router, edge generator, message pass, expert FFN, epilogue, block
         forward (torch on the CPU, float32 math)
+fp8_blocks  group-limited routing, block-scaled fp8 quantizer, linear and
+        expert FFN (torch on the CPU, 64-bit math), and how far a right result
+        may be off; no counterpart in the reference
 lm      the SpiderWebLM shell around the block (attention prelude / coda)
 ref     ctypes binding of the reference's own scalar C++ library, compiled
         from its sources into ``oracle/_ref`` by ``oracle/Makefile``

@@ -12,8 +12,8 @@ int device_cus();
 namespace {
 
 // 1 x 128 blocks (quant_row_block), sixteen a workgroup, a block's 128 columns
-// by 16 lanes in one load each.  Bound by the bytes: bf16 16384 x 2048 in 12.8
-// us, 101 MB at 7.9 TB/s (the input is in the last-level cache).
+// by 16 lanes in one load each.  Bound by the bytes: bf16 16384 x 1024 in 12.8
+// us, 51 MB at 4.0 TB/s.
 template <int XDT>
 __global__ __launch_bounds__(256) void k_quant_row_blocks(const BlockQuant q, int nblk, int64_t total) {
   quant_row_block<XDT>(q, nblk, total, (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 4,

@@ -182,7 +182,7 @@ __device__ __forceinline__ void groups64(const BlockGemm& p, int BM, int b, int&
 // other, so that the rows in use stay in an L2 while the strips' weights pass.
 // Workgroup ids are dealt to the 8 XCDs round robin and each XCD takes one
 // contiguous part of the order.  SUPER: an XCD holds 32 tiles of 256 rows (64 of
-// 128) at a time (32768 routed rows, 2048 -> 1408 SwiGLU, 256 rows a tile: 2
+// 128) at a time (32768 routed rows, 1024 -> 2816 SwiGLU, 256 rows a tile: 2
 // row tiles 250 us, 4 252, 8 260, 16 256; 1024 -> 5632: 119, 117, 118, 121).
 template <int BM, int BN>
 __device__ __forceinline__ bool block_tile(const BlockGemm& p, int bid, int& g, int& m0, int& mrows,
