@@ -132,14 +132,12 @@ def select_topk(logits: torch.Tensor, k: int, mode: int):
     return w.view(*lead, k).to(out_dtype), idx.view(*lead, k).long()
 
 
-def _select_groups_fwd(x, idx, k, score, bias, num_groups, top_groups, renormalize, scale):
-    """x: contiguous logits; fills idx, returns the weights."""
-    dev = x.device
-    w = torch.empty(idx.shape, dtype=torch.float32, device=dev)
-    e = x.shape[-1]
-    nat.launch(dev, "smoe_select_groups", x.data_ptr(), nat.float_code(x.dtype),
-               x.numel() // e if e else 0, e, k, score, None if bias is None else bias.data_ptr(),
-               num_groups, top_groups, renormalize, scale, w.data_ptr(), idx.data_ptr())
+def _select_groups_fwd(x, n, e, idx, k, score, bias, num_groups, top_groups, renormalize, scale):
+    """x: contiguous logits, n rows of e; fills idx, returns the weights."""
+    w = torch.empty(idx.shape, dtype=torch.float32, device=x.device)
+    nat.launch(x.device, "smoe_select_groups", x.data_ptr(), nat.float_code(x.dtype), n, e, k, score,
+               None if bias is None else bias.data_ptr(), num_groups, top_groups, renormalize, scale,
+               w.data_ptr(), idx.data_ptr())
     return w
 
 
@@ -147,47 +145,48 @@ class _SelectGroups(torch.autograd.Function):
     # idx is filled, not returned: a second output and its bookkeeping cost the
     # host 4 us of a step's 86
     @staticmethod
-    def forward(ctx, logits, idx, how):
+    def forward(ctx, logits, n, e, idx, how):
         x = logits.contiguous()
         ctx.save_for_backward(x, idx)
-        ctx.how = how
-        return _select_groups_fwd(x, idx, *how)
+        ctx.how = n, e, how
+        return _select_groups_fwd(x, n, e, idx, *how)
 
     @staticmethod
     def backward(ctx, d_w):
         if torch.is_grad_enabled():
             raise RuntimeError("route_groups is not twice differentiable")
         x, idx = ctx.saved_tensors
-        k, score, _, _, _, renormalize, scale = ctx.how
+        n, e, (k, score, _, _, _, renormalize, scale) = ctx.how
         d = torch.empty_like(x)
-        e = x.shape[-1]
         d_w = d_w.contiguous()
-        nat.launch(x.device, "smoe_select_groups_backward", x.data_ptr(), nat.float_code(x.dtype),
-                   x.numel() // e, e, k, score, renormalize, scale, idx.data_ptr(), d_w.data_ptr(),
-                   d.data_ptr())
-        return d, None, None
+        nat.launch(x.device, "smoe_select_groups_backward", x.data_ptr(), nat.float_code(x.dtype), n, e, k,
+                   score, renormalize, scale, idx.data_ptr(), d_w.data_ptr(), d.data_ptr())
+        return d, None, None, None, None
 
 
 def select_groups(logits: torch.Tensor, k: int, *, score: str = "sigmoid", bias=None,
                   num_groups: int = 1, top_groups: int = 1, renormalize: bool = True,
                   scale: float = 1.0):
     """smoe_select_groups over the last dimension (ForgeSelect.route_groups)."""
-    nat.require_gpu(logits, bias)
-    if logits.ndim < 1 or logits.numel() > 0x7fffffff * logits.shape[-1]:
-        raise ValueError(f"logits must be [.., E], got {tuple(logits.shape)}")
+    dev = nat.require_gpu(logits, bias)
+    shape = logits.shape
+    e = shape[-1] if shape else 0
+    n = logits.numel() // e if e else 0
+    if not shape or n > 0x7fffffff:
+        raise ValueError(f"logits must be [.., E], got {tuple(shape)}")
     if score not in nat.SCORES:
         raise ValueError("score must be 'softmax' or 'sigmoid'")
     if bias is not None:
-        if bias.shape != logits.shape[-1:]:
-            raise ValueError(f"bias must be [{logits.shape[-1]}], got {tuple(bias.shape)}")
+        if bias.shape != shape[-1:]:
+            raise ValueError(f"bias must be [{e}], got {tuple(bias.shape)}")
         if bias.dtype != torch.float32:
             bias = bias.float()
-        bias = bias.detach().contiguous()
-    idx = torch.empty((*logits.shape[:-1], k), dtype=torch.int32, device=logits.device)
+        bias = bias.contiguous()
+    idx = torch.empty((*shape[:-1], k), dtype=torch.int32, device=dev)
     how = (k, nat.SCORES[score], bias, num_groups, top_groups, renormalize, scale)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _SelectGroups.apply(logits, idx, how), idx
-    return _select_groups_fwd(logits.contiguous(), idx, *how), idx
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _SelectGroups.apply(logits, n, e, idx, how), idx
+    return _select_groups_fwd(logits.contiguous(), n, e, idx, *how), idx
 
 
 # ------------------------------------------------------------------ gemm ----
@@ -226,7 +225,7 @@ def _linear_fp8_blocks(x, codes, scale, bias, act):
     if bias is not None:
         if bias.shape != (n_out,):
             raise ValueError(f"bias must be [{n_out}], got {tuple(bias.shape)}")
-        bias = bias.detach().float().contiguous()
+        bias = bias.float().contiguous()
     if x.ndim == 2 and x.stride(1) == 1 and x.stride(0) >= k:
         ldx = x.stride(0)
     else:
@@ -394,14 +393,13 @@ class ForgeGEMM:
         self.calls += 1
         return self._run(x, weight, bias, None, True, quantize_input).to(x.dtype)
 
-    @torch.no_grad()
     def linear_fp8_blocks(self, x, codes, scale, bias=None, *, act: str | None = None):
         """act(x . W^T + bias) with W held as e4m3 codes [N_out, K] and one
         scale per 128 x 128 block (quantize_fp8_blocks), x [..., K] quantized
         in 1 x 128 blocks on the way (smoe_linear_fp8_blocks); act None or
         "gelu" (erf).  Result in x's dtype: bfloat16 from e4m3 x e4m3
         products, float32 (and float16) from the same values' products with
-        f32 sums throughout."""
+        f32 sums throughout.  No gradient."""
         self.calls += 1
         return _linear_fp8_blocks(x, codes, scale, bias, act)
 

@@ -177,7 +177,6 @@ def quantize_fp8_blocks(x: torch.Tensor, *, block_rows: int = FP8_BLOCK):
         raise ValueError("block_rows must be 1 or 128")
     if x.ndim < 2 or x.shape[-1] < 1:
         raise ValueError("x must be [.., rows, cols] with cols >= 1")
-    x = x.detach()
     if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         x = x.float()
     *lead, rows, cols = x.shape
@@ -195,7 +194,8 @@ def quantize_fp8_blocks(x: torch.Tensor, *, block_rows: int = FP8_BLOCK):
         scale = torch.empty(*lead, rb, cb, dtype=torch.float32, device=x.device)
         nat.launch(x.device, "smoe_quantize_fp8_blocks", x.data_ptr(), nat.float_code(x.dtype), g, rows,
                    cols, ldx, block_rows, codes.data_ptr(), ld, scale.data_ptr())
-        return (codes if ld == cols else codes[..., :cols]), scale
+        return (codes if ld == cols else codes.narrow(-1, 0, cols)), scale
+    x = x.detach()
     p = torch.zeros(*lead, rb * block_rows, cb * FP8_BLOCK)
     p[..., :rows, :cols] = x
     p = p.view(*lead, rb, block_rows, cb, FP8_BLOCK)

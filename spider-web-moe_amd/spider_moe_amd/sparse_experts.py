@@ -152,13 +152,13 @@ class Fp8BlockExperts:
         return cls(q, s, qd, sd, b_up=b_up, b_down=b_down, activation=activation)
 
 
-@torch.no_grad()
 def sparse_expert_delta_fp8_blocks(messages: torch.Tensor, top_indices: torch.Tensor,
                                    top_weights: torch.Tensor, experts: Fp8BlockExperts) -> torch.Tensor:
     """sparse_expert_delta on Fp8BlockExperts: messages [..,H] (float32 or
     bfloat16), top_indices / top_weights [..,K] -> delta [..,H] in messages'
     dtype.  Messages and hidden activations are quantized in 1 x 128 blocks on
-    the way into the two products; everything else is summed in f32."""
+    the way into the two products; everything else is summed in f32.  No
+    gradient."""
     dev = nat.require_gpu(messages, top_indices, top_weights, experts.w_up)
     h, k = messages.shape[-1], top_indices.shape[-1]
     if h != experts.hidden_size:
