@@ -22,7 +22,8 @@ __global__ __launch_bounds__(256) void k_quant_row_blocks(const BlockQuant q, in
 
 // 128 x 128 blocks: a workgroup holds a block in registers (one read, one
 // write), thread t the columns 8 (t % 16) .. + 7 of rows t / 16, t / 16 + 16, ..
-// Bound by the bytes: bf16 16384 x 2816 in 27.5 us, 138 MB at 5.0 TB/s.
+// Bound by the bytes: bf16 16384 x 2816, 138 MB, one call after another 26.8 us
+// at 5.2 TB/s (30.8 with plain stores).
 template <int XDT>
 __global__ __launch_bounds__(256) void k_quant_square_blocks(const BlockQuant q, int rblk, int nblk) {
   __shared__ uint32_t red[4];
@@ -50,8 +51,8 @@ __global__ __launch_bounds__(256) void k_quant_square_blocks(const BlockQuant q,
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = r0 + (threadIdx.x >> 4) + 16 * i;
-    if (r < q.rows)
-      *reinterpret_cast<u32x2*>(q.codes + (g * q.rows + r) * q.ld_out + c) = codes8(v[i], sc);
+    if (r < q.rows)  // past the L2s, which would write them back at the kernel's end
+      __builtin_nontemporal_store(codes8(v[i], sc), reinterpret_cast<u32x2*>(q.codes + (g * q.rows + r) * q.ld_out + c));
   }
 }
 
