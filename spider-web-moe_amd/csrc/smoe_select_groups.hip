@@ -300,7 +300,9 @@ __global__ __launch_bounds__(256) void k_select_groups(const void* __restrict__ 
 }
 
 // d loss / d z_e.  With S = sum of the chosen s and g_j = d loss / d w_j:
-//   renorm, S >= 1e-9: ds_j = scale / S * (g_j - sum_i g_i s_i / S)
+//   renorm, S >= 1e-9: ds_j = scale / S * (g_j - g_0 - sum_i (g_i - g_0) s_i / S),
+//                      g_0 that of the first slot: 0 where the weights cannot
+//                      change the loss (one slot, or equal g), and no worse else
 //   renorm, otherwise: ds_j = scale / 1e-9 * g_j       (the clamped sum is a constant)
 //   else               ds_j = scale * g_j
 //   sigmoid: dz_e = ds_e s_e (1 - s_e);  softmax: dz_e = s_e (ds_e - sum_i s_i ds_i)
@@ -352,10 +354,14 @@ __global__ __launch_bounds__(256) void k_select_groups_bwd(const void* __restric
   };
   float unused;
   const float ss = used ? score(zs, unused) : 0.f;
-  const float total = wave_sum(ss), dot = wave_sum(used ? g * ss : 0.f);
+  const float total = wave_sum(ss);
   const bool over = total >= 1e-9f || total != total;
   const float f = a.renorm ? a.scale / (over ? total : 1e-9f) : a.scale;
-  const float ds_slot = used ? f * (g - (a.renorm && over ? dot / total : 0.f)) : 0.f;
+  const bool centred = a.renorm && over;  // uniform
+  const uint64_t slots = __ballot(used);
+  const float gc = centred && slots ? g - lane_f(g, __builtin_ctzll(slots)) : g;
+  const float dot = wave_sum(used ? gc * ss : 0.f);
+  const float ds_slot = used ? f * (gc - (centred ? dot / total : 0.f)) : 0.f;
   const float mean = a.sigmoid ? 0.f : wave_sum(used ? ss * ds_slot : 0.f);
   float d[V];
 #pragma unroll

@@ -315,3 +315,16 @@ def test_routes_into_the_dispatch_plan():
     assert plan.counts.cpu().numpy().tolist() == cnt.tolist()
     assert plan.rows.cpu().numpy().tolist() == perm.tolist()
     assert np.array_equal(plan.row_weights.cpu().numpy(), pw)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("n,e,k", [(597, 16, 1), (40, 255, 7)])
+def test_gradient_is_zero_where_the_weights_cannot_matter(score, n, e, k):
+    """Renormalised weights add up to the scale: one slot, or slots of equal
+    gradients, cannot change the loss, and the gradient is 0, not a rounding."""
+    say("zero gradient", score, n, e, k)
+    g = torch.Generator().manual_seed(n)
+    zg = (torch.randn(n, e, generator=g) * 2).to(dev).requires_grad_(True)
+    w, _ = _route(zg, k, score=score, scale=2.5)
+    (d,) = torch.autograd.grad(w, zg, torch.randn(n, 1, generator=g).expand(n, k).to(dev))
+    assert not bool(d.any())
