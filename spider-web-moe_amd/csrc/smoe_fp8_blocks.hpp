@@ -76,7 +76,6 @@ bool linear_quantizes_inside(int N, int K);
 
 // A small step's dispatch plan (smoe_dispatch_plan's: offsets [E + 1], rows,
 // row weights, tokrow [N, K]) and the quantized messages in one launch.
-constexpr int kPrepMaxN = 1024;
 struct PrepArgs {
   const int32_t* idx = nullptr;
   const float* w = nullptr;

@@ -400,23 +400,22 @@ __global__ __launch_bounds__(512, 4) void k_tokens_down(const TokensArgs a) {
   }
 }
 
-// The plan of a decode step or a short prompt (K <= KB) and its quantized
-// messages in one launch: workgroup 0 makes the plan (the one
+// The plan of a decode step or a short prompt (K <= KB, N <= 1024 T) and its
+// quantized messages in one launch: workgroup 0 makes the plan (the one
 // smoe_dispatch_plan makes), the others quantize 64 blocks each.
 //
-// A token per thread, its slots in registers: ids that occur twice are merged
-// into their first slot (weights added in slot order from 0), ids outside
-// [0, E) and sums that are not > 0 left out.  Every kept (token, expert) sets
-// the token's bit in the expert's masks, one word for 64 tokens, by an LDS
-// atomic OR (its result does not depend on the order); a row is then the
-// expert's offset, its counts in the words before and the bits below.
+// T tokens per thread, their slots in registers: ids that occur twice are
+// merged into their first slot (weights added in slot order from 0), ids
+// outside [0, E) and sums that are not > 0 left out.  Every kept (token,
+// expert) sets the token's bit in the expert's masks, one word for 64 tokens,
+// by an LDS atomic OR (its result does not depend on the order); a row is then
+// the expert's offset, its counts in the words before and the bits below.
+// LDS: E * C masks (C words an expert), then as many counts.
 // 777 tokens of 1024 channels, top-4 of 32: 15.6 -> 6.8 us against ranking by
 // ballots through memory; what is left is the plan's one workgroup.
-template <int KB>
+template <int KB, int T>
 __global__ __launch_bounds__(1024) void k_prep(const PrepArgs a, const BlockQuant bq, int nblk, int64_t total) {
-  constexpr int MAXC = kPrepMaxN / 64;
-  __shared__ unsigned long long mask[kPlanMaxG * MAXC];
-  __shared__ uint16_t before[kPlanMaxG * MAXC];
+  extern __shared__ unsigned long long mask[];
   __shared__ int tot[kPlanMaxG], goff[kPlanMaxG + 1], wsum[4];
   const int tid = threadIdx.x;
   if (blockIdx.x > 0) {
@@ -429,61 +428,81 @@ __global__ __launch_bounds__(1024) void k_prep(const PrepArgs a, const BlockQuan
     return;
   }
   const int N = a.N, K = a.K, E = a.E, C = (N + 63) / 64;
-  int id[KB];
-  float w[KB], sum[KB];
-  bool use[KB];
-  const int tc = min(tid, N - 1);
+  uint16_t* before = reinterpret_cast<uint16_t*>(mask + E * C);
+  int id[T][KB];
+  float w[T][KB], sum[T][KB];
+  bool use[T][KB];
 #pragma unroll
-  for (int j = 0; j < KB; ++j) {  // unconditional loads at clamped indices
-    id[j] = a.idx[tc * K + min(j, K - 1)];
-    w[j] = a.w[tc * K + min(j, K - 1)];
-  }
+  for (int u = 0; u < T; ++u)
+#pragma unroll
+    for (int j = 0; j < KB; ++j) {  // unconditional loads at clamped indices
+      const int at = min(u * 1024 + tid, N - 1) * K + min(j, K - 1);
+      id[u][j] = a.idx[at];
+      w[u][j] = a.w[at];
+    }
   for (int i = tid; i < E * C; i += 1024) mask[i] = 0ull;
 #pragma unroll
-  for (int j = 0; j < KB; ++j) {
-    use[j] = tid < N && j < K && id[j] >= 0 && id[j] < E;
-    sum[j] = 0.f;
+  for (int u = 0; u < T; ++u)
 #pragma unroll
-    for (int i = 0; i < KB; ++i) {
-      if (i < j) use[j] = use[j] && id[i] != id[j];  // its first slot speaks for an id
-      sum[j] = i < K && id[i] == id[j] ? sum[j] + w[i] : sum[j];
-    }
-    use[j] = use[j] && sum[j] > 0.f;
-  }
-  __syncthreads();
-  const int c = tid >> 6;
-  const unsigned long long bit = 1ull << (tid & 63);
+    for (int j = 0; j < KB; ++j) {
+      use[u][j] = u * 1024 + tid < N && j < K && id[u][j] >= 0 && id[u][j] < E;
+      sum[u][j] = 0.f;
 #pragma unroll
-  for (int j = 0; j < KB; ++j)
-    if (use[j]) atomicOr(&mask[id[j] * C + c], bit);
-  __syncthreads();
-  if (tid < E) {
-    int n = 0;
-    for (int i = 0; i < C; ++i) {
-      before[tid * C + i] = static_cast<uint16_t>(n);
-      n += __popcll(mask[tid * C + i]);
+      for (int i = 0; i < KB; ++i) {
+        if (i < j) use[u][j] = use[u][j] && id[u][i] != id[u][j];  // its first slot speaks for an id
+        sum[u][j] = i < K && id[u][i] == id[u][j] ? sum[u][j] + w[u][i] : sum[u][j];
+      }
+      use[u][j] = use[u][j] && sum[u][j] > 0.f;
     }
-    tot[tid] = n;
+  __syncthreads();
+  const int c = tid >> 6, lane = tid & 63;
+  const unsigned long long bit = 1ull << lane;
+#pragma unroll
+  for (int u = 0; u < T; ++u)
+#pragma unroll
+    for (int j = 0; j < KB; ++j)
+      if (use[u][j]) atomicOr(&mask[id[u][j] * C + 16 * u + c], bit);
+  __syncthreads();
+  if constexpr (T == 1) {  // a thread an expert
+    if (tid < E) {
+      int n = 0;
+      for (int i = 0; i < C; ++i) {
+        before[tid * C + i] = static_cast<uint16_t>(n);
+        n += __popcll(mask[tid * C + i]);
+      }
+      tot[tid] = n;
+    }
+  } else {
+    for (int e = c; e < E; e += 16) {  // a wave an expert, a lane a word: C <= 64
+      const int n = lane < C ? __popcll(mask[e * C + lane]) : 0;
+      const int upto = wave_incl_scan(n);
+      if (lane < C) before[e * C + lane] = static_cast<uint16_t>(upto - n);
+      if (lane == 63) tot[e] = upto;
+    }
   }
   __syncthreads();
   block_group_offsets(tot, E, goff, wsum);
   for (int g = tid; g <= E; g += 1024) a.off[g] = goff[g];
-  if (tid >= N) return;
-  int n = 0;
 #pragma unroll
-  for (int j = 0; j < KB; ++j) {
-    int rank = 0;  // among the token's experts, ascending
+  for (int u = 0; u < T; ++u) {
+    const int t = u * 1024 + tid;
+    if (t >= N) return;
+    int n = 0;
 #pragma unroll
-    for (int i = 0; i < KB; ++i) rank += use[i] && id[i] < id[j] ? 1 : 0;
-    if (!use[j]) continue;
-    const int at = id[j] * C + c;
-    const int row = goff[id[j]] + before[at] + __popcll(mask[at] & (bit - 1ull));
-    a.rows[row] = tid;
-    a.roww[row] = sum[j];
-    a.tokrow[tid * K + rank] = row;
-    ++n;
+    for (int j = 0; j < KB; ++j) {
+      int rank = 0;  // among the token's experts, ascending
+#pragma unroll
+      for (int i = 0; i < KB; ++i) rank += use[u][i] && id[u][i] < id[u][j] ? 1 : 0;
+      if (!use[u][j]) continue;
+      const int at = id[u][j] * C + 16 * u + c;
+      const int row = goff[id[u][j]] + before[at] + __popcll(mask[at] & (bit - 1ull));
+      a.rows[row] = t;
+      a.roww[row] = sum[u][j];
+      a.tokrow[t * K + rank] = row;
+      ++n;
+    }
+    for (int j = n; j < K; ++j) a.tokrow[t * K + j] = -1;
   }
-  for (int j = n; j < K; ++j) a.tokrow[tid * K + j] = -1;
 }
 
 int rc() { return hipGetLastError() == hipSuccess ? SMOE_OK : SMOE_EHIP; }
@@ -520,20 +539,33 @@ int launch_gemm_blocks_few(const BlockGemm& a, hipStream_t s) {
   return SMOE_EINVAL;
 }
 
+// Up to 1024 tokens, and up to 4096 of few choices: the plan's one workgroup
+// against three launches and the quantizer's.  Whole steps of 1500 tokens: top-4
+// of 32 68 -> 63 us, top-2 of 96 44 -> 36; 4096, top-2 of 64: 182 -> 176; 3000,
+// top-4 of 32: 101 -> 103.
 bool prep_fits(int N, int K, int E) {
-  return N <= kPrepMaxN && K <= 16 && E <= kPlanMaxG;
+  return K <= 16 && N <= 4096 && (N <= 1024 || N * K <= 8192) && E <= kPlanMaxG &&
+         E * ((N + 63) / 64) <= 6144;  // 60 KB of LDS
 }
 
 int launch_prep(const PrepArgs& a, const BlockQuant& q, hipStream_t s) {
   const int nblk = fp8_blocks_of(q.cols);
   const int64_t total = static_cast<int64_t>(q.rows) * nblk, wgs = (total + 63) / 64 + 1;
-  if (wgs * 1024 > 0xffffffffll) return SMOE_EINVAL;  // threads of a launch
-  const dim3 grid(static_cast<unsigned>(wgs)), block(1024);
-  if (a.K <= 2) hipLaunchKernelGGL((k_prep<2>), grid, block, 0, s, a, q, nblk, total);
-  else if (a.K <= 4) hipLaunchKernelGGL((k_prep<4>), grid, block, 0, s, a, q, nblk, total);
-  else if (a.K <= 8) hipLaunchKernelGGL((k_prep<8>), grid, block, 0, s, a, q, nblk, total);
-  else hipLaunchKernelGGL((k_prep<16>), grid, block, 0, s, a, q, nblk, total);
-  return rc();
+  if (!prep_fits(a.N, a.K, a.E) || wgs * 1024 > 0xffffffffll) return SMOE_EINVAL;  // threads of a launch
+  const size_t lds = static_cast<size_t>(a.E) * ((a.N + 63) / 64) * 10;
+  auto go = [&](auto kb, auto t) {
+    SMOE_LAUNCH((k_prep<decltype(kb)::value, decltype(t)::value>), dim3(static_cast<unsigned>(wgs)), dim3(1024), lds, s,
+                a, q, nblk, total);
+    return rc();
+  };
+  using I1 = std::integral_constant<int, 1>;
+  using I2 = std::integral_constant<int, 2>;
+  using I4 = std::integral_constant<int, 4>;
+  using I8 = std::integral_constant<int, 8>;
+  using I16 = std::integral_constant<int, 16>;
+  if (a.N <= 1024) return a.K <= 2 ? go(I2{}, I1{}) : a.K <= 4 ? go(I4{}, I1{}) : a.K <= 8 ? go(I8{}, I1{}) : go(I16{}, I1{});
+  if (a.N <= 2048) return a.K <= 2 ? go(I2{}, I2{}) : a.K <= 4 ? go(I4{}, I2{}) : go(I8{}, I2{});
+  return a.K <= 2 ? go(I2{}, I4{}) : go(I4{}, I4{});
 }
 
 // LDS of the two launches: quantized rows of up to N messages or N * K

@@ -49,11 +49,13 @@ def test_expert_delta_over_many_tiles(activation, bias, n, e, k, h, u):
                                      activation))
 
 
-@pytest.mark.parametrize("n,e,k", [(3, 70, 4), (300, 70, 6), (300, 5, 20), (1300, 70, 6), (1300, 24, 20)])
+@pytest.mark.parametrize("n,e,k", [(3, 70, 4), (300, 70, 6), (300, 5, 20), (1300, 70, 6), (1300, 24, 20), (1024, 256, 16),
+                                   (1025, 3, 1), (2048, 190, 8), (2048, 200, 4), (2049, 90, 4), (4096, 96, 2),
+                                   (4095, 97, 2), (4097, 8, 2), (3000, 40, 5)])
 def test_expert_delta_every_plan(n, e, k):
-    """The few-token step, the plan by bit masks and the general one: more
-    experts than a wave has lanes, more choices than the bit masks take
-    (k > 16), the same id several times in a row of choices, int64 ids past 32
+    """The few-token step, the plan by bit masks (one, two and four tokens a
+    thread, up to its limits) and the general one: more experts than a wave
+    has lanes, more choices than the bit masks take (k > 16), the same id several times in a row of choices, int64 ids past 32
     bits (outside [0, E), as any other id there)."""
     from spider_moe_amd import sparse_expert_delta_fp8_blocks
     say("expert delta, plans", n, e, k)
@@ -63,7 +65,7 @@ def test_expert_delta_every_plan(n, e, k):
     idx = torch.randint(0, e, (n, k), generator=g)
     w = torch.rand(n, k, generator=g)
     idx[0] = e - 1
-    idx[1, :2] = torch.tensor([1 << 32, -(1 << 32)])
+    idx[1, :2] = torch.tensor([1 << 32, -(1 << 32)])[:k]
     got = sparse_expert_delta_fp8_blocks(msg.to(dev), idx.to(dev), w.to(dev), ex)
     ids = torch.where((idx >= 0) & (idx < e), idx, torch.full_like(idx, -1))
     _check_delta(got, O.expert_delta(msg, ids, w, ex.w_up, ex.s_up, ex.w_down, ex.s_down, ex.b_up, ex.b_down, "swiglu"))
