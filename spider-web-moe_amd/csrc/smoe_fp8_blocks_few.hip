@@ -400,6 +400,9 @@ __global__ __launch_bounds__(512, 4) void k_tokens_down(const TokensArgs a) {
   }
 }
 
+// words of 64 tokens an expert takes: an odd number
+__host__ __device__ inline int prep_pitch(int N) { return ((N + 63) / 64) | 1; }
+
 // The plan of a decode step or a short prompt (K <= KB, N <= 1024 T) and its
 // quantized messages in one launch: workgroup 0 makes the plan (the one
 // smoe_dispatch_plan makes), the others quantize 64 blocks each.
@@ -410,8 +413,9 @@ __global__ __launch_bounds__(512, 4) void k_tokens_down(const TokensArgs a) {
 // expert) sets the token's bit in the expert's masks, one word for 64 tokens,
 // by an LDS atomic OR (its result does not depend on the order); a row is then
 // the expert's offset, its counts in the words before and the bits below.
-// LDS: E * C masks (C words an expert), then as many counts.
-// 777 tokens of 1024 channels, top-4 of 32: 15.6 -> 6.8 us against ranking by
+// LDS: E * P masks, then as many counts; an odd pitch P, without which the
+// experts' words of 64 tokens meet in one bank; after them the plan's rows.
+// 777 tokens of 1024 channels, top-4 of 32: 15.6 -> 5.9 us against ranking by
 // ballots through memory; what is left is the plan's one workgroup.
 template <int KB, int T>
 __global__ __launch_bounds__(1024) void k_prep(const PrepArgs a, const BlockQuant bq, int nblk, int64_t total) {
@@ -427,8 +431,8 @@ __global__ __launch_bounds__(1024) void k_prep(const PrepArgs a, const BlockQuan
     else run(std::integral_constant<int, SMOE_BF16>{});
     return;
   }
-  const int N = a.N, K = a.K, E = a.E, C = (N + 63) / 64;
-  uint16_t* before = reinterpret_cast<uint16_t*>(mask + E * C);
+  const int N = a.N, K = a.K, E = a.E, C = (N + 63) / 64, P = prep_pitch(N);
+  uint16_t* before = reinterpret_cast<uint16_t*>(mask + E * P);
   int id[T][KB];
   float w[T][KB], sum[T][KB];
   bool use[T][KB];
@@ -440,7 +444,7 @@ __global__ __launch_bounds__(1024) void k_prep(const PrepArgs a, const BlockQuan
       id[u][j] = a.idx[at];
       w[u][j] = a.w[at];
     }
-  for (int i = tid; i < E * C; i += 1024) mask[i] = 0ull;
+  for (int i = tid; i < E * P; i += 1024) mask[i] = 0ull;
 #pragma unroll
   for (int u = 0; u < T; ++u)
 #pragma unroll
@@ -461,32 +465,32 @@ __global__ __launch_bounds__(1024) void k_prep(const PrepArgs a, const BlockQuan
   for (int u = 0; u < T; ++u)
 #pragma unroll
     for (int j = 0; j < KB; ++j)
-      if (use[u][j]) atomicOr(&mask[id[u][j] * C + 16 * u + c], bit);
+      if (use[u][j]) atomicOr(&mask[id[u][j] * P + 16 * u + c], bit);
   __syncthreads();
   if constexpr (T == 1) {  // a thread an expert
     if (tid < E) {
       int n = 0;
       for (int i = 0; i < C; ++i) {
-        before[tid * C + i] = static_cast<uint16_t>(n);
-        n += __popcll(mask[tid * C + i]);
+        before[tid * P + i] = static_cast<uint16_t>(n);
+        n += __popcll(mask[tid * P + i]);
       }
       tot[tid] = n;
     }
   } else {
     for (int e = c; e < E; e += 16) {  // a wave an expert, a lane a word: C <= 64
-      const int n = lane < C ? __popcll(mask[e * C + lane]) : 0;
+      const int n = lane < C ? __popcll(mask[e * P + lane]) : 0;
       const int upto = wave_incl_scan(n);
-      if (lane < C) before[e * C + lane] = static_cast<uint16_t>(upto - n);
+      if (lane < C) before[e * P + lane] = static_cast<uint16_t>(upto - n);
       if (lane == 63) tot[e] = upto;
     }
   }
   __syncthreads();
   block_group_offsets(tot, E, goff, wsum);
   for (int g = tid; g <= E; g += 1024) a.off[g] = goff[g];
+  int row[T][KB];
 #pragma unroll
   for (int u = 0; u < T; ++u) {
     const int t = u * 1024 + tid;
-    if (t >= N) return;
     int n = 0;
 #pragma unroll
     for (int j = 0; j < KB; ++j) {
@@ -494,14 +498,30 @@ __global__ __launch_bounds__(1024) void k_prep(const PrepArgs a, const BlockQuan
 #pragma unroll
       for (int i = 0; i < KB; ++i) rank += use[u][i] && id[u][i] < id[u][j] ? 1 : 0;
       if (!use[u][j]) continue;
-      const int at = id[u][j] * C + 16 * u + c;
-      const int row = goff[id[u][j]] + before[at] + __popcll(mask[at] & (bit - 1ull));
-      a.rows[row] = t;
-      a.roww[row] = sum[u][j];
-      a.tokrow[t * K + rank] = row;
+      const int at = id[u][j] * P + 16 * u + c;
+      row[u][j] = goff[id[u][j]] + before[at] + __popcll(mask[at] & (bit - 1ull));
+      a.tokrow[t * K + rank] = row[u][j];
       ++n;
     }
-    for (int j = n; j < K; ++j) a.tokrow[t * K + j] = -1;
+    for (int j = n; j < K && t < N; ++j) a.tokrow[t * K + j] = -1;
+  }
+  __syncthreads();  // the masks are read
+  // rows and their weights leave in order: scattered from here, each store of a
+  // wave took a cycle per lane
+  float* const lw = reinterpret_cast<float*>(mask);
+  uint16_t* const lt = reinterpret_cast<uint16_t*>(lw + N * K);
+#pragma unroll
+  for (int u = 0; u < T; ++u)
+#pragma unroll
+    for (int j = 0; j < KB; ++j)
+      if (use[u][j]) {
+        lw[row[u][j]] = sum[u][j];
+        lt[row[u][j]] = static_cast<uint16_t>(u * 1024 + tid);
+      }
+  __syncthreads();
+  for (int r = tid; r < goff[E]; r += 1024) {
+    a.rows[r] = lt[r];
+    a.roww[r] = lw[r];
   }
 }
 
@@ -539,20 +559,19 @@ int launch_gemm_blocks_few(const BlockGemm& a, hipStream_t s) {
   return SMOE_EINVAL;
 }
 
-// Up to 1024 tokens, and up to 4096 of few choices: the plan's one workgroup
+// Up to 8192 choices, which the plan's one workgroup holds in registers and LDS,
 // against three launches and the quantizer's.  Whole steps of 1500 tokens: top-4
-// of 32 68 -> 63 us, top-2 of 96 44 -> 36; 4096, top-2 of 64: 182 -> 176; 3000,
-// top-4 of 32: 101 -> 103.
+// of 32 69 -> 65 us, top-2 of 96 44 -> 34; 4096 tokens, top-2 of 64: 181 -> 175.
 bool prep_fits(int N, int K, int E) {
-  return K <= 16 && N <= 4096 && (N <= 1024 || N * K <= 8192) && E <= kPlanMaxG &&
-         E * ((N + 63) / 64) <= 6144;  // 60 KB of LDS
+  return K <= 16 && N <= 4096 && N * K <= 8192 && E <= kPlanMaxG &&
+         E * prep_pitch(N) <= 6300;  // 62 KB of LDS
 }
 
 int launch_prep(const PrepArgs& a, const BlockQuant& q, hipStream_t s) {
   const int nblk = fp8_blocks_of(q.cols);
   const int64_t total = static_cast<int64_t>(q.rows) * nblk, wgs = (total + 63) / 64 + 1;
   if (!prep_fits(a.N, a.K, a.E) || wgs * 1024 > 0xffffffffll) return SMOE_EINVAL;  // threads of a launch
-  const size_t lds = static_cast<size_t>(a.E) * ((a.N + 63) / 64) * 10;
+  const size_t lds = std::max(static_cast<size_t>(a.E) * prep_pitch(a.N) * 10, static_cast<size_t>(a.N) * a.K * 6);
   auto go = [&](auto kb, auto t) {
     SMOE_LAUNCH((k_prep<decltype(kb)::value, decltype(t)::value>), dim3(static_cast<unsigned>(wgs)), dim3(1024), lds, s,
                 a, q, nblk, total);
