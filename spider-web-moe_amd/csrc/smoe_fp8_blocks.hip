@@ -28,8 +28,8 @@ template <int XDT>
 __global__ __launch_bounds__(256) void k_quant_square_blocks(const BlockQuant q, int rblk, int nblk) {
   __shared__ uint32_t red[4];
   const int kb = blockIdx.x % nblk;
-  const int64_t grb = blockIdx.x / nblk;  // group * row blocks + row block
-  const int64_t g = grb / rblk;
+  const uint32_t grb = blockIdx.x / nblk;  // group * row blocks + row block
+  const int64_t g = grb / static_cast<uint32_t>(rblk);
   const int r0 = static_cast<int>(grb - g * rblk) * kFp8Block;
   const int c = kb * kFp8Block + 8 * (threadIdx.x & 15);
   const bool vec = (reinterpret_cast<uintptr_t>(q.x) | static_cast<uintptr_t>(q.ldx * elt_bytes<XDT>())) % 16 == 0;

@@ -128,9 +128,9 @@ __device__ __forceinline__ u32x2 codes8(const float (&v)[8], float sc) {
 // calls it (blocks past `total` compute on the last one and store nothing).
 template <int XDT>
 __device__ __forceinline__ void quant_row_block(const BlockQuant& q, int nblk, int64_t total, int64_t b, int l16) {
-  const int64_t bc = b < total ? b : total - 1;
-  const int64_t row = bc / nblk;
-  const int kb = static_cast<int>(bc - row * nblk);
+  const uint32_t bc = static_cast<uint32_t>(b < total ? b : total - 1);  // total <= 2^28
+  const int64_t row = bc / static_cast<uint32_t>(nblk);  // a 64-bit division is longer than the rest
+  const int kb = static_cast<int>(bc - static_cast<uint32_t>(row) * nblk);
   const int c = kb * kFp8Block + 8 * l16;
   const char* rp = reinterpret_cast<const char*>(q.x) + row * q.ldx * elt_bytes<XDT>();
   const bool vec = (reinterpret_cast<uintptr_t>(q.x) | static_cast<uintptr_t>(q.ldx * elt_bytes<XDT>())) % 16 == 0;
