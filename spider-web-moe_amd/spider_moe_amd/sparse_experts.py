@@ -152,6 +152,17 @@ class Fp8BlockExperts:
         return cls(q, s, qd, sd, b_up=b_up, b_down=b_down, activation=activation)
 
 
+def _expert_ids(idx: torch.Tensor, num_experts: int) -> torch.Tensor:
+    """idx as int32, ids outside [0, num_experts) still outside.  Narrow types
+    go straight to int32: they need not hold the limits of a clamp (-1 in
+    uint8 is 255)."""
+    if idx.dtype == torch.int32:
+        return idx
+    if idx.dtype not in (torch.uint8, torch.int8, torch.int16):
+        idx = idx.clamp(-1, num_experts)
+    return idx.to(torch.int32)
+
+
 def sparse_expert_delta_fp8_blocks(messages: torch.Tensor, top_indices: torch.Tensor,
                                    top_weights: torch.Tensor, experts: Fp8BlockExperts) -> torch.Tensor:
     """sparse_expert_delta on Fp8BlockExperts: messages [..,H] (float32 or
@@ -166,9 +177,7 @@ def sparse_expert_delta_fp8_blocks(messages: torch.Tensor, top_indices: torch.Te
     if top_indices.shape[:-1] != messages.shape[:-1] or top_weights.shape != top_indices.shape:
         raise ValueError("top_indices and top_weights must be messages' shape with K last")
     code = nat.dtype_code(messages.dtype)
-    idx, wts = top_indices, top_weights
-    if idx.dtype != torch.int32:  # ids past 32 bits stay outside [0, E)
-        idx = idx.clamp(-1, experts.num_experts).to(torch.int32)
+    idx, wts = _expert_ids(top_indices, experts.num_experts), top_weights
     if wts.dtype != torch.float32:
         wts = wts.float()
     msg, idx, wts = messages.contiguous(), idx.contiguous(), wts.contiguous()
