@@ -139,12 +139,15 @@ def _act_codes(a, d):
     return c * sf, off * sf + c.abs() * sf * _spread(rel, u)
 
 
-# The matrix unit cuts each product below 2^-18 of its block's largest (test_
-# gpu_fp8_blocks.py's docstring): 128 of them are 2^-11 of it.
+# What the matrix unit's e4m3 x e4m3 sums of a block are off by on codes of
+# random data: 2^-11 of the block's largest product.  At worst (7 of each eight
+# products cut by 2^-13 of the eight's largest) it is 7 * 16 * 2^-13 of it:
+# tests/test_gpu_fp8_block_sums.py.
 BLOCK_CUT = 2.0 ** -11
 
 
-def expert_delta(msg, idx, w, w_up, s_up, w_down, s_down, b_up=None, b_down=None, activation="gelu"):
+def expert_delta(msg, idx, w, w_up, s_up, w_down, s_down, b_up=None, b_down=None, activation="gelu",
+                 f32_sums=False):
     """msg [N,H], idx / w [N,K] -> (delta f64 [N,H], how far a right result
     may be off before its last rounding); slots of one expert merged, weights
     <= 0 and ids outside [0, E) dropped.
@@ -154,7 +157,10 @@ def expert_delta(msg, idx, w, w_up, s_up, w_down, s_down, b_up=None, b_down=None
     at most 1.13, SiLU's 1.1; their own errors in f32 3e-7 of the argument and
     2e-6 of the value); where a border between two codes lies that near, the
     other code is as right; the down product carries on the codes' distance
-    and adds its own cut."""
+    and adds its own cut.
+
+    f32_sums: both products summed in f32, with no cut: off by 2^-24 of the
+    magnitudes for each of a sum's K + K / 128 + 8 operations."""
     n, h = msg.shape
     e, u = w_down.shape[0], w_down.shape[2]
     ub = -(-u // B)
@@ -165,7 +171,13 @@ def expert_delta(msg, idx, w, w_up, s_up, w_down, s_down, b_up=None, b_down=None
     def product(a, codes, scale, bias):
         wv = values(codes, scale)
         y = a @ wv.t()
-        d = 2.0 ** -20 * (a.abs() @ wv.abs().t())
+        mag = a.abs() @ wv.abs().t()
+        if f32_sums:
+            d = (a.shape[1] * (1 + 1 / B) + 8) * 2.0 ** -24 * mag
+            if bias is not None:
+                d = d + 2.0 ** -24 * (y + bias.cpu().double()).abs()
+            return (y if bias is None else y + bias.cpu().double()), d, wv
+        d = 2.0 ** -20 * mag
         for k in range(0, a.shape[1], B):
             d += BLOCK_CUT * a[:, k:k + B].abs().amax(1, keepdim=True) * wv[:, k:k + B].abs().amax(1)[None]
         return (y if bias is None else y + bias.cpu().double()), d, wv

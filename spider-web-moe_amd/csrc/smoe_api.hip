@@ -1671,6 +1671,7 @@ SMOE_API int smoe_expert_delta_fp8_blocks(const smoe_experts_fp8_blocks* ex, con
   up.max_rows = N * K;
   up.bias = ex->b_up;
   up.bias_gstride = U;
+  up.wide = out_dtype == SMOE_F32;
   up.out = at<void>(ws, l.act);
   up.ldo = U;
   up.out_scale = at<float>(ws, l.ascale);
@@ -1696,6 +1697,7 @@ SMOE_API int smoe_expert_delta_fp8_blocks(const smoe_experts_fp8_blocks* ex, con
   dn.bias = ex->b_down;
   dn.bias_gstride = H;
   dn.row_scale = roww;
+  dn.wide = up.wide;
   dn.out = at<void>(ws, l.y);
   dn.ldo = H;
   SMOE_TRY(launch_gemm_fp8_blocks(dn, s), "expert down GEMM");

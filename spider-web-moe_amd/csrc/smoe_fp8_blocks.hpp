@@ -64,6 +64,7 @@ struct BlockGemm {
   void* out = nullptr;
   int out_dtype = SMOE_F32;
   int64_t ldo = 0;             // elements (codes: bytes)
+  bool wide = false;           // BLK_UP_*, BLK_DOWN: products summed in f32 (BLK_LINEAR, BLK_GELU: with f32 outputs)
   float* out_scale = nullptr;  // BLK_UP_*: scale of (row, block): out_scale[block * os_col + row]
   int64_t os_col = 0;
 };

@@ -213,7 +213,7 @@ constexpr int kTokensMax = 16;  // entries (and so tokens, experts and rows)
 // into LDS under the first weights' loads; activations leave in f32 at their
 // plan rows.  Bound by the latency of its loads: 2 of 64 experts, 2048 -> 1408,
 // 5.8 MB in 6 us.
-template <bool SWIGLU, int XDT>
+template <bool SWIGLU, int XDT, bool WIDE>
 __global__ __launch_bounds__(256, 4) void k_tokens_up(const TokensArgs a) {
   constexpr int NT = SWIGLU ? 2 : 1, D = SWIGLU ? 3 : 4;
   __shared__ __attribute__((aligned(16))) float red[4 * NT * 256];
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(256, 4) void k_tokens_up(const TokensArgs a) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         if (a.H - 128 * b < 128) w[d][j] = cut_piece(w[d][j], q, a.H - 128 * b);
-        const f32x4 part = block_product<false>(w[d][j], x);
+        const f32x4 part = block_product<WIDE>(w[d][j], x);
         const float sc = xs * ws[d][j];
 #pragma unroll
         for (int v = 0; v < 4; ++v) acc[j][v] = fmaf(part[v], sc, acc[j][v]);
@@ -317,6 +317,7 @@ __global__ __launch_bounds__(256, 4) void k_tokens_up(const TokensArgs a) {
 template <int ODT>
 __global__ __launch_bounds__(512, 4) void k_tokens_down(const TokensArgs a) {
   constexpr int D = 4;
+  constexpr bool WIDE = ODT == SMOE_F32;
   __shared__ __attribute__((aligned(16))) float red[8 * 256];
   __shared__ int s_row[kTokensMax * kTokensMax], s_exp[kTokensMax];
   __shared__ float s_w[kTokensMax * kTokensMax];
@@ -370,7 +371,7 @@ __global__ __launch_bounds__(512, 4) void k_tokens_down(const TokensArgs a) {
       const int o = i / KB, b = i - o * KB;
       const int r = s_row[o * kTokensMax + l16], rc = max(r, 0);
       if (a.U - 128 * b < 128) w[d] = cut_piece(w[d], q, a.U - 128 * b);
-      const f32x4 part = block_product<false>(w[d], load_piece(xlds + rc * ldl, 128 * b, q, ldl));
+      const f32x4 part = block_product<WIDE>(w[d], load_piece(xlds + rc * ldl, 128 * b, q, ldl));
       const float sc = xsl[b * rows + rc] * ws[d] * s_w[o * kTokensMax + l16];
 #pragma unroll
       for (int v = 0; v < 4; ++v) acc[v] = r >= 0 ? fmaf(part[v], sc, acc[v]) : acc[v];
@@ -600,11 +601,16 @@ int launch_tokens(const TokensArgs& a, hipStream_t s) {
   const dim3 up(static_cast<unsigned>(std::min(a.E, a.N * a.K) * ((a.U + 15) / 16)));
   const size_t lds_up = static_cast<size_t>(a.N) * fp8_blocks_of(a.H) * 132;
   const size_t lds_down = static_cast<size_t>(a.N) * a.K * fp8_blocks_of(a.U) * 132;
-  const bool sw = a.act_fn == SMOE_ACT_SWIGLU, f32 = a.msg_dtype == SMOE_F32;
-  if (sw && f32) hipLaunchKernelGGL((k_tokens_up<true, SMOE_F32>), up, dim3(256), lds_up, s, a);
-  else if (sw) hipLaunchKernelGGL((k_tokens_up<true, SMOE_BF16>), up, dim3(256), lds_up, s, a);
-  else if (f32) hipLaunchKernelGGL((k_tokens_up<false, SMOE_F32>), up, dim3(256), lds_up, s, a);
-  else hipLaunchKernelGGL((k_tokens_up<false, SMOE_BF16>), up, dim3(256), lds_up, s, a);
+  const bool f32 = a.msg_dtype == SMOE_F32, wide = a.out_dtype == SMOE_F32;
+  auto go_up = [&](auto sw, auto w) {
+    constexpr bool SW = decltype(sw)::value, WD = decltype(w)::value;
+    if (f32) hipLaunchKernelGGL((k_tokens_up<SW, SMOE_F32, WD>), up, dim3(256), lds_up, s, a);
+    else hipLaunchKernelGGL((k_tokens_up<SW, SMOE_BF16, WD>), up, dim3(256), lds_up, s, a);
+  };
+  using Y = std::true_type;
+  using N = std::false_type;
+  if (a.act_fn == SMOE_ACT_SWIGLU) wide ? go_up(Y{}, Y{}) : go_up(Y{}, N{});
+  else wide ? go_up(N{}, Y{}) : go_up(N{}, N{});
   const dim3 down(static_cast<unsigned>((a.H + 15) / 16));
   if (a.out_dtype == SMOE_F32) hipLaunchKernelGGL((k_tokens_down<SMOE_F32>), down, dim3(512), lds_down, s, a);
   else hipLaunchKernelGGL((k_tokens_down<SMOE_BF16>), down, dim3(512), lds_down, s, a);

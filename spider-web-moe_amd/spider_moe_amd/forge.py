@@ -398,7 +398,8 @@ class ForgeGEMM:
         scale per 128 x 128 block (quantize_fp8_blocks), x [..., K] quantized
         in 1 x 128 blocks on the way (smoe_linear_fp8_blocks); act None or
         "gelu" (erf).  Result in x's dtype: bfloat16 from e4m3 x e4m3
-        products, float32 (and float16) from the same values' products with
+        products, each cut by less than 2^-13 of the largest of its eight
+        neighbours; float32 (and float16) from the same values' products with
         f32 sums throughout.  No gradient."""
         self.calls += 1
         return _linear_fp8_blocks(x, codes, scale, bias, act)

@@ -168,8 +168,10 @@ def sparse_expert_delta_fp8_blocks(messages: torch.Tensor, top_indices: torch.Te
     """sparse_expert_delta on Fp8BlockExperts: messages [..,H] (float32 or
     bfloat16), top_indices / top_weights [..,K] -> delta [..,H] in messages'
     dtype.  Messages and hidden activations are quantized in 1 x 128 blocks on
-    the way into the two products; everything else is summed in f32.  No
-    gradient."""
+    the way into the two products.  float32: both products and all that
+    follows are summed in f32; bfloat16: the products by the e4m3 x e4m3 matrix
+    instruction, which cuts each one by less than 2^-13 of the largest of its
+    eight neighbours, the rest in f32.  No gradient."""
     dev = nat.require_gpu(messages, top_indices, top_weights, experts.w_up)
     h, k = messages.shape[-1], top_indices.shape[-1]
     if h != experts.hidden_size:
