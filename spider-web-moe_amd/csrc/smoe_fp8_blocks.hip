@@ -326,9 +326,9 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm_blocks(const BlockGemm
     // of 128 channels through LDS; codes staged in the ring
     constexpr int JN = SWIGLU ? 2 : 4, BW = 128 / CHW;  // BW waves share a block
     uint32_t* red = reinterpret_cast<uint32_t*>(ring);     // [WN][BM]
-    float* inv = reinterpret_cast<float*>(red + WN * BM);  // [CH / 128][BM]
-    uint8_t* stg = ring + (WN + CH / 128) * BM * 4;        // [BM][CH], 16-byte chunks swizzled by row
-    static_assert((WN + CH / 128) * BM * 4 + BM * CH <= NS * STAGE, "staging in the ring");
+    Divisor* div = reinterpret_cast<Divisor*>(red + WN * BM);  // [CH / 128][BM]
+    uint8_t* stg = ring + (WN + 2 * (CH / 128)) * BM * 4;      // [BM][CH], 16-byte chunks swizzled by row
+    static_assert((WN + 2 * (CH / 128)) * BM * 4 + BM * CH <= NS * STAGE, "staging in the ring");
     uint32_t m[FM];
 #pragma unroll
     for (int i = 0; i < FM; ++i) m[i] = 0u;
@@ -369,21 +369,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm_blocks(const BlockGemm
 #pragma unroll
       for (int w = 1; w < BW; ++w) a = max(a, red[(blk * BW + w) * BM + r]);
       const float sc = block_scale(a);
-      inv[e] = __fdiv_rn(1.0f, sc);
+      div[e] = divisor(sc);
       if (r < mrows && n0 + 128 * blk < p.N_out) p.out_scale[(n0 / 128 + blk) * p.os_col + m0 + r] = sc;
     }
     __syncthreads();
-    // times the reciprocal: within 2^-23 of the quotient, where the activation
-    // itself is known to about 2^-16
+    // the quantizer's own quotients (with the reciprocal alone 1 of 15 ties went
+    // to the other code), one division for a row's block
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int r = wm * TM + i * 16 + fr;
-      const float d = inv[wn / BW * BM + r];
+      const Divisor d = div[wn / BW * BM + r];
 #pragma unroll
       for (int j = 0; j < JN; ++j) {
         const int c = CHW * wn + j * 16 + 4 * q;
         *reinterpret_cast<uint32_t*>(stg + r * CH + (((c >> 4) ^ (r & 7)) << 4) + (c & 15)) =
-            pack_e4m3(acc[j][i][0] * d, acc[j][i][1] * d, acc[j][i][2] * d, acc[j][i][3] * d);
+            pack_e4m3(quotient(acc[j][i][0], d), quotient(acc[j][i][1], d), quotient(acc[j][i][2], d),
+                      quotient(acc[j][i][3], d));
       }
     }
     __syncthreads();
