@@ -38,6 +38,7 @@ from enum import Enum
 from typing import Any, Callable
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 from .dispatch import DispatchPlan, build_dispatch_plan, dispatch_expert_ffn
@@ -101,8 +102,9 @@ class ForgeSelect:
         with renormalize.  Experts whose logit is -inf are chosen last, with
         weight 0.
 
-        Differentiable in logits (the choice held fixed; the bias gets no
-        gradient)."""
+        Differentiable in logits, once and in reverse mode (the choice held
+        fixed; the bias gets no gradient); a tangent of forward mode is
+        refused."""
         self.calls += 1
         k = int(top_k if top_k is not None else self.config.select_top_k)
         return select_groups(logits, k, score=score, bias=bias, num_groups=num_groups,
@@ -169,6 +171,8 @@ def select_groups(logits: torch.Tensor, k: int, *, score: str = "sigmoid", bias=
                   scale: float = 1.0):
     """smoe_select_groups over the last dimension (ForgeSelect.route_groups)."""
     dev = nat.require_gpu(logits, bias)
+    if forward_ad.unpack_dual(logits).tangent is not None:
+        raise RuntimeError("route_groups has no forward-mode derivative")
     shape = logits.shape
     e = shape[-1] if shape else 0
     n = logits.numel() // e if e else 0
