@@ -89,18 +89,38 @@ class Fp8BlockExperts:
     [E, 2 ceil(U/128), ceil(H/128)] (gate and up projection are quantized
     each on its own).  w_down [E,H,U], s_down [E, ceil(H/128), ceil(U/128)].
     b_up [E,U] (swiglu: added to the up projection) and b_down [E,H] or None.
-    H % 16 == 0 and U % 16 == 0.  The tensors are kept, not copied (a copy is
-    made of what is not contiguous); a kept object follows in-place changes
-    of them.  Fp8BlockExperts.quantize makes one from float weights."""
+    H % 16 == 0 and U % 16 == 0.
+
+    The tensors are kept, not copied, and every call takes them as they are
+    then: changed in place, with other memory (`t.data = ..`, Module.to) or set
+    anew as an attribute.  Scales that are not contiguous and biases that are
+    not contiguous float32 are converted in each call.  Only codes that are not
+    contiguous or not 16-byte aligned are copied once and no longer followed.
+    Fp8BlockExperts.quantize makes one from float weights."""
+
+    _TENSORS = ("w_up", "s_up", "w_down", "s_down", "b_up", "b_down")
 
     def __init__(self, w_up, s_up, w_down, s_down, *, b_up=None, b_down=None,
                  activation: str = "gelu"):
-        if activation not in ("gelu", "swiglu"):
+        self.w_up, self.s_up, self.w_down, self.s_down = w_up, s_up, w_down, s_down
+        self.b_up, self.b_down = b_up, b_down
+        self.activation = activation
+        self._bind()
+
+    def __setattr__(self, name, value):
+        super().__setattr__(name, value)
+        if name in self._TENSORS or name == "activation":
+            super().__setattr__("_at", None)  # the next call looks at it
+
+    def _bind(self):
+        """Checks the tensors and describes them to the library."""
+        w_up, s_up, w_down, s_down, b_up, b_down = (getattr(self, n) for n in self._TENSORS)
+        if self.activation not in ("gelu", "swiglu"):
             raise ValueError("activation must be 'gelu' or 'swiglu'")
-        self.device = nat.require_gpu(w_up, s_up, w_down, s_down, b_up, b_down)
+        device = nat.require_gpu(w_up, s_up, w_down, s_down, b_up, b_down)
         if w_up.ndim != 3 or w_down.ndim != 3:
             raise ValueError("w_up and w_down must be stacked over experts: [E, .., ..]")
-        halves = 2 if activation == "swiglu" else 1
+        halves = 2 if self.activation == "swiglu" else 1
         e, h, u = w_down.shape
         hb, ub = -(-h // FP8_BLOCK), -(-u // FP8_BLOCK)
         if w_up.shape != (e, halves * u, h):
@@ -116,25 +136,44 @@ class Fp8BlockExperts:
                 raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
         if h % 16 or u % 16 or not 1 <= e <= 256:
             raise ValueError("Fp8BlockExperts: H % 16 == 0, U % 16 == 0, 1 <= E <= 256")
+        self.device = device
         self.num_experts, self.hidden_size, self.expert_ffn_size = e, h, u
-        self.activation = activation
-
-        def whole(t):
-            t = t.contiguous()
-            return t if t.data_ptr() % 16 == 0 else t.clone()
-
-        self.w_up, self.s_up = whole(w_up), s_up.contiguous()
-        self.w_down, self.s_down = whole(w_down), s_down.contiguous()
-        self.b_up = None if b_up is None else b_up.detach().float().contiguous()
-        self.b_down = None if b_down is None else b_down.detach().float().contiguous()
+        for name, t in (("w_up", w_up), ("w_down", w_down)):
+            if not t.is_contiguous():
+                setattr(self, name, t.contiguous())
+            elif t.data_ptr() % 16:
+                setattr(self, name, t.clone())
+        at = self._addresses()
+        if 0 in at:
+            raise ValueError("Fp8BlockExperts: a tensor's memory was released")
         d = nat.SmoeExpertsFp8Blocks()
         d.act = nat.ACT_SWIGLU if halves == 2 else nat.ACT_GELU
         d.E, d.H, d.U = e, h, u
-        d.w_up, d.w_down = self.w_up.data_ptr(), self.w_down.data_ptr()
-        d.s_up, d.s_down = self.s_up.data_ptr(), self.s_down.data_ptr()
-        d.b_up, d.b_down = nat.ptr(self.b_up), nat.ptr(self.b_down)
+        d.w_up, d.s_up, d.w_down, d.s_down, d.b_up, d.b_down = at
         self._desc = d
         self._ref = ctypes.byref(d)
+        self._convert = [n for n, t in zip(self._TENSORS, (w_up, s_up, w_down, s_down, b_up, b_down))
+                         if n not in ("w_up", "w_down") and t is not None and
+                         not (t.dtype == torch.float32 and t.is_contiguous())]
+        self._at = at
+
+    def _addresses(self):
+        u, d = self.b_up, self.b_down
+        return (self.w_up.data_ptr(), self.s_up.data_ptr(), self.w_down.data_ptr(), self.s_down.data_ptr(),
+                None if u is None else u.data_ptr(), None if d is None else d.data_ptr())
+
+    def _descriptor(self):
+        """The C descriptor of the tensors as they are now, and what has to
+        live until the call on it is made."""
+        if self._at is None or self._at != self._addresses():
+            self._bind()
+        if not self._convert:
+            return self._ref, None
+        d = nat.SmoeExpertsFp8Blocks.from_buffer_copy(self._desc)
+        keep = [getattr(self, n).detach().float().contiguous() for n in self._convert]
+        for n, t in zip(self._convert, keep):
+            setattr(d, n, t.data_ptr())
+        return ctypes.byref(d), keep
 
     @classmethod
     def quantize(cls, w_up, w_down, *, b_up=None, b_down=None, activation: str = "gelu"):
@@ -172,6 +211,7 @@ def sparse_expert_delta_fp8_blocks(messages: torch.Tensor, top_indices: torch.Te
     follows are summed in f32; bfloat16: the products by the e4m3 x e4m3 matrix
     instruction, which cuts each one by less than 2^-13 of the largest of its
     eight neighbours, the rest in f32.  No gradient."""
+    ref, keep = experts._descriptor()
     dev = nat.require_gpu(messages, top_indices, top_weights, experts.w_up)
     h, k = messages.shape[-1], top_indices.shape[-1]
     if h != experts.hidden_size:
@@ -188,11 +228,12 @@ def sparse_expert_delta_fp8_blocks(messages: torch.Tensor, top_indices: torch.Te
         raise ValueError("more than 2^31 - 1 tokens")
     delta = torch.empty(messages.shape, dtype=messages.dtype, device=dev)
     lib = nat.lib()
-    need = lib.smoe_expert_delta_fp8_blocks_workspace_bytes(experts._ref, n, k)
+    need = lib.smoe_expert_delta_fp8_blocks_workspace_bytes(ref, n, k)
     if need == 0:
         raise RuntimeError("smoe_expert_delta_fp8_blocks: "
                            f"unsupported shapes ({lib.smoe_last_error().decode()})")
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    nat.launch(dev, "smoe_expert_delta_fp8_blocks", experts._ref, msg.data_ptr(), code,
+    nat.launch(dev, "smoe_expert_delta_fp8_blocks", ref, msg.data_ptr(), code,
                idx.data_ptr(), wts.data_ptr(), n, k, delta.data_ptr(), code, ws.data_ptr(), need)
+    del keep
     return delta
