@@ -413,8 +413,8 @@ SMOE_API int smoe_combine_rows(const void* y, int y_dtype, const float* row_w,
  * is 0, it is chosen after every other, with weight 0 (which the dispatch plan
  * drops), so a row that masks every expert gets weights 0.  NaN compares as
  * +infinity and gives NaN weights.  The choices are those of scores in
- * 64 bits.  N < 2^26, 1 <= E <= 256, 1 <= K <= min(64, top_groups * E / groups), groups divides E,
- * 1 <= top_groups <= groups.  No workspace. */
+ * 64 bits.  N <= 2^26 - 4, 1 <= E <= 256, 1 <= K <= min(64, top_groups * E /
+ * groups), groups divides E, 1 <= top_groups <= groups.  No workspace. */
 #define SMOE_SCORE_SOFTMAX 0
 #define SMOE_SCORE_SIGMOID 1
 SMOE_API int smoe_select_groups(const void* logits, int logits_dtype, int N, int E, int K, int score,
@@ -438,8 +438,8 @@ SMOE_API int smoe_select_groups_backward(const void* logits, int logits_dtype, i
  * smoe_quantize_fp8_tensor has them; a NaN in a block makes its scale and its
  * codes NaN.  codes [G, rows, ld_out] (ld_out % 16 == 0, cols <= ld_out <= cols
  * rounded up to 128; 16-byte aligned; code 0 past cols), scale f32
- * [G, ceil(rows / block_rows), ceil(cols / 128)].  Fewer than 2^28 blocks of
- * 1 x 128, 2^24 of 128 x 128.  No workspace. */
+ * [G, ceil(rows / block_rows), ceil(cols / 128)].  At most 2^28 - 16 blocks of
+ * 1 x 128, 2^24 - 1 of 128 x 128.  No workspace. */
 SMOE_API int smoe_quantize_fp8_blocks(const void* x, int x_dtype, int G, int rows, int cols,
                                       int64_t ldx, int block_rows, uint8_t* codes, int64_t ld_out,
                                       float* scale, void* stream);

@@ -1374,8 +1374,9 @@ namespace {
 
 int check_select_groups(int zdt, int N, int E, int K, int score) {
   if (zdt != SMOE_F32 && zdt != SMOE_BF16 && zdt != SMOE_F16) return fail(SMOE_EUNSUPPORTED, "logits dtype");
-  if (N < 0 || N >= 1 << 26 || E < 1 || E > 256 || K < 1 || K > E || K > 64)
-    return fail(SMOE_EINVAL, "select shape (N < 2^26, 1 <= K <= min(E, 64), E <= 256)");
+  // (N + 3) / 4 workgroups of 256 threads, fewer than 2^32 of them
+  if (N < 0 || N > (1 << 26) - 4 || E < 1 || E > 256 || K < 1 || K > E || K > 64)
+    return fail(SMOE_EINVAL, "select shape (N <= 2^26 - 4, 1 <= K <= min(E, 64), E <= 256)");
   if (score != SMOE_SCORE_SOFTMAX && score != SMOE_SCORE_SIGMOID) return fail(SMOE_EINVAL, "score");
   return SMOE_OK;
 }
@@ -1424,8 +1425,9 @@ SMOE_API int smoe_quantize_fp8_blocks(const void* x, int x_dtype, int G, int row
       ld_out > static_cast<int64_t>(fp8_blocks_of(cols)) * kFp8Block)
     return fail(SMOE_EINVAL, "quantize shape (ldx >= cols, cols <= ld_out <= cols rounded up to 128, ld_out % 16 == 0)");
   const int64_t blocks = static_cast<int64_t>(G) * (block_rows == 1 ? rows : fp8_blocks_of(rows));
-  if (blocks > ((block_rows == 1 ? 1 << 28 : 1 << 24) - 1) / fp8_blocks_of(cols))
-    return fail(SMOE_EINVAL, "quantize shape (fewer than 2^28 blocks of 1 x 128, 2^24 of 128 x 128)");
+  // sixteen row blocks, or one square one, a workgroup of 256 threads
+  if (blocks > (block_rows == 1 ? (1 << 28) - 16 : (1 << 24) - 1) / fp8_blocks_of(cols))
+    return fail(SMOE_EINVAL, "quantize shape (at most 2^28 - 16 blocks of 1 x 128, 2^24 - 1 of 128 x 128)");
   if (G == 0 || rows == 0) return SMOE_OK;
   if (!x || !codes || !scale) return fail(SMOE_EINVAL, "null buffer");
   if (!aligned16(codes)) return fail(SMOE_EINVAL, "codes must be 16-byte aligned");

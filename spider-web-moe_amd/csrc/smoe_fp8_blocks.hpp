@@ -11,7 +11,7 @@
 namespace smoe {
 
 constexpr int kFp8Block = 128;
-inline int fp8_blocks_of(int n) { return (n + kFp8Block - 1) / kFp8Block; }
+inline int fp8_blocks_of(int n) { return n / kFp8Block + (n % kFp8Block != 0); }  // any n >= 0
 
 // x [groups * rows, cols] (rows ldx elements apart) -> codes (rows ld_out
 // bytes apart, code 0 past cols) and the scale of block (row block r of
