@@ -44,11 +44,16 @@ __device__ __forceinline__ float block_scale(uint32_t amax) {
   return s < 1e-12f ? 1e-12f : s;
 }
 
-// Quotients by one divisor, correctly rounded: with r the correctly rounded
-// reciprocal and q0 = x r, the residual e = x - q0 s is exact and q0 + e r
-// rounds to x / s (P. Markstein, IBM J. Res. Dev. 34, 1990), where neither q0
-// nor e underflows; below, the code is 0 either way.  4 operations for an
-// IEEE division's 12.  s = infinity: 0 for finite x, NaN for infinite x.
+// Quotients by one divisor, as good as correctly rounded ones: r the correctly
+// rounded reciprocal, q0 = x r, e = x - q0 s, q0 + e r (P. Markstein, IBM J.
+// Res. Dev. 34, 1990).  His theorem asks for a q0 within a unit, which this one
+// exceeds by half a unit at times; but the sum is within 12 * 2^-49 (of x / s
+// brought to 1 .. 2) before it is rounded, and the few pairs where that could
+// move a quotient over the middle between two codes are tried one by one in
+// tests/test_fp8_blocks_quotient.py: the code is always that of the rounded
+// x / s.  Below 2^-10, where e could underflow, the code is 0 either way.  4
+// operations for an IEEE division's 12.  s = infinity: 0 for finite x, NaN for
+// infinite x.
 struct Divisor {
   float r, s;
 };
