@@ -121,7 +121,7 @@ __device__ __forceinline__ bool choose(const float (&z)[V], const SelectArgs& a,
 #pragma unroll
     for (int v = 0; v < V; ++v) s[v] = z[v] == -INFINITY ? T(0) : T(1) / (T(1) + exp_of(-T(z[v])));
   } else {
-    float m = -INFINITY;  // NaN if there is one: then every score is
+    float m = -INFINITY;  // of the numbers: a NaN makes the sum, and so every score, NaN
 #pragma unroll
     for (int v = 0; v < V; ++v) m = z[v] > m ? z[v] : m;
     m = wave_max(m);
