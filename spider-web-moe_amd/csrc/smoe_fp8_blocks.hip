@@ -72,7 +72,7 @@ __global__ __launch_bounds__(256) void k_quant_square_blocks(const BlockQuant q,
 // bf16 rounding; where large products cancel it can be all of it.  It suits
 // outputs of 8 to 16 bits, whose operands were themselves rounded by up to 2^-4.
 // WIDE (f32 outputs): the codes are widened to bf16, exactly, and multiplied at
-// half the rate with f32 sums.
+// half the rate with f32 sums (16384 x 1024 -> 5632: 265 to 288 us).
 //
 // 16384 x 1024 -> 5632 in bf16: 118 to 124 us, 1.5 to 1.6 PFLOP/s.  Stages alone
 // 86 (a stage of 256 x 256 tiles: 2048 cycles of products beside 1536 of LDS
@@ -522,7 +522,9 @@ int go_dense(const BlockGemm& a, hipStream_t s) {
 // 32), 128 above (1500 tokens, top-2 of 16 SwiGLU: 81, 84, 114), 256 from 512 on
 // (6000 tokens: 208 -> 181 us; 2500: 102 -> 119).  GELU's up product keeps 128
 // rows, whose two workgroups a CU hide one's epilogue under the other's products
-// (6000 tokens, top-4 of 32: 183 us with 256, 172).
+// (6000 tokens, top-4 of 32: 183 us with 256, 172).  WIDE has no registers for
+// 256 rows and keeps 128 (16384 tokens, top-2 of 16 SwiGLU: up 581 us, down 252;
+// 254 and 129 without).
 template <int EPI, bool WIDE>
 int go_grouped(const BlockGemm& a, hipStream_t s) {
   constexpr int O = SMOE_F32;

@@ -270,11 +270,12 @@ __device__ __forceinline__ bool choose(const float (&z)[V], const SelectArgs& a,
 }
 
 // One wave per token.  The choice is made in f32 and, where two values that
-// decide lie nearer than f32 tells apart, once more in f64 (sigmoid scores of
-// 256 experts: about 1 token in 100), so that it is the order of the real
-// values: 16384 tokens over 256 experts in 8 groups, top 8 of 4 groups, 66 us
-// all in f64, 37 so.  Bound by instructions: about 1200 a token, half of them
-// the K rounds of a maximum over the wave; the bytes are 4 us.
+// decide lie nearer than f32 tells apart, once more in f64, so that it is the
+// order of the real values.  16384 tokens over 256 experts in 8 groups, top 8 of
+// 4 groups: 37 us with normal f32 logits (about 1 token in 100 needs both), 60
+// at most, where every token does (uniform, saturated or equal logits).  Bound
+// by instructions: about 1200 a token, half of them the K rounds of a maximum
+// over the wave; the bytes are 4 us.
 template <int DT, int V>
 __global__ __launch_bounds__(256) void k_select_groups(const void* __restrict__ logits, int N, bool vec,
                                                        const SelectArgs a, float* __restrict__ top_w,

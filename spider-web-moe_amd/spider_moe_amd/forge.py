@@ -93,8 +93,8 @@ class ForgeSelect:
         indices int32) [..., k], as the dispatch plan and the experts read
         them.
 
-        s = softmax(logits) or sigmoid(logits); s + bias (bias [E], which
-        evens out the experts' load) decides the choice, s alone the weights.
+        s = softmax(logits) or sigmoid(logits); s + bias (bias [E], taken as
+        float32, which evens out the experts' load) decides the choice, s alone the weights.
         With num_groups > 1 consecutive experts form groups, a group's value
         is the sum of its two largest s + bias, and only the top_groups best
         groups take part.  The k largest are chosen, ties to the lower index,
