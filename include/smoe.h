@@ -429,6 +429,34 @@ SMOE_API int smoe_select_groups_backward(const void* logits, int logits_dtype, i
                                          int score, int renorm, float scale, const int32_t* top_idx,
                                          const float* d_top_w, void* d_logits, void* stream);
 
+/* Balance loss of a router over S sequences of T tokens: logits z [S,T,E]
+ * (SMOE_F32 / SMOE_BF16 / SMOE_F16), the choices top_idx i32 [S,T,K] (ids
+ * outside [0, E) count nowhere, equal ids of a token each for itself), mask u8
+ * [S,T] (0: the token is padding; whatever its logits hold plays no part) or
+ * NULL.  Per sequence, n its tokens that are not masked:
+ *   p = softmax(z) of a token, or sigmoid(z) over its sum; 0 where z = -inf, and
+ *       for a token whose logits all are
+ *   counts_e = choices of expert e, load_e = counts_e / sum of counts,
+ *   loss = E sum_e load_e (sum over tokens of p_e) / n
+ * (SpiderMoELayer's aux_loss is the softmax form over the whole batch,
+ * model.py:330-337: S = 1).  No tokens or no choices: loss 0.  loss f32 [S],
+ * counts i32 [S,E], slope f32 [S,E] or NULL: what the backward pass takes,
+ * (E load_e - 1) / n.  Sums over tokens are in f32 over one workgroup's and in
+ * 64 bits over those; their order depends on the sizes alone.
+ * S * T <= 2^26 - 4, S < 2^22, 1 <= E <= 256, 1 <= K <= 64, S * T * K < 2^31.
+ * Where the workspace query gives 0 the workspace may be NULL. */
+SMOE_API size_t smoe_balance_loss_workspace_bytes(int S, int T, int E);
+SMOE_API int smoe_balance_loss(const void* logits, int logits_dtype, int S, int T, int E, int K,
+                               int score, const int32_t* top_idx, const uint8_t* mask, float* loss,
+                               int32_t* counts, float* slope, void* workspace,
+                               size_t workspace_bytes, void* stream);
+/* Its gradient in the logits, the counts held fixed: d_loss f32 [S] ->
+ * d_logits [S,T,E] in logits_dtype, every entry written (0 for masked tokens).
+ * slope as smoe_balance_loss wrote it. */
+SMOE_API int smoe_balance_loss_backward(const void* logits, int logits_dtype, int S, int T, int E,
+                                        int score, const uint8_t* mask, const float* slope,
+                                        const float* d_loss, void* d_logits, void* stream);
+
 /* Block-scaled e4m3: x [G, rows, cols] (SMOE_F32 / SMOE_BF16 / SMOE_F16; rows
  * ldx elements apart, ldx >= cols) cut into blocks of block_rows x 128,
  * block_rows 1 (activations: one scale per token and 128 channels) or 128
@@ -498,6 +526,77 @@ SMOE_API int smoe_expert_delta_fp8_blocks(const smoe_experts_fp8_blocks* ex, con
                                           int msg_dtype, const int32_t* idx, const float* w, int N,
                                           int K, void* delta, int out_dtype, void* workspace,
                                           size_t workspace_bytes, void* stream);
+
+/* ---- microscaled 4-bit floating point (OCP Microscaling Formats v1.0, MXFP4) ----
+ * x [rows, cols] (SMOE_F32 / SMOE_BF16 / SMOE_F16; rows ldx elements apart) cut
+ * along its rows into blocks of 32 (the last one of a row may be shorter).  Per
+ * block the power of two X = 2^(floor(log2 amax|x|) - 2), at least 2^-127, kept
+ * as its biased exponent (E8M0: byte b is 2^(b - 127)), and codes of x / X in
+ * e2m1 (sign, then 0, 0.5, 1, 1.5, 2, 3, 4, 6), rounded to nearest even, past 6
+ * to 6.  A block of zeros has X = 2^-127; a block with an infinity or a NaN has
+ * byte 255 (NaN) and codes 0, and so stands for NaN.
+ * codes: two a byte, the even column in the low half; rows ld_codes bytes apart
+ * (ld_codes % 16 == 0, 16 ceil(cols / 32) <= ld_codes <= 64 ceil(cols / 128);
+ * 16-byte aligned; code 0 past cols).  scale: a byte a block, rows ld_scale
+ * bytes apart (ld_scale % 4 == 0, >= ceil(cols / 32); 4-byte aligned; whole
+ * words are written).  At most 2^28 - 16 pieces of 1 x 128.  No workspace. */
+SMOE_API int smoe_quantize_mxfp4(const void* x, int x_dtype, int64_t rows, int cols, int64_t ldx,
+                                 uint8_t* codes, int64_t ld_codes, uint8_t* scale,
+                                 int64_t ld_scale, void* stream);
+/* The values of such codes (any ld_codes >= cols / 2 rounded up, any ld_scale
+ * >= ceil(cols / 32), any alignment): out [rows, cols] (SMOE_F32 / SMOE_BF16,
+ * exact; SMOE_F16 rounded to nearest).  Fewer than 2^32 - 512 pieces of 1 x 8. */
+SMOE_API int smoe_dequantize_mxfp4(const uint8_t* codes, int64_t ld_codes, const uint8_t* scale,
+                                   int64_t ld_scale, int64_t rows, int cols, void* out,
+                                   int out_dtype, void* stream);
+
+/* out [N, N_out] = act(x [N,K] . W^T + bias), W in such codes [N_out, K] (rows
+ * of whole blocks: ldw % 16 == 0, ldw >= 16 ceil(K / 32), 16-byte aligned; what
+ * lies past K in a row's last block plays no part) and scales (rows ld_ws bytes
+ * apart, ld_ws % 4 == 0, ld_ws >= ceil(K / 32), 4-byte aligned).  x (SMOE_F32 /
+ * SMOE_BF16 / SMOE_F16, rows ldx elements apart) is quantized by the call as
+ * smoe_quantize_mxfp4 does.  Products of the two operands' values, summed in f32;
+ * act SMOE_LINEAR_NONE / SMOE_LINEAR_GELU; bias f32 [N_out] or NULL; any K, any
+ * N_out.  Where the workspace query gives 0 (a few rows) the workspace may be
+ * NULL. */
+SMOE_API size_t smoe_linear_mxfp4_workspace_bytes(int N, int K);
+SMOE_API int smoe_linear_mxfp4(const void* x, int x_dtype, int64_t ldx, int N, int K,
+                               const uint8_t* wq, int64_t ldw, const uint8_t* w_scale,
+                               int64_t ld_ws, const float* bias, int N_out, int act, void* out,
+                               int out_dtype, void* workspace, size_t workspace_bytes,
+                               void* stream);
+
+/* Expert FFN weights in that format, stacked over experts: rows of whole
+ * blocks, one after another, and scales in rows of whole words.
+ *   w_up codes of [E,U,H] ([E,2U,H] with SMOE_ACT_SWIGLU, the gate's U rows,
+ *   then the up projection's), H / 2 bytes a row; s_up H / 32 bytes a row,
+ *   rounded up to a multiple of 4; w_down codes of [E,H,U], s_down alike;
+ *   b_up f32 [E,U] (SwiGLU: added to the up projection), b_down [E,H], or NULL.
+ * H % 32 == 0, U % 32 == 0, 1 <= E <= 256, codes 16-byte, scales 4-byte aligned. */
+typedef struct smoe_experts_mxfp4 {
+  int act; /* SMOE_ACT_GELU / SMOE_ACT_SWIGLU */
+  int E, H, U;
+  const uint8_t* w_up;
+  const uint8_t* w_down;
+  const uint8_t* s_up;
+  const uint8_t* s_down;
+  const float* b_up;
+  const float* b_down;
+} smoe_experts_mxfp4;
+
+/* smoe_expert_delta on such experts: the messages msg [N,H] (SMOE_F32 /
+ * SMOE_BF16) and the hidden activations (in f32) are quantized on the way into
+ * the two products; delta [N,H] (SMOE_F32 / SMOE_BF16) = per token the sum over
+ * its experts of w * (W_down act(W_up m + b_up) + b_down), in f32 until the end.
+ * idx i32 / w f32 [N,K] as smoe_dispatch_plan takes them (equal ids merged,
+ * weights <= 0 and ids outside [0, E) dropped; a token left without experts gets
+ * 0).  1 <= K <= 64, N * K < 2^31 - 128, N <= 4194240, with H > 4096 N <= 65535,
+ * N * ceil(H / 128) <= 2^28 - 16. */
+SMOE_API size_t smoe_expert_delta_mxfp4_workspace_bytes(const smoe_experts_mxfp4* ex, int N, int K);
+SMOE_API int smoe_expert_delta_mxfp4(const smoe_experts_mxfp4* ex, const void* msg, int msg_dtype,
+                                     const int32_t* idx, const float* w, int N, int K, void* delta,
+                                     int out_dtype, void* workspace, size_t workspace_bytes,
+                                     void* stream);
 
 /* ---- Dobu expert residency (spider_moe/expert_store.py:121-166) ----
  * out[i] = map[ids[i]] for ids in [0, E), else -1: routed expert ids ->

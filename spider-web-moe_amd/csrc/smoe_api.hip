@@ -21,6 +21,7 @@
 #include "smoe_common.hpp"
 #include "smoe_fp8_blocks.hpp"
 #include "smoe_internal.hpp"
+#include "smoe_mxfp4.hpp"
 
 using namespace smoe;
 
@@ -1414,6 +1415,70 @@ SMOE_API int smoe_select_groups_backward(const void* logits, int logits_dtype, i
   return SMOE_OK;
 }
 
+// ----------------------------------------------------- balance loss ----
+namespace {
+
+int check_balance(int dt, int S, int T, int E, int score) {
+  if (dt != SMOE_F32 && dt != SMOE_BF16 && dt != SMOE_F16) return fail(SMOE_EUNSUPPORTED, "logits dtype");
+  if (S < 0 || T < 0 || static_cast<int64_t>(S) * T > (1 << 26) - 4 || S > (1 << 22) - 1 || E < 1 || E > 256)
+    return fail(SMOE_EINVAL, "balance shape (S * T <= 2^26 - 4, S < 2^22, 1 <= E <= 256)");
+  if (score != SMOE_SCORE_SOFTMAX && score != SMOE_SCORE_SIGMOID) return fail(SMOE_EINVAL, "score");
+  return SMOE_OK;
+}
+
+struct BalanceWs {
+  size_t part_p, part_c, total;
+};
+BalanceWs balance_ws(int S, int T, int E) {
+  const size_t n = static_cast<size_t>(S) * balance_chunks(S, T);
+  BalanceWs w;
+  Bump z;
+  w.part_p = z.take(n * E * 4);
+  w.part_c = z.take(n * (E + 1) * 4);
+  w.total = z.off;
+  return w;
+}
+
+}  // namespace
+
+SMOE_API size_t smoe_balance_loss_workspace_bytes(int S, int T, int E) {
+  if (check_balance(SMOE_F32, S, T, E, SMOE_SCORE_SOFTMAX) != SMOE_OK || S == 0 || balance_chunks(S, T) == 1) return 0;
+  return balance_ws(S, T, E).total;
+}
+
+SMOE_API int smoe_balance_loss(const void* logits, int logits_dtype, int S, int T, int E, int K, int score,
+                               const int32_t* top_idx, const uint8_t* mask, float* loss, int32_t* counts,
+                               float* slope, void* ws, size_t ws_bytes, void* stream) {
+  const int rc = check_balance(logits_dtype, S, T, E, score);
+  if (rc != SMOE_OK) return rc;
+  if (K < 1 || K > 64 || static_cast<int64_t>(S) * T * K > 0x7fffffff)
+    return fail(SMOE_EINVAL, "1 <= K <= 64, S * T * K < 2^31");
+  if (S == 0) return SMOE_OK;
+  const size_t need = smoe_balance_loss_workspace_bytes(S, T, E);
+  if ((T > 0 && (!logits || !top_idx)) || !loss || !counts || (need && !ws)) return fail(SMOE_EINVAL, "null buffer");
+  if (need && !aligned16(ws)) return fail(SMOE_EINVAL, "workspace must be 16-byte aligned");
+  if (ws_bytes < need) return fail(SMOE_ECAPACITY, "workspace");
+  const BalanceWs l = balance_ws(S, T, E);
+  SMOE_TRY(launch_balance_loss(logits, logits_dtype, S, T, E, K, score == SMOE_SCORE_SIGMOID, top_idx, mask, loss,
+                               counts, slope, need ? at<float>(ws, l.part_p) : nullptr,
+                               need ? at<int32_t>(ws, l.part_c) : nullptr, static_cast<hipStream_t>(stream)),
+           "balance loss");
+  return SMOE_OK;
+}
+
+SMOE_API int smoe_balance_loss_backward(const void* logits, int logits_dtype, int S, int T, int E, int score,
+                                        const uint8_t* mask, const float* slope, const float* d_loss,
+                                        void* d_logits, void* stream) {
+  const int rc = check_balance(logits_dtype, S, T, E, score);
+  if (rc != SMOE_OK) return rc;
+  if (S == 0 || T == 0) return SMOE_OK;
+  if (!logits || !slope || !d_loss || !d_logits) return fail(SMOE_EINVAL, "null buffer");
+  SMOE_TRY(launch_balance_loss_bwd(logits, logits_dtype, S, T, E, score == SMOE_SCORE_SIGMOID, mask, slope, d_loss,
+                                   d_logits, static_cast<hipStream_t>(stream)),
+           "balance loss backward");
+  return SMOE_OK;
+}
+
 // ----------------------------------------------- block-scaled fp8 ----
 SMOE_API int smoe_quantize_fp8_blocks(const void* x, int x_dtype, int G, int rows, int cols, int64_t ldx,
                                       int block_rows, uint8_t* codes, int64_t ld_out, float* scale,
@@ -1703,6 +1768,291 @@ SMOE_API int smoe_expert_delta_fp8_blocks(const smoe_experts_fp8_blocks* ex, con
   dn.out = at<void>(ws, l.y);
   dn.ldo = H;
   SMOE_TRY(launch_gemm_fp8_blocks(dn, s), "expert down GEMM");
+  SMOE_TRY(launch_delta_combine(at<void>(ws, l.y), SMOE_F32, tokrow, N, K, H, delta, out_dtype, s), "delta combine");
+  return SMOE_OK;
+}
+
+// ------------------------------------------------- microscaled 4-bit ----
+SMOE_API int smoe_quantize_mxfp4(const void* x, int x_dtype, int64_t rows, int cols, int64_t ldx, uint8_t* codes,
+                                 int64_t ld_codes, uint8_t* scale, int64_t ld_scale, void* stream) {
+  if (x_dtype != SMOE_F32 && x_dtype != SMOE_BF16 && x_dtype != SMOE_F16)
+    return fail(SMOE_EUNSUPPORTED, "quantize input dtype");
+  if (rows < 0 || cols < 1 || cols > 0x7fffff80 || ldx < cols) return fail(SMOE_EINVAL, "quantize shape (cols >= 1, ldx >= cols)");
+  const int64_t npc = (static_cast<int64_t>(cols) + 127) / 128;
+  if (ld_codes % 16 || ld_codes < mx_code_pitch(cols) || ld_codes > 64 * npc || ld_scale % 4 || ld_scale < mx_scale_pitch(cols))
+    return fail(SMOE_EINVAL, "16 bytes of codes a block, at most cols rounded up to 128 (ld_codes % 16 == 0), ld_scale % 4 == 0");
+  if (rows > ((1 << 28) - 16) / npc) return fail(SMOE_EINVAL, "quantize shape (at most 2^28 - 16 pieces of 1 x 128)");
+  if (rows == 0) return SMOE_OK;
+  if (!x || !codes || !scale) return fail(SMOE_EINVAL, "null buffer");
+  if (!aligned16(codes) || reinterpret_cast<uintptr_t>(scale) % 4) return fail(SMOE_EINVAL, "codes must be 16-byte, scale 4-byte aligned");
+  MxQuant q;
+  q.x = x;
+  q.x_dtype = x_dtype;
+  q.ldx = ldx;
+  q.rows = rows;
+  q.cols = cols;
+  q.codes = codes;
+  q.ld_codes = ld_codes;
+  q.scale = scale;
+  q.ld_scale = ld_scale;
+  SMOE_TRY(launch_quantize_mxfp4(q, static_cast<hipStream_t>(stream)), "quantize mxfp4");
+  return SMOE_OK;
+}
+
+SMOE_API int smoe_dequantize_mxfp4(const uint8_t* codes, int64_t ld_codes, const uint8_t* scale, int64_t ld_scale,
+                                   int64_t rows, int cols, void* out, int out_dtype, void* stream) {
+  if (out_dtype != SMOE_F32 && out_dtype != SMOE_BF16 && out_dtype != SMOE_F16) return fail(SMOE_EUNSUPPORTED, "out dtype");
+  if (rows < 0 || cols < 1 || cols > 0x7fffff80 || ld_codes < (static_cast<int64_t>(cols) + 1) / 2 || ld_scale < mx_blocks_of(cols))
+    return fail(SMOE_EINVAL, "dequantize shape (rows of at least cols / 2 codes' bytes and cols / 32 scales)");
+  if (rows > 0xfffffe00ll / ((static_cast<int64_t>(cols) + 7) / 8)) return fail(SMOE_EINVAL, "dequantize shape (fewer than 2^32 - 512 pieces of 8)");
+  if (rows == 0) return SMOE_OK;
+  if (!codes || !scale || !out) return fail(SMOE_EINVAL, "null buffer");
+  SMOE_TRY(launch_dequantize_mxfp4(codes, ld_codes, scale, ld_scale, rows, cols, out, out_dtype, static_cast<hipStream_t>(stream)),
+           "dequantize mxfp4");
+  return SMOE_OK;
+}
+
+namespace {
+
+// x quantized: codes in rows of whole blocks, scales in rows of whole words
+struct MxWs {
+  size_t codes, scale, total;
+};
+MxWs mx_ws(int64_t N, int K) {
+  MxWs w;
+  Bump z;
+  w.codes = z.take(static_cast<size_t>(N) * mx_code_pitch(K));
+  w.scale = z.take(static_cast<size_t>(N) * mx_scale_pitch(K));
+  w.total = z.off;
+  return w;
+}
+
+MxQuant mx_rows(const void* x, int xdt, int64_t ldx, int N, int K, void* ws, const MxWs& l) {
+  MxQuant q;
+  q.x = x;
+  q.x_dtype = xdt;
+  q.ldx = ldx;
+  q.rows = N;
+  q.cols = K;
+  q.codes = at<uint8_t>(ws, l.codes);
+  q.ld_codes = mx_code_pitch(K);
+  q.scale = at<uint8_t>(ws, l.scale);
+  q.ld_scale = mx_scale_pitch(K);
+  return q;
+}
+
+}  // namespace
+
+SMOE_API size_t smoe_linear_mxfp4_workspace_bytes(int N, int K) {
+  return N < 1 || K < 1 || mx_linear_quantizes_inside(N, K) ? 0 : mx_ws(N, K).total;
+}
+
+SMOE_API int smoe_linear_mxfp4(const void* x, int x_dtype, int64_t ldx, int N, int K, const uint8_t* wq, int64_t ldw,
+                               const uint8_t* w_scale, int64_t ld_ws, const float* bias, int N_out, int act, void* out,
+                               int out_dtype, void* ws, size_t ws_bytes, void* stream) {
+  if (x_dtype != SMOE_F32 && x_dtype != SMOE_BF16 && x_dtype != SMOE_F16) return fail(SMOE_EUNSUPPORTED, "linear input dtype");
+  if (N < 0 || N > 0x7fffff00 || K < 1 || K > 0x7fffff00 || N_out < 1 || N_out > 0x7fffff00 || ldx < K ||
+      ldw < mx_code_pitch(K) || ldw % 16 || ld_ws < mx_scale_pitch(K) || ld_ws % 4)
+    return fail(SMOE_EINVAL, "mxfp4 linear shape (ldx >= K; weight rows of whole blocks, ldw % 16 == 0; ld_ws % 4 == 0)");
+  if (N > ((1 << 28) - 16) / ((static_cast<int64_t>(K) + 127) / 128)) return fail(SMOE_EINVAL, "mxfp4 linear shape (at most 2^28 - 16 pieces of 1 x 128 of x)");
+  if (act != SMOE_LINEAR_NONE && act != SMOE_LINEAR_GELU) return fail(SMOE_EINVAL, "act");
+  if (out_dtype != SMOE_F32 && out_dtype != SMOE_BF16) return fail(SMOE_EUNSUPPORTED, "out dtype");
+  if (N == 0) return SMOE_OK;
+  const bool inside = mx_linear_quantizes_inside(N, K);
+  if (!x || !wq || !w_scale || !out || (!inside && !ws)) return fail(SMOE_EINVAL, "null buffer");
+  if (!aligned16(wq) || reinterpret_cast<uintptr_t>(w_scale) % 4 || (!inside && !aligned16(ws)))
+    return fail(SMOE_EINVAL, "codes and workspace must be 16-byte, scales 4-byte aligned");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  MxGemm g;
+  g.epi = act == SMOE_LINEAR_GELU ? MX_GELU : MX_LINEAR;
+  if (inside) {
+    g.x_float = x;
+    g.x_dtype = x_dtype;
+    g.ld_float = ldx;
+  } else {
+    const MxWs l = mx_ws(N, K);
+    if (ws_bytes < l.total) return fail(SMOE_ECAPACITY, "workspace");
+    const MxQuant q = mx_rows(x, x_dtype, ldx, N, K, ws, l);
+    SMOE_TRY(launch_quantize_mxfp4(q, s), "quantize mxfp4");
+    g.X = q.codes;
+    g.ldx = q.ld_codes;
+    g.xs = q.scale;
+    g.ld_xs = q.ld_scale;
+  }
+  g.W = wq;
+  g.ldw = ldw;
+  g.ws = w_scale;
+  g.ld_ws = ld_ws;
+  g.K = K;
+  g.N_out = N_out;
+  g.single_rows = N;
+  g.bias = bias;
+  g.out = out;
+  g.out_dtype = out_dtype;
+  g.ldo = N_out;
+  SMOE_TRY(launch_gemm_mxfp4(g, s), "mxfp4 GEMM");
+  return SMOE_OK;
+}
+
+namespace {
+
+int check_experts_mxfp4(const smoe_experts_mxfp4* ex, int N, int K) {
+  if (!ex) return fail(SMOE_EINVAL, "null experts");
+  if (ex->act != SMOE_ACT_GELU && ex->act != SMOE_ACT_SWIGLU) return fail(SMOE_EINVAL, "act");
+  if (ex->E < 1 || ex->E > 256 || ex->H < 32 || ex->H % 32 || ex->U < 32 || ex->U % 32 || ex->H > (1 << 24) ||
+      ex->U > (1 << 24))
+    return fail(SMOE_EINVAL, "mxfp4 experts: 1 <= E <= 256, H % 32 == 0, U % 32 == 0");
+  if (!ex->w_up || !ex->w_down || !ex->s_up || !ex->s_down) return fail(SMOE_EINVAL, "expert weights or scales missing");
+  if (!aligned16(ex->w_up) || !aligned16(ex->w_down) || reinterpret_cast<uintptr_t>(ex->s_up) % 4 ||
+      reinterpret_cast<uintptr_t>(ex->s_down) % 4)
+    return fail(SMOE_EINVAL, "expert codes must be 16-byte, scales 4-byte aligned");
+  if (N < 0 || K < 1 || K > 64 || static_cast<int64_t>(N) * K > 0x7fffff7f)
+    return fail(SMOE_EINVAL, "shape (1 <= top_k <= 64, N * top_k < 2^31 - 128)");
+  if (N > (ex->H > 4096 ? 65535 : 65535 * 64)) return fail(SMOE_EINVAL, "N <= 4194240, with H > 4096 N <= 65535");
+  if (N > ((1 << 28) - 16) / ((ex->H + 127) / 128)) return fail(SMOE_EINVAL, "N * ceil(H / 128) <= 2^28 - 16");
+  return SMOE_OK;
+}
+
+struct MxExpertsWs {
+  size_t plan, off, cnt, rows, roww, tokrow, act, ascale, y, total;
+  MxWs x;
+  size_t x_at;
+};
+MxExpertsWs mx_experts_ws(const smoe_experts_mxfp4& ex, int N, int K) {
+  const size_t n = N > 0 ? N : 1, r = n * K;
+  MxExpertsWs w;
+  Bump z;
+  w.plan = z.take(smoe_dispatch_workspace_bytes(N, K, ex.E));
+  w.off = z.take((ex.E + 1) * 4);
+  w.cnt = z.take(ex.E * 4);
+  w.rows = z.take(r * 4);
+  w.roww = z.take(r * 4);
+  w.tokrow = z.take(r * 4);
+  w.x = mx_ws(n, ex.H);
+  w.x_at = z.take(w.x.total);
+  w.act = z.take(r * mx_code_pitch(ex.U));
+  w.ascale = z.take(r * mx_scale_pitch(ex.U));
+  w.y = z.take(r * ex.H * 4);
+  w.total = z.off;
+  return w;
+}
+
+}  // namespace
+
+SMOE_API size_t smoe_expert_delta_mxfp4_workspace_bytes(const smoe_experts_mxfp4* ex, int N, int K) {
+  if (check_experts_mxfp4(ex, N, K) != SMOE_OK) return 0;
+  if (N > 0 && mx_tokens_fit(N, K, ex->H, ex->U)) return align_up(static_cast<size_t>(N) * K * ex->U * 4);
+  return mx_experts_ws(*ex, N, K).total;
+}
+
+SMOE_API int smoe_expert_delta_mxfp4(const smoe_experts_mxfp4* ex, const void* msg, int msg_dtype, const int32_t* idx,
+                                     const float* w, int N, int K, void* delta, int out_dtype, void* ws,
+                                     size_t ws_bytes, void* stream) {
+  int rc = check_experts_mxfp4(ex, N, K);
+  if (rc != SMOE_OK) return rc;
+  if (msg_dtype != SMOE_F32 && msg_dtype != SMOE_BF16) return fail(SMOE_EUNSUPPORTED, "message dtype");
+  if (out_dtype != SMOE_F32 && out_dtype != SMOE_BF16) return fail(SMOE_EUNSUPPORTED, "out dtype");
+  if (N == 0) return SMOE_OK;
+  if (!msg || !idx || !w || !delta || !ws) return fail(SMOE_EINVAL, "null buffer");
+  if (!aligned16(ws)) return fail(SMOE_EINVAL, "workspace must be 16-byte aligned");
+  if (ws_bytes < smoe_expert_delta_mxfp4_workspace_bytes(ex, N, K)) return fail(SMOE_ECAPACITY, "workspace");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (mx_tokens_fit(N, K, ex->H, ex->U)) {
+    MxTokensArgs t;
+    t.msg = msg;
+    t.msg_dtype = msg_dtype;
+    t.idx = idx;
+    t.w = w;
+    t.N = N;
+    t.K = K;
+    t.E = ex->E;
+    t.H = ex->H;
+    t.U = ex->U;
+    t.act_fn = ex->act;
+    t.w_up = ex->w_up;
+    t.w_down = ex->w_down;
+    t.s_up = ex->s_up;
+    t.s_down = ex->s_down;
+    t.b_up = ex->b_up;
+    t.b_down = ex->b_down;
+    t.act = static_cast<float*>(ws);
+    t.out = delta;
+    t.out_dtype = out_dtype;
+    SMOE_TRY(launch_mx_tokens(t, s), "expert step of a few tokens");
+    return SMOE_OK;
+  }
+  const MxExpertsWs l = mx_experts_ws(*ex, N, K);
+  const int E = ex->E, H = ex->H, U = ex->U;
+  const int halves = ex->act == SMOE_ACT_SWIGLU ? 2 : 1;
+  int32_t *off = at<int32_t>(ws, l.off), *rows = at<int32_t>(ws, l.rows), *tokrow = at<int32_t>(ws, l.tokrow);
+  float* roww = at<float>(ws, l.roww);
+  const MxQuant mq = mx_rows(msg, msg_dtype, H, N, H, at<void>(ws, l.x_at), l.x);
+  if (prep_fits(N, K, E)) {
+    PrepArgs pa;
+    pa.idx = idx;
+    pa.w = w;
+    pa.N = N;
+    pa.K = K;
+    pa.E = E;
+    pa.off = off;
+    pa.rows = rows;
+    pa.tokrow = tokrow;
+    pa.roww = roww;
+    SMOE_TRY(launch_prep_mx(pa, mq, s), "plan and messages");
+  } else {
+    rc = smoe_dispatch_plan(idx, w, N, K, E, at<int32_t>(ws, l.cnt), off, rows, roww, tokrow, at<void>(ws, l.plan),
+                            smoe_dispatch_workspace_bytes(N, K, E), stream);
+    if (rc != SMOE_OK) return rc;
+    SMOE_TRY(launch_quantize_mxfp4(mq, s), "quantize messages");
+  }
+  MxGemm up;
+  up.epi = halves == 2 ? MX_UP_SWIGLU : MX_UP_GELU;
+  up.X = mq.codes;
+  up.ldx = mq.ld_codes;
+  up.xs = mq.scale;
+  up.ld_xs = mq.ld_scale;
+  up.a_rows = rows;
+  up.W = ex->w_up;
+  up.ldw = mx_code_pitch(H);
+  up.w_gstride = static_cast<int64_t>(halves) * U * up.ldw;
+  up.ws = ex->s_up;
+  up.ld_ws = mx_scale_pitch(H);
+  up.ws_gstride = static_cast<int64_t>(halves) * U * up.ld_ws;
+  up.K = H;
+  up.N_out = U;
+  up.grp_off = off;
+  up.G = E;
+  up.max_rows = N * K;
+  up.bias = ex->b_up;
+  up.bias_gstride = U;
+  up.out = at<void>(ws, l.act);
+  up.ldo = mx_code_pitch(U);
+  up.out_scale = at<uint8_t>(ws, l.ascale);
+  up.ld_os = mx_scale_pitch(U);
+  SMOE_TRY(launch_gemm_mxfp4(up, s), "expert up GEMM");
+  MxGemm dn;
+  dn.epi = MX_DOWN;
+  dn.X = at<uint8_t>(ws, l.act);
+  dn.ldx = up.ldo;
+  dn.xs = up.out_scale;
+  dn.ld_xs = up.ld_os;
+  dn.W = ex->w_down;
+  dn.ldw = mx_code_pitch(U);
+  dn.w_gstride = H * dn.ldw;
+  dn.ws = ex->s_down;
+  dn.ld_ws = mx_scale_pitch(U);
+  dn.ws_gstride = H * dn.ld_ws;
+  dn.K = U;
+  dn.N_out = H;
+  dn.grp_off = off;
+  dn.G = E;
+  dn.max_rows = N * K;
+  dn.bias = ex->b_down;
+  dn.bias_gstride = H;
+  dn.row_scale = roww;
+  dn.out = at<void>(ws, l.y);
+  dn.ldo = H;
+  SMOE_TRY(launch_gemm_mxfp4(dn, s), "expert down GEMM");
   SMOE_TRY(launch_delta_combine(at<void>(ws, l.y), SMOE_F32, tokrow, N, K, H, delta, out_dtype, s), "delta combine");
   return SMOE_OK;
 }

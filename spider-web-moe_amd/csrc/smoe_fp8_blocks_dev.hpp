@@ -148,8 +148,8 @@ __device__ __forceinline__ void quant_row_block(const BlockQuant& q, int nblk, i
 }
 
 // Four output channels n .. n + 3 of row r (those below N_out)
-template <int ODT>
-__device__ __forceinline__ void store4(const BlockGemm& p, int64_t r, int n, const float (&o)[4]) {
+template <int ODT, typename P>
+__device__ __forceinline__ void store4(const P& p, int64_t r, int n, const float (&o)[4]) {
   const int64_t at = r * p.ldo + n;
   if constexpr (ODT == SMOE_F32) {
     float* po = reinterpret_cast<float*>(p.out) + at;
@@ -173,8 +173,9 @@ __device__ __forceinline__ void store4(const BlockGemm& p, int64_t r, int n, con
 }
 
 // Rows of the 64 groups from b on: first, end and BM-row tiles of group
-// b + lane.
-__device__ __forceinline__ void groups64(const BlockGemm& p, int BM, int b, int& lo, int& hi, int& t) {
+// b + lane.  P: BlockGemm or MxGemm.
+template <typename P>
+__device__ __forceinline__ void groups64(const P& p, int BM, int b, int& lo, int& hi, int& t) {
   const int i = b + static_cast<int>(threadIdx.x & 63);
   const int ic = i < p.G ? i : p.G - 1;
   lo = p.grp_off[ic];
@@ -189,8 +190,8 @@ __device__ __forceinline__ void groups64(const BlockGemm& p, int BM, int b, int&
 // contiguous part of the order.  SUPER: an XCD holds 32 tiles of 256 rows (64 of
 // 128) at a time (32768 routed rows, 1024 -> 2816 SwiGLU, 256 rows a tile: 2
 // row tiles 250 us, 4 252, 8 260, 16 256; 1024 -> 5632: 119, 117, 118, 121).
-template <int BM, int BN>
-__device__ __forceinline__ bool block_tile(const BlockGemm& p, int bid, int& g, int& m0, int& mrows,
+template <int BM, int BN, typename P>
+__device__ __forceinline__ bool block_tile(const P& p, int bid, int& g, int& m0, int& mrows,
                                            int& n0) {
   const int strips = (p.N_out + BN - 1) / BN;
   int tiles = 0;

@@ -240,6 +240,16 @@ int launch_select_groups(const void* logits, int zdt, int N, int E, int K, int s
 int launch_select_groups_bwd(const void* logits, int zdt, int N, int E, int K, int sigmoid,
                              int renorm, float scale, const int32_t* top_idx, const float* d_w,
                              void* d_logits, hipStream_t s);
+
+// Balance loss and its gradient (smoe_balance.hip); the entry points check the
+// shapes.  Workspace: part_p f32 [S * chunks, E], part_c i32 [S * chunks, E + 1]
+// where a sequence takes more than one chunk.
+int balance_chunks(int64_t S, int64_t T);
+int launch_balance_loss(const void* logits, int dt, int S, int T, int E, int K, int sigmoid, const int32_t* idx,
+                        const uint8_t* mask, float* loss, int32_t* counts, float* slope, float* part_p,
+                        int32_t* part_c, hipStream_t s);
+int launch_balance_loss_bwd(const void* logits, int dt, int S, int T, int E, int sigmoid, const uint8_t* mask,
+                            const float* slope, const float* d_loss, void* d_logits, hipStream_t s);
 // out[t] = sum over the token's rows tok_row [N, K] of y[row] * row_w[row]
 int launch_combine_rows(const void* y, int ydt, const float* row_w, const int32_t* tok_row,
                         int N, int K, int H, void* out, int odt, hipStream_t s);

@@ -38,6 +38,10 @@ class SmoeExpertsFp8Blocks(ctypes.Structure):
                 ("w_down", _vp), ("s_up", _vp), ("s_down", _vp), ("b_up", _vp), ("b_down", _vp)]
 
 
+class SmoeExpertsMxfp4(ctypes.Structure):
+    _fields_ = SmoeExpertsFp8Blocks._fields_
+
+
 class SmoeBlock(ctypes.Structure):
     _fields_ = [("act_dtype", _c_int), ("H", _c_int), ("E", _c_int), ("K", _c_int),
                 ("M", _c_int), ("L", _c_int), ("R", _c_int),
@@ -116,6 +120,20 @@ SIGNATURES = {
     "smoe_expert_delta_fp8_blocks": (_c_int, [ctypes.POINTER(SmoeExpertsFp8Blocks), _vp, _c_int,
                                               _vp, _vp, _c_int, _c_int, _vp, _c_int, _vp, _sz,
                                               _vp]),
+    "smoe_balance_loss_workspace_bytes": (_sz, [_c_int, _c_int, _c_int]),
+    "smoe_balance_loss": (_c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp,
+                                   _vp, _vp, _vp, _vp, _sz, _vp]),
+    "smoe_balance_loss_backward": (_c_int, [_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _vp, _vp,
+                                            _vp, _vp, _vp]),
+    "smoe_quantize_mxfp4": (_c_int, [_vp, _c_int, _i64, _c_int, _i64, _vp, _i64, _vp, _i64, _vp]),
+    "smoe_dequantize_mxfp4": (_c_int, [_vp, _i64, _vp, _i64, _i64, _c_int, _vp, _c_int, _vp]),
+    "smoe_linear_mxfp4_workspace_bytes": (_sz, [_c_int, _c_int]),
+    "smoe_linear_mxfp4": (_c_int, [_vp, _c_int, _i64, _c_int, _c_int, _vp, _i64, _vp, _i64, _vp,
+                                   _c_int, _c_int, _vp, _c_int, _vp, _sz, _vp]),
+    "smoe_expert_delta_mxfp4_workspace_bytes": (_sz, [ctypes.POINTER(SmoeExpertsMxfp4), _c_int,
+                                                      _c_int]),
+    "smoe_expert_delta_mxfp4": (_c_int, [ctypes.POINTER(SmoeExpertsMxfp4), _vp, _c_int, _vp, _vp,
+                                         _c_int, _c_int, _vp, _c_int, _vp, _sz, _vp]),
     "smoe_combine_rows": (_c_int, [_vp, _c_int, _vp, _vp, _c_int, _c_int, _c_int, _vp, _c_int,
                                    _vp]),
     "smoe_remap_ids": (_c_int, [_vp, ctypes.c_int64, _vp, _c_int, _vp, _vp]),

@@ -24,8 +24,12 @@ Beside them, without a counterpart in the reference:
   ForgeSelect.route_groups   softmax or sigmoid scores, a balance bias,
                        top-k within the best groups of experts, with its
                        gradient -> smoe_select_groups(_backward)
+  ForgeSelect.balance_loss   how evenly the choices spread, with its gradient,
+                       and the experts' counts -> smoe_balance_loss(_backward)
   ForgeGEMM.linear_fp8_blocks   fp8 with a scale per block of 128 ->
                        smoe_linear_fp8_blocks
+  ForgeGEMM.linear_mxfp4   4-bit floats with a power of two per 32 ->
+                       smoe_linear_mxfp4
 
 One GPU: the cross-rank combine is the identity (no process group), as
 the reference's combine_across_ranks is at world size 1.
@@ -33,6 +37,7 @@ the reference's combine_across_ranks is at world size 1.
 from __future__ import annotations
 
 import ctypes
+import math
 from dataclasses import dataclass
 from enum import Enum
 from typing import Any, Callable
@@ -42,7 +47,8 @@ from torch.autograd import forward_ad
 
 from . import _native as nat
 from .dispatch import DispatchPlan, build_dispatch_plan, dispatch_expert_ffn
-from .quant import FP8_BLOCK, quantize_fp8_per_tensor
+from .quant import FP8_BLOCK, MX_BLOCK, _as_bytes, _pitched, mx_pitches, quantize_fp8_per_tensor
+from .sparse_experts import _expert_ids
 
 
 class ForgeBackend(str, Enum):
@@ -109,6 +115,28 @@ class ForgeSelect:
         k = int(top_k if top_k is not None else self.config.select_top_k)
         return select_groups(logits, k, score=score, bias=bias, num_groups=num_groups,
                              top_groups=top_groups, renormalize=renormalize, scale=scale)
+
+    def balance_loss(self, logits: torch.Tensor, top_indices: torch.Tensor, *, score: str = "softmax",
+                     mask: torch.Tensor | None = None, per_sequence: bool = False):
+        """(loss float32, counts int32 [.., E]) of a router's logits [.., E]
+        (float32, bfloat16 or float16) and its choices top_indices [.., k]:
+
+          p = softmax(logits), or sigmoid(logits) over its sum
+          load_e = share of the choices that went to expert e
+          loss = E * sum_e load_e * (mean over tokens of p_e)
+
+        1 where both are even; the aux_loss of SpiderMoELayer's statistics
+        (model.py:330-337) over all tokens.  mask [..] (bool, or 0 / 1): tokens
+        that count; what the others' logits hold plays no part.  per_sequence:
+        logits [.., T, E], a loss and counts for each sequence of T tokens
+        (loss [..], counts [.., E]).  Ids outside [0, E) count nowhere; a
+        sequence without tokens or choices has loss 0.  An expert with logit
+        -inf has p = 0.
+
+        Differentiable in logits, once and in reverse mode (the counts held
+        fixed)."""
+        self.calls += 1
+        return balance_loss(logits, top_indices, score=score, mask=mask, per_sequence=per_sequence)
 
     def top_dobu_budget(self) -> int:
         return int(self.config.select_top_dobu)
@@ -193,6 +221,80 @@ def select_groups(logits: torch.Tensor, k: int, *, score: str = "sigmoid", bias=
     return _select_groups_fwd(logits.contiguous(), n, e, idx, *how), idx
 
 
+def _balance_fwd(x, idx, mask, how, slope):
+    """x: contiguous logits of s sequences of t tokens -> (loss [s], counts [s, e])."""
+    s, t, e, k, score = how
+    dev = x.device
+    loss = torch.empty(s, dtype=torch.float32, device=dev)
+    counts = torch.empty(s, e, dtype=torch.int32, device=dev)
+    need = nat.lib().smoe_balance_loss_workspace_bytes(s, t, e)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    nat.launch(dev, "smoe_balance_loss", x.data_ptr(), nat.float_code(x.dtype), s, t, e, k, score,
+               idx.data_ptr(), nat.ptr(mask), loss.data_ptr(), counts.data_ptr(), nat.ptr(slope),
+               nat.ptr(ws), need)
+    return loss, counts
+
+
+class _BalanceLoss(torch.autograd.Function):
+    # the counts are kept on ctx's holder, not returned: no bookkeeping for them
+    @staticmethod
+    def forward(ctx, logits, idx, mask, how, shape, out):
+        x = logits.contiguous()
+        slope = torch.empty(how[0], how[2], dtype=torch.float32, device=x.device)
+        loss, counts = _balance_fwd(x, idx, mask, how, slope)
+        out.append(counts)
+        ctx.save_for_backward(x, mask, slope)
+        ctx.how = how
+        return loss.view(shape)
+
+    @staticmethod
+    def backward(ctx, d_loss):
+        if torch.is_grad_enabled():
+            raise RuntimeError("balance_loss is not twice differentiable")
+        x, mask, slope = ctx.saved_tensors
+        s, t, e, _, score = ctx.how
+        d = torch.empty_like(x)
+        d_loss = d_loss.contiguous()
+        nat.launch(x.device, "smoe_balance_loss_backward", x.data_ptr(), nat.float_code(x.dtype), s, t, e,
+                   score, nat.ptr(mask), slope.data_ptr(), d_loss.data_ptr(), d.data_ptr())
+        return d, None, None, None, None, None
+
+
+def balance_loss(logits: torch.Tensor, top_indices: torch.Tensor, *, score: str = "softmax", mask=None,
+                 per_sequence: bool = False):
+    """smoe_balance_loss over the last dimension (ForgeSelect.balance_loss)."""
+    nat.require_gpu(logits, top_indices, mask)
+    if forward_ad.unpack_dual(logits).tangent is not None:
+        raise RuntimeError("balance_loss has no forward-mode derivative")
+    if score not in nat.SCORES:
+        raise ValueError("score must be 'softmax' or 'sigmoid'")
+    shape = logits.shape
+    if len(shape) < (2 if per_sequence else 1):
+        raise ValueError(f"logits must be [.., {'T, ' if per_sequence else ''}E], got {tuple(shape)}")
+    if top_indices.ndim != len(shape) or top_indices.shape[:-1] != shape[:-1]:
+        raise ValueError("top_indices must be logits' shape with k last")
+    e, k = shape[-1], top_indices.shape[-1]
+    lead = tuple(shape[:-2]) if per_sequence else ()
+    s = math.prod(lead)
+    t = shape[-2] if per_sequence else math.prod(shape[:-1])
+    if mask is not None:
+        if mask.shape != shape[:-1]:
+            raise ValueError(f"mask must be {tuple(shape[:-1])}, got {tuple(mask.shape)}")
+        mask = (mask if mask.dtype == torch.bool else mask != 0).contiguous()
+    if max(s, t) > 0x7fffffff:
+        raise ValueError("more than 2^31 - 1 tokens")
+    idx = _expert_ids(top_indices, e).contiguous()
+    how = (s, t, e, k, nat.SCORES[score])
+    if logits.requires_grad and torch.is_grad_enabled():
+        out = []
+        loss = _BalanceLoss.apply(logits, idx, mask, how, lead, out)
+        counts = out[0]
+    else:
+        loss, counts = _balance_fwd(logits.contiguous(), idx, mask, how, None)
+        loss = loss.view(lead)
+    return loss, counts.view(*lead, e)
+
+
 # ------------------------------------------------------------------ gemm ----
 _ACT = {None: 0, "gelu": 1}
 
@@ -262,6 +364,46 @@ def _rows16(codes):
     c = torch.zeros(rows, ld, dtype=torch.uint8, device=codes.device)
     c[:, :cols] = codes.view(torch.uint8)
     return c, ld
+
+
+def _linear_mxfp4(x, codes, scale, bias, act):
+    dev = nat.require_gpu(x, codes, scale, bias)
+    if x.ndim < 1 or x.shape[-1] < 1:
+        raise ValueError("x must be [.., K] with K >= 1")
+    k, lead = x.shape[-1], x.shape[:-1]
+    codes, scale = _as_bytes(codes, "codes"), _as_bytes(scale, "scale")
+    if codes.ndim != 2 or codes.shape[1] != -(-k // 2):
+        raise ValueError(f"codes must be [N_out, {-(-k // 2)}], got {tuple(codes.shape)}")
+    n_out = codes.shape[0]
+    if scale.shape != (n_out, -(-k // MX_BLOCK)):
+        raise ValueError(f"scale must be {(n_out, -(-k // MX_BLOCK))}, got {tuple(scale.shape)}")
+    if act not in _ACT:
+        raise ValueError("act must be None or 'gelu'")
+    if max(k, n_out) > 0x7fffff00 or x.numel() > 0x7fffff00 * k:
+        raise ValueError("more than 2^31 - 256 rows, K or N_out")
+    if bias is not None:
+        if bias.shape != (n_out,):
+            raise ValueError(f"bias must be [{n_out}], got {tuple(bias.shape)}")
+        bias = bias.float().contiguous()
+    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise RuntimeError(f"unsupported activation dtype {x.dtype} (float32, bfloat16 or float16)")
+    if x.ndim == 2 and x.stride(1) == 1 and x.stride(0) >= k:
+        ldx = x.stride(0)
+    else:
+        x, ldx = x.contiguous(), k
+    ldc, lds = mx_pitches(k)
+    codes, ldw = _pitched(codes, ldc, 16)
+    scale, ld_ws = _pitched(scale, lds, 4)
+    out_dtype = torch.bfloat16 if x.dtype == torch.bfloat16 else torch.float32
+    out = torch.empty(*lead, n_out, dtype=out_dtype, device=dev)
+    n = out.numel() // n_out if n_out else 0
+    if n:
+        need = nat.lib().smoe_linear_mxfp4_workspace_bytes(n, k)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        nat.launch(dev, "smoe_linear_mxfp4", x.data_ptr(), nat.float_code(x.dtype), ldx, n, k,
+                   codes.data_ptr(), ldw, scale.data_ptr(), ld_ws, nat.ptr(bias), n_out, _ACT[act],
+                   out.data_ptr(), nat.dtype_code(out_dtype), nat.ptr(ws), need)
+    return out if out_dtype == x.dtype else out.to(x.dtype)
 
 
 class _Fp8Cache:
@@ -408,6 +550,15 @@ class ForgeGEMM:
         self.calls += 1
         return _linear_fp8_blocks(x, codes, scale, bias, act)
 
+    def linear_mxfp4(self, x, codes, scale, bias=None, *, act: str | None = None):
+        """act(x . W^T + bias) with W held as quantize_mxfp4 gives it: e2m1
+        codes [N_out, ceil(K / 2)] and a power of two per 32 along K
+        [N_out, ceil(K / 32)]; x [..., K] is quantized the same way on the way
+        (smoe_linear_mxfp4).  act None or "gelu" (erf).  Products of the two
+        operands' values, summed in f32; result in x's dtype.  No gradient."""
+        self.calls += 1
+        return _linear_mxfp4(x, codes, scale, bias, act)
+
     @torch.no_grad()
     def expert_ffn(self, x, w_up, b_up, w_down, b_down):
         self.calls += 1
@@ -535,5 +686,5 @@ def get_forge() -> ForgeRuntime:
 
 
 __all__ = ["ForgeBackend", "ForgeConfig", "ForgeSelect", "ForgeGEMM", "ForgeEP", "ForgeRuntime",
-           "init_forge", "get_forge", "select_topk", "select_groups", "fp8_linear", "fp8_expert_ffn",
+           "init_forge", "get_forge", "select_topk", "select_groups", "balance_loss", "fp8_linear", "fp8_expert_ffn",
            "get_last_fp8_gemm_backend", "quantize_fp8_input"]

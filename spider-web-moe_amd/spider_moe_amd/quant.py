@@ -15,6 +15,10 @@ codes = (w / scale).to(float8_e4m3fn), as quantize_fp8_with_scale_tensor
 fp8 in blocks: e4m3 codes with one f32 scale per 128 x 128 block of a weight
 or per 1 x 128 block of activations (no counterpart in the reference):
 quantize_fp8_blocks / dequantize_fp8_blocks.
+
+microscaled 4-bit floating point (OCP MXFP4, no counterpart in the reference):
+e2m1 codes with one power of two per 32 elements of a row: quantize_mxfp4 /
+dequantize_mxfp4.
 """
 from __future__ import annotations
 
@@ -216,6 +220,130 @@ def dequantize_fp8_blocks(codes: torch.Tensor, scale: torch.Tensor, *, block_row
     if block_rows > 1:
         s = s.repeat_interleave(block_rows, dim=-2)[..., :rows, :]
     return (codes.float() * s).to(dtype)
+
+
+# -------------------------------------------- microscaled 4-bit floats ----
+MX_BLOCK = 32
+_E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
+_BYTES = tuple(getattr(torch, n) for n in ("uint8", "float4_e2m1fn_x2", "float8_e8m0fnu") if hasattr(torch, n))
+
+
+def _as_bytes(t: torch.Tensor, name: str) -> torch.Tensor:
+    """Codes or scales as uint8, whichever of torch's names for them they
+    carry."""
+    if t.dtype not in _BYTES:
+        raise ValueError(f"{name} must be uint8 (or float4_e2m1fn_x2 codes, float8_e8m0fnu scales), got {t.dtype}")
+    return t if t.dtype == torch.uint8 else t.view(torch.uint8)
+
+
+def mx_pitches(cols: int):
+    """Bytes from row to row that the kernels want at least: codes (whole
+    blocks) and scales (whole words)."""
+    nb = -(-cols // MX_BLOCK)
+    return 16 * nb, -(-nb // 4) * 4
+
+
+def _pitched(t: torch.Tensor, pitch: int, align: int):
+    """t [rows, n] bytes with rows `ld` apart, ld a multiple of `align` and
+    every row's `pitch` bytes inside the storage: t itself, else a copy.
+    Returns it and ld."""
+    rows, n = t.shape
+    ld = t.stride(0) if rows > 1 else pitch
+    if (t.stride(1) == 1 or n == 1) and ld >= pitch and ld % align == 0 and t.data_ptr() % align == 0 and \
+            t.untyped_storage().nbytes() - t.storage_offset() >= (rows - 1) * ld + pitch:
+        return t, ld
+    c = torch.zeros(rows, pitch, dtype=torch.uint8, device=t.device)
+    c[:, :n] = t
+    return c[:, :n], pitch
+
+
+def _flat_rows(t: torch.Tensor):
+    """t [.., n] as (tensor, elements from row to row): t itself where its rows
+    lie at one distance, else a contiguous copy."""
+    t2 = t if t.ndim > 1 else t.unsqueeze(0)
+    ld = t2.shape[-1] if t2.is_contiguous() else _row_stride(t2)
+    return (t2, ld) if ld is not None else (t2.contiguous(), t2.shape[-1])
+
+
+def quantize_mxfp4(x: torch.Tensor):
+    """x [.., cols] -> (codes uint8 [.., ceil(cols / 2)], scale uint8
+    [.., ceil(cols / 32)]): blocks of 32 along the last dimension (the last one
+    may be shorter), each a power of two 2^(scale - 127) = 2^(floor(log2 amax)
+    - 2), at least 2^-127, times e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a
+    sign) rounded to nearest even, past 6 to 6; element 2i in the low half of
+    byte i.  An infinity or a NaN makes its block NaN (scale 255, codes 0).
+    The codes' rows start a multiple of 16 bytes apart and the scales' a
+    multiple of 4, as the products read them (views where cols does not fill
+    them).  On a GPU: the HIP quantizer (same bits as the CPU formula)."""
+    if x.ndim < 1 or x.shape[-1] < 1:
+        raise ValueError("x must be [.., cols] with cols >= 1")
+    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        x = x.float()
+    *lead, cols = x.shape
+    nb = -(-cols // MX_BLOCK)
+    ldc, lds = mx_pitches(cols)
+    if x.is_cuda:
+        from . import _native as nat
+        rows = math.prod(lead)
+        if max(rows, cols) > 0x7fffffff:
+            raise ValueError("more than 2^31 - 1 rows or columns")
+        x, ldx = _flat_rows(x)
+        codes = torch.empty(*lead, ldc, dtype=torch.uint8, device=x.device)
+        scale = torch.empty(*lead, lds, dtype=torch.uint8, device=x.device)
+        nat.launch(x.device, "smoe_quantize_mxfp4", x.data_ptr(), nat.float_code(x.dtype), rows, cols, ldx,
+                   codes.data_ptr(), ldc, scale.data_ptr(), lds)
+    else:
+        p = torch.zeros(*lead, nb * MX_BLOCK)
+        p[..., :cols] = x.detach()
+        p = p.view(*lead, nb, MX_BLOCK)
+        biased = p.abs().amax(dim=-1).view(torch.int32) >> 23  # NaN is the largest magnitude
+        biased = torch.where(torch.isfinite(p).all(dim=-1), (biased - 2).clamp_min(0), 255)
+        v = p.double().abs() * torch.exp2(127.0 - biased.double()).unsqueeze(-1)
+        c = torch.zeros(p.shape, dtype=torch.uint8)
+        for i in range(1, 8):  # a tie goes to the even code
+            middle = (_E2M1[i - 1] + _E2M1[i]) / 2
+            c += (v >= middle) if i % 2 == 0 else (v > middle)
+        c = torch.where(biased.unsqueeze(-1) == 255, 0, c + 8 * torch.signbit(p).to(torch.uint8))
+        c = c.to(torch.uint8).view(*lead, -1)
+        codes = c[..., 0::2] | (c[..., 1::2] << 4)
+        scale = torch.zeros(*lead, lds, dtype=torch.uint8)
+        scale[..., :nb] = biased.to(torch.uint8)
+    if ldc != -(-cols // 2):
+        codes = codes.narrow(-1, 0, -(-cols // 2))
+    return codes, (scale if lds == nb else scale.narrow(-1, 0, nb))
+
+
+def dequantize_mxfp4(codes: torch.Tensor, scale: torch.Tensor, *, cols: int | None = None,
+                     dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """The values [.., cols] of quantize_mxfp4's codes and scale, as dtype
+    (float32 and bfloat16 hold them exactly); cols: 2 * codes.shape[-1] by
+    default, one less where the last byte holds one code."""
+    codes, scale = _as_bytes(codes, "codes"), _as_bytes(scale, "scale")
+    if codes.ndim < 1 or codes.shape[-1] < 1:
+        raise ValueError("codes must be [.., ceil(cols / 2)] with cols >= 1")
+    cols = 2 * codes.shape[-1] if cols is None else int(cols)
+    lead = codes.shape[:-1]
+    if codes.shape[-1] != -(-cols // 2):
+        raise ValueError(f"{cols} columns take {-(-cols // 2)} bytes of codes, got {codes.shape[-1]}")
+    if scale.shape != (*lead, -(-cols // MX_BLOCK)):
+        raise ValueError(f"scale must be {(*lead, -(-cols // MX_BLOCK))}, got {tuple(scale.shape)}")
+    if codes.is_cuda:
+        from . import _native as nat
+        nat.require_gpu(codes, scale)
+        rows = math.prod(lead)
+        if max(rows, cols) > 0x7fffffff:
+            raise ValueError("more than 2^31 - 1 rows or columns")
+        out = torch.empty(*lead, cols, device=codes.device,
+                          dtype=dtype if dtype in (torch.float32, torch.bfloat16, torch.float16) else torch.float32)
+        (c, ldc), (s, lds) = _flat_rows(codes), _flat_rows(scale)
+        nat.launch(codes.device, "smoe_dequantize_mxfp4", c.data_ptr(), ldc, s.data_ptr(), lds, rows, cols,
+                   out.data_ptr(), nat.float_code(out.dtype))
+        return out if out.dtype == dtype else out.to(dtype)
+    table = torch.tensor(_E2M1 + tuple(-v for v in _E2M1))
+    v = table[torch.stack([codes & 15, codes >> 4], dim=-1).flatten(-2)[..., :cols].long()]
+    two = torch.exp2(scale.double() - 127.0)
+    two = torch.where(scale == 255, float("nan"), two).float()
+    return (v * two.repeat_interleave(MX_BLOCK, dim=-1)[..., :cols]).to(dtype)
 
 
 # ------------------------------------------------------ SwiGLU layout ----

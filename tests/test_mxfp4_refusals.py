@@ -1,0 +1,215 @@
+"""CPU checks of microscaled 4-bit floats and of the balance loss: what the
+entry points refuse before any launch, the quantizer's CPU form against known
+answers and against oracle/mxfp4.py."""
+import ctypes
+
+import pytest
+import torch
+
+from oracle import mxfp4 as O
+
+FAKE = 0x1000  # never dereferenced: every call below is refused, or has no rows
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from spider_moe_amd import _native
+    return _native.lib()
+
+
+def test_balance_refusals(lib):
+    from spider_moe_amd import _native as nat
+
+    def go(dt=nat.F32, s=2, t=5, e=16, k=2, score=0, z=FAKE, i=FAKE, m=None, lo=FAKE, c=FAKE, sl=None, ws=None, wb=0):
+        return lib.smoe_balance_loss(z, dt, s, t, e, k, score, i, m, lo, c, sl, ws, wb, None)
+
+    assert go(dt=nat.FP8_E4M3) == -2
+    for bad in (dict(s=-1), dict(t=-1), dict(e=0), dict(e=257), dict(k=0), dict(k=65), dict(score=2), dict(z=None),
+                dict(i=None), dict(lo=None), dict(c=None), dict(s=1 << 13, t=1 << 13), dict(s=1 << 22, t=1),
+                dict(s=1 << 10, t=1 << 15, k=64)):
+        assert go(**bad) == 1, bad
+    assert go(s=0, z=None, i=None, lo=None, c=None) == 0
+    need = lib.smoe_balance_loss_workspace_bytes(2, 5000, 16)
+    assert need > 0 and lib.smoe_balance_loss_workspace_bytes(2, 100, 16) == 0
+    assert lib.smoe_balance_loss_workspace_bytes(2, 5000, 300) == 0
+    assert go(t=5000, ws=None, wb=need) == 1 and go(t=5000, ws=FAKE + 4, wb=need) == 1
+    assert go(t=5000, ws=FAKE, wb=need - 1) == 3
+
+    def back(dt=nat.F32, s=2, t=5, e=16, score=0, z=FAKE, sl=FAKE, g=FAKE, d=FAKE):
+        return lib.smoe_balance_loss_backward(z, dt, s, t, e, score, None, sl, g, d, None)
+
+    assert back(dt=7) == -2
+    for bad in (dict(s=-1), dict(e=300), dict(score=-1), dict(z=None), dict(sl=None), dict(g=None), dict(d=None)):
+        assert back(**bad) == 1, bad
+    assert back(s=0) == 0 and back(t=0, z=None) == 0
+
+
+def test_quantizer_refusals(lib):
+    from spider_moe_amd import _native as nat
+
+    def go(dt=nat.BF16, r=4, c=100, ldx=100, q=FAKE, ld=64, s=FAKE, ls=4, x=FAKE):
+        return lib.smoe_quantize_mxfp4(x, dt, r, c, ldx, q, ld, s, ls, None)
+
+    assert go(dt=nat.INT4) == -2
+    for bad in (dict(r=-1), dict(c=0), dict(ldx=99), dict(ld=48), dict(ld=72), dict(ld=80), dict(ls=3), dict(ls=6),
+                dict(q=FAKE + 8), dict(s=FAKE + 2), dict(q=None), dict(s=None), dict(x=None)):
+        assert go(**bad) == 1, bad
+    assert go(r=0) == 0
+    assert go(r=1 << 27, c=129, ldx=129, ld=80, ls=8) == 1  # 2^28 pieces
+
+    def back(dt=nat.BF16, r=4, c=100, q=FAKE, ld=50, s=FAKE, ls=4, o=FAKE):
+        return lib.smoe_dequantize_mxfp4(q, ld, s, ls, r, c, o, dt, None)
+
+    assert back(dt=nat.FP8_E4M3) == -2
+    for bad in (dict(r=-1), dict(c=0), dict(ld=49), dict(ls=3), dict(q=None), dict(s=None), dict(o=None),
+                dict(r=1 << 32, c=8, ld=4, ls=1)):
+        assert back(**bad) == 1, bad
+    assert back(r=0) == 0
+
+
+def test_linear_refusals(lib):
+    from spider_moe_amd import _native as nat
+
+    def go(x=FAKE, dt=nat.BF16, ldx=100, n=40, k=100, w=FAKE, ldw=64, ws=FAKE, ls=4, no=30, act=0, out=FAKE,
+           od=nat.BF16, wk=FAKE, wb=1 << 20):
+        return lib.smoe_linear_mxfp4(x, dt, ldx, n, k, w, ldw, ws, ls, None, no, act, out, od, wk, wb, None)
+
+    assert go(dt=nat.INT4) == -2 and go(dt=nat.FP8_E4M3) == -2 and go(od=nat.F16) == -2
+    for bad in (dict(n=-1), dict(k=0), dict(no=0), dict(ldx=99), dict(ldw=48), dict(ldw=72), dict(ls=3), dict(ls=6),
+                dict(act=2), dict(x=None), dict(w=None), dict(ws=None), dict(out=None), dict(wk=None), dict(w=FAKE + 4),
+                dict(ws=FAKE + 1), dict(wk=FAKE + 1), dict(n=1 << 28)):
+        assert go(**bad) == 1, bad
+    need = lib.smoe_linear_mxfp4_workspace_bytes(40, 100)
+    assert need >= 40 * 64 + 40 * 4 and go(wb=need - 1) == 3
+    assert go(n=0) == 0
+    assert lib.smoe_linear_mxfp4_workspace_bytes(4, 100) == 0  # a few rows are quantized by the product itself
+    assert lib.smoe_linear_mxfp4_workspace_bytes(0, 100) == 0
+
+
+def test_expert_refusals(lib):
+    from spider_moe_amd import _native as nat
+
+    def desc(act=0, e=4, h=64, u=96, up=FAKE, down=FAKE, su=FAKE, sd=FAKE):
+        d = nat.SmoeExpertsMxfp4()
+        d.act, d.E, d.H, d.U = act, e, h, u
+        d.w_up, d.w_down, d.s_up, d.s_down = up, down, su, sd
+        return d
+
+    def need(d, n=30, k=2):
+        return lib.smoe_expert_delta_mxfp4_workspace_bytes(ctypes.byref(d), n, k)
+
+    for bad in (dict(act=2), dict(e=0), dict(e=257), dict(h=48), dict(h=0), dict(u=16), dict(u=80), dict(up=None),
+                dict(down=None), dict(su=None), dict(sd=None), dict(up=FAKE + 8), dict(sd=FAKE + 2)):
+        assert need(desc(**bad)) == 0, bad
+    ok = desc()
+    assert need(ok) > 0 and need(ok, n=8) == 8 * 2 * 96 * 4
+    for n, k in ((-1, 2), (4, 0), (4, 65), (1 << 30, 2), (4194241, 1)):
+        assert need(ok, n, k) == 0
+    assert need(desc(h=4128), 65536, 1) == 0 and need(desc(h=1 << 20), 40000, 1) == 0
+
+    def go(d=ok, m=FAKE, dt=nat.BF16, i=FAKE, w=FAKE, n=30, k=2, o=FAKE, od=nat.BF16, ws=FAKE, wb=1 << 24):
+        return lib.smoe_expert_delta_mxfp4(ctypes.byref(d), m, dt, i, w, n, k, o, od, ws, wb, None)
+
+    assert go(dt=nat.F16) == -2 and go(od=nat.F16) == -2
+    for bad in (dict(m=None), dict(i=None), dict(w=None), dict(o=None), dict(ws=None), dict(ws=FAKE + 8), dict(k=0)):
+        assert go(**bad) == 1, bad
+    assert go(wb=need(ok) - 1) == 3 and go(n=0, m=None) == 0
+    assert lib.smoe_expert_delta_mxfp4(None, FAKE, 0, FAKE, FAKE, 3, 2, FAKE, 0, FAKE, 1 << 24, None) == 1
+
+
+def test_python_refusals():
+    from spider_moe_amd import ForgeGEMM, ForgeSelect, MxFp4Experts, dequantize_mxfp4, quantize_mxfp4
+    x = torch.randn(3, 40)
+    q, s = quantize_mxfp4(x)
+    with pytest.raises(ValueError):
+        quantize_mxfp4(torch.zeros(()))
+    with pytest.raises(ValueError):
+        quantize_mxfp4(torch.zeros(3, 0))
+    for bad in (dict(cols=41), dict(cols=38), dict(cols=0)):
+        with pytest.raises(ValueError):
+            dequantize_mxfp4(q, s, **bad)
+    with pytest.raises(ValueError):
+        dequantize_mxfp4(q, s[:, :1])
+    with pytest.raises(ValueError):
+        dequantize_mxfp4(q.float(), s)
+    with pytest.raises(RuntimeError):  # a GPU call
+        ForgeGEMM().linear_mxfp4(x, q, s)
+    with pytest.raises(RuntimeError):
+        ForgeSelect().balance_loss(x, torch.zeros(3, 2, dtype=torch.int32))
+    with pytest.raises(RuntimeError):
+        MxFp4Experts.quantize(torch.randn(2, 64, 32), torch.randn(2, 32, 64))
+
+
+# ------------------------------------------------- the quantizer's CPU form ----
+def test_known_codes():
+    from spider_moe_amd import dequantize_mxfp4, quantize_mxfp4
+    # amax 6: power 1; every tie between neighbours goes to the even code
+    x = torch.tensor([[0.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, -0.0, -0.25, -0.76, 0.26, 5.01, -5.0, -6.0]])
+    q, s = quantize_mxfp4(x)
+    nib = torch.stack([q & 15, q >> 4], -1).flatten(1)
+    assert s.tolist() == [[127]]
+    assert nib.tolist() == [[0, 0, 2, 2, 4, 4, 6, 6, 7, 8, 8, 10, 1, 7, 14, 15]]
+    assert dequantize_mxfp4(q, s).tolist() == [[0, 0, 1, 1, 2, 2, 4, 4, 6, -0.0, -0.0, -1, 0.5, 6, -4, -6]]
+    # past 6 to 6, up to the next power (3.99 is 7.98 halves)
+    for top, want in ((7.0, 6.0), (7.99, 6.0), (8.0, 8.0), (4.0, 4.0), (3.99, 3.0)):
+        q, s = quantize_mxfp4(torch.tensor([[top]]))
+        assert q.shape == (1, 1) and dequantize_mxfp4(q, s, cols=1).item() == want
+
+
+def test_extreme_blocks():
+    from spider_moe_amd import dequantize_mxfp4, quantize_mxfp4
+    inf = float("inf")
+    x = torch.zeros(6, 64)
+    x[1, 3], x[2, 40], x[3, 0] = inf, float("nan"), 3.4e38
+    x[4, :32] = 2.0 ** -126
+    x[5, 0], x[5, 1] = 1e-45, 2.0 ** -127
+    q, s = quantize_mxfp4(x)
+    assert s.tolist() == [[0, 0], [255, 0], [0, 255], [252, 0], [0, 0], [0, 0]]
+    v = dequantize_mxfp4(q, s)
+    assert torch.isnan(v[1, :32]).all() and (v[1, 32:] == 0).all()
+    assert torch.isnan(v[2, 32:]).all() and (v[2, :32] == 0).all()
+    assert v[3, 0].item() == 6 * 2.0 ** 125 and (v[4, :32] == 2.0 ** -126).all()
+    assert v[5, 0] == 0 and v[5, 1] == 2.0 ** -127
+    assert (q[1, :16] == 0).all() and (q[2, 16:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(1,), (31,), (3, 32), (4, 33), (2, 3, 100), (7, 257)])
+def test_cpu_form_is_the_oracle(dtype, shape):
+    from spider_moe_amd import dequantize_mxfp4, quantize_mxfp4
+    g = torch.Generator().manual_seed(sum(shape))
+    x = (torch.randn(*shape, generator=g) * torch.exp(3 * torch.randn(*shape[:-1], 1, generator=g))).to(dtype)
+    q, s = quantize_mxfp4(x)
+    cols = shape[-1]
+    assert q.dtype == s.dtype == torch.uint8
+    assert q.shape == (*shape[:-1], -(-cols // 2)) and s.shape == (*shape[:-1], -(-cols // 32))
+    v, e = O.quantize(x.reshape(-1, cols))
+    assert torch.equal(dequantize_mxfp4(q, s, cols=cols).double().view(-1, cols), v)
+    assert torch.equal(s.reshape(-1, s.shape[-1]).double(), e)
+    assert torch.equal(O.values(q.reshape(-1, q.shape[-1]), s.reshape(-1, s.shape[-1]), cols), v)
+
+
+def test_bytes_by_torchs_names():
+    from spider_moe_amd import dequantize_mxfp4, quantize_mxfp4
+    q, s = quantize_mxfp4(torch.randn(4, 64))
+    want = dequantize_mxfp4(q, s)
+    if hasattr(torch, "float8_e8m0fnu"):
+        assert torch.equal(dequantize_mxfp4(q, s.contiguous().view(torch.float8_e8m0fnu)), want)
+    if hasattr(torch, "float4_e2m1fn_x2"):
+        assert torch.equal(dequantize_mxfp4(q.view(torch.float4_e2m1fn_x2), s), want)
+
+
+def test_oracle_pins():
+    """The oracle's pieces against each other: codes that are values already,
+    the spread of an exact input, a balanced router's loss and gradient."""
+    x = torch.tensor([[6.0, -3.0, 1.5, 0.5] + [0.0] * 28])
+    assert torch.equal(O.quantize(x)[0], x.double())
+    assert O.spread(x, torch.zeros_like(x)).abs().max() == 0
+    near = torch.full((1, 32), 5.0)  # a tie: 4 for 5, 6 for anything above
+    assert O.spread(near, torch.full_like(near, 1e-9)).unique().tolist() == [2.0]
+    z = torch.zeros(1, 8, 4, dtype=torch.float64, requires_grad=True)
+    idx = (torch.arange(8).view(1, 8, 1) % 4).int()
+    loss, counts, u, _ = O.balance(z, idx)
+    assert loss.item() == 1.0 and counts.tolist() == [[2, 2, 2, 2]] and u.abs().max() == 0
+    (g,) = torch.autograd.grad(loss.sum(), z)
+    assert g.abs().max() < 1e-17
