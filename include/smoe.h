@@ -556,10 +556,10 @@ SMOE_API int smoe_dequantize_mxfp4(const uint8_t* codes, int64_t ld_codes, const
  * apart, ld_ws % 4 == 0, ld_ws >= ceil(K / 32), 4-byte aligned).  x (SMOE_F32 /
  * SMOE_BF16 / SMOE_F16, rows ldx elements apart) is quantized by the call as
  * smoe_quantize_mxfp4 does.  Products of the two operands' values, summed in f32;
- * act SMOE_LINEAR_NONE / SMOE_LINEAR_GELU; bias f32 [N_out] or NULL; any K, any
- * N_out.  Where the workspace query gives 0 (a few rows) the workspace may be
- * NULL. */
-SMOE_API size_t smoe_linear_mxfp4_workspace_bytes(int N, int K);
+ * act SMOE_LINEAR_NONE / SMOE_LINEAR_GELU; bias f32 [N_out] or NULL; K <= 2^23,
+ * N_out <= 2^22, ldw <= 2^22.  Where the workspace query gives 0 (a few rows) the workspace
+ * may be NULL. */
+SMOE_API size_t smoe_linear_mxfp4_workspace_bytes(int N, int K, int N_out);
 SMOE_API int smoe_linear_mxfp4(const void* x, int x_dtype, int64_t ldx, int N, int K,
                                const uint8_t* wq, int64_t ldw, const uint8_t* w_scale,
                                int64_t ld_ws, const float* bias, int N_out, int act, void* out,
@@ -572,7 +572,8 @@ SMOE_API int smoe_linear_mxfp4(const void* x, int x_dtype, int64_t ldx, int N, i
  *   then the up projection's), H / 2 bytes a row; s_up H / 32 bytes a row,
  *   rounded up to a multiple of 4; w_down codes of [E,H,U], s_down alike;
  *   b_up f32 [E,U] (SwiGLU: added to the up projection), b_down [E,H], or NULL.
- * H % 32 == 0, U % 32 == 0, 1 <= E <= 256, codes 16-byte, scales 4-byte aligned. */
+ * H % 32 == 0, U % 32 == 0, both <= 2^22, 1 <= E <= 256, codes 16-byte, scales
+ * 4-byte aligned. */
 typedef struct smoe_experts_mxfp4 {
   int act; /* SMOE_ACT_GELU / SMOE_ACT_SWIGLU */
   int E, H, U;
@@ -591,7 +592,7 @@ typedef struct smoe_experts_mxfp4 {
  * idx i32 / w f32 [N,K] as smoe_dispatch_plan takes them (equal ids merged,
  * weights <= 0 and ids outside [0, E) dropped; a token left without experts gets
  * 0).  1 <= K <= 64, N * K < 2^31 - 128, N <= 4194240, with H > 4096 N <= 65535,
- * N * ceil(H / 128) <= 2^28 - 16. */
+ * U * H <= 2^32, N * H <= 2^32. */
 SMOE_API size_t smoe_expert_delta_mxfp4_workspace_bytes(const smoe_experts_mxfp4* ex, int N, int K);
 SMOE_API int smoe_expert_delta_mxfp4(const smoe_experts_mxfp4* ex, const void* msg, int msg_dtype,
                                      const int32_t* idx, const float* w, int N, int K, void* delta,

@@ -1794,8 +1794,10 @@ SMOE_API int smoe_quantize_mxfp4(const void* x, int x_dtype, int64_t rows, int c
   q.codes = codes;
   q.ld_codes = ld_codes;
   q.scale = scale;
-  q.ld_scale = ld_scale;
-  SMOE_TRY(launch_quantize_mxfp4(q, static_cast<hipStream_t>(stream)), "quantize mxfp4");
+  q.s_row = ld_scale;
+  q.s_word = 4;
+  const MxPlanes none[2];
+  SMOE_TRY(launch_quantize_mxfp4(q, none, static_cast<hipStream_t>(stream)), "quantize mxfp4");
   return SMOE_OK;
 }
 
@@ -1814,7 +1816,9 @@ SMOE_API int smoe_dequantize_mxfp4(const uint8_t* codes, int64_t ld_codes, const
 
 namespace {
 
-// x quantized: codes in rows of whole blocks, scales in rows of whole words
+size_t mx_planes_bytes(int64_t rows, int K) { return static_cast<size_t>(mx_plane_pitch(rows)) * (mx_scale_pitch(K) / 4); }
+
+// x quantized: codes in rows of whole blocks, scales in planes or (less) in rows of whole words
 struct MxWs {
   size_t codes, scale, total;
 };
@@ -1822,12 +1826,23 @@ MxWs mx_ws(int64_t N, int K) {
   MxWs w;
   Bump z;
   w.codes = z.take(static_cast<size_t>(N) * mx_code_pitch(K));
-  w.scale = z.take(static_cast<size_t>(N) * mx_scale_pitch(K));
+  w.scale = z.take(mx_planes_bytes(N, K));
   w.total = z.off;
   return w;
 }
 
-MxQuant mx_rows(const void* x, int xdt, int64_t ldx, int N, int K, void* ws, const MxWs& l) {
+MxPlanes mx_planes(const uint8_t* src, int64_t ld, int groups, int rows, int K, void* dst) {
+  MxPlanes p;
+  p.src = src;
+  p.ld = ld;
+  p.groups = groups;
+  p.rows = rows;
+  p.blocks = static_cast<int>(mx_blocks_of(K));
+  p.dst = static_cast<uint32_t*>(dst);
+  return p;
+}
+
+MxQuant mx_rows(const void* x, int xdt, int64_t ldx, int N, int K, void* ws, const MxWs& l, bool planes) {
   MxQuant q;
   q.x = x;
   q.x_dtype = xdt;
@@ -1837,23 +1852,25 @@ MxQuant mx_rows(const void* x, int xdt, int64_t ldx, int N, int K, void* ws, con
   q.codes = at<uint8_t>(ws, l.codes);
   q.ld_codes = mx_code_pitch(K);
   q.scale = at<uint8_t>(ws, l.scale);
-  q.ld_scale = mx_scale_pitch(K);
+  q.s_row = planes ? 4 : mx_scale_pitch(K);
+  q.s_word = planes ? mx_plane_pitch(N) : 4;
   return q;
 }
 
 }  // namespace
 
-SMOE_API size_t smoe_linear_mxfp4_workspace_bytes(int N, int K) {
-  return N < 1 || K < 1 || mx_linear_quantizes_inside(N, K) ? 0 : mx_ws(N, K).total;
+SMOE_API size_t smoe_linear_mxfp4_workspace_bytes(int N, int K, int N_out) {
+  if (N < 1 || K < 1 || N_out < 1 || mx_linear_quantizes_inside(N, K)) return 0;
+  return mx_ws(N, K).total + (mx_large_linear(N, N_out) ? align_up(mx_planes_bytes(N_out, K)) : 0);
 }
 
 SMOE_API int smoe_linear_mxfp4(const void* x, int x_dtype, int64_t ldx, int N, int K, const uint8_t* wq, int64_t ldw,
                                const uint8_t* w_scale, int64_t ld_ws, const float* bias, int N_out, int act, void* out,
                                int out_dtype, void* ws, size_t ws_bytes, void* stream) {
   if (x_dtype != SMOE_F32 && x_dtype != SMOE_BF16 && x_dtype != SMOE_F16) return fail(SMOE_EUNSUPPORTED, "linear input dtype");
-  if (N < 0 || N > 0x7fffff00 || K < 1 || K > 0x7fffff00 || N_out < 1 || N_out > 0x7fffff00 || ldx < K ||
-      ldw < mx_code_pitch(K) || ldw % 16 || ld_ws < mx_scale_pitch(K) || ld_ws % 4)
-    return fail(SMOE_EINVAL, "mxfp4 linear shape (ldx >= K; weight rows of whole blocks, ldw % 16 == 0; ld_ws % 4 == 0)");
+  if (N < 0 || N > 0x7fffff00 || K < 1 || K > 0x7fffff00 || N_out < 1 || N_out > (1 << 22) || ldx < K || K > (1 << 23) ||
+      ldw > (1 << 22) || ldw < mx_code_pitch(K) || ldw % 16 || ld_ws < mx_scale_pitch(K) || ld_ws % 4)
+    return fail(SMOE_EINVAL, "mxfp4 linear shape (ldx >= K; K <= 2^23, N_out <= 2^22, ldw <= 2^22; weight rows of whole blocks, ldw % 16 == 0; ld_ws % 4 == 0)");
   if (N > ((1 << 28) - 16) / ((static_cast<int64_t>(K) + 127) / 128)) return fail(SMOE_EINVAL, "mxfp4 linear shape (at most 2^28 - 16 pieces of 1 x 128 of x)");
   if (act != SMOE_LINEAR_NONE && act != SMOE_LINEAR_GELU) return fail(SMOE_EINVAL, "act");
   if (out_dtype != SMOE_F32 && out_dtype != SMOE_BF16) return fail(SMOE_EUNSUPPORTED, "out dtype");
@@ -1871,17 +1888,24 @@ SMOE_API int smoe_linear_mxfp4(const void* x, int x_dtype, int64_t ldx, int N, i
     g.ld_float = ldx;
   } else {
     const MxWs l = mx_ws(N, K);
-    if (ws_bytes < l.total) return fail(SMOE_ECAPACITY, "workspace");
-    const MxQuant q = mx_rows(x, x_dtype, ldx, N, K, ws, l);
-    SMOE_TRY(launch_quantize_mxfp4(q, s), "quantize mxfp4");
+    if (ws_bytes < smoe_linear_mxfp4_workspace_bytes(N, K, N_out)) return fail(SMOE_ECAPACITY, "workspace");
+    const bool large = mx_large_linear(N, N_out);
+    const MxQuant q = mx_rows(x, x_dtype, ldx, N, K, ws, l, large);
+    MxPlanes planes[2];
+    if (large) {
+      planes[0] = mx_planes(w_scale, ld_ws, 1, N_out, K, at<void>(ws, l.total));
+      g.ws_plane = mx_plane_pitch(N_out);
+    }
+    SMOE_TRY(launch_quantize_mxfp4(q, planes, s), "quantize mxfp4");
     g.X = q.codes;
     g.ldx = q.ld_codes;
     g.xs = q.scale;
-    g.ld_xs = q.ld_scale;
+    g.xs_plane = q.s_word;
+    g.ld_xs = q.s_row;
   }
   g.W = wq;
   g.ldw = ldw;
-  g.ws = w_scale;
+  g.ws = g.ws_plane ? at<uint8_t>(ws, mx_ws(N, K).total) : w_scale;
   g.ld_ws = ld_ws;
   g.K = K;
   g.N_out = N_out;
@@ -1899,9 +1923,9 @@ namespace {
 int check_experts_mxfp4(const smoe_experts_mxfp4* ex, int N, int K) {
   if (!ex) return fail(SMOE_EINVAL, "null experts");
   if (ex->act != SMOE_ACT_GELU && ex->act != SMOE_ACT_SWIGLU) return fail(SMOE_EINVAL, "act");
-  if (ex->E < 1 || ex->E > 256 || ex->H < 32 || ex->H % 32 || ex->U < 32 || ex->U % 32 || ex->H > (1 << 24) ||
-      ex->U > (1 << 24))
-    return fail(SMOE_EINVAL, "mxfp4 experts: 1 <= E <= 256, H % 32 == 0, U % 32 == 0");
+  if (ex->E < 1 || ex->E > 256 || ex->H < 32 || ex->H % 32 || ex->U < 32 || ex->U % 32 || ex->H > (1 << 22) ||
+      ex->U > (1 << 22))
+    return fail(SMOE_EINVAL, "mxfp4 experts: 1 <= E <= 256, H % 32 == 0, U % 32 == 0, neither above 2^22");
   if (!ex->w_up || !ex->w_down || !ex->s_up || !ex->s_down) return fail(SMOE_EINVAL, "expert weights or scales missing");
   if (!aligned16(ex->w_up) || !aligned16(ex->w_down) || reinterpret_cast<uintptr_t>(ex->s_up) % 4 ||
       reinterpret_cast<uintptr_t>(ex->s_down) % 4)
@@ -1910,11 +1934,13 @@ int check_experts_mxfp4(const smoe_experts_mxfp4* ex, int N, int K) {
     return fail(SMOE_EINVAL, "shape (1 <= top_k <= 64, N * top_k < 2^31 - 128)");
   if (N > (ex->H > 4096 ? 65535 : 65535 * 64)) return fail(SMOE_EINVAL, "N <= 4194240, with H > 4096 N <= 65535");
   if (N > ((1 << 28) - 16) / ((ex->H + 127) / 128)) return fail(SMOE_EINVAL, "N * ceil(H / 128) <= 2^28 - 16");
+  if (static_cast<int64_t>(ex->U) * ex->H > (1ll << 32) || static_cast<int64_t>(N) * ex->H > (1ll << 32))
+    return fail(SMOE_EINVAL, "mxfp4 experts: U * H and N * H <= 2^32");
   return SMOE_OK;
 }
 
 struct MxExpertsWs {
-  size_t plan, off, cnt, rows, roww, tokrow, act, ascale, y, total;
+  size_t plan, off, cnt, rows, roww, tokrow, act, ascale, y, sup, sdown, total;
   MxWs x;
   size_t x_at;
 };
@@ -1931,8 +1957,11 @@ MxExpertsWs mx_experts_ws(const smoe_experts_mxfp4& ex, int N, int K) {
   w.x = mx_ws(n, ex.H);
   w.x_at = z.take(w.x.total);
   w.act = z.take(r * mx_code_pitch(ex.U));
-  w.ascale = z.take(r * mx_scale_pitch(ex.U));
+  w.ascale = z.take(mx_planes_bytes(r, ex.U));
   w.y = z.take(r * ex.H * 4);
+  const size_t large = mx_large_experts(N, K, ex.E) ? ex.E : 0;  // the weights' scales in planes
+  w.sup = z.take(large * (ex.act == SMOE_ACT_SWIGLU ? 2 : 1) * ex.U * mx_scale_pitch(ex.H));
+  w.sdown = z.take(large * ex.H * mx_scale_pitch(ex.U));
   w.total = z.off;
   return w;
 }
@@ -1986,8 +2015,9 @@ SMOE_API int smoe_expert_delta_mxfp4(const smoe_experts_mxfp4* ex, const void* m
   const int halves = ex->act == SMOE_ACT_SWIGLU ? 2 : 1;
   int32_t *off = at<int32_t>(ws, l.off), *rows = at<int32_t>(ws, l.rows), *tokrow = at<int32_t>(ws, l.tokrow);
   float* roww = at<float>(ws, l.roww);
-  const MxQuant mq = mx_rows(msg, msg_dtype, H, N, H, at<void>(ws, l.x_at), l.x);
-  if (prep_fits(N, K, E)) {
+  const bool large = mx_large_experts(N, K, E);
+  const MxQuant mq = mx_rows(msg, msg_dtype, H, N, H, at<void>(ws, l.x_at), l.x, large);
+  if (!large && prep_fits(N, K, E)) {
     PrepArgs pa;
     pa.idx = idx;
     pa.w = w;
@@ -2003,21 +2033,29 @@ SMOE_API int smoe_expert_delta_mxfp4(const smoe_experts_mxfp4* ex, const void* m
     rc = smoe_dispatch_plan(idx, w, N, K, E, at<int32_t>(ws, l.cnt), off, rows, roww, tokrow, at<void>(ws, l.plan),
                             smoe_dispatch_workspace_bytes(N, K, E), stream);
     if (rc != SMOE_OK) return rc;
-    SMOE_TRY(launch_quantize_mxfp4(mq, s), "quantize messages");
+    MxPlanes planes[2];
+    if (large) {
+      planes[0] = mx_planes(ex->s_up, mx_scale_pitch(H), E, halves * U, H, at<void>(ws, l.sup));
+      planes[1] = mx_planes(ex->s_down, mx_scale_pitch(U), E, H, U, at<void>(ws, l.sdown));
+    }
+    SMOE_TRY(launch_quantize_mxfp4(mq, planes, s), "quantize messages");
   }
   MxGemm up;
   up.epi = halves == 2 ? MX_UP_SWIGLU : MX_UP_GELU;
   up.X = mq.codes;
   up.ldx = mq.ld_codes;
   up.xs = mq.scale;
-  up.ld_xs = mq.ld_scale;
+  up.xs_plane = mq.s_word;
+  up.ld_xs = mq.s_row;
   up.a_rows = rows;
+  up.x_rows = N;
   up.W = ex->w_up;
   up.ldw = mx_code_pitch(H);
   up.w_gstride = static_cast<int64_t>(halves) * U * up.ldw;
-  up.ws = ex->s_up;
+  up.ws = large ? at<uint8_t>(ws, l.sup) : ex->s_up;
+  up.ws_plane = large ? mx_plane_pitch(halves * U) : 0;
   up.ld_ws = mx_scale_pitch(H);
-  up.ws_gstride = static_cast<int64_t>(halves) * U * up.ld_ws;
+  up.ws_gstride = static_cast<int64_t>(halves) * U * mx_scale_pitch(H);
   up.K = H;
   up.N_out = U;
   up.grp_off = off;
@@ -2028,6 +2066,7 @@ SMOE_API int smoe_expert_delta_mxfp4(const smoe_experts_mxfp4* ex, const void* m
   up.out = at<void>(ws, l.act);
   up.ldo = mx_code_pitch(U);
   up.out_scale = at<uint8_t>(ws, l.ascale);
+  up.os_plane = mx_plane_pitch(static_cast<int64_t>(N) * K);
   up.ld_os = mx_scale_pitch(U);
   SMOE_TRY(launch_gemm_mxfp4(up, s), "expert up GEMM");
   MxGemm dn;
@@ -2035,13 +2074,15 @@ SMOE_API int smoe_expert_delta_mxfp4(const smoe_experts_mxfp4* ex, const void* m
   dn.X = at<uint8_t>(ws, l.act);
   dn.ldx = up.ldo;
   dn.xs = up.out_scale;
+  dn.xs_plane = up.os_plane;
   dn.ld_xs = up.ld_os;
   dn.W = ex->w_down;
   dn.ldw = mx_code_pitch(U);
   dn.w_gstride = H * dn.ldw;
-  dn.ws = ex->s_down;
+  dn.ws = large ? at<uint8_t>(ws, l.sdown) : ex->s_down;
+  dn.ws_plane = large ? mx_plane_pitch(H) : 0;
   dn.ld_ws = mx_scale_pitch(U);
-  dn.ws_gstride = H * dn.ld_ws;
+  dn.ws_gstride = H * mx_scale_pitch(U);
   dn.K = U;
   dn.N_out = H;
   dn.grp_off = off;

@@ -173,39 +173,43 @@ __device__ __forceinline__ void store4(const P& p, int64_t r, int n, const float
 }
 
 // Rows of the 64 groups from b on: first, end and BM-row tiles of group
-// b + lane.  P: BlockGemm or MxGemm.
-template <typename P>
-__device__ __forceinline__ void groups64(const P& p, int BM, int b, int& lo, int& hi, int& t) {
+// b + lane; off: the G + 1 offsets, in global memory or LDS.
+template <typename O>
+__device__ __forceinline__ void groups64(O off, int G, int BM, int b, int& lo, int& hi, int& t) {
   const int i = b + static_cast<int>(threadIdx.x & 63);
-  const int ic = i < p.G ? i : p.G - 1;
-  lo = p.grp_off[ic];
-  hi = p.grp_off[ic + 1];
-  t = i < p.G ? (hi - lo + BM - 1) / BM : 0;
+  const int ic = i < G ? i : G - 1;
+  lo = off[ic];
+  hi = off[ic + 1];
+  t = i < G ? (hi - lo + BM - 1) / BM : 0;
 }
 
-// The tile of workgroup bid: group by group; within a group SUPER row tiles at
-// a time, over them strip by strip with the strip's row tiles next to each
-// other, so that the rows in use stay in an L2 while the strips' weights pass.
-// Workgroup ids are dealt to the 8 XCDs round robin and each XCD takes one
-// contiguous part of the order.  SUPER: an XCD holds 32 tiles of 256 rows (64 of
-// 128) at a time (32768 routed rows, 1024 -> 2816 SwiGLU, 256 rows a tile: 2
-// row tiles 250 us, 4 252, 8 260, 16 256; 1024 -> 5632: 119, 117, 118, 121).
-template <int BM, int BN, typename P>
-__device__ __forceinline__ bool block_tile(const P& p, int bid, int& g, int& m0, int& mrows,
-                                           int& n0) {
-  const int strips = (p.N_out + BN - 1) / BN;
+// Tiles of BM rows x BN channels in all.  P: BlockGemm or MxGemm.
+template <int BM, int BN, typename P, typename O>
+__device__ __forceinline__ int count_tiles(const P& p, O off) {
   int tiles = 0;
   if (p.G == 0) {
     tiles = (p.single_rows + BM - 1) / BM;
   } else {
     for (int b = 0; b < p.G; b += 64) {
       int lo, hi, t;
-      groups64(p, BM, b, lo, hi, t);
+      groups64(off, p.G, BM, b, lo, hi, t);
       tiles += __builtin_amdgcn_readlane(wave_incl_scan(t), 63);
     }
   }
-  const int T = tiles * strips;
-  if (bid >= T) return false;
+  return tiles * ((p.N_out + BN - 1) / BN);
+}
+
+// Tile bid of T, for a workgroup of id bid modulo 8: group by group; within a
+// group SUPER row tiles at a time, over them strip by strip with the strip's row
+// tiles next to each other, so that the rows in use stay in an L2 while the
+// strips' weights pass.  Workgroup ids are dealt to the 8 XCDs round robin and
+// each XCD takes one contiguous part of the order.  SUPER: an XCD holds 32 tiles
+// of 256 rows (64 of 128) at a time (32768 routed rows, 1024 -> 2816 SwiGLU, 256
+// rows a tile: 2 row tiles 250 us, 4 252, 8 260, 16 256; 1024 -> 5632: 119, 117,
+// 118, 121).
+template <int BM, int BN, typename P, typename O>
+__device__ __forceinline__ void tile_at(const P& p, O off, int T, int bid, int& g, int& m0, int& mrows, int& n0) {
+  const int strips = (p.N_out + BN - 1) / BN;
   const int x = bid & 7, base = T >> 3, rem = T & 7;
   const int logical = x * base + min(x, rem) + (bid >> 3);
   int lo = 0, hi = p.single_rows, in = logical;
@@ -214,7 +218,7 @@ __device__ __forceinline__ bool block_tile(const P& p, int bid, int& g, int& m0,
     int acc = 0;
     for (int b = 0; b < p.G; b += 64) {
       int l, h, t;
-      groups64(p, BM, b, l, h, t);
+      groups64(off, p.G, BM, b, l, h, t);
       const int incl = wave_incl_scan(t) * strips + acc;
       const uint64_t m = __ballot(logical < incl);
       if (m) {
@@ -232,9 +236,18 @@ __device__ __forceinline__ bool block_tile(const P& p, int bid, int& g, int& m0,
   constexpr int SUPER = BM == 256 ? 4 : 8;
   const int super = in / (SUPER * strips), rest = in - super * SUPER * strips;
   const int sr = min(SUPER, tm - super * SUPER);  // row tiles of this part
-  m0 = lo + (super * SUPER + rest % sr) * BM;
+  const int strip = sr == SUPER ? rest / SUPER : rest / sr;  // uniform: a shift but for the last part
+  m0 = lo + (super * SUPER + rest - strip * sr) * BM;
   mrows = min(BM, hi - m0);
-  n0 = (rest / sr) * BN;
+  n0 = strip * BN;
+}
+
+// The tile of workgroup bid, if there is one
+template <int BM, int BN, typename P>
+__device__ __forceinline__ bool block_tile(const P& p, int bid, int& g, int& m0, int& mrows, int& n0) {
+  const int T = count_tiles<BM, BN>(p, p.grp_off);
+  if (bid >= T) return false;
+  tile_at<BM, BN>(p, p.grp_off, T, bid, g, m0, mrows, n0);
   return true;
 }
 

@@ -12,10 +12,18 @@ namespace {
 
 int rc() { return hipGetLastError() == hipSuccess ? SMOE_OK : SMOE_EHIP; }
 
-// 128 columns of a row by 16 lanes (mx_quant_piece), sixteen pieces a workgroup.
+// 128 columns of a row by 16 lanes (mx_quant_piece), sixteen pieces a workgroup;
+// behind them workgroups for the planes, 256 words each
 template <int XDT>
-__global__ __launch_bounds__(256) void k_quant_mx(const MxQuant q, int npc, int64_t total) {
-  mx_quant_piece<XDT>(q, npc, total, (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 4, threadIdx.x & 15);
+__global__ __launch_bounds__(256) void k_quant_mx(const MxQuant q, int npc, int64_t total, uint32_t quant_wgs,
+                                                  const MxPlanes p0, const MxPlanes p1) {
+  if (blockIdx.x < quant_wgs) {
+    mx_quant_piece<XDT>(q, npc, total, (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) >> 4, threadIdx.x & 15);
+    return;
+  }
+  const uint32_t i = (blockIdx.x - quant_wgs) * 256 + threadIdx.x, n0 = static_cast<uint32_t>(mx_plane_words(p0));
+  if (i < n0) mx_plane_word(p0, i);
+  else if (i - n0 < static_cast<uint32_t>(mx_plane_words(p1))) mx_plane_word(p1, i - n0);
 }
 
 // The values of codes: eight columns a thread.  Exact but for f16, whose range
@@ -74,332 +82,439 @@ __global__ __launch_bounds__(256) void k_dequant_mx(const uint8_t* __restrict__ 
 }
 
 // ------------------------------------------------------------------ GEMM ----
-// BM rows x BN weight rows a workgroup (SwiGLU: BN / 2 gate channels and the
-// up channels of the same outputs), 256 k (128 bytes of codes and 8 of scales a
-// row) a stage through an LDS ring of NS stages filled by DMA.  WM x WN waves,
-// wave tile BM / WM rows x BN / WN weight rows (SwiGLU: half gate, half up).
-// The matrix instruction takes the scales beside the codes, so a stage is 2
-// instructions for each 16 x 16 tile straight into the f32 accumulators.
+// Where chunk c of row r of a stage lies (an involution).  Rows are 64 bytes;
+// the four groups of lanes that a ds_read_b128 serves together (0-3, 12-15,
+// 20-23, 24-27: rows 4 R .. of R = 0 and 3 at one chunk, 1 and 2 at its
+// neighbour) meet in four different quarters of the banks.
+__device__ __forceinline__ int mx_chunk(int r, int c) {
+  const int R = (r >> 2) & 3;
+  return c ^ ((R & 1) << 1 ^ (R >> 1) * 3);
+}
+
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+constexpr int kNowhere = static_cast<int>(0x80000000u);  // an offset that a buffer store drops
+
+// BM rows x BN weight rows a tile (SwiGLU: BN / 2 gate channels and the up
+// channels of the same outputs), 128 k (64 bytes of codes and 4 of scales a row)
+// a stage through an LDS ring of NS stages filled by DMA.  WM x WN waves, wave
+// tile BM / WM rows x BN / WN weight rows (SwiGLU: half gate, half up).  The
+// matrix instruction takes the scales beside the codes, so a stage is one
+// instruction for each 16 x 16 tile straight into the f32 accumulators.
 //
-// A lane's 32 codes and their scale: the instruction wants lane q = l / 16 to
-// hold one block of each row; with blocks 2 q and 2 q + 1 of a stage in its two
-// steps the two scales are neighbours, one 16-bit LDS read whose bytes the two
-// instructions name.  The DMA puts block 2 q at chunk q and 2 q + 1 at q + 4, so
-// that the fragment reads keep the conflict-free pattern of 128-byte rows.
-template <int EPI, int ODT, int BM, int BN, int WM, int WN, int NS>
-__global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm_mx(const MxGemm p) {
-  constexpr bool SWIGLU = EPI == MX_UP_SWIGLU, UP = EPI == MX_UP_GELU || SWIGLU;
+// A workgroup walks over the tiles bid, bid + grid, ..: the next tile's first
+// stages are requested before the last products and the epilogue, which uses no
+// LDS.  For that a lane holds four rows of one channel of each 16 x 16 tile, and
+// channels are dealt to the tiles so that the lane's are neighbours: a row leaves
+// in 256-byte pieces of 16 lanes, and a block of 32 activations is quantized by a
+// quad of lanes.
+//
+// The last two of a stage's FN steps come after the barrier that opens the next
+// stage, over the latency of that stage's first fragments.
+template <int EPI, int ODT, int BM, int BN, int WM, int WN, int NS, int OCC>
+__global__ __launch_bounds__(64 * WM * WN, OCC) void k_gemm_mx(const MxGemm p) {
+  constexpr bool SWIGLU = EPI == MX_UP_SWIGLU, UP = EPI == MX_UP_GELU || SWIGLU, GATHER = UP;
   constexpr int NW = WM * WN, CH = SWIGLU ? BN / 2 : BN, CHW = CH / WN, TM = BM / WM, TN = BN / WN, FM = TM / 16, FN = TN / 16;
-  static_assert(TM % 16 == 0 && TN % (SWIGLU ? 64 : 32) == 0, "whole blocks of 32 channels a wave");
-  constexpr int XB = BM * 128, WB = BN * 128, SB = (BM + BN) * 8, STAGE = XB + WB + SB;
-  constexpr int XI = BM / 8, WI = BN / 8, SI = SB / 256;  // DMA instructions of a stage (fewer than waves: some load the same)
-  constexpr int X_LD = (XI + NW - 1) / NW, W_LD = (WI + NW - 1) / NW, S_LD = (SI + NW - 1) / NW, LD = X_LD + W_LD + S_LD;
-  static_assert((XI % NW == 0 || NW % XI == 0) && (WI % NW == 0 || NW % WI == 0) && SB % 256 == 0, "whole DMA instructions");
+  constexpr int JC = SWIGLU ? FN / 2 : FN;  // channels of a lane
+  static_assert(TM % 16 == 0 && TM <= 64 && FN >= 4 && (JC == 4 || JC == 8 || (!SWIGLU && !UP && JC == 2)), "wave tile");
+  constexpr int XI = BM / 16, WI = BN / 16;  // DMA instructions of a stage (fewer than waves: some load the same)
+  // scales: BN words of the weights by channel, then the rows', from the one at or
+  // before the first whose word is 16-byte aligned; GATHER: the rows' word by word
+  constexpr int SLOTS = BN / 4 + (GATHER ? 0 : BM / 4 + 1), SI = (SLOTS + 63) / 64, GI = GATHER ? (BM + 63) / 64 : 0;
+  constexpr int XB = XI * 1024, WB = WI * 1024, XS = SI * 1024 - (GATHER ? 0 : (64 * SI - BN / 4) * 16), STAGE = XB + WB + SI * 1024 + GI * 256;
+  constexpr int X_LD = (XI + NW - 1) / NW, W_LD = (WI + NW - 1) / NW, S_LD = (SI + NW - 1) / NW, G_LD = (GI + NW - 1) / NW, LD = X_LD + W_LD + S_LD + G_LD;
+  static_assert((XI % NW == 0 || NW % XI == 0) && (WI % NW == 0 || NW % WI == 0), "whole DMA instructions");
+  constexpr int EB = UP ? 0 : (ODT == SMOE_F32 ? 4 : 2);
+  constexpr int STORES = UP ? FM * 8 : FM * 4 * (JC * EB / 16 > 0 ? JC * EB / 16 : 1);  // of a wave and tile
+  static_assert((NS - 1) * LD < 64, "counted by vmcnt");
   __shared__ __attribute__((aligned(1024))) uint8_t ring[NS * STAGE];
-  int g, m0, mrows, n0;
-  if (!block_tile<BM, CH>(p, blockIdx.x, g, m0, mrows, n0)) return;  // uniform
+  __shared__ int s_off[257];
+  __shared__ __attribute__((aligned(16))) i32x4 s_tile[NW][8];  // a wave's: tiles requested, not yet finished
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
-  const int nb = (p.K + kMxBlock - 1) / kMxBlock, KS = (nb + 7) / 8, nd = (nb + 3) / 4;
-
-  // the weight row of row r of the tile
-  auto wrow = [&](int r) {
-    const int w = r / TN, t = r % TN;
-    const int ch = SWIGLU ? n0 + CHW * w + t % CHW : n0 + r;
-    return static_cast<int64_t>(min(ch, p.N_out - 1)) + (SWIGLU && t >= CHW ? p.N_out : 0);
-  };
-  auto xrow = [&](int r) {  // rows past the end: a valid one, never stored
-    const int pr = m0 + min(r, mrows - 1);
-    return static_cast<int64_t>(p.a_rows ? p.a_rows[pr] : pr);
-  };
-  // DMA sources: lane i of instruction j loads 16 bytes of row 8 j + i / 8, the
-  // block that belongs at the chunk the swizzle puts at i % 8 (the same one for
-  // every instruction of a wave: their rows are a multiple of 16 apart, or it
-  // has one)
-  static_assert(8 * NW % 16 == 0, "one chunk per lane");
-  const int cl = sw_chunk<8>(8 * wave + (lane >> 3), lane & 7);
-  const int blk = 2 * (cl & 3) + (cl >> 2);
-  const uint8_t* xsrc[X_LD];
-  const uint8_t* wsrc[W_LD];
-  const uint8_t* ssrc[S_LD];
-#pragma unroll
-  for (int j = 0; j < X_LD; ++j) xsrc[j] = p.X + xrow(8 * ((NW * j + wave) % XI) + (lane >> 3)) * p.ldx;
-#pragma unroll
-  for (int j = 0; j < W_LD; ++j) wsrc[j] = p.W + g * p.w_gstride + wrow(8 * ((NW * j + wave) % WI) + (lane >> 3)) * p.ldw;
-#pragma unroll
-  for (int j = 0; j < S_LD; ++j) {  // 32 rows' two words of scales an instruction, X's rows before W's
-    const int r = 32 * ((NW * j + wave) % SI) + (lane >> 1);
-    ssrc[j] = r < BM ? p.xs + xrow(r) * p.ld_xs : p.ws + g * p.ws_gstride + wrow(r - BM) * p.ld_ws;
-  }
-  // DMA d of stage s; what lies past K is the row's first chunk or word instead, cut before use
-  auto issue = [&](int s) {
-    uint8_t* base = ring + (s % NS) * STAGE;
-    const int at = 8 * s + blk < nb ? (8 * s + blk) * 16 : 0;
-    const int sat = 2 * s + (lane & 1) < nd ? (2 * s + (lane & 1)) * 4 : 0;
-#pragma unroll
-    for (int d = 0; d < X_LD; ++d)
-      __builtin_amdgcn_global_load_lds((gbl_vptr)(xsrc[d] + at), (lds_vptr)(base + (NW * d + wave) % XI * 1024), 16, 0, 0);
-#pragma unroll
-    for (int d = 0; d < W_LD; ++d)
-      __builtin_amdgcn_global_load_lds((gbl_vptr)(wsrc[d] + at), (lds_vptr)(base + XB + (NW * d + wave) % WI * 1024), 16, 0, 0);
-#pragma unroll
-    for (int d = 0; d < S_LD; ++d)
-      __builtin_amdgcn_global_load_lds((gbl_vptr)(ssrc[d] + sat), (lds_vptr)(base + XB + WB + (NW * d + wave) % SI * 256), 4, 0, 0);
-  };
   const int fr = lane & 15, q = lane >> 4;
-  const int flo = fr * 128 + (sw_chunk<8>(fr, q) << 4);  // step h: flo ^ 64 h
+  const int nb = (p.K + kMxBlock - 1) / kMxBlock, KS = (nb + 3) / 4;
+  for (int i = tid; i <= p.G && p.G > 0; i += NW * 64) s_off[i] = p.grp_off[i];
+  __syncthreads();
+  const int T = count_tiles<BM, CH>(p, s_off);
+  if (static_cast<int>(blockIdx.x) >= T) return;  // uniform
 
-  f32x4 acc[FN][FM];
-#pragma unroll
-  for (int j = 0; j < FN; ++j)
-#pragma unroll
-    for (int i = 0; i < FM; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int s = 0; s < NS; ++s)
-    if (s < KS) issue(s);
-
-  auto stage = [&](int s) {
-    const uint8_t* sx = ring + (s % NS) * STAGE;
-    const uint8_t* ss = sx + XB + WB + 2 * q;
-    uint32_t xsc[FM], wsc[FN];
-#pragma unroll
-    for (int j = 0; j < FN; ++j) wsc[j] = *reinterpret_cast<const uint16_t*>(ss + (BM + wn * TN + j * 16 + fr) * 8);
-#pragma unroll
-    for (int i = 0; i < FM; ++i) xsc[i] = *reinterpret_cast<const uint16_t*>(ss + (wm * TM + i * 16 + fr) * 8);
-    auto step = [&](auto h) {
-      constexpr int H = decltype(h)::value;
-      u32x4 w[FN];
-#pragma unroll
-      for (int j = 0; j < FN; ++j) w[j] = *reinterpret_cast<const u32x4*>(sx + XB + (wn * TN + j * 16) * 128 + (flo ^ (64 * H)));
-#pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(sx + (wm * TM + i * 16) * 128 + (flo ^ (64 * H)));
-#pragma unroll
-        for (int j = 0; j < FN; ++j) acc[j][i] = mx_mfma<H>(w[j], wsc[j], x, xsc[i], acc[j][i]);
-      }
+  // a lane's number anew: what is computed from it stays where it is used (kept
+  // over the products it would take their registers)
+  auto anew = [](int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+  };
+  // The channel of weight row r, from the tile's first (SwiGLU: of its half):
+  // tile j = t / 16 of its wave, place c = t % 16; lane c's channels of a wave are
+  // JC c + j, in f32 4 c + j % 4 of every 64
+  auto channel = [](int r) {
+    const int w = r / TN, t = r % TN, j = (t >> 4) % JC, c = t & 15;
+    return CHW * w + (EB == 4 ? 64 * (j >> 2) + 4 * c + (j & 3) : JC * c + j);
+  };
+  // DMA sources of the tile that is requested: lane i of instruction j loads 16
+  // bytes of row 16 j + i / 4, the block whose chunk lies at i % 4 (the same one
+  // for every j), or slot 64 j + i of the scales
+  // (an address is a base of the tile's and 32 bits of a lane's: launch_gemm_mxfp4
+  // checks that they suffice)
+  const int blk = mx_chunk(lane >> 2, lane & 3);
+  const uint8_t *xbase = nullptr, *wbase = nullptr;
+  uint32_t xoff[X_LD], woff[W_LD];
+  const uint8_t* ssrc[S_LD];
+  int64_t splane[S_LD];
+  uint32_t goff[G_LD > 0 ? G_LD : 1];
+  int pbid = blockIdx.x, ps = 0;  // tile and stage to request next
+  int asked = 0;                  // tiles
+  auto sources = [&] {
+    int g, m0, mrows, n0;
+    tile_at<BM, CH>(p, s_off, T, pbid, g, m0, mrows, n0);
+    const int ln = anew(lane);
+    s_tile[wave][asked++ & 7] = i32x4{g, m0, mrows, n0};  // every lane the same
+    // rows past the end: a valid one, never stored
+    auto xrow = [&](int r) {
+      const int pr = min(r, mrows - 1);
+      return static_cast<uint32_t>(GATHER ? p.a_rows[m0 + pr] : pr);
     };
-    step(std::integral_constant<int, 0>{});
-    step(std::integral_constant<int, 1>{});
+    xbase = p.X + (GATHER ? 0 : m0 * p.ldx);
+    wbase = p.W + g * p.w_gstride + n0 * p.ldw;
+#pragma unroll
+    for (int j = 0; j < X_LD; ++j)
+      xoff[j] = xrow(16 * ((NW * j + wave) % XI) + (ln >> 2)) * static_cast<uint32_t>(p.ldx) + blk * 16;
+#pragma unroll
+    for (int j = 0; j < W_LD; ++j) {  // SwiGLU: gate rows, then up
+      const int r = 16 * ((NW * j + wave) % WI) + (ln >> 2);
+      woff[j] = static_cast<uint32_t>(min(channel(r), p.N_out - 1 - n0) + (SWIGLU && r % TN >= TN / 2 ? p.N_out : 0)) *
+                    static_cast<uint32_t>(p.ldw) + blk * 16;
+    }
+#pragma unroll
+    for (int j = 0; j < S_LD; ++j) {
+      const int t = min(64 * ((NW * j + wave) % SI) + ln, SLOTS - 1);
+      const bool up = SWIGLU && t >= BN / 8, wt = t < BN / 4;
+      const int64_t at = wt ? min(n0 + 4 * (up ? t - BN / 8 : t), p.N_out - 1) + (up ? p.N_out : 0)
+                            : min((m0 & ~3) + 4 * (t - BN / 4), m0 + mrows - 1);
+      ssrc[j] = (wt ? p.ws + g * p.ws_gstride : p.xs) + (at & ~3ll) * 4;  // whole slots: planes are
+      splane[j] = wt ? p.ws_plane : p.xs_plane;
+    }
+#pragma unroll
+    for (int j = 0; j < G_LD; ++j) goff[j] = xrow(min(64 * ((NW * j + wave) % (GI > 0 ? GI : 1)) + ln, BM - 1)) * 4;
+  };
+  // The next stage of the sequence (behind the last one that one again, never
+  // read): its tile's sources, then DMA d of it into slot `base`.  Blocks past K
+  // are the row's first one instead, cut before use.
+  uint32_t fwd = 0;  // bytes from the block of stage 0 to this stage's (an offset holds 16 blk, which may go again)
+  auto next_stage = [&] {
+    if (ps == KS && pbid + static_cast<int>(gridDim.x) < T) {  // uniform
+      pbid += gridDim.x;
+      ps = 0;
+      sources();
+    }
+    ps = min(ps, KS - 1) + 1;
+    fwd = 4 * (ps - 1) + blk < nb ? 64u * (ps - 1) : -16u * blk;
+  };
+  auto dma = [&](uint8_t* base, int d) {
+    if (d < X_LD) {
+      __builtin_amdgcn_global_load_lds((gbl_vptr)(xbase + (xoff[d < X_LD ? d : 0] + fwd)), (lds_vptr)(base + (NW * d + wave) % XI * 1024), 16, 0, 0);
+    } else if (d < X_LD + W_LD) {
+      const int e = d - X_LD;
+      __builtin_amdgcn_global_load_lds((gbl_vptr)(wbase + (woff[e >= 0 && e < W_LD ? e : 0] + fwd)), (lds_vptr)(base + XB + (NW * e + wave) % WI * 1024), 16, 0, 0);
+    } else if (d < X_LD + W_LD + S_LD) {
+      const int e = d - X_LD - W_LD, i = e >= 0 && e < S_LD ? e : 0;
+      __builtin_amdgcn_global_load_lds((gbl_vptr)(ssrc[i] + (ps - 1) * splane[i]), (lds_vptr)(base + XB + WB + (NW * e + wave) % SI * 1024), 16, 0, 0);
+    } else {
+      const int e = d - X_LD - W_LD - S_LD, i = e >= 0 && e < G_LD ? e : 0;
+      __builtin_amdgcn_global_load_lds((gbl_vptr)(p.xs + (ps - 1) * p.xs_plane + goff[i]), (lds_vptr)(base + XB + WB + XS + (NW * e + wave) % (GI > 0 ? GI : 1) * 256), 4, 0, 0);
+    }
   };
   // The last stage of a K that ends inside it: code 0 for what lies past K in
-  // the rows, and scale 1 in both operands (a byte of another row may be NaN).
-  // The weights' codes there may be anything: none of them is NaN.
-  auto cut = [&](int s) {
-    const int left = nb - 8 * s;
-    if (left >= 8) return;  // uniform
-    uint8_t* base = ring + (s % NS) * STAGE;
-    const int per = 8 - left;
-    for (int e = tid; e < BM * per; e += NW * 64) {
+  // the rows.  The weights' codes there may be anything: none of them is NaN, nor
+  // is a scale there.
+  auto cut = [&](int s, uint8_t* base) {
+    const int left = nb - 4 * s;
+    if (left >= 4) return;  // uniform
+    const int per = 4 - left;
+    for (int e = anew(tid); e < BM * per; e += NW * 64) {
       const int r = e / per, b = left + e % per;
-      *reinterpret_cast<u32x4*>(base + r * 128 + (sw_chunk<8>(r, (b >> 1) | (b & 1) << 2) << 4)) = u32x4{0u, 0u, 0u, 0u};
+      *reinterpret_cast<u32x4*>(base + r * 64 + (mx_chunk(r, b) << 4)) = u32x4{0u, 0u, 0u, 0u};
     }
-    for (int e = tid; e < (BM + BN) * per; e += NW * 64) base[XB + WB + e / per * 8 + left + e % per] = 127;
     lds_barrier();
   };
-  // own part of a stage landed (the later ones may be on their way); after the
-  // barrier everybody's, and nobody reads the stage before any more
-  if (KS >= NS) wait_vmcnt<(NS - 1) * LD>();
-  else wait_vmcnt<0>();
-  __builtin_amdgcn_s_barrier();
-  cut(0);
-  stage(0);
-  int s = 1;
-  for (; s - 1 + NS < KS; ++s) {
-    wait_vmcnt<(NS - 2) * LD>();
-    wait_lgkm0();
-    __builtin_amdgcn_s_barrier();
-    issue(s - 1 + NS);
-    stage(s);
-  }
-  for (; s < KS; ++s) {
-    wait_vmcnt<0>();
-    wait_lgkm0();
-    __builtin_amdgcn_s_barrier();
-    cut(s);
-    stage(s);
-  }
 
-  // epilogue: lane holds channels 4 q + v of row fr of each 16 x 16 tile
-  const float* bias = p.bias ? p.bias + g * p.bias_gstride : nullptr;
-  if constexpr (UP) {
-    // a block of 32 channels is two tiles of one wave: its amax by the four
-    // lanes of a row; codes and scales leave through the ring in whole rows
-    constexpr int JN = SWIGLU ? FN / 2 : FN, CPR = CH / 32;  // 16-byte chunks (blocks) a row
-    static_assert(BM * CH / 2 + BM * CPR <= NS * STAGE, "staging in the ring");
-    uint8_t* stg = ring;
-    uint8_t* sst = ring + BM * (CH / 2);
-    __syncthreads();  // every wave is done with the ring
+  const int flo = fr * 64 + (mx_chunk(fr, q) << 4);
+  u32x4 x[FM], w[FN];
+  uint32_t xsc[FM], wsc[FN];
+  f32x4 acc[FN][FM];
+  const int wch = (CHW * wn + (EB == 4 ? 4 : JC) * fr) * 4;  // the lane's first channel's word
+  int shift = 0;  // rows before the tile's first in the first slot
+  uint8_t *cur = ring, *prev = ring + (NS - 1) * STAGE;  // slots of this stage and of the one before
+  bool stored = false;                                   // a tile's stores lie behind
+  // Stage s of a tile: its DMAs landed (own ones by the count, in which the
+  // stages requested since, and the stores of the tile before if they are newer,
+  // may be under way; everybody's behind the barrier, after which nobody reads
+  // the slot before any more), and that slot filled again.
+  auto open = [&](int s) {
+    constexpr int C = (NS - 2) * LD;
+    wait_lgkm0();
+    if (stored && s < NS - 1) wait_vmcnt<(C + STORES < 63 ? C + STORES : 63)>();
+    else wait_vmcnt<C>();
+    __builtin_amdgcn_s_barrier();
+    if (s == KS - 1) cut(s, cur);
+    next_stage();
+  };
+  auto read_w = [&](int j) { w[j] = *reinterpret_cast<const u32x4*>(cur + XB + (wn * TN + j * 16) * 64 + flo); };
+  auto products = [&](int j) {
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int b = 0; b < JN / 2; ++b) {
-      const int c = n0 + CHW * wn + 32 * b;
-      float bb[2][4] = {};
-      if (bias && c < p.N_out) {  // uniform: N_out % 32 == 0
+    for (int i = 0; i < FM; ++i) acc[j][i] = mx_mfma<0>(x[i], xsc[i], w[j], wsc[j], acc[j][i]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // The products of an open stage but for the last two steps', which run
+  // (`before`: those of the stage before) over the latency of its first reads
+  auto stage = [&](auto before) {
+    const uint8_t* sc = cur + XB + WB + q;
+    const uint8_t* sx = sc + XS + (wm * TM + fr + shift) * 4;
+    u32x4 nx[FM];
+    uint32_t nxs[FM];
+    u32x4 nwv[FN / 4];
+    read_w(0);
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+    for (int i = 0; i < FM; ++i) {
+      nx[i] = *reinterpret_cast<const u32x4*>(cur + (wm * TM + i * 16) * 64 + flo);
+      nxs[i] = sx[i * 64];
+    }
+    // the lane's channels' words, four at a time: byte q of each
 #pragma unroll
-          for (int v = 0; v < 4; ++v) bb[j][v] = bias[c + 16 * j + 4 * q + v];
+    for (int h = 0; h < FN / 4; ++h)
+      nwv[h] = *reinterpret_cast<const u32x4*>(cur + XB + WB + wch + (4 * h >= JC ? CH * 4 : 0) + 4 * h % JC * (EB == 4 ? 64 : 4));
+    read_w(1);
+    if constexpr (FN > 4) read_w(2);  // w[2], w[3] of four still hold the stage before
+    // the DMAs go under the products, evenly: all at once they hold up every wave
+    // of the workgroup (16384 x 1024 -> 5632: 75 us)
+    constexpr int FIRST = decltype(before)::value ? 0 : 2;
+    auto dmas = [&](int step) {
+#pragma unroll
+      for (int d = 0; d < LD; ++d)
+        if (max(d * FN / LD, FIRST) == step) dma(prev, d);
+    };
+    if constexpr (decltype(before)::value) {
+      products(FN - 2);
+      dmas(0);
+      products(FN - 1);
+      dmas(1);
+    }
+    if constexpr (FN == 4) read_w(2);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      x[i] = nx[i];
+      xsc[i] = nxs[i];
+    }
+#pragma unroll
+    for (int j = 0; j < FN; ++j) wsc[j] = nwv[j / 4][j % 4] >> (8 * q);
+#pragma unroll
+    for (int j = 0; j < FN - 2; ++j) {
+      if (j + 3 < FN) read_w(j + 3);
+      products(j);
+      dmas(j + 2);
+    }
+    prev = cur;
+    cur = cur + STAGE == ring + NS * STAGE ? ring : cur + STAGE;
+  };
+  static_assert(FN >= 4, "steps of a stage");
+
+  sources();
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) {
+    next_stage();
+#pragma unroll
+    for (int d = 0; d < LD; ++d) dma(ring + i * STAGE, d);
+  }
+  static_assert(NS <= 8, "s_tile: at most NS - 1 tiles ahead");
+  for (int bid = blockIdx.x, turn = 0; bid < T; bid += gridDim.x, ++turn) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j)
+#pragma unroll
+      for (int i = 0; i < FM; ++i) acc[j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    open(0);
+    float rows_w[(TM + 63) / 64];  // MX_DOWN: the weights of the wave's rows lane, lane + 64
+    const i32x4 tile = s_tile[wave][turn & 7];
+    const int cg = __builtin_amdgcn_readfirstlane(tile.x), cm0 = __builtin_amdgcn_readfirstlane(tile.y),
+              cmrows = __builtin_amdgcn_readfirstlane(tile.z), cn0 = __builtin_amdgcn_readfirstlane(tile.w);
+    if constexpr (!GATHER) shift = cm0 & 3;
+    if constexpr (EPI == MX_DOWN) {
+#pragma unroll
+      for (int h = 0; h < (TM + 63) / 64; ++h) rows_w[h] = p.row_scale[cm0 + min(wm * TM + 64 * h + lane, cmrows - 1)];
+    }
+    stage(std::false_type{});
+    if constexpr (EPI == MX_DOWN) {
+#pragma unroll
+      for (int h = 0; h < (TM + 63) / 64; ++h) rows_w[h] = __int_as_float(anew(__float_as_int(rows_w[h])));  // here, not behind the last DMAs
+    }
+#pragma unroll 1
+    for (int s = 1; s < KS; ++s) {
+      open(s);
+      stage(std::true_type{});
+    }
+    products(FN - 2);
+    products(FN - 1);
+
+    // epilogue: lane (q, fr) holds channels ch0 .. of rows 4 q + v of each 16
+    const int row0 = wm * TM, eq = anew(q), ef = anew(fr);
+    const int ch0 = cn0 + CHW * wn + (EB == 4 ? 4 : JC) * ef;  // the lane's first channel
+    float bias[JC];
+#pragma unroll
+    for (int j = 0; j < JC; ++j) bias[j] = 0.f;
+    if (p.bias) {  // uniform; such loads wait for every DMA under way
+#pragma unroll
+      for (int j = 0; j < JC; ++j) {
+        const int ch = ch0 + (EB == 4 ? 64 * (j >> 2) + (j & 3) : j);
+        bias[j] = p.bias[cg * p.bias_gstride + min(ch, p.N_out - 1)];
       }
-      const int cb = wn * (CHW / 32) + b;
+    }
+    // A buffer ends behind the tile's last row: what a lane holds past it is not
+    // stored (the range check counts the scalar offset of a row too)
+    const int rows_left = max(cmrows - row0, 0);
+    if constexpr (UP) {
+      const int64_t rb = static_cast<int64_t>(cm0) + row0;
+      const int ldo = static_cast<int>(p.ldo);
+      const rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(static_cast<uint8_t*>(p.out) + rb * p.ldo, 0, rows_left * ldo, 0x00027000);
+      // the scales of the wave's channels: four blocks a plane, TM rows of it
+      const int64_t plane0 = (cn0 + CHW * wn) / 128;
+      const rsrc_t osc = __builtin_amdgcn_make_buffer_rsrc(p.out_scale + plane0 * p.os_plane + rb * 4, 0, rows_left * 4, 0x00027000);
+      const bool in = ch0 < p.N_out;                // N_out % 32 == 0: whole blocks
+      const bool word = ch0 / 128 * 128 < p.N_out;  // blocks behind the last one of its word get scale 1
+      const int to = in ? eq * 4 * ldo + ch0 / 2 : kNowhere;
+      const int sto = word && ef % (32 / JC) == 0 ? eq * 16 + ch0 / 32 - static_cast<int>(plane0) * 4 : kNowhere;
+      if (p.bias) {  // uniform
 #pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        float y[2][4];
-        uint32_t m = 0u;
+        for (int j = 0; j < JC; ++j)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+          for (int i = 0; i < FM; ++i) acc[FN - JC + j][i] += bias[j];
+      }
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          float y[JC], m = 0.f;
+#pragma unroll
+          for (int j = 0; j < JC; ++j) {
+            if constexpr (SWIGLU) y[j] = silu(acc[j][i][v]) * acc[JC + j][i][v];
+            else y[j] = gelu_tail(acc[j][i][v]);
+            m = __builtin_elementwise_maximum(m, fabsf(y[j]));  // a NaN stays
+          }
+          uint32_t mb = quad_max(__float_as_uint(m) & 0x7FFFFFFFu);
+          if constexpr (JC == 4) mb = max(mb, static_cast<uint32_t>(dpp_i<kDppHalfMirror>(static_cast<int>(mb))));
+          // mx_scale_byte and mx_scale_value at once; the codes of a block whose
+          // scale is NaN do not matter
+          const int two = max(static_cast<int>(mb & 0x7F800000u) - 0x01000000, 0x00400000);
+          const float sv = __int_as_float(two);
+          uint32_t c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, y[0], y[1], sv, 0);
+          c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[2], y[3], sv, 1);
+          if constexpr (JC == 8) {
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[JC - 4], y[JC - 3], sv, 2);
+            c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, y[JC - 2], y[JC - 1], sv, 3);
+          }
+          const int byte = mb >= 0x7F800000u ? 255 : two >> 23;
+          const int rr = i * 16 + v;
+          if constexpr (JC == 4) __builtin_amdgcn_raw_buffer_store_b16(static_cast<uint16_t>(c), out, to, rr * ldo, 0);
+          else __builtin_amdgcn_raw_buffer_store_b32(c, out, to, rr * ldo, 0);
+          __builtin_amdgcn_raw_buffer_store_b8(static_cast<uint8_t>(in ? byte : 127), osc, sto, rr * 4, 0);
+        }
+    } else {
+      // whole vectors of a row, or its elements one by one (then the stores are
+      // not counted: waited for)
+      const bool whole = (static_cast<int64_t>(p.N_out) * EB) % 16 == 0 && (p.ldo * EB) % 16 == 0 &&
+                         reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+      auto value = [&](int j, int i, int v, float rs) {
+        const float y = acc[j][i][v] + bias[j];
+        return EPI == MX_GELU ? gelu_tail(y) : (EPI == MX_DOWN ? y * rs : y);
+      };
+      const int ldb = static_cast<int>(p.ldo) * EB;
+      const rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(static_cast<uint8_t*>(p.out) + (static_cast<int64_t>(cm0) + row0) * ldb, 0,
+                                                           rows_left * ldb, 0x00027000);
+      if (whole) {
+        // a row's offset in the lanes' registers, not in the scalar one, with which
+        // 16-byte stores gave wrong values here where the next vector operation
+        // wrote their data's registers (two of 16 columns, GELU)
+        constexpr int HS = EB == 4 ? JC / 4 : 1;
+        int to[HS];
+#pragma unroll
+        for (int h = 0; h < HS; ++h) to[h] = ch0 + 64 * h < p.N_out ? eq * 4 * ldb + (ch0 + 64 * h) * EB : kNowhere;
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            if constexpr (SWIGLU) y[j][v] = silu(acc[2 * b + j][i][v]) * (acc[JN + 2 * b + j][i][v] + bb[j][v]);
-            else y[j][v] = gelu_tail(acc[2 * b + j][i][v] + bb[j][v]);
-            m = amax_bits(m, y[j][v]);
-          }
-        const int byte = mx_scale_byte(quarters_max(m));
-        const int r = wm * TM + i * 16 + fr;
-        uint8_t* to = stg + r * (CH / 2) + (sw_chunk<CPR>(r, cb) << 4) + 2 * q;
+            const int rr = i * 16 + v, at = rr * ldb;
+            const float rs = EPI == MX_DOWN ? __shfl(rows_w[i / 4], (rr + 4 * eq) & 63) : 1.f;
+            if constexpr (EB == 4) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          *reinterpret_cast<uint16_t*>(to + 8 * j) = static_cast<uint16_t>(mx_codes4(y[j][0], y[j][1], y[j][2], y[j][3], byte));
-        if (q == 0) sst[r * CPR + cb] = static_cast<uint8_t>(byte);
+              for (int h = 0; h < HS; ++h) {
+                const f32x4 o = {value(4 * h, i, v, rs), value(4 * h + 1, i, v, rs), value(4 * h + 2, i, v, rs), value(4 * h + 3, i, v, rs)};
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), out, to[h] + at, 0, 2);
+              }
+            } else {
+              const u32x2 a = {pack_bf2(value(0, i, v, rs), value(1, i, v, rs)), pack_bf2(value(2, i, v, rs), value(3, i, v, rs))};
+              if constexpr (JC == 4) {
+                __builtin_amdgcn_raw_buffer_store_b64(a, out, to[0] + at, 0, 2);
+              } else {
+                const u32x4 o = {a.x, a.y, pack_bf2(value(JC - 4, i, v, rs), value(JC - 3, i, v, rs)),
+                                 pack_bf2(value(JC - 2, i, v, rs), value(JC - 1, i, v, rs))};
+                __builtin_amdgcn_raw_buffer_store_b128(o, out, to[0] + at, 0, 2);
+              }
+            }
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int r = row0 + i * 16 + 4 * eq + v;
+            const float rs = EPI == MX_DOWN ? __shfl(rows_w[i / 4], (r - row0) & 63) : 1.f;
+#pragma unroll
+            for (int j = 0; j < JC; ++j) {
+              const int ch = ch0 + (EB == 4 ? 64 * (j >> 2) + (j & 3) : j);
+              if (r < cmrows && ch < p.N_out) {
+                const int64_t at = (static_cast<int64_t>(cm0) + r) * p.ldo + ch;
+                if constexpr (EB == 4) static_cast<float*>(p.out)[at] = value(j, i, v, rs);
+                else static_cast<uint16_t*>(p.out)[at] = f2bf(value(j, i, v, rs));
+              }
+            }
+          }
+        wait_vmcnt<0>();
       }
     }
-    __syncthreads();
-    uint8_t* out = static_cast<uint8_t*>(p.out);
-    for (int e = tid; e < BM * CPR; e += NW * 64) {
-      const int r = e / CPR, c = e % CPR;
-      if (r < mrows && n0 + 32 * c < p.N_out) {
-        *reinterpret_cast<u32x4*>(out + static_cast<int64_t>(m0 + r) * p.ldo + n0 / 2 + 16 * c) =
-            *reinterpret_cast<const u32x4*>(stg + r * (CH / 2) + (sw_chunk<CPR>(r, c) << 4));
-        p.out_scale[static_cast<int64_t>(m0 + r) * p.ld_os + n0 / 32 + c] = sst[r * CPR + c];
-      }
-    }
-  } else {
-    float b4[FN][4];
-#pragma unroll
-    for (int j = 0; j < FN; ++j)
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const int n = n0 + wn * TN + j * 16 + 4 * q + v;
-        b4[j][v] = (bias && n < p.N_out) ? bias[n] : 0.f;
-      }
-    auto value = [&](int j, int i, float rs, float (&o)[4]) {
-#pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const float y = acc[j][i][v] + b4[j][v];
-        o[v] = EPI == MX_GELU ? gelu_tail(y) : (EPI == MX_DOWN ? y * rs : y);
-      }
-    };
-    // whole 16-byte chunks: the tile is staged in the ring (chunk c of row r at
-    // c ^ (r & 7)) and leaves in whole rows
-    constexpr int EB = ODT == SMOE_F32 ? 4 : 2, CPR = BN * EB / 16;
-    constexpr int PASS = BM * BN * EB <= NS * STAGE ? 1 : 2, FP = FM / PASS, TP = TM / PASS;
-    static_assert(BM / PASS * BN * EB <= NS * STAGE && FM % PASS == 0, "staging in the ring");
-    const bool whole = (static_cast<int64_t>(p.N_out) * EB) % 16 == 0 && (p.ldo * EB) % 16 == 0 &&
-                       reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
-    if (whole) {
-#pragma unroll
-      for (int h = 0; h < PASS; ++h) {
-        __syncthreads();  // every wave is done with the ring (or the pass before)
-#pragma unroll
-        for (int i = h * FP; i < (h + 1) * FP; ++i) {
-          const int r = wm * TM + i * 16 + fr, lr = wm * TP + (i - h * FP) * 16 + fr;
-          const float rs = EPI == MX_DOWN ? p.row_scale[m0 + min(r, mrows - 1)] : 1.f;
-#pragma unroll
-          for (int j = 0; j < FN; ++j) {
-            float o[4];
-            value(j, i, rs, o);
-            const int c4 = wn * (TN / 4) + j * 4 + q;  // group of four channels
-            if constexpr (ODT == SMOE_F32)
-              *reinterpret_cast<f32x4*>(ring + (lr * CPR + (c4 ^ (lr & 7))) * 16) = f32x4{o[0], o[1], o[2], o[3]};
-            else
-              *reinterpret_cast<u32x2*>(ring + (lr * CPR + ((c4 >> 1) ^ (lr & 7))) * 16 + (c4 & 1) * 8) =
-                  u32x2{pack_bf2(o[0], o[1]), pack_bf2(o[2], o[3])};
-          }
-        }
-        __syncthreads();
-        for (int e = tid; e < BM / PASS * CPR; e += NW * 64) {
-          const int lr = e / CPR, c = e % CPR;
-          const int r = lr / TP * TM + h * FP * 16 + lr % TP;
-          if (r < mrows && n0 + c * (16 / EB) < p.N_out) {
-            u32x4* to = reinterpret_cast<u32x4*>(static_cast<uint8_t*>(p.out) + ((m0 + static_cast<int64_t>(r)) * p.ldo + n0) * EB + c * 16);
-            const u32x4 o = *reinterpret_cast<const u32x4*>(ring + (lr * CPR + (c ^ (lr & 7))) * 16);
-            if constexpr (BM == 256 || EPI == MX_DOWN) __builtin_nontemporal_store(o, to);
-            else *to = o;
-          }
-        }
-      }
-      return;
-    }
-#pragma unroll
-    for (int j = 0; j < FN; ++j)
-#pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        const int r = wm * TM + i * 16 + fr;
-        if (r >= mrows) continue;
-        float o[4];
-        value(j, i, EPI == MX_DOWN ? p.row_scale[m0 + r] : 1.f, o);
-        store4<ODT>(p, m0 + r, n0 + wn * TN + j * 16 + 4 * q, o);
-      }
+    stored = true;
   }
+  wait_vmcnt<0>();  // nothing may land in the LDS of the workgroup that comes next
 }
 
-template <int EPI, int ODT, int BM, int BN, int WM, int WN, int NS>
-int go_tile(const MxGemm& a, hipStream_t s) {
-  constexpr int CH = EPI == MX_UP_SWIGLU ? BN / 2 : BN;
+// Tiles of 128 x 256, two workgroups a CU
+template <int EPI, int ODT>
+int go(const MxGemm& a, hipStream_t s) {
+  constexpr int BM = 128, CH = EPI == MX_UP_SWIGLU ? 128 : 256;
   const int rows = a.G > 0 ? a.max_rows : a.single_rows;
   // at most one partly filled row tile for every group with rows
   const int64_t tiles = (static_cast<int64_t>(rows) + BM - 1) / BM + (a.G > 0 ? std::min(a.G, rows) : 0);
-  const int64_t grid = tiles * ((static_cast<int64_t>(a.N_out) + CH - 1) / CH);
-  if (grid * 64 * WM * WN > 0xffffffffll) return SMOE_EINVAL;  // threads of a launch
-  SMOE_LAUNCH((k_gemm_mx<EPI, ODT, BM, BN, WM, WN, NS>), dim3(static_cast<unsigned>(grid)),
-              dim3(64 * WM * WN), 0, s, a);
+  const int64_t all = tiles * ((static_cast<int64_t>(a.N_out) + CH - 1) / CH);
+  if (all > 0x7fff0000ll) return SMOE_EINVAL;  // tiles are counted in 32 bits
+  const int64_t grid = std::min<int64_t>(all, std::max<int64_t>(device_cus() * 2 / 8 * 8, 8));
+  SMOE_LAUNCH((k_gemm_mx<EPI, ODT, BM, 256, 2, 2, 3, 2>), dim3(static_cast<unsigned>(grid)), dim3(256), 0, s, a);
   return rc();
-}
-
-// Tiles of BM rows and CH channels: over groups, as if the rows were spread
-// evenly (the host does not know the counts).
-int64_t tiles_of(const MxGemm& a, int BM, int CH) {
-  const int64_t strips = (static_cast<int64_t>(a.N_out) + CH - 1) / CH;
-  if (a.G == 0) return (static_cast<int64_t>(a.single_rows) + BM - 1) / BM * strips;
-  const int64_t per = (static_cast<int64_t>(a.max_rows) + a.G - 1) / a.G;
-  return std::min(a.G, a.max_rows) * ((per + BM - 1) / BM) * strips;
-}
-
-template <int EPI, int ODT>
-int go_dense(const MxGemm& a, hipStream_t s) {
-  const int64_t cus = device_cus();
-  if (tiles_of(a, 32, 64) <= cus) return go_tile<EPI, ODT, 32, 64, 2, 1, 4>(a, s);
-  if (tiles_of(a, 64, 128) <= cus) return go_tile<EPI, ODT, 64, 128, 2, 2, 3>(a, s);
-  if (tiles_of(a, 256, 256) * 8 >= cus * 5) return go_tile<EPI, ODT, 256, 256, 2, 4, 2>(a, s);
-  return go_tile<EPI, ODT, 128, 128, 2, 2, 2>(a, s);
-}
-
-template <int EPI>
-int go_grouped(const MxGemm& a, hipStream_t s) {
-  constexpr int O = SMOE_F32;
-  constexpr bool SW = EPI == MX_UP_SWIGLU;
-  const int64_t cus = device_cus(), per = (static_cast<int64_t>(a.max_rows) + a.G - 1) / a.G;
-  if (per >= 512 && tiles_of(a, 256, SW ? 128 : 256) * 8 >= cus * 5) return go_tile<EPI, O, 256, 256, 2, 4, 2>(a, s);
-  int BM = per <= 40 ? 32 : (per <= 112 ? 64 : 128);
-  while (BM > 32 && tiles_of(a, BM, 128) < cus) BM /= 2;
-  constexpr int BN = SW ? 256 : 128, WN = BN / 64;
-  if (BM == 32) return go_tile<EPI, O, 32, BN, 2, WN, 3>(a, s);
-  if (BM == 64) return go_tile<EPI, O, 64, BN, 2, WN, 2>(a, s);
-  return go_tile<EPI, O, 128, BN, 2, WN, 2>(a, s);
 }
 
 }  // namespace
 
-int launch_quantize_mxfp4(const MxQuant& q, hipStream_t s) {
+int launch_quantize_mxfp4(const MxQuant& q, const MxPlanes (&planes)[2], hipStream_t s) {
   if (q.rows < 0 || q.cols < 1 || q.ldx < q.cols || q.ld_codes < mx_code_pitch(q.cols) || q.ld_codes % 16 ||
-      q.ld_scale < mx_scale_pitch(q.cols) || q.ld_scale % 4 || reinterpret_cast<uintptr_t>(q.codes) % 16 ||
-      reinterpret_cast<uintptr_t>(q.scale) % 4)
+      q.s_row % 4 || q.s_word % 4 || reinterpret_cast<uintptr_t>(q.codes) % 16 || reinterpret_cast<uintptr_t>(q.scale) % 4)
     return SMOE_EINVAL;
   if (q.rows == 0) return SMOE_OK;
   const int npc = (q.cols - 1) / 128 + 1;
   if (q.ld_codes > 64 * static_cast<int64_t>(npc) || q.rows > ((1 << 28) - 16) / npc) return SMOE_EINVAL;
   const int64_t total = q.rows * npc, wgs = (total + 15) / 16;
+  const int64_t words = mx_plane_words(planes[0]) + mx_plane_words(planes[1]), all = wgs + (words + 255) / 256;
+  if (words > 0x7fffffffll || all * 256 > 0xffffffffll) return SMOE_EINVAL;  // threads of a launch
   return by_xdt(q.x_dtype, [&](auto xd) {
-    hipLaunchKernelGGL((k_quant_mx<decltype(xd)::value>), dim3(static_cast<unsigned>(wgs)), dim3(256), 0, s, q, npc, total);
+    hipLaunchKernelGGL((k_quant_mx<decltype(xd)::value>), dim3(static_cast<unsigned>(all)), dim3(256), 0, s, q, npc, total,
+                       static_cast<uint32_t>(wgs), planes[0], planes[1]);
     return rc();
   });
 }
@@ -421,21 +536,36 @@ int launch_dequantize_mxfp4(const uint8_t* codes, int64_t ld_codes, const uint8_
 int launch_gemm_mxfp4(const MxGemm& a, hipStream_t s) {
   const int rows = a.G > 0 ? a.max_rows : a.single_rows;
   if (rows <= 0) return SMOE_OK;
-  const int64_t pitch = mx_code_pitch(a.K), sp = mx_scale_pitch(a.K);
-  if (a.K < 1 || a.N_out < 1 || a.ldw < pitch || a.ldw % 16 || a.w_gstride % 16 || a.ld_ws < sp || a.ld_ws % 4 || a.ws_gstride % 4)
-    return SMOE_EINVAL;
-  if (!a.x_float && (a.ldx < pitch || a.ldx % 16 || a.ld_xs < sp || a.ld_xs % 4)) return SMOE_EINVAL;
+  const int64_t pitch = mx_code_pitch(a.K);
+  if (a.K < 1 || a.N_out < 1 || a.ldw < pitch || a.ldw % 16 || a.w_gstride % 16 || a.ws_gstride % 4) return SMOE_EINVAL;
+  if (!a.x_float && (a.ldx < pitch || a.ldx % 16 || a.xs_plane % 4)) return SMOE_EINVAL;
   if (gemm_mx_few_fits(a)) return launch_gemm_mx_few(a, s);
   if (a.x_float) return SMOE_EINVAL;
+  if (a.ws_plane == 0) return launch_gemm_mx_mid(a, s);
+  if (a.ws_plane % 16 || a.xs_plane % 16) return SMOE_EINVAL;
+  // 32-bit offsets: weight rows of a tile (SwiGLU: and those of the up half), rows
+  // of X of a tile (gathered: all), a wave's rows of the output
+  const bool up = a.epi == MX_UP_GELU || a.epi == MX_UP_SWIGLU;
+  const int64_t lim = (1ll << 32) - (1 << 20);
+  if (a.ldw > lim / 512 || a.ldx > lim / 512 || a.N_out > (1 << 22) ||
+      (a.epi == MX_UP_SWIGLU && (a.N_out + 256ll) * a.ldw > lim) || (up && a.x_rows > lim / a.ldx))
+    return SMOE_EINVAL;
   const bool f32 = a.out_dtype == SMOE_F32;
   switch (a.epi) {
-    case MX_LINEAR: return f32 ? go_dense<MX_LINEAR, SMOE_F32>(a, s) : go_dense<MX_LINEAR, SMOE_BF16>(a, s);
-    case MX_GELU: return f32 ? go_dense<MX_GELU, SMOE_F32>(a, s) : go_dense<MX_GELU, SMOE_BF16>(a, s);
-    case MX_UP_GELU: return go_grouped<MX_UP_GELU>(a, s);
-    case MX_UP_SWIGLU: return go_grouped<MX_UP_SWIGLU>(a, s);
-    case MX_DOWN: return go_grouped<MX_DOWN>(a, s);
+    case MX_LINEAR: return f32 ? go<MX_LINEAR, SMOE_F32>(a, s) : go<MX_LINEAR, SMOE_BF16>(a, s);
+    case MX_GELU: return f32 ? go<MX_GELU, SMOE_F32>(a, s) : go<MX_GELU, SMOE_BF16>(a, s);
+    case MX_UP_GELU: return go<MX_UP_GELU, SMOE_F32>(a, s);
+    case MX_UP_SWIGLU: return go<MX_UP_SWIGLU, SMOE_F32>(a, s);
+    case MX_DOWN: return go<MX_DOWN, SMOE_F32>(a, s);
     default: return SMOE_EINVAL;
   }
 }
+
+// From five tiles of 256 x 256 for every eight of the 256 CUs on, and 512 rows a
+// group (a workspace's size goes by it: the same on every device)
+bool mx_large_linear(int N, int N_out) {
+  return (static_cast<int64_t>(N) + 255) / 256 * ((static_cast<int64_t>(N_out) + 255) / 256) >= 160;
+}
+bool mx_large_experts(int N, int K, int E) { return static_cast<int64_t>(N) * K >= 512ll * E; }
 
 }  // namespace smoe

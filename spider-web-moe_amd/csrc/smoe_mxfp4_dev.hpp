@@ -70,8 +70,21 @@ __device__ __forceinline__ void mx_quant_piece(const MxQuant& q, int npc, int64_
   uint32_t scales;
   const uint32_t codes = mx_quant128(v, scales);
   if (b >= total) return;
-  if (l16 == 0) *reinterpret_cast<uint32_t*>(q.scale + row * q.ld_scale + 4 * kb) = scales;
+  if (l16 == 0) *reinterpret_cast<uint32_t*>(q.scale + row * q.s_row + kb * q.s_word) = scales;
   if (c / 2 < q.ld_codes) *reinterpret_cast<uint32_t*>(q.codes + row * q.ld_codes + c / 2) = codes;
+}
+
+// Word i of the planes, rows fastest
+inline __host__ __device__ int64_t mx_plane_words(const MxPlanes& p) {
+  return static_cast<int64_t>(p.groups) * p.rows * ((p.blocks + 3) / 4);
+}
+__device__ __forceinline__ void mx_plane_word(const MxPlanes& p, uint32_t i) {
+  const uint32_t rest = i / static_cast<uint32_t>(p.rows), r = i - rest * p.rows, nd = (p.blocks + 3) / 4;
+  const uint32_t g = rest / nd, s = rest - g * nd;
+  uint32_t w = *reinterpret_cast<const uint32_t*>(p.src + (static_cast<int64_t>(g) * p.rows + r) * p.ld + 4 * s);
+  const int left = p.blocks - 4 * static_cast<int>(s);
+  if (left < 4) w = (w & ((1u << 8 * left) - 1u)) | (0x7F7F7F7Fu << 8 * left);
+  p.dst[static_cast<int64_t>(rest) * (mx_plane_pitch(p.rows) / 4) + r] = w;
 }
 
 // The matrix instruction on 128 k: lane l holds 32 codes of row l % 16 of each

@@ -127,7 +127,7 @@ SIGNATURES = {
                                             _vp, _vp, _vp]),
     "smoe_quantize_mxfp4": (_c_int, [_vp, _c_int, _i64, _c_int, _i64, _vp, _i64, _vp, _i64, _vp]),
     "smoe_dequantize_mxfp4": (_c_int, [_vp, _i64, _vp, _i64, _i64, _c_int, _vp, _c_int, _vp]),
-    "smoe_linear_mxfp4_workspace_bytes": (_sz, [_c_int, _c_int]),
+    "smoe_linear_mxfp4_workspace_bytes": (_sz, [_c_int, _c_int, _c_int]),
     "smoe_linear_mxfp4": (_c_int, [_vp, _c_int, _i64, _c_int, _c_int, _vp, _i64, _vp, _i64, _vp,
                                    _c_int, _c_int, _vp, _c_int, _vp, _sz, _vp]),
     "smoe_expert_delta_mxfp4_workspace_bytes": (_sz, [ctypes.POINTER(SmoeExpertsMxfp4), _c_int,

@@ -398,7 +398,7 @@ def _linear_mxfp4(x, codes, scale, bias, act):
     out = torch.empty(*lead, n_out, dtype=out_dtype, device=dev)
     n = out.numel() // n_out if n_out else 0
     if n:
-        need = nat.lib().smoe_linear_mxfp4_workspace_bytes(n, k)
+        need = nat.lib().smoe_linear_mxfp4_workspace_bytes(n, k, n_out)
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         nat.launch(dev, "smoe_linear_mxfp4", x.data_ptr(), nat.float_code(x.dtype), ldx, n, k,
                    codes.data_ptr(), ldw, scale.data_ptr(), ld_ws, nat.ptr(bias), n_out, _ACT[act],

@@ -79,11 +79,11 @@ def test_linear_refusals(lib):
                 dict(act=2), dict(x=None), dict(w=None), dict(ws=None), dict(out=None), dict(wk=None), dict(w=FAKE + 4),
                 dict(ws=FAKE + 1), dict(wk=FAKE + 1), dict(n=1 << 28)):
         assert go(**bad) == 1, bad
-    need = lib.smoe_linear_mxfp4_workspace_bytes(40, 100)
+    need = lib.smoe_linear_mxfp4_workspace_bytes(40, 100, 30)
     assert need >= 40 * 64 + 40 * 4 and go(wb=need - 1) == 3
     assert go(n=0) == 0
-    assert lib.smoe_linear_mxfp4_workspace_bytes(4, 100) == 0  # a few rows are quantized by the product itself
-    assert lib.smoe_linear_mxfp4_workspace_bytes(0, 100) == 0
+    assert lib.smoe_linear_mxfp4_workspace_bytes(4, 100, 30) == 0  # a few rows are quantized by the product itself
+    assert lib.smoe_linear_mxfp4_workspace_bytes(0, 100, 30) == 0
 
 
 def test_expert_refusals(lib):
