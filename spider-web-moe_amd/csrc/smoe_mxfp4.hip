@@ -541,6 +541,7 @@ int launch_gemm_mxfp4(const MxGemm& a, hipStream_t s) {
   if (!a.x_float && (a.ldx < pitch || a.ldx % 16 || a.xs_plane % 4)) return SMOE_EINVAL;
   if (gemm_mx_few_fits(a)) return launch_gemm_mx_few(a, s);
   if (a.x_float) return SMOE_EINVAL;
+  if (gemm_mx_stream_fits(a)) return launch_gemm_mx_stream(a, s);
   if (a.ws_plane == 0) return launch_gemm_mx_mid(a, s);
   if (a.ws_plane % 16 || a.xs_plane % 16) return SMOE_EINVAL;
   // 32-bit offsets: weight rows of a tile (SwiGLU: and those of the up half), rows

@@ -92,6 +92,9 @@ int launch_gemm_mx_mid(const MxGemm& g, hipStream_t s);  // smoe_mxfp4_mid.hip
 // the dense products of a few rows (smoe_mxfp4_few.hip)
 bool gemm_mx_few_fits(const MxGemm& g);
 int launch_gemm_mx_few(const MxGemm& g, hipStream_t s);
+// grouped products of decode steps (smoe_mxfp4_few.hip)
+bool gemm_mx_stream_fits(const MxGemm& g);
+int launch_gemm_mx_stream(const MxGemm& g, hipStream_t s);
 // whether a linear product of N rows takes x_float
 bool mx_linear_quantizes_inside(int N, int K);
 // whether a product runs on large tiles, with scales in planes

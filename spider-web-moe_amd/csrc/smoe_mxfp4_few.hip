@@ -158,6 +158,108 @@ __global__ __launch_bounds__(256, 4) void k_mx_few(const MxGemm p) {
   store4<ODT>(p, m0 + r, n, o);
 }
 
+// -------------------------------------------------- decode-size experts ----
+// Grouped products of decode steps, a few rows a group.  The weights' bytes bound
+// them, and a workgroup of few rows has too little to do between two barriers of
+// a staged pipeline: here a strip of a group's channels (32 for the up products,
+// a block of activations; 16 for the down product) is a workgroup, its four waves
+// take every fourth 256 of K, and weights and rows go straight into registers,
+// D pieces at once, without a barrier; the waves' sums are added through LDS in
+// wave order.  16 rows at a time: a group with more reads its strip again, from
+// the L2.  64 tokens, 2 of 16 experts of 1024 x 2816 (SwiGLU): 14.4 us the up
+// product, 7.7 the down one (staged: 15.4 and 9.0); non-temporal weight loads 15.2
+// and 8.8; blocks q and q + 4 a lane, so that a load covers whole 64-byte pieces,
+// 17.2 and 8.2.
+template <int EPI>
+__global__ __launch_bounds__(256, 4) void k_mx_stream(const MxGemm p) {
+  constexpr bool SWIGLU = EPI == MX_UP_SWIGLU, UP = EPI == MX_UP_GELU || SWIGLU;
+  constexpr int NT = SWIGLU ? 4 : (UP ? 2 : 1), CH = UP ? 32 : 16, D = SWIGLU ? 1 : (UP ? 2 : 3), NW = 4;
+  __shared__ __attribute__((aligned(16))) float red[NW * NT * 256];
+  const int strips = p.N_out / CH;  // N_out % 32 == 0
+  const int g = static_cast<int>(blockIdx.x) / strips, n0 = (static_cast<int>(blockIdx.x) - g * strips) * CH;
+  const int lo = p.grp_off[g], hi = p.grp_off[g + 1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int q = lane >> 4, l16 = lane & 15;
+  const int nb = (p.K + kMxBlock - 1) / kMxBlock, KS = (nb + 7) / 8;
+  const uint8_t *wrow[NT], *wsrow[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {  // SwiGLU: two tiles of gate rows, two of up rows
+    const int64_t r = n0 + 16 * (t & 1) + l16 + (t >= 2 ? p.N_out : 0);
+    wrow[t] = p.W + g * p.w_gstride + r * p.ldw;
+    wsrow[t] = p.ws + g * p.ws_gstride + r * p.ld_ws;
+  }
+  for (int m0 = lo; m0 < hi; m0 += 16) {
+    const int mrows = min(16, hi - m0);
+    const int r = m0 + min(l16, mrows - 1);  // rows past the end: a valid one, never stored
+    const int64_t xr = p.a_rows ? p.a_rows[r] : r;
+    const uint8_t *xrow = p.X + xr * p.ldx, *xsrow = p.xs + xr * p.ld_xs;
+    f32x4 acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int b0 = wave; b0 < KS; b0 += D * NW) {
+      Piece w[D][NT], x[D];
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        const int b = b0 + d * NW;
+        if (b >= KS) break;  // uniform
+#pragma unroll
+        for (int t = 0; t < NT; ++t) w[d][t] = load_piece(wrow[t], wsrow[t], b, q, nb);
+        x[d] = load_piece(xrow, xsrow, b, q, nb);
+      }
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        const int b = b0 + d * NW;
+        if (b >= KS) break;  // uniform
+        if (8 * b + 8 > nb) x[d] = cut_piece(x[d], b, q, nb);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[t] = product(w[d][t], x[d], acc[t]);
+      }
+    }
+    if (m0 > lo) __syncthreads();  // the rows before are read
+#pragma unroll
+    for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(red + (wave * NT + t) * 256 + lane * 4) = acc[t];
+    __syncthreads();
+    if (wave) continue;
+    f32x4 sum[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      sum[t] = *reinterpret_cast<const f32x4*>(red + t * 256 + lane * 4);
+#pragma unroll
+      for (int u = 1; u < NW; ++u) sum[t] += *reinterpret_cast<const f32x4*>(red + (u * NT + t) * 256 + lane * 4);
+    }
+    // lane: channels 4 q + v of each tile, of row l16
+    const int64_t row = m0 + l16;
+    const bool live = l16 < mrows;
+    const float* bias = p.bias ? p.bias + g * p.bias_gstride + n0 + 4 * q : nullptr;
+    if constexpr (UP) {
+      float y[2][4], m = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const float b = bias ? bias[16 * h + v] : 0.f;
+          if constexpr (SWIGLU) y[h][v] = silu(sum[h][v]) * (sum[NT - 2 + h][v] + b);
+          else y[h][v] = gelu_tail(sum[h][v] + b);
+          m = __builtin_elementwise_maximum(m, fabsf(y[h][v]));  // a NaN stays
+        }
+      const int byte = mx_scale_byte(quarters_max(__float_as_uint(m) & 0x7FFFFFFFu));
+      if (!live) continue;
+      uint8_t* to = static_cast<uint8_t*>(p.out) + row * p.ldo + n0 / 2 + 2 * q;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<uint16_t*>(to + 8 * h) = static_cast<uint16_t>(mx_codes4(y[h][0], y[h][1], y[h][2], y[h][3], byte));
+      if (q == 0) p.out_scale[row * p.ld_os + n0 / 32] = static_cast<uint8_t>(byte);
+    } else {
+      if (!live) continue;
+      const float rs = p.row_scale[row];
+      f32x4 o;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) o[v] = (sum[0][v] + (bias ? bias[v] : 0.f)) * rs;
+      *reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + row * p.ldo + n0 + 4 * q) = o;
+    }
+  }
+}
+
 // ------------------------------------------------- a few tokens' experts ----
 // At most kTokensMax (token, slot) entries: the whole expert step in two launches
 // that keep the dispatch plan in registers and quantize their own operands.
@@ -375,6 +477,28 @@ int launch_gemm_mx_few(const MxGemm& a, hipStream_t s) {
   if (a.epi == MX_LINEAR) return f32 ? go_rows<MX_LINEAR, SMOE_F32>(a, s) : go_rows<MX_LINEAR, SMOE_BF16>(a, s);
   if (a.epi == MX_GELU) return f32 ? go_rows<MX_GELU, SMOE_F32>(a, s) : go_rows<MX_GELU, SMOE_BF16>(a, s);
   return SMOE_EINVAL;
+}
+
+// Up to 8 rows a group on average.  Both products and the plan, us, streamed and
+// staged, tokens spread evenly and unevenly (a group over 16 rows reads its weights
+// again): 16 experts of 1024 x 2816, SwiGLU, 48 tokens (6 rows) 26.6 / 26.6 and
+// 29.6, 64 tokens (8 rows) 27.3 / 30.7 and 29.6, 80 tokens 30.6 / 31.3 and 29.8;
+// 32 experts of 1024 x 1408, 64 tokens (8 rows) 24.3 / 25.5 and 25.3, 96 tokens
+// 27.6 and 25.4; 64 experts of 2048 x 1408, 64 tokens (2 rows) 40.0 and 45.1,
+// 256 tokens (8 rows) 50.5 / 56.0 and 49.8.
+bool gemm_mx_stream_fits(const MxGemm& a) {
+  return a.G > 0 && a.ws_plane == 0 && a.max_rows <= 8ll * a.G;
+}
+
+int launch_gemm_mx_stream(const MxGemm& a, hipStream_t s) {
+  const bool up = a.epi == MX_UP_GELU || a.epi == MX_UP_SWIGLU;
+  const int64_t grid = static_cast<int64_t>(a.G) * (a.N_out / (up ? 32 : 16));
+  if (a.N_out % 32 || (!up && a.epi != MX_DOWN) || grid * 256 > 0xffffffffll) return SMOE_EINVAL;  // threads of a launch
+  const dim3 g(static_cast<unsigned>(grid)), b(256);
+  if (a.epi == MX_UP_GELU) SMOE_LAUNCH((k_mx_stream<MX_UP_GELU>), g, b, 0, s, a);
+  else if (a.epi == MX_UP_SWIGLU) SMOE_LAUNCH((k_mx_stream<MX_UP_SWIGLU>), g, b, 0, s, a);
+  else SMOE_LAUNCH((k_mx_stream<MX_DOWN>), g, b, 0, s, a);
+  return rc();
 }
 
 int launch_prep_mx(const PrepArgs& a, const MxQuant& q, hipStream_t s) {
