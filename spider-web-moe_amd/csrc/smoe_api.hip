@@ -1430,7 +1430,7 @@ struct BalanceWs {
   size_t part_p, part_c, total;
 };
 BalanceWs balance_ws(int S, int T, int E) {
-  const size_t n = static_cast<size_t>(S) * balance_chunks(S, T);
+  const size_t n = static_cast<size_t>(S) * balance_chunks(S, T, E);
   BalanceWs w;
   Bump z;
   w.part_p = z.take(n * E * 4);
@@ -1442,7 +1442,7 @@ BalanceWs balance_ws(int S, int T, int E) {
 }  // namespace
 
 SMOE_API size_t smoe_balance_loss_workspace_bytes(int S, int T, int E) {
-  if (check_balance(SMOE_F32, S, T, E, SMOE_SCORE_SOFTMAX) != SMOE_OK || S == 0 || balance_chunks(S, T) == 1) return 0;
+  if (check_balance(SMOE_F32, S, T, E, SMOE_SCORE_SOFTMAX) != SMOE_OK || S == 0 || balance_chunks(S, T, E) == 1) return 0;
   return balance_ws(S, T, E).total;
 }
 

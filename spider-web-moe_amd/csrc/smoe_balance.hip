@@ -55,25 +55,43 @@ __device__ __forceinline__ void load_row(const void* z, int64_t base, int e0, in
   }
 }
 
-// p of a token whose experts lie in SEG lanes, V each.  sigmoid(z) =
-// exp(min(z, 0)) / (1 + exp(-|z|)) with the largest min(z, 0) taken out first:
-// the shares of far negative logits are those of their exponentials.
+__device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
+
+// p of a token whose experts lie in SEG lanes, V each, and with sigmoid also
+// 1 - sigmoid(z).  t = exp(-|z|) gives both sigmoid(z) and 1 - sigmoid(z): they
+// are 1 / (1 + t) and t / (1 + t).  A token whose logits are all below -16 takes
+// the largest out first, exp(z - m) / (1 + t): the shares of far negative logits
+// are those of their exponentials (above, a t that is 0 has a share below e^-71).
 template <int SEG, int V>
-__device__ __forceinline__ void shares(const float (&z)[V], bool sigmoid, float (&p)[V]) {
+__device__ __forceinline__ void shares(const float (&z)[V], bool sigmoid, float (&p)[V], float (&rest)[V]) {
   float m = -INFINITY;  // of the numbers: a NaN makes the sum, and so every share, NaN
 #pragma unroll
   for (int v = 0; v < V; ++v) m = fmaxf(m, z[v]);
   m = seg_max<SEG>(m);
-  if (sigmoid) m = fminf(m, 0.f);  // uniform
   float sum = 0.f;
+  if (sigmoid) {  // uniform
+    float one[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
-    const float x = sigmoid ? fminf(z[v], 0.f) : z[v];
-    float e = expf(x - m);
-    if (sigmoid) e = __fdividef(e, 1.f + expf(-fabsf(z[v])));
-    p[v] = z[v] == -INFINITY ? 0.f : e;
-    sum += p[v];
+    for (int v = 0; v < V; ++v) {
+      const float t = exp_of(-fabsf(z[v]));
+      one[v] = __builtin_amdgcn_rcpf(1.f + t);
+      const float far = t * one[v];
+      p[v] = z[v] > 0.f ? one[v] : far;
+      rest[v] = z[v] > 0.f ? far : one[v];
+    }
+    if (__builtin_amdgcn_ballot_w64(m < -16.f)) {  // uniform
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float e = z[v] == -INFINITY ? 0.f : exp_of(z[v] - m) * one[v];
+        p[v] = m < -16.f ? e : p[v];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < V; ++v) p[v] = z[v] == -INFINITY ? 0.f : exp_of(z[v] - m);
   }
+#pragma unroll
+  for (int v = 0; v < V; ++v) sum += p[v];
   sum = seg_sum<SEG>(sum);
   const float r = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
@@ -155,12 +173,16 @@ __device__ __forceinline__ void finish(const BalanceArgs& a, int seq, int chunks
   }
 }
 
-// `rows` tokens of a sequence a workgroup, 64 / SEG a wave at a time; the
-// shares' sums stay in registers, the counts in LDS.  With one chunk a sequence
-// the workgroup goes on to the loss itself.
+// `rows` tokens of a sequence a workgroup, kTokens * 64 / SEG a wave at a time
+// (their logits are loaded together); the shares' sums stay in registers, the
+// counts in LDS.  With one chunk a sequence the workgroup goes on to the loss
+// itself.  The logits are read once; latency and the exponentials bound it.  8
+// sequences of 2048 tokens over 256 experts, sigmoid: 9.7 us, 1.7 TB/s (a token at
+// a time in 128 workgroups 36.6; accurate expf and a second exponential for
+// the sigmoid 11.9).
 template <int DT, int SEG, int V>
 __global__ __launch_bounds__(256) void k_balance_part(const BalanceArgs a) {
-  constexpr int PW = 64 / SEG;  // tokens of a wave
+  constexpr int PW = 64 / SEG, kTokens = SEG == 16 ? 2 : 4;
   __shared__ float s_p[4 * PW * SEG * V];
   __shared__ int32_t s_c[257];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -180,16 +202,24 @@ __global__ __launch_bounds__(256) void k_balance_part(const BalanceArgs a) {
 #pragma unroll
   for (int v = 0; v < V; ++v) sum[v] = 0.f;
   int n = 0;
-  for (int t = t0 + wave * PW; t < t1; t += 4 * PW) {  // uniform
-    const int mine = t + lane / SEG;
-    const int64_t at = first + min(mine, t1 - 1);
-    const bool on = mine < t1 && (!a.mask || a.mask[at]);
-    float z[V], p[V];
-    load_row<DT, V>(a.logits, at * E, e0, E, a.vec, z);
-    shares<SEG, V>(z, a.sigmoid, p);
+  for (int t = t0 + wave * PW; t < t1; t += 4 * PW * kTokens) {  // uniform
+    float z[kTokens][V];
+    bool on[kTokens];
 #pragma unroll
-    for (int v = 0; v < V; ++v) sum[v] += on ? p[v] : 0.f;  // a masked token's may be NaN
-    n += on && lane % SEG == 0 ? 1 : 0;
+    for (int u = 0; u < kTokens; ++u) {
+      const int mine = t + u * 4 * PW + lane / SEG;
+      const int64_t at = first + min(mine, t1 - 1);
+      on[u] = mine < t1 && (!a.mask || a.mask[at]);
+      load_row<DT, V>(a.logits, at * E, e0, E, a.vec, z[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kTokens; ++u) {
+      float p[V], rest[V];
+      shares<SEG, V>(z[u], a.sigmoid, p, rest);
+#pragma unroll
+      for (int v = 0; v < V; ++v) sum[v] += on[u] ? p[v] : 0.f;  // a masked token's may be NaN
+      n += on[u] && lane % SEG == 0 ? 1 : 0;
+    }
   }
   if (n) atomicAdd(&s_c[E], n);
 #pragma unroll
@@ -214,6 +244,9 @@ __global__ __launch_bounds__(1024) void k_balance_loss(const BalanceArgs a) {
   finish<1024>(a, blockIdx.x, a.chunks, a.part_p + at * a.E, a.part_c + at * (a.E + 1));
 }
 
+// Logits in, gradients out, 64 / SEG tokens a wave: bound by both.  16384 tokens
+// over 256 experts, f32: 10.0 us, 3.4 TB/s (with expf and a division for
+// 1 - sigmoid 14.7).
 template <int DT, int SEG, int V>
 __global__ __launch_bounds__(256) void k_balance_bwd(const BalanceArgs a, const float* __restrict__ d_loss,
                                                      void* __restrict__ d_logits) {
@@ -225,12 +258,12 @@ __global__ __launch_bounds__(256) void k_balance_bwd(const BalanceArgs a, const 
   const int64_t mine = t0 + lane / SEG, at = mine < N ? mine : N - 1;
   const int64_t seq = at / a.T;
   const bool on = !a.mask || a.mask[at];
-  float z[V], p[V], u[V];
+  float z[V], p[V], rest[V], u[V];
   load_row<DT, V>(a.logits, at * E, e0, E, a.vec, z);
 #pragma unroll
   for (int v = 0; v < V; ++v) u[v] = e0 + v < E ? a.slope[seq * E + e0 + v] : 0.f;
   const float dl = d_loss[seq];
-  shares<SEG, V>(z, a.sigmoid, p);
+  shares<SEG, V>(z, a.sigmoid, p, rest);
   float dot = 0.f;
 #pragma unroll
   for (int v = 0; v < V; ++v) dot = fmaf(p[v], u[v], dot);
@@ -239,7 +272,7 @@ __global__ __launch_bounds__(256) void k_balance_bwd(const BalanceArgs a, const 
 #pragma unroll
   for (int v = 0; v < V; ++v) {
     d[v] = dl * (p[v] * (u[v] - dot));
-    if (a.sigmoid) d[v] = z[v] == INFINITY ? 0.f : __fdividef(d[v], 1.f + expf(z[v]));
+    if (a.sigmoid) d[v] *= rest[v];
     d[v] = on ? d[v] : 0.f;
   }
   if (mine >= N || e0 >= E) return;
@@ -295,22 +328,29 @@ bool vec4(const void* p, int dt, int E) {
 
 }  // namespace
 
-// Tokens of a workgroup: at least 128, so that a short batch is one launch, and
-// about 512 workgroups over the batch.
-int balance_rows(int64_t S, int64_t T) {
-  const int64_t even = (S * T + 511) / 512;
-  return static_cast<int>(std::max<int64_t>(128, even));
+// Tokens of a workgroup.  A short sequence is one launch, up to two times what a
+// workgroup has in flight: 128 tokens of up to 64 experts (one launch 7.2 us, two
+// 7.7), 64 of up to 128 (7.0 and 7.5), 32 of up to 256 (7.2 and 7.9; 64 tokens
+// 10.9 and 8.0).  Else about 512 workgroups over the batch, and at least 32
+// tokens each: 8 sequences of 2048 tokens over 256 experts, both kernels, 13.4 us
+// (16 tokens each 14.1, 64 tokens 22.8).  At most 256 chunks a sequence, since one workgroup
+// adds them up: 16384 tokens over 256 experts as one sequence 22.1 us (512 chunks
+// 23.6, 128 chunks 32.2 before the shares had one exponential).
+int balance_rows(int64_t S, int64_t T, int E) {
+  const int64_t one = 2048 / (E <= 64 ? 16 : (E <= 128 ? 32 : 64));
+  if (T <= one) return static_cast<int>(one);
+  return static_cast<int>(std::max({int64_t{32}, (S * T + 511) / 512, (T + 255) / 256}));
 }
-int balance_chunks(int64_t S, int64_t T) {
-  const int64_t r = balance_rows(S, T);
+int balance_chunks(int64_t S, int64_t T, int E) {
+  const int64_t r = balance_rows(S, T, E);
   return static_cast<int>(std::max<int64_t>(1, (T + r - 1) / r));
 }
 
 int launch_balance_loss(const void* logits, int dt, int S, int T, int E, int K, int sigmoid, const int32_t* idx,
                         const uint8_t* mask, float* loss, int32_t* counts, float* slope, float* part_p,
                         int32_t* part_c, hipStream_t s) {
-  const BalanceArgs a{logits, idx, mask, S, T, E, K, sigmoid != 0, vec4(logits, dt, E), balance_rows(S, T),
-                      balance_chunks(S, T), part_p, part_c, loss, counts, slope};
+  const BalanceArgs a{logits, idx, mask, S, T, E, K, sigmoid != 0, vec4(logits, dt, E), balance_rows(S, T, E),
+                      balance_chunks(S, T, E), part_p, part_c, loss, counts, slope};
   const int64_t grid = static_cast<int64_t>(S) * a.chunks;
   if (grid * 256 > 0xffffffffll) return SMOE_EINVAL;  // threads of a launch
   const int r = by_shape(dt, E, [&](auto d, auto seg, auto v) {

@@ -244,7 +244,7 @@ int launch_select_groups_bwd(const void* logits, int zdt, int N, int E, int K, i
 // Balance loss and its gradient (smoe_balance.hip); the entry points check the
 // shapes.  Workspace: part_p f32 [S * chunks, E], part_c i32 [S * chunks, E + 1]
 // where a sequence takes more than one chunk.
-int balance_chunks(int64_t S, int64_t T);
+int balance_chunks(int64_t S, int64_t T, int E);
 int launch_balance_loss(const void* logits, int dt, int S, int T, int E, int K, int sigmoid, const int32_t* idx,
                         const uint8_t* mask, float* loss, int32_t* counts, float* slope, float* part_p,
                         int32_t* part_c, hipStream_t s);
