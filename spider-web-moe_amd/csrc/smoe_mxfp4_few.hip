@@ -6,6 +6,8 @@
 #include "smoe_small_plan.hpp"
 
 namespace smoe {
+
+int device_cus();
 namespace {
 
 // A lane's part of 256 k of a row: blocks 2 q and 2 q + 1 (q = lane / 16; the
@@ -167,9 +169,8 @@ __global__ __launch_bounds__(256, 4) void k_mx_few(const MxGemm p) {
 // D pieces at once, without a barrier; the waves' sums are added through LDS in
 // wave order.  16 rows at a time: a group with more reads its strip again, from
 // the L2.  64 tokens, 2 of 16 experts of 1024 x 2816 (SwiGLU): 14.4 us the up
-// product, 7.7 the down one (staged: 15.4 and 9.0); non-temporal weight loads 15.2
-// and 8.8; blocks q and q + 4 a lane, so that a load covers whole 64-byte pieces,
-// 17.2 and 8.2.
+// product, 7.8 the down one; non-temporal weight loads 15.2 and 8.8; blocks q and
+// q + 4 a lane, so that a load covers whole 64-byte pieces, 17.2 and 8.2.
 template <int EPI>
 __global__ __launch_bounds__(256, 4) void k_mx_stream(const MxGemm p) {
   constexpr bool SWIGLU = EPI == MX_UP_SWIGLU, UP = EPI == MX_UP_GELU || SWIGLU;
@@ -479,15 +480,20 @@ int launch_gemm_mx_few(const MxGemm& a, hipStream_t s) {
   return SMOE_EINVAL;
 }
 
-// Up to 8 rows a group on average.  Both products and the plan, us, streamed and
-// staged, tokens spread evenly and unevenly (a group over 16 rows reads its weights
-// again): 16 experts of 1024 x 2816, SwiGLU, 48 tokens (6 rows) 26.6 / 26.6 and
-// 29.6, 64 tokens (8 rows) 27.3 / 30.7 and 29.6, 80 tokens 30.6 / 31.3 and 29.8;
-// 32 experts of 1024 x 1408, 64 tokens (8 rows) 24.3 / 25.5 and 25.3, 96 tokens
-// 27.6 and 25.4; 64 experts of 2048 x 1408, 64 tokens (2 rows) 40.0 and 45.1,
-// 256 tokens (8 rows) 50.5 / 56.0 and 49.8.
+// Up to 4 rows a group on average, and up to 8 where the staged kernel's tiles (32
+// rows, 64 channels of SwiGLU or 128) do not give every CU one.  Both products and
+// the plan, us, streamed and staged: 64 experts of 2048 x 1408, 64 tokens (2 rows)
+// 40.1 and 41.5, 128 tokens (4 rows) 45.5 and 46.8; 32 experts of 1024 x 1408, 32
+// tokens (4 rows) 23.7 and 25.2; 16 experts of 1024 x 2816, SwiGLU, 32 tokens (4
+// rows) 26.3 and 26.5, 64 tokens (8 rows) 30.8 and 27.0, but only the down product,
+// of 128 tiles, streamed 26.6; 12 experts of 544 x 1184, 32 tokens (8 rows) 15.4
+// and 18.5; 8 experts of 256 x 512, 32 tokens (8 rows) 11.8 and 15.3, 64 tokens (16
+// rows) 16.2 and 15.2.
 bool gemm_mx_stream_fits(const MxGemm& a) {
-  return a.G > 0 && a.ws_plane == 0 && a.max_rows <= 8ll * a.G;
+  if (a.G < 1 || a.ws_plane != 0) return false;
+  const int ch = a.epi == MX_UP_SWIGLU ? 64 : 128;
+  const int64_t tiles = static_cast<int64_t>(std::min(a.G, a.max_rows)) * ((a.N_out - 1) / ch + 1);
+  return a.max_rows <= (tiles <= device_cus() ? 8ll : 4ll) * a.G;
 }
 
 int launch_gemm_mx_stream(const MxGemm& a, hipStream_t s) {

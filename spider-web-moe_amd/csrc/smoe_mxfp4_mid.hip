@@ -302,25 +302,36 @@ int64_t tiles_of(const MxGemm& a, int BM, int CH) {
   return std::min(a.G, a.max_rows) * ((per + BM - 1) / BM) * strips;
 }
 
+// 32 x 64 tiles where they leave no CU a second one, 64 x 64 up to four for a CU.
+// Whole products with the activations' quantizer, us, in a graph: 100 x 1000 ->
+// 2800 6.7 (two waves a tile 7.1; three stages 6.9), 30 x 2048 -> 1408 7.4 (8.1);
+// 200 x 1000 -> 2800 7.4 on 64 x 64 and 8.4 on 64 x 128, 777 x 2816 -> 1024 10.8
+// and 13.0, 1500 x 1024 -> 1408 10.1 and 10.7 on 128 x 128.
 template <int EPI, int ODT>
 int go_dense(const MxGemm& a, hipStream_t s) {
   const int64_t cus = device_cus();
-  if (tiles_of(a, 32, 64) <= cus) return go_tile<EPI, ODT, 32, 64, 2, 1, 4>(a, s);
-  if (tiles_of(a, 64, 128) <= cus) return go_tile<EPI, ODT, 64, 128, 2, 2, 3>(a, s);
+  if (tiles_of(a, 32, 64) <= cus) return go_tile<EPI, ODT, 32, 64, 2, 2, 4>(a, s);
+  if (tiles_of(a, 64, 64) <= 4 * cus) return go_tile<EPI, ODT, 64, 64, 2, 2, 3>(a, s);
   return go_tile<EPI, ODT, 128, 128, 2, 2, 2>(a, s);
 }
 
+// 128 weight rows a tile (SwiGLU: 64 channels; 256 rows on eight waves left fewer
+// workgroups: 800 tokens over 16 experts of 1024 x 2816 37 us for both products and
+// the plan, 41.4 before), two stages (the third takes LDS from a workgroup beside:
+// 1024 tokens over 64 experts of 2048 x 1408 59.6 and 64.6), and rows by the groups'
+// average: 32 up to 56 (400 tokens over 32 experts of 1024 x 1408, 50 rows, 29.6;
+// on 64 rows 32.1), 64 up to 112 (777 tokens, 97 rows, 36.6; on 128 rows 42.3, on
+// 32 rows 48.0), 128 (1500 tokens over 16 SwiGLU experts, 188 rows, 50.6; on 64
+// rows 58.8), fewer where those tiles do not give every CU one.
 template <int EPI>
 int go_grouped(const MxGemm& a, hipStream_t s) {
-  constexpr int O = SMOE_F32;
-  constexpr bool SW = EPI == MX_UP_SWIGLU;
+  constexpr int O = SMOE_F32, CH = EPI == MX_UP_SWIGLU ? 64 : 128;
   const int64_t cus = device_cus(), per = (static_cast<int64_t>(a.max_rows) + a.G - 1) / a.G;
-  int BM = per <= 40 ? 32 : (per <= 112 ? 64 : 128);
-  while (BM > 32 && tiles_of(a, BM, 128) < cus) BM /= 2;
-  constexpr int BN = SW ? 256 : 128, WN = BN / 64;
-  if (BM == 32) return go_tile<EPI, O, 32, BN, 2, WN, 3>(a, s);
-  if (BM == 64) return go_tile<EPI, O, 64, BN, 2, WN, 2>(a, s);
-  return go_tile<EPI, O, 128, BN, 2, WN, 2>(a, s);
+  int BM = per <= 56 ? 32 : (per <= 112 ? 64 : 128);
+  while (BM > 32 && tiles_of(a, BM, CH) < cus) BM /= 2;
+  if (BM == 32) return go_tile<EPI, O, 32, 128, 2, 2, 2>(a, s);
+  if (BM == 64) return go_tile<EPI, O, 64, 128, 2, 2, 2>(a, s);
+  return go_tile<EPI, O, 128, 128, 2, 2, 2>(a, s);
 }
 
 }  // namespace
