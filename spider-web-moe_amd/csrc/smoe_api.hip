@@ -1860,7 +1860,7 @@ MxQuant mx_rows(const void* x, int xdt, int64_t ldx, int N, int K, void* ws, con
 }  // namespace
 
 SMOE_API size_t smoe_linear_mxfp4_workspace_bytes(int N, int K, int N_out) {
-  if (N < 1 || K < 1 || N_out < 1 || mx_linear_quantizes_inside(N, K)) return 0;
+  if (N < 1 || K < 1 || K > (1 << 23) || N_out < 1 || N_out > (1 << 22) || mx_linear_quantizes_inside(N, K)) return 0;
   return mx_ws(N, K).total + (mx_large_linear(N, N_out) ? align_up(mx_planes_bytes(N_out, K)) : 0);
 }
 

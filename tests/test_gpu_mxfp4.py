@@ -116,8 +116,8 @@ def check_linear(x, codes, scale, bias=None, act=None):
     (1, 1, 1), (1, 32, 16), (1, 2048, 1408), (2, 31, 33), (5, 1000, 70), (16, 257, 48), (16, 1024, 64),   # quantized inside
     (9, 2816, 40), (17, 96, 100), (24, 2048, 130),                                                   # a few rows of codes
     (25, 64, 60), (33, 300, 65), (40, 1000, 2800), (64, 256, 512),                                    # 32 x 64 tiles
-    (200, 1000, 2800), (257, 288, 1300),                                                              # 64 x 128
-    (1000, 544, 2000), (515, 96, 5632),                                                               # 128 x 128
+    (200, 1000, 2800), (257, 288, 1300), (1000, 544, 2000), (515, 96, 5632),                          # 64 x 64
+    (2000, 96, 5000), (4000, 352, 2500),                                                              # 128 x 128
     (2100, 352, 5632), (4096, 64, 2816)])                                                             # 256 x 256
 def test_linear(dtype, shape):
     n, k, n_out = shape
