@@ -76,6 +76,7 @@ __device__ __forceinline__ void quant_to_lds(const XLds& x, const void* row, int
 //
 // XQ: -1 X is codes; else its dtype (x_float), which the workgroup quantizes
 // into LDS while its first weights are on their way: one launch for a few tokens.
+// Latency bounds it: 1 x 2048 -> 1408 4.4 us, about an empty launch.
 template <int EPI, int ODT, int MT, int XQ>
 __global__ __launch_bounds__(256, 4) void k_mx_few(const MxGemm p) {
   constexpr int BM = 16 * MT, NW = 4, D = MT == 1 ? 4 : 2;
@@ -263,7 +264,9 @@ __global__ __launch_bounds__(256, 4) void k_mx_stream(const MxGemm p) {
 
 // ------------------------------------------------- a few tokens' experts ----
 // At most kTokensMax (token, slot) entries: the whole expert step in two launches
-// that keep the dispatch plan in registers and quantize their own operands.
+// that keep the dispatch plan in registers and quantize their own operands.  Bound
+// by the latency of the two: 1 token, 2 of 64 experts of 2048 x 1408 5.7 and 5.9 us
+// (weights of 6 MB, 1.3 us of a copy's rate).
 
 // Up product of one expert's rows and 16 channels (SwiGLU: of gate and up):
 // four waves take every fourth 256 of K, the rows' messages are quantized into
@@ -433,7 +436,8 @@ __global__ __launch_bounds__(512, 4) void k_mx_tokens_down(const MxTokensArgs a)
 }
 
 // A small step's plan and its quantized messages in one launch: workgroup 0
-// makes the plan, the others quantize 64 pieces each.
+// makes the plan, the others quantize 64 pieces each.  The plan bounds it: 64
+// tokens, 2 of 16 experts 3.0 us, 777 tokens, 4 of 32 experts 5.7 us.
 template <int KB, int T>
 __global__ __launch_bounds__(1024) void k_prep_mx(const PrepArgs a, const MxQuant mq, int npc, int64_t total) {
   if (blockIdx.x > 0) {
