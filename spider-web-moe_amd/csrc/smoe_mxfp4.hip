@@ -576,7 +576,7 @@ int launch_gemm_mxfp4(const MxGemm& a, hipStream_t s) {
 // From five tiles of 256 x 256 for every eight of the 256 CUs on, and 512 rows a
 // group (a workspace's size goes by it: the same on every device)
 bool mx_large_linear(int N, int N_out) {
-  return (static_cast<int64_t>(N) + 255) / 256 * ((static_cast<int64_t>(N_out) + 255) / 256) >= 160;
+  return N > kMxFewRows && (static_cast<int64_t>(N) + 255) / 256 * ((static_cast<int64_t>(N_out) + 255) / 256) >= 160;
 }
 bool mx_large_experts(int N, int K, int E) { return static_cast<int64_t>(N) * K >= 512ll * E; }
 

@@ -95,9 +95,12 @@ int launch_gemm_mx_few(const MxGemm& g, hipStream_t s);
 // grouped products of decode steps (smoe_mxfp4_few.hip)
 bool gemm_mx_stream_fits(const MxGemm& g);
 int launch_gemm_mx_stream(const MxGemm& g, hipStream_t s);
+// Dense products of up to this many rows run on gemm_mx_few, whatever N_out is
+constexpr int kMxFewRows = 24;
 // whether a linear product of N rows takes x_float
 bool mx_linear_quantizes_inside(int N, int K);
-// whether a product runs on large tiles, with scales in planes
+// whether a product runs on large tiles, with scales in planes (ws_plane > 0; the
+// other kernels read rows of scales and refuse planes)
 bool mx_large_linear(int N, int N_out);
 bool mx_large_experts(int N, int K, int E);
 

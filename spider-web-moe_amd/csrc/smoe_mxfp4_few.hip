@@ -471,13 +471,14 @@ constexpr int64_t kXLds = 49152;
 
 }  // namespace
 
-bool gemm_mx_few_fits(const MxGemm& a) { return a.G == 0 && a.single_rows <= 24; }
+bool gemm_mx_few_fits(const MxGemm& a) { return a.G == 0 && a.ws_plane == 0 && a.single_rows <= kMxFewRows; }
 
 bool mx_linear_quantizes_inside(int N, int K) {
   return N <= 16 && static_cast<int64_t>(N) * K <= 16384 && static_cast<int64_t>(N) * xlds_row(K) <= kXLds;
 }
 
 int launch_gemm_mx_few(const MxGemm& a, hipStream_t s) {
+  if (a.ws_plane) return SMOE_EINVAL;  // the kernel reads rows of scales
   const bool f32 = a.out_dtype == SMOE_F32;
   if (a.epi == MX_LINEAR) return f32 ? go_rows<MX_LINEAR, SMOE_F32>(a, s) : go_rows<MX_LINEAR, SMOE_BF16>(a, s);
   if (a.epi == MX_GELU) return f32 ? go_rows<MX_GELU, SMOE_F32>(a, s) : go_rows<MX_GELU, SMOE_BF16>(a, s);
@@ -503,7 +504,7 @@ bool gemm_mx_stream_fits(const MxGemm& a) {
 int launch_gemm_mx_stream(const MxGemm& a, hipStream_t s) {
   const bool up = a.epi == MX_UP_GELU || a.epi == MX_UP_SWIGLU;
   const int64_t grid = static_cast<int64_t>(a.G) * (a.N_out / (up ? 32 : 16));
-  if (a.N_out % 32 || (!up && a.epi != MX_DOWN) || grid * 256 > 0xffffffffll) return SMOE_EINVAL;  // threads of a launch
+  if (a.ws_plane || a.N_out % 32 || (!up && a.epi != MX_DOWN) || grid * 256 > 0xffffffffll) return SMOE_EINVAL;  // threads of a launch
   const dim3 g(static_cast<unsigned>(grid)), b(256);
   if (a.epi == MX_UP_GELU) SMOE_LAUNCH((k_mx_stream<MX_UP_GELU>), g, b, 0, s, a);
   else if (a.epi == MX_UP_SWIGLU) SMOE_LAUNCH((k_mx_stream<MX_UP_SWIGLU>), g, b, 0, s, a);

@@ -341,7 +341,7 @@ int go_grouped(const MxGemm& a, hipStream_t s) {
 }  // namespace
 
 int launch_gemm_mx_mid(const MxGemm& a, hipStream_t s) {
-  if (a.ld_ws % 4 || a.ld_xs % 4) return SMOE_EINVAL;
+  if (a.ws_plane || a.ld_ws % 4 || a.ld_xs % 4) return SMOE_EINVAL;
   const bool f32 = a.out_dtype == SMOE_F32;
   switch (a.epi) {
     case MX_LINEAR: return f32 ? go_dense<MX_LINEAR, SMOE_F32>(a, s) : go_dense<MX_LINEAR, SMOE_BF16>(a, s);

@@ -1,0 +1,105 @@
+"""Microscaled 4-bit linear products into many channels (a vocabulary), from one
+row to a batch, against oracle/mxfp4.py in 64 bits with the bounds of
+test_gpu_mxfp4.py: the products' f32 sums as the oracle bounds them, and half a
+step of the output's type.  From 40705 channels on more than 24 rows run on
+large tiles, which lay the scales out anew, and fewer never do."""
+import pytest
+import torch
+
+from oracle import mxfp4 as O
+from test_gpu_mxfp4 import assert_within, check_linear, dev, say, weight
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def room():
+    yield
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("n_out", [40704, 40705, 50257, 65536])
+@pytest.mark.parametrize("k", [96, 257])
+def test_rows_by_channels(k, n_out):
+    codes, scale = weight(n_out, k)
+    g = torch.Generator().manual_seed(n_out + k)
+    bias = (torch.randn(n_out, generator=g) * 0.1).to(dev)
+    for n in (1, 2, 17, 24, 25, 100, 129):
+        for dtype in (torch.bfloat16, torch.float32):
+            say("channels", n, k, n_out, dtype)
+            x = (torch.randn(n, k, generator=g) * torch.exp(torch.randn(n, 1, generator=g))).to(dtype).to(dev)
+            check_linear(x, codes, scale)
+            check_linear(x, codes, scale, bias, "gelu")
+
+
+@pytest.mark.parametrize("n,k,n_out", [(8, 4096, 50257), (12, 2048, 40705), (16, 2816, 65536)])
+def test_rows_past_the_ones_quantized_inside(n, k, n_out):
+    say("decode batch", n, k, n_out)
+    codes, scale = weight(n_out, k)
+    x = torch.randn(n, k, generator=torch.Generator().manual_seed(n)).bfloat16().to(dev)
+    check_linear(x, codes, scale)
+
+
+@pytest.mark.parametrize("n", [2, 17, 24, 25, 60])
+def test_scale_rows_further_apart(n):
+    """Scales as columns of a wider table, NaN around them; codes likewise."""
+    from spider_moe_amd import ForgeGEMM
+    for k, n_out in ((257, 40705), (128, 50257)):
+        say("wider", n, k, n_out)
+        codes, scale = weight(n_out, k)
+        nb = -(-k // 32)
+        wide = torch.full((n_out, 64), 0xFF, dtype=torch.uint8, device=dev)
+        wide[:, 8:8 + nb] = scale
+        far = torch.full((n_out, 16 * nb + 64), 0x77, dtype=torch.uint8, device=dev)
+        far[:, 16:16 + codes.shape[1]] = codes
+        x = torch.randn(n, k, generator=torch.Generator().manual_seed(n)).to(dev)
+        want = check_linear(x, codes, scale)
+        got = ForgeGEMM().linear_mxfp4(x, far[:, 16:16 + codes.shape[1]], wide[:, 8:8 + nb])
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("n", [3, 20, 40])
+def test_codes_past_32_bits(n):
+    """More than 2^32 bytes of codes: the last channels."""
+    from spider_moe_amd import ForgeGEMM
+    k, n_out = 65536, 140033
+    say("codes past 2^32", n)
+    g = torch.Generator(device=dev).manual_seed(n)
+    codes = torch.randint(0, 256, (n_out, k // 2), dtype=torch.uint8, device=dev, generator=g)
+    scale = torch.randint(116, 122, (n_out, k // 32), dtype=torch.uint8, device=dev, generator=g)
+    x = torch.randn(n, k, device=dev, generator=g).bfloat16()
+    got = ForgeGEMM().linear_mxfp4(x, codes, scale)
+    for at in (slice(0, 48), slice(131040, 131104), slice(n_out - 65, n_out)):
+        want, err = O.linear(x, codes[at], scale[at])
+        assert_within(got[:, at], want, err)
+
+
+def test_outputs_past_31_bits():
+    from spider_moe_amd import ForgeGEMM
+    n, k, n_out = 60001, 40, 40705  # 2.4e9 outputs
+    say("outputs past 2^31")
+    codes, scale = weight(n_out, k)
+    x = torch.randn(n, k, device=dev, generator=torch.Generator(device=dev).manual_seed(1)).bfloat16()
+    got = ForgeGEMM().linear_mxfp4(x, codes, scale)
+    for at in (slice(0, 130), slice(52700, 52900), slice(n - 150, n)):
+        want, err = O.linear(x[at], codes, scale)
+        assert_within(got[at], want, err)
+
+
+def test_expert_rows_past_31_bits():
+    """More than 2^31 message, output and routed elements: the first and the
+    last tokens."""
+    from spider_moe_amd import sparse_expert_delta_mxfp4
+    from test_gpu_mxfp4 import experts_of
+    n, h = 600_007, 4096
+    say("experts past 2^31")
+    ex = experts_of(2, h, 32, "gelu", True)
+    g = torch.Generator(device=dev).manual_seed(2)
+    x = torch.randn(n, h, device=dev, generator=g, dtype=torch.bfloat16)
+    idx = torch.randint(0, 2, (n, 1), device=dev, generator=g, dtype=torch.int32)
+    w = torch.rand(n, 1, device=dev, generator=g) + 0.5
+    got = sparse_expert_delta_mxfp4(x, idx, w, ex)
+    for at in (slice(0, 200), slice(n // 2, n // 2 + 200), slice(n - 200, n)):
+        want, err = O.expert_delta(x[at], idx[at], w[at], ex.w_up, ex.s_up, ex.w_down, ex.s_down, ex.b_up, ex.b_down,
+                                   ex.activation)
+        assert_within(got[at], want, err)
