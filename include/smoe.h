@@ -441,8 +441,9 @@ SMOE_API int smoe_select_groups_backward(const void* logits, int logits_dtype, i
  * (SpiderMoELayer's aux_loss is the softmax form over the whole batch,
  * model.py:330-337: S = 1).  No tokens or no choices: loss 0.  loss f32 [S],
  * counts i32 [S,E], slope f32 [S,E] or NULL: what the backward pass takes,
- * (E load_e - 1) / n.  Sums over tokens are in f32 over one workgroup's and in
- * 64 bits over those; their order depends on the sizes alone.
+ * (E load_e - 1) / n.  Sums over tokens are in f32 over runs of at
+ * most 128 a lane and over a workgroup's lanes, in 64 bits over the runs and the
+ * workgroups; their order depends on the sizes alone.
  * S * T <= 2^26 - 4, S < 2^22, 1 <= E <= 256, 1 <= K <= 64, S * T * K < 2^31.
  * Where the workspace query gives 0 the workspace may be NULL. */
 SMOE_API size_t smoe_balance_loss_workspace_bytes(int S, int T, int E);

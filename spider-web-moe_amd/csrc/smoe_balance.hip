@@ -198,10 +198,17 @@ __global__ __launch_bounds__(256) void k_balance_part(const BalanceArgs a) {
     const bool on = !a.mask || a.mask[first + t0 + i / static_cast<uint32_t>(a.K)];
     if (on && id >= 0 && id < E) atomicAdd(&s_c[id], 1);
   }
+  // f32 sums of at most kRun trips (128 tokens a lane: 2^-17 of the sum), those in
+  // 64 bits: a workgroup's tokens grow with the batch
+  constexpr int kRun = 128 / kTokens;
   float sum[V];
+  double runs[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) sum[v] = 0.f;
-  int n = 0;
+  for (int v = 0; v < V; ++v) {
+    sum[v] = 0.f;
+    runs[v] = 0.0;
+  }
+  int n = 0, trips = 0;
   for (int t = t0 + wave * PW; t < t1; t += 4 * PW * kTokens) {  // uniform
     float z[kTokens][V];
     bool on[kTokens];
@@ -220,10 +227,18 @@ __global__ __launch_bounds__(256) void k_balance_part(const BalanceArgs a) {
       for (int v = 0; v < V; ++v) sum[v] += on[u] ? p[v] : 0.f;  // a masked token's may be NaN
       n += on[u] && lane % SEG == 0 ? 1 : 0;
     }
+    if (++trips == kRun) {  // uniform
+      trips = 0;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        runs[v] += static_cast<double>(sum[v]);
+        sum[v] = 0.f;
+      }
+    }
   }
   if (n) atomicAdd(&s_c[E], n);
 #pragma unroll
-  for (int v = 0; v < V; ++v) s_p[(wave * PW + lane / SEG) * SEG * V + e0 + v] = sum[v];
+  for (int v = 0; v < V; ++v) s_p[(wave * PW + lane / SEG) * SEG * V + e0 + v] = static_cast<float>(runs[v] + static_cast<double>(sum[v]));
   __syncthreads();
   float all = 0.f;
   if (tid < E)
