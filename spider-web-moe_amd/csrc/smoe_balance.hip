@@ -168,8 +168,10 @@ __device__ __forceinline__ void finish(const BalanceArgs& a, int seq, int chunks
   }
   if (tid < E) {
     a.counts[static_cast<int64_t>(seq) * E + tid] = c;
-    if (a.slope)
-      a.slope[static_cast<int64_t>(seq) * E + tid] = tot > 0 && n > 0 ? static_cast<float>((E * load - 1.0) / n) : 0.f;
+    if (a.slope) {  // E c and tot are whole numbers: 0 exactly where they are equal (49 * (1 / 49) is not 1)
+      const double u = (static_cast<double>(E) * c - tot) / std::max(tot, 1);
+      a.slope[static_cast<int64_t>(seq) * E + tid] = tot > 0 && n > 0 ? static_cast<float>(u / n) : 0.f;
+    }
   }
 }
 
