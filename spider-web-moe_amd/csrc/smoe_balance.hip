@@ -55,6 +55,10 @@ __device__ __forceinline__ void load_row(const void* z, int64_t base, int e0, in
   }
 }
 
+// e^x within (3 + 2.3 |x|) 2^-24 of its value (the product's rounding, the
+// constant's, the instruction's), 0 below 2^-126.  With the argument split, so that
+// |x| plays no part, 8 sequences of 2048 tokens over 256 experts take 13.4 us
+// forward instead of 12.8, 2^20 tokens over 64 experts 198 instead of 188.
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
 
 // p of a token whose experts lie in SEG lanes, V each, and with sigmoid also
