@@ -560,7 +560,9 @@ SMOE_API int smoe_dequantize_mxfp4(const uint8_t* codes, int64_t ld_codes, const
  * SMOE_BF16 / SMOE_F16, rows ldx elements apart) is quantized by the call as
  * smoe_quantize_mxfp4 does.  Products of the two operands' values, summed in f32;
  * act SMOE_LINEAR_NONE / SMOE_LINEAR_GELU; bias f32 [N_out] or NULL; K <= 2^23,
- * N_out <= 2^22, ldw <= 2^22.  Where the workspace query gives 0 (a few rows) the workspace
+ * N_out <= 2^22, ldw <= 2^22, N * ceil(K / 128) <= 2^28 - 16, N_out * ceil(K / 128)
+ * <= 2^32 - 512.  Sizes whose tiles pass a launch's limits (2^32 threads, 2^31 - 2^16
+ * tiles: outputs past 2^45 elements) are refused before anything is launched.  Where the workspace query gives 0 (a few rows) the workspace
  * may be NULL. */
 SMOE_API size_t smoe_linear_mxfp4_workspace_bytes(int N, int K, int N_out);
 SMOE_API int smoe_linear_mxfp4(const void* x, int x_dtype, int64_t ldx, int N, int K,
@@ -595,7 +597,10 @@ typedef struct smoe_experts_mxfp4 {
  * idx i32 / w f32 [N,K] as smoe_dispatch_plan takes them (equal ids merged,
  * weights <= 0 and ids outside [0, E) dropped; a token left without experts gets
  * 0).  1 <= K <= 64, N * K < 2^31 - 128, N <= 4194240, with H > 4096 N <= 65535,
- * U * H <= 2^32, N * H <= 2^32. */
+ * U * H <= 2^32, N * H <= 2^32.  Refused before anything is
+ * launched: sizes whose tiles pass a launch's 2^32 threads (none with E * max(U, H)
+ * below 2^28 and (N * K + 32 E) * max(U, H) below 2^34) and, from N * K = 512 E on,
+ * weights of more than 2^32 - 512 pieces of 1 x 128. */
 SMOE_API size_t smoe_expert_delta_mxfp4_workspace_bytes(const smoe_experts_mxfp4* ex, int N, int K);
 SMOE_API int smoe_expert_delta_mxfp4(const smoe_experts_mxfp4* ex, const void* msg, int msg_dtype,
                                      const int32_t* idx, const float* w, int N, int K, void* delta,

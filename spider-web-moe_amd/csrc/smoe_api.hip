@@ -1816,6 +1816,9 @@ SMOE_API int smoe_dequantize_mxfp4(const uint8_t* codes, int64_t ld_codes, const
 
 namespace {
 
+// words of scales that rows of K values have
+int64_t mx_words(int64_t rows, int K) { return rows * (mx_scale_pitch(K) / 4); }
+
 size_t mx_planes_bytes(int64_t rows, int K) { return static_cast<size_t>(mx_plane_pitch(rows)) * (mx_scale_pitch(K) / 4); }
 
 // x quantized: codes in rows of whole blocks, scales in planes or (less) in rows of whole words
@@ -1860,7 +1863,9 @@ MxQuant mx_rows(const void* x, int xdt, int64_t ldx, int N, int K, void* ws, con
 }  // namespace
 
 SMOE_API size_t smoe_linear_mxfp4_workspace_bytes(int N, int K, int N_out) {
-  if (N < 1 || K < 1 || K > (1 << 23) || N_out < 1 || N_out > (1 << 22) || mx_linear_quantizes_inside(N, K)) return 0;
+  if (N < 1 || K < 1 || K > (1 << 23) || N_out < 1 || N_out > (1 << 22) || mx_words(N_out, K) > kMxPlaneWords ||
+      mx_linear_quantizes_inside(N, K))
+    return 0;
   return mx_ws(N, K).total + (mx_large_linear(N, N_out) ? align_up(mx_planes_bytes(N_out, K)) : 0);
 }
 
@@ -1872,6 +1877,7 @@ SMOE_API int smoe_linear_mxfp4(const void* x, int x_dtype, int64_t ldx, int N, i
       ldw > (1 << 22) || ldw < mx_code_pitch(K) || ldw % 16 || ld_ws < mx_scale_pitch(K) || ld_ws % 4)
     return fail(SMOE_EINVAL, "mxfp4 linear shape (ldx >= K; K <= 2^23, N_out <= 2^22, ldw <= 2^22; weight rows of whole blocks, ldw % 16 == 0; ld_ws % 4 == 0)");
   if (N > ((1 << 28) - 16) / ((static_cast<int64_t>(K) + 127) / 128)) return fail(SMOE_EINVAL, "mxfp4 linear shape (at most 2^28 - 16 pieces of 1 x 128 of x)");
+  if (mx_words(N_out, K) > kMxPlaneWords) return fail(SMOE_EINVAL, "mxfp4 linear shape (at most 2^32 - 512 pieces of 1 x 128 of the weights)");
   if (act != SMOE_LINEAR_NONE && act != SMOE_LINEAR_GELU) return fail(SMOE_EINVAL, "act");
   if (out_dtype != SMOE_F32 && out_dtype != SMOE_BF16) return fail(SMOE_EUNSUPPORTED, "out dtype");
   if (N == 0) return SMOE_OK;
@@ -1881,6 +1887,8 @@ SMOE_API int smoe_linear_mxfp4(const void* x, int x_dtype, int64_t ldx, int N, i
     return fail(SMOE_EINVAL, "codes and workspace must be 16-byte, scales 4-byte aligned");
   hipStream_t s = static_cast<hipStream_t>(stream);
   MxGemm g;
+  MxQuant q;
+  MxPlanes planes[2];
   g.epi = act == SMOE_LINEAR_GELU ? MX_GELU : MX_LINEAR;
   if (inside) {
     g.x_float = x;
@@ -1890,13 +1898,11 @@ SMOE_API int smoe_linear_mxfp4(const void* x, int x_dtype, int64_t ldx, int N, i
     const MxWs l = mx_ws(N, K);
     if (ws_bytes < smoe_linear_mxfp4_workspace_bytes(N, K, N_out)) return fail(SMOE_ECAPACITY, "workspace");
     const bool large = mx_large_linear(N, N_out);
-    const MxQuant q = mx_rows(x, x_dtype, ldx, N, K, ws, l, large);
-    MxPlanes planes[2];
+    q = mx_rows(x, x_dtype, ldx, N, K, ws, l, large);
     if (large) {
       planes[0] = mx_planes(w_scale, ld_ws, 1, N_out, K, at<void>(ws, l.total));
       g.ws_plane = mx_plane_pitch(N_out);
     }
-    SMOE_TRY(launch_quantize_mxfp4(q, planes, s), "quantize mxfp4");
     g.X = q.codes;
     g.ldx = q.ld_codes;
     g.xs = q.scale;
@@ -1914,6 +1920,12 @@ SMOE_API int smoe_linear_mxfp4(const void* x, int x_dtype, int64_t ldx, int N, i
   g.out = out;
   g.out_dtype = out_dtype;
   g.ldo = N_out;
+  if (!inside) {  // refusals before the first launch
+    g.dry = true;
+    if (launch_gemm_mxfp4(g, s) != SMOE_OK) return fail(SMOE_EINVAL, "mxfp4 linear shape (tiles past a launch)");
+    g.dry = false;
+    SMOE_TRY(launch_quantize_mxfp4(q, planes, s), "quantize mxfp4");
+  }
   SMOE_TRY(launch_gemm_mxfp4(g, s), "mxfp4 GEMM");
   return SMOE_OK;
 }
@@ -1936,6 +1948,10 @@ int check_experts_mxfp4(const smoe_experts_mxfp4* ex, int N, int K) {
   if (N > ((1 << 28) - 16) / ((ex->H + 127) / 128)) return fail(SMOE_EINVAL, "N * ceil(H / 128) <= 2^28 - 16");
   if (static_cast<int64_t>(ex->U) * ex->H > (1ll << 32) || static_cast<int64_t>(N) * ex->H > (1ll << 32))
     return fail(SMOE_EINVAL, "mxfp4 experts: U * H and N * H <= 2^32");
+  const int halves = ex->act == SMOE_ACT_SWIGLU ? 2 : 1;
+  if (mx_large_experts(N, K, ex->E) &&
+      ex->E * (mx_words(static_cast<int64_t>(halves) * ex->U, ex->H) + mx_words(ex->H, ex->U)) > kMxPlaneWords)
+    return fail(SMOE_EINVAL, "mxfp4 experts: from 512 choices an expert on at most 2^32 - 512 pieces of 1 x 128 of the weights");
   return SMOE_OK;
 }
 
@@ -2017,29 +2033,6 @@ SMOE_API int smoe_expert_delta_mxfp4(const smoe_experts_mxfp4* ex, const void* m
   float* roww = at<float>(ws, l.roww);
   const bool large = mx_large_experts(N, K, E);
   const MxQuant mq = mx_rows(msg, msg_dtype, H, N, H, at<void>(ws, l.x_at), l.x, large);
-  if (!large && prep_fits(N, K, E)) {
-    PrepArgs pa;
-    pa.idx = idx;
-    pa.w = w;
-    pa.N = N;
-    pa.K = K;
-    pa.E = E;
-    pa.off = off;
-    pa.rows = rows;
-    pa.tokrow = tokrow;
-    pa.roww = roww;
-    SMOE_TRY(launch_prep_mx(pa, mq, s), "plan and messages");
-  } else {
-    rc = smoe_dispatch_plan(idx, w, N, K, E, at<int32_t>(ws, l.cnt), off, rows, roww, tokrow, at<void>(ws, l.plan),
-                            smoe_dispatch_workspace_bytes(N, K, E), stream);
-    if (rc != SMOE_OK) return rc;
-    MxPlanes planes[2];
-    if (large) {
-      planes[0] = mx_planes(ex->s_up, mx_scale_pitch(H), E, halves * U, H, at<void>(ws, l.sup));
-      planes[1] = mx_planes(ex->s_down, mx_scale_pitch(U), E, H, U, at<void>(ws, l.sdown));
-    }
-    SMOE_TRY(launch_quantize_mxfp4(mq, planes, s), "quantize messages");
-  }
   MxGemm up;
   up.epi = halves == 2 ? MX_UP_SWIGLU : MX_UP_GELU;
   up.X = mq.codes;
@@ -2068,7 +2061,6 @@ SMOE_API int smoe_expert_delta_mxfp4(const smoe_experts_mxfp4* ex, const void* m
   up.out_scale = at<uint8_t>(ws, l.ascale);
   up.os_plane = mx_plane_pitch(static_cast<int64_t>(N) * K);
   up.ld_os = mx_scale_pitch(U);
-  SMOE_TRY(launch_gemm_mxfp4(up, s), "expert up GEMM");
   MxGemm dn;
   dn.epi = MX_DOWN;
   dn.X = at<uint8_t>(ws, l.act);
@@ -2093,6 +2085,34 @@ SMOE_API int smoe_expert_delta_mxfp4(const smoe_experts_mxfp4* ex, const void* m
   dn.row_scale = roww;
   dn.out = at<void>(ws, l.y);
   dn.ldo = H;
+  up.dry = dn.dry = true;  // refusals before the first launch
+  if (launch_gemm_mxfp4(up, s) != SMOE_OK || launch_gemm_mxfp4(dn, s) != SMOE_OK)
+    return fail(SMOE_EINVAL, "mxfp4 experts: tiles past a launch");
+  up.dry = dn.dry = false;
+  if (!large && prep_fits(N, K, E)) {
+    PrepArgs pa;
+    pa.idx = idx;
+    pa.w = w;
+    pa.N = N;
+    pa.K = K;
+    pa.E = E;
+    pa.off = off;
+    pa.rows = rows;
+    pa.tokrow = tokrow;
+    pa.roww = roww;
+    SMOE_TRY(launch_prep_mx(pa, mq, s), "plan and messages");
+  } else {
+    rc = smoe_dispatch_plan(idx, w, N, K, E, at<int32_t>(ws, l.cnt), off, rows, roww, tokrow, at<void>(ws, l.plan),
+                            smoe_dispatch_workspace_bytes(N, K, E), stream);
+    if (rc != SMOE_OK) return rc;
+    MxPlanes planes[2];
+    if (large) {
+      planes[0] = mx_planes(ex->s_up, mx_scale_pitch(H), E, halves * U, H, at<void>(ws, l.sup));
+      planes[1] = mx_planes(ex->s_down, mx_scale_pitch(U), E, H, U, at<void>(ws, l.sdown));
+    }
+    SMOE_TRY(launch_quantize_mxfp4(mq, planes, s), "quantize messages");
+  }
+  SMOE_TRY(launch_gemm_mxfp4(up, s), "expert up GEMM");
   SMOE_TRY(launch_gemm_mxfp4(dn, s), "expert down GEMM");
   SMOE_TRY(launch_delta_combine(at<void>(ws, l.y), SMOE_F32, tokrow, N, K, H, delta, out_dtype, s), "delta combine");
   return SMOE_OK;

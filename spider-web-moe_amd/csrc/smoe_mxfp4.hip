@@ -506,6 +506,7 @@ int go(const MxGemm& a, hipStream_t s) {
   const int64_t tiles = (static_cast<int64_t>(rows) + BM - 1) / BM + (a.G > 0 ? std::min(a.G, rows) : 0);
   const int64_t all = tiles * ((static_cast<int64_t>(a.N_out) + CH - 1) / CH);
   if (all > 0x7fff0000ll) return SMOE_EINVAL;  // tiles are counted in 32 bits
+  if (a.dry) return SMOE_OK;
   const int64_t grid = std::min<int64_t>(all, std::max<int64_t>(device_cus() * 2 / 8 * 8, 8));
   SMOE_LAUNCH((k_gemm_mx<EPI, ODT, BM, 256, 2, 2, 3, 2>), dim3(static_cast<unsigned>(grid)), dim3(256), 0, s, a);
   return rc();
@@ -522,11 +523,16 @@ int launch_quantize_mxfp4(const MxQuant& q, const MxPlanes (&planes)[2], hipStre
   if (q.ld_codes > 64 * static_cast<int64_t>(npc) || q.rows > ((1 << 28) - 16) / npc) return SMOE_EINVAL;
   const int64_t total = q.rows * npc, wgs = (total + 15) / 16;
   const int64_t words = mx_plane_words(planes[0]) + mx_plane_words(planes[1]), all = wgs + (words + 255) / 256;
-  if (words > 0x7fffffffll || all * 256 > 0xffffffffll) return SMOE_EINVAL;  // threads of a launch
+  if (words > kMxPlaneWords) return SMOE_EINVAL;
   return by_xdt(q.x_dtype, [&](auto xd) {
-    hipLaunchKernelGGL((k_quant_mx<decltype(xd)::value>), dim3(static_cast<unsigned>(all)), dim3(256), 0, s, q, npc, total,
-                       static_cast<uint32_t>(wgs), planes[0], planes[1]);
-    return rc();
+    auto go = [&](int64_t grid, int64_t quant_wgs) {
+      hipLaunchKernelGGL((k_quant_mx<decltype(xd)::value>), dim3(static_cast<unsigned>(grid)), dim3(256), 0, s, q, npc,
+                         total, static_cast<uint32_t>(quant_wgs), planes[0], planes[1]);
+      return rc();
+    };
+    if (all * 256 <= 0xffffffffll) return go(all, wgs);  // threads of a launch
+    const int r = go(wgs, wgs);
+    return r != SMOE_OK ? r : go(all - wgs, 0);
   });
 }
 

@@ -43,6 +43,7 @@ struct MxPlanes {
   int blocks = 0;            // of a row
   uint32_t* dst = nullptr;
 };
+constexpr int64_t kMxPlaneWords = 0xfffffe00ll;  // words that a call lays out in planes at most
 int launch_quantize_mxfp4(const MxQuant& q, const MxPlanes (&planes)[2], hipStream_t s);
 int launch_dequantize_mxfp4(const uint8_t* codes, int64_t ld_codes, const uint8_t* scale, int64_t ld_scale,
                             int64_t rows, int cols, void* out, int out_dtype, hipStream_t s);
@@ -86,6 +87,7 @@ struct MxGemm {
   int64_t ldo = 0;               // elements (codes: bytes)
   uint8_t* out_scale = nullptr;  // MX_UP_*
   int64_t os_plane = 0, ld_os = 0;
+  bool dry = false;  // says whether the launch would be refused, and launches nothing
 };
 int launch_gemm_mxfp4(const MxGemm& g, hipStream_t s);
 int launch_gemm_mx_mid(const MxGemm& g, hipStream_t s);  // smoe_mxfp4_mid.hip

@@ -455,6 +455,7 @@ template <int EPI, int ODT, int MT, int XQ>
 int go_few(const MxGemm& a, hipStream_t s) {
   const int64_t grid = (static_cast<int64_t>(a.single_rows) + 16 * MT - 1) / (16 * MT) * ((static_cast<int64_t>(a.N_out) + 15) / 16);
   if (grid * 256 > 0xffffffffll) return SMOE_EINVAL;  // threads of a launch
+  if (a.dry) return SMOE_OK;
   const size_t lds = XQ >= 0 ? static_cast<size_t>(std::min(16 * MT, a.single_rows)) * xlds_row(a.K) : 0;
   SMOE_LAUNCH((k_mx_few<EPI, ODT, MT, XQ>), dim3(static_cast<unsigned>(grid)), dim3(256), lds, s, a);
   return rc();
@@ -505,6 +506,7 @@ int launch_gemm_mx_stream(const MxGemm& a, hipStream_t s) {
   const bool up = a.epi == MX_UP_GELU || a.epi == MX_UP_SWIGLU;
   const int64_t grid = static_cast<int64_t>(a.G) * (a.N_out / (up ? 32 : 16));
   if (a.ws_plane || a.N_out % 32 || (!up && a.epi != MX_DOWN) || grid * 256 > 0xffffffffll) return SMOE_EINVAL;  // threads of a launch
+  if (a.dry) return SMOE_OK;
   const dim3 g(static_cast<unsigned>(grid)), b(256);
   if (a.epi == MX_UP_GELU) SMOE_LAUNCH((k_mx_stream<MX_UP_GELU>), g, b, 0, s, a);
   else if (a.epi == MX_UP_SWIGLU) SMOE_LAUNCH((k_mx_stream<MX_UP_SWIGLU>), g, b, 0, s, a);

@@ -292,6 +292,7 @@ int go_tile(const MxGemm& a, hipStream_t s) {
   const int64_t tiles = (static_cast<int64_t>(rows) + BM - 1) / BM + (a.G > 0 ? std::min(a.G, rows) : 0);
   const int64_t grid = tiles * ((static_cast<int64_t>(a.N_out) + CH - 1) / CH);
   if (grid * 64 * WM * WN > 0xffffffffll) return SMOE_EINVAL;  // threads of a launch
+  if (a.dry) return SMOE_OK;
   SMOE_LAUNCH((k_gemm_mx_mid<EPI, ODT, BM, BN, WM, WN, NS>), dim3(static_cast<unsigned>(grid)),
               dim3(64 * WM * WN), 0, s, a);
   return rc();
