@@ -392,7 +392,7 @@ def _linear_mxfp4(x, codes, scale, bias, act):
     else:
         x, ldx = x.contiguous(), k
     ldc, lds = mx_pitches(k)
-    codes, ldw = _pitched(codes, ldc, 16)
+    codes, ldw = _pitched(codes, ldc, 16, most=1 << 22)
     scale, ld_ws = _pitched(scale, lds, 4)
     out_dtype = torch.bfloat16 if x.dtype == torch.bfloat16 else torch.float32
     out = torch.empty(*lead, n_out, dtype=out_dtype, device=dev)

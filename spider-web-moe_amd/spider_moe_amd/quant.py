@@ -243,13 +243,13 @@ def mx_pitches(cols: int):
     return 16 * nb, -(-nb // 4) * 4
 
 
-def _pitched(t: torch.Tensor, pitch: int, align: int):
-    """t [rows, n] bytes with rows `ld` apart, ld a multiple of `align` and
-    every row's `pitch` bytes inside the storage: t itself, else a copy.
-    Returns it and ld."""
+def _pitched(t: torch.Tensor, pitch: int, align: int, most: int | None = None):
+    """t [rows, n] bytes with rows `ld` apart, ld a multiple of `align`, at most
+    `most`, and every row's `pitch` bytes inside the storage: t itself, else a
+    copy.  Returns it and ld."""
     rows, n = t.shape
     ld = t.stride(0) if rows > 1 else pitch
-    if (t.stride(1) == 1 or n == 1) and ld >= pitch and ld % align == 0 and t.data_ptr() % align == 0 and \
+    if (t.stride(1) == 1 or n == 1) and pitch <= ld <= (most or ld) and ld % align == 0 and t.data_ptr() % align == 0 and \
             t.untyped_storage().nbytes() - t.storage_offset() >= (rows - 1) * ld + pitch:
         return t, ld
     c = torch.zeros(rows, pitch, dtype=torch.uint8, device=t.device)

@@ -34,3 +34,15 @@ def test_large_products_take_planes(need, n, n_out):
 @pytest.mark.parametrize("n,n_out", [(25, 40704), (256, 40704), (257, 20224)])
 def test_products_below_take_none(need, n, n_out):
     assert need(n, 257, n_out) == rows_only(n, 257)
+
+
+def test_rows_further_apart_than_the_product_takes_are_copied():
+    """Codes as columns of a table whose rows lie more than 2^22 bytes apart."""
+    import torch
+    from spider_moe_amd.quant import _pitched
+    table = torch.zeros(3, (1 << 22) + 16, dtype=torch.uint8)
+    table[:, :48] = torch.arange(3 * 48).view(3, 48)
+    far = table[:, :48]
+    t, ld = _pitched(far, 48, 16, most=1 << 22)
+    assert ld == 48 and t.data_ptr() != far.data_ptr() and torch.equal(t, far)
+    assert _pitched(far, 48, 16)[0] is far and _pitched(far[:1], 48, 16, most=1 << 22)[0].data_ptr() == far.data_ptr()
