@@ -261,7 +261,7 @@ __global__ __launch_bounds__(256) void k_balance_part(const BalanceArgs a) {
 }
 
 // One workgroup a sequence; latency bounds it: 8 sequences of 64 chunks of 256
-// experts 5.4 us.
+// experts 5.0-5.8 us.
 __global__ __launch_bounds__(1024) void k_balance_loss(const BalanceArgs a) {
   const int64_t at = static_cast<int64_t>(blockIdx.x) * a.chunks;
   finish<1024>(a, blockIdx.x, a.chunks, a.part_p + at * a.E, a.part_c + at * (a.E + 1));

@@ -16,7 +16,7 @@ int rc() { return hipGetLastError() == hipSuccess ? SMOE_OK : SMOE_EHIP; }
 // behind them workgroups for the planes, 256 words each.  Bytes bound it: a piece
 // is read once, its amax goes over quads of lanes, the conversion instruction
 // rounds.  16384 x 1024 bf16 and the planes of 5632 weight rows 10.0 us, 16384 x
-// 2816 20.8 us (5.6 TB/s, the input partly from the last-level cache).
+// 2816 23.8 us (4.9 TB/s).
 template <int XDT>
 __global__ __launch_bounds__(256) void k_quant_mx(const MxQuant q, int npc, int64_t total, uint32_t quant_wgs,
                                                   const MxPlanes p0, const MxPlanes p1) {
@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256) void k_quant_mx(const MxQuant q, int npc, int6
 }
 
 // The values of codes: eight columns a thread.  Exact but for f16, whose range
-// is smaller.  Bound by the bytes written: 16384 x 2816 to bf16 27.2 us, 4.3 TB/s.
+// is smaller.  Bound by the bytes written: 16384 x 2816 to bf16 27.8 us, 4.2 TB/s.
 template <int ODT>
 __global__ __launch_bounds__(256) void k_dequant_mx(const uint8_t* __restrict__ codes, int64_t ld_codes,
                                                     const uint8_t* __restrict__ scale, int64_t ld_scale,
@@ -118,9 +118,11 @@ constexpr int kNowhere = static_cast<int>(0x80000000u);  // an offset that a buf
 // 128 x 256 tiles and two workgroups a CU, one's epilogue under the other's
 // products: 16384 x 1024 -> 5632 bf16 70 us (2.7 PFLOP/s; 86 in one tile a
 // workgroup, 55 of them the loop without DMA and epilogue), 32768 rows of 16
-// experts of 1024 x 2816 150-167 us the up product (SwiGLU; 178 before) and
-// 88-99 the down one.  Slower: 256 x 256 on four waves (one a SIMD), 128 x 128, and
-// eight waves of 64 x 64.
+// experts of 1024 x 2816 135 us the up product (SwiGLU, 2.8 PFLOP/s) and 85 the
+// down one (2.2: some 264 row tiles x 4 are two rounds of the 512 workgroups and a
+// few tiles of a third; evenly loaded, 256 x 4, it takes 75); in the first calls after an idle second 150-167 (178 in
+// one tile a workgroup) and 88-99.  Slower: 256 x 256 on four waves (one a SIMD),
+// 128 x 128, and eight waves of 64 x 64.
 template <int EPI, int ODT, int BM, int BN, int WM, int WN, int NS, int OCC>
 __global__ __launch_bounds__(64 * WM * WN, OCC) void k_gemm_mx(const MxGemm p) {
   constexpr bool SWIGLU = EPI == MX_UP_SWIGLU, UP = EPI == MX_UP_GELU || SWIGLU, GATHER = UP;
@@ -579,8 +581,20 @@ int launch_gemm_mxfp4(const MxGemm& a, hipStream_t s) {
   }
 }
 
-// From five tiles of 256 x 256 for every eight of the 256 CUs on, and 512 rows a
-// group (a workspace's size goes by it: the same on every device)
+// From 160 pieces of 256 x 256 outputs on (tiles of 128 x 256 for more than 320 of
+// the 512 workgroups), and 512 rows a group; a workspace's size goes by it, so it is
+// the same on every device.  Whole calls in a graph, us, middle and large kernel:
+// 1024 x 1024 -> 5632 (88 pieces) 14.8 and 15.1, 1792 (154) 20.5 and 18.5, 2048
+// (176) 20.4 and 18.4, 4096 (352) 30.2 and 28.4; 2048 x 2816 -> 4096 (128) 27.0 and
+// 32.5, -> 5120 (160) 33.6 and 33.1; 10240 x 2816 -> 1024 (160) 41.8 and 42.6, 16384
+// (256) 56.3 and 54.8; 512 x 1024 -> 20480 (160) 18.9 and 17.0.  Where one or two
+// row tiles meet a vocabulary the middle one would be ahead: 40 x 1024 -> 50257 13.7
+// and 28.7, 128 rows 21.3 and 35.2, 256 rows 35.6 and 39.3.
+// Expert steps at 384, 512, 640 and 768 rows a group: 16 experts of 1024 x 2816
+// (SwiGLU) 74.1, 96.1, 115.2, 128.6 and 80.8, 96.1, 107.1, 117.1; 32 of 1024 x 1408
+// 89.4, 110.4, 123.2, 139.6 and 87.8, 114.4, 124.9, 134.4; 64 of 2048 x 1408 281.6,
+// 356.1, 424.9, 495.2 and 271.5, 332.4, 398.1, 467.8 (from 192 on, 171.2 and 166.6);
+// 8 of 256 x 512 stay behind (1024 rows 34.2 and 39.7).
 bool mx_large_linear(int N, int N_out) {
   return N > kMxFewRows && (static_cast<int64_t>(N) + 255) / 256 * ((static_cast<int64_t>(N_out) + 255) / 256) >= 160;
 }

@@ -169,9 +169,11 @@ __global__ __launch_bounds__(256, 4) void k_mx_few(const MxGemm p) {
 // take every fourth 256 of K, and weights and rows go straight into registers,
 // D pieces at once, without a barrier; the waves' sums are added through LDS in
 // wave order.  16 rows at a time: a group with more reads its strip again, from
-// the L2.  64 tokens, 2 of 16 experts of 1024 x 2816 (SwiGLU): 14.4 us the up
-// product, 7.8 the down one; non-temporal weight loads 15.2 and 8.8; blocks q and
-// q + 4 a lane, so that a load covers whole 64-byte pieces, 17.2 and 8.2.
+// the L2.  32 tokens, 2 of 16 experts of 1024 x 2816 (SwiGLU, 49 MB of weights):
+// 14.2 us the up product, 7.5 the down one.  At 64 tokens, whose up product now runs
+// on staged tiles (11.2), the two took 14.4 and 7.8 here; with non-temporal weight
+// loads 15.2 and 8.8; with blocks q and q + 4 a lane, so that a load covers whole
+// 64-byte pieces, 17.2 and 8.2.
 template <int EPI>
 __global__ __launch_bounds__(256, 4) void k_mx_stream(const MxGemm p) {
   constexpr bool SWIGLU = EPI == MX_UP_SWIGLU, UP = EPI == MX_UP_GELU || SWIGLU;
@@ -472,8 +474,18 @@ constexpr int64_t kXLds = 49152;
 
 }  // namespace
 
+// Whole calls in a graph, us, this kernel and tiles: 17 x 2048 -> 1408 5.9 and 6.9,
+// 24 rows 6.4 and 7.0, 48 rows 6.6 and 7.2; 24 x 1000 -> 2800 6.3 and 6.2, 40 rows
+// 7.7 and 6.3.  With many channels it reads every row once for 16 of them, and tiles
+// would be ahead: 24 x 1024 -> 5632 8.0 and 6.1, 17 x 4096 -> 40000 34.7 and 19.8.
 bool gemm_mx_few_fits(const MxGemm& a) { return a.G == 0 && a.ws_plane == 0 && a.single_rows <= kMxFewRows; }
 
+// Up to one row tile, and while each workgroup's own quantizing costs about what a
+// launch does.  Inside and by a launch of its own, us in a graph (from the host a
+// launch is 4 more): into 1408 channels 1 x 4096 4.3 and 5.7, 4 x 1024 4.3 and 5.9,
+// 16 x 1024 6.6 and 6.8, 4 x 4096 6.7 and 6.2, 8 x 2048 6.7 and 6.3, 2 x 8192 8.1 and
+// 7.9; past it 16 x 1536 8.0 and 6.5, 8 x 4096 10.0 and 6.5; into 50257 channels 4 x
+// 1024 21.0 and 28.0, 8 x 2048 32.4 and 33.1, past it 8 x 4096 47.9 and 33.9.
 bool mx_linear_quantizes_inside(int N, int K) {
   return N <= 16 && static_cast<int64_t>(N) * K <= 16384 && static_cast<int64_t>(N) * xlds_row(K) <= kXLds;
 }

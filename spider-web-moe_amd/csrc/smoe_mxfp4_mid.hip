@@ -26,7 +26,7 @@ int rc() { return hipGetLastError() == hipSuccess ? SMOE_OK : SMOE_EHIP; }
 // that the fragment reads keep the conflict-free pattern of 128-byte rows.
 //
 // The weights' bytes and the stages' latency bound it: 777 tokens, 4 of 32 experts of
-// 1024 x 1408 (GELU) 15.0 us the up product and 11.8 the down one, 23 MB of weights
+// 1024 x 1408 (GELU) 14.4 us the up product and 11-14 the down one, 23 MB of weights
 // each; 200 x 1000 -> 2800 5.9 us.
 template <int EPI, int ODT, int BM, int BN, int WM, int WN, int NS>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm_mx_mid(const MxGemm p) {

@@ -103,3 +103,43 @@ def test_expert_rows_past_31_bits():
         want, err = O.expert_delta(x[at], idx[at], w[at], ex.w_up, ex.s_up, ex.w_down, ex.s_down, ex.b_up, ex.b_down,
                                    ex.activation)
         assert_within(got[at], want, err)
+
+
+@pytest.mark.parametrize("n", [20, 60])
+def test_nan_stays_in_its_row_and_channel(n):
+    say("channels nan", n)
+    k, n_out = 200, 40705
+    x = torch.randn(n, k, generator=torch.Generator().manual_seed(n)).to(dev)
+    codes, scale = weight(n_out, k)
+    x[1, 7] = float("nan")
+    scale = scale.clone()
+    scale[40001, 3] = 255
+    nan = torch.isnan(check_linear(x, codes, scale))
+    assert nan[1].all() and nan[:, 40001].all() and int(nan.sum()) == n_out + n - 1
+
+
+@pytest.mark.parametrize("n", [20, 60])
+def test_captured_and_on_another_stream(n):
+    from spider_moe_amd import ForgeGEMM
+    say("channels graph", n)
+    k, n_out = 288, 50257
+    codes, scale = weight(n_out, k)
+    g = torch.Generator().manual_seed(n)
+    xs = [torch.randn(n, k, generator=g).bfloat16().to(dev) for _ in range(3)]
+    want = [ForgeGEMM().linear_mxfp4(x, codes, scale) for x in xs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ForgeGEMM().linear_mxfp4(xs[0], codes, scale)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want[0])
+    held = xs[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ForgeGEMM().linear_mxfp4(held, codes, scale)
+    for i in range(4):
+        held.copy_(xs[i % 3])
+        graph.replay()
+        again = ForgeGEMM().linear_mxfp4(xs[i % 3], codes, scale)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want[i % 3]) and torch.equal(again, want[i % 3])
