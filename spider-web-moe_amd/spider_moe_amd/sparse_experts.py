@@ -102,9 +102,14 @@ class _HeldExperts:
             super().__setattr__("_at", None)  # the next call looks at it
 
     def _addresses(self):
+        """Where the tensors lie and how large they are: what the description
+        rests on."""
         u, d = self.b_up, self.b_down
         return (self.w_up.data_ptr(), self.s_up.data_ptr(), self.w_down.data_ptr(), self.s_down.data_ptr(),
-                None if u is None else u.data_ptr(), None if d is None else d.data_ptr())
+                None if u is None else u.data_ptr(), None if d is None else d.data_ptr(),
+                # a tensor may get another size where it lies (`t.data = t.data[:3]`)
+                self.w_up.numel(), self.s_up.numel(), self.w_down.numel(), self.s_down.numel(),
+                None if u is None else u.numel(), None if d is None else d.numel())
 
     def _describe(self, desc, e, h, u, convert):
         """desc: an empty structure of the library's; convert: the names that
@@ -115,7 +120,7 @@ class _HeldExperts:
         self.num_experts, self.hidden_size, self.expert_ffn_size = e, h, u
         desc.act = nat.ACT_SWIGLU if self.activation == "swiglu" else nat.ACT_GELU
         desc.E, desc.H, desc.U = e, h, u
-        desc.w_up, desc.s_up, desc.w_down, desc.s_down, desc.b_up, desc.b_down = at
+        desc.w_up, desc.s_up, desc.w_down, desc.s_down, desc.b_up, desc.b_down = at[:6]
         self._desc = desc
         self._ref = ctypes.byref(desc)
         self._convert = [n for n in convert if getattr(self, n) is not None and
@@ -152,6 +157,8 @@ class Fp8BlockExperts(_HeldExperts):
     not contiguous float32 are converted in each call.  Only codes that are not
     contiguous or not 16-byte aligned are copied once and no longer followed.
     Fp8BlockExperts.quantize makes one from float weights."""
+
+    _WORKSPACE = "smoe_expert_delta_fp8_blocks_workspace_bytes"
 
     def _bind(self):
         """Checks the tensors and describes them to the library."""
@@ -219,6 +226,8 @@ class MxFp4Experts(_HeldExperts):
     that was given is no longer followed.  MxFp4Experts.quantize makes one from
     float weights, laid out as it is read."""
 
+    _WORKSPACE = "smoe_expert_delta_mxfp4_workspace_bytes"
+
     def _bind(self):
         """Checks the tensors and describes them to the library."""
         w_up, s_up, w_down, s_down, b_up, b_down = (getattr(self, n) for n in self._TENSORS)
@@ -275,7 +284,7 @@ def _expert_ids(idx: torch.Tensor, num_experts: int) -> torch.Tensor:
 
 
 def _delta(name, kind, messages, top_indices, top_weights, experts):
-    """smoe_<name>(messages, ..) on kept experts of class `kind`."""
+    """Entry point `name` (messages, ..) on kept experts of class `kind`."""
     if not isinstance(experts, kind):  # the library would read one format as the other
         raise TypeError(f"experts must be {kind.__name__}, got {type(experts).__name__}")
     ref, keep = experts._descriptor()
@@ -295,11 +304,11 @@ def _delta(name, kind, messages, top_indices, top_weights, experts):
         raise ValueError("more than 2^31 - 1 tokens")
     delta = torch.empty(messages.shape, dtype=messages.dtype, device=dev)
     lib = nat.lib()
-    need = getattr(lib, f"smoe_{name}_workspace_bytes")(ref, n, k)
+    need = getattr(lib, kind._WORKSPACE)(ref, n, k)
     if need == 0:
-        raise RuntimeError(f"smoe_{name}: unsupported shapes ({lib.smoe_last_error().decode()})")
+        raise RuntimeError(f"{name}: unsupported shapes ({lib.smoe_last_error().decode()})")
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    nat.launch(dev, f"smoe_{name}", ref, msg.data_ptr(), code,
+    nat.launch(dev, name, ref, msg.data_ptr(), code,
                idx.data_ptr(), wts.data_ptr(), n, k, delta.data_ptr(), code, ws.data_ptr(), need)
     del keep
     return delta
@@ -314,7 +323,7 @@ def sparse_expert_delta_fp8_blocks(messages: torch.Tensor, top_indices: torch.Te
     follows are summed in f32; bfloat16: the products by the e4m3 x e4m3 matrix
     instruction, which cuts each one by less than 2^-13 of the largest of its
     eight neighbours, the rest in f32.  No gradient."""
-    return _delta("expert_delta_fp8_blocks", Fp8BlockExperts, messages, top_indices, top_weights, experts)
+    return _delta("smoe_expert_delta_fp8_blocks", Fp8BlockExperts, messages, top_indices, top_weights, experts)
 
 
 def sparse_expert_delta_mxfp4(messages: torch.Tensor, top_indices: torch.Tensor,
@@ -324,4 +333,4 @@ def sparse_expert_delta_mxfp4(messages: torch.Tensor, top_indices: torch.Tensor,
     dtype.  Messages and hidden activations are quantized as quantize_mxfp4
     does on the way into the two products, whose sums, and all that follows,
     are in f32.  No gradient."""
-    return _delta("expert_delta_mxfp4", MxFp4Experts, messages, top_indices, top_weights, experts)
+    return _delta("smoe_expert_delta_mxfp4", MxFp4Experts, messages, top_indices, top_weights, experts)
